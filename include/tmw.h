@@ -442,6 +442,112 @@ TMW_API int tmw_cross_entropy(int32_t dtype, int32_t batch, int32_t tokens, int3
                       void* stream);
 
 /*
+ * Keys and values in pages.  The reference has no cache at all (its generation helper re-runs the forward per token,
+ * examples/train_math.py:146-161); the ring of tmw_cache_desc holds window+1 slots for every sequence, this form holds what
+ * the sequences have, in pages of a pool that they share.
+ *
+ * k_pages, v_pages : [pages, kv_heads, page_size, head_dim] contiguous, on a 16-byte boundary.
+ * page_table       : [batch, columns] int32 (device), rows table_stride elements apart: token t of sequence b lives in slot
+ *                    t % page_size of page page_table[b][t / page_size].  Entries that no token of a call needs are not read.
+ * Sequences may share pages that no call writes.  head_dim: a multiple of 8, at most 256.  columns * page_size < 2^31.
+ */
+typedef struct tmw_pages {
+    int32_t dtype; /* tmw_dtype of the pages and of every q, k, v and o that goes with them */
+    int32_t batch, kv_heads, head_dim;
+    int32_t page_size, pages, columns;
+    int32_t reserved; /* 0 */
+    int64_t table_stride;
+    void* k_pages;
+    void* v_pages;
+    const int32_t* page_table;
+} tmw_pages;
+
+/*
+ * New tokens into the pages.  k, v: [batch, kv_heads, rows, head_dim] through {batch, head, row} strides; row r of sequence b is
+ * its token start[b] + r and is stored if r < counts[b] (counts NULL: every row).  start[b] = -1: the sequence is not there,
+ * nothing of it is touched.
+ *
+ * rotated > 0 (even, at most head_dim) turns the first `rotated` numbers of every key by the token's position t on the way:
+ * pair i by the angle t * inv_freq[i] (inv_freq: rotated / 2 fp32 numbers, device), pairs being (i, i + rotated / 2) or, with
+ * interleaved, (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin), with the angle in 64 bits and one rounding at the end.
+ * q (may be NULL): [batch, heads, rows, head_dim], turned likewise into q_out, which may be q itself with the same strides; rows
+ * behind a sequence's last new token stay as they are.  Buffers must not overlap otherwise.
+ *
+ * The device checks what the host cannot see: a token without a place (a position or a page outside the table or the pool, or a
+ * count outside 0 .. rows, a start below -1, which takes the whole sequence) is not stored, its q_out is NaN, and tmw_poll_status
+ * reports TMW_ERR_INVALID_ARGUMENT.
+ */
+typedef struct tmw_paged_append_desc {
+    tmw_pages at;
+    int32_t rows, heads; /* heads: of q, 0 without */
+    int32_t rotated, interleaved;
+    const void *k, *v, *q;
+    void* q_out;
+    int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
+    const int32_t* start;
+    const int32_t* counts;
+    const float* inv_freq;
+} tmw_paged_append_desc;
+
+TMW_API int tmw_paged_append(const tmw_paged_append_desc* desc, void* stream);
+
+/*
+ * Attention of one new token per sequence over its pages: o[b, h] = softmax(q[b, h] kᵀ · scale) v over the persistent keys
+ * (k_pers, v_pers: [kv_heads, n_persistent, head_dim] contiguous, shared by the batch) and the sequence's tokens
+ * max(0, pos[b] - window) .. pos[b] (window -1: all of them), the new one at pos[b] among them: it has been appended before.
+ * q, o: [batch, heads, head_dim] through {batch, head} strides; heads is a multiple of kv_heads, and head h reads the keys of
+ * head h / (heads / kv_heads).  pos[b] = -1: a sequence without tokens; it sees the persistent keys, and without these its output
+ * is zero.  A position or a page outside the table or the pool makes the sequence's output NaN and is reported by
+ * tmw_poll_status (TMW_ERR_INVALID_ARGUMENT).
+ *
+ * The keys of all sequences are shared out evenly over the GPU, however long each sequence is; the parts of one that came to
+ * several CTAs are joined by a second launch.  `scratch`: device memory of tmw_paged_attention_scratch_bytes() bytes on a 16-byte
+ * boundary, of any content, used until the call's kernels have finished.  The result does not depend on the schedule.
+ */
+typedef struct tmw_paged_attention_desc {
+    tmw_pages at;
+    int32_t heads, n_persistent, window;
+    float scale; /* 0 selects 1/sqrt(head_dim) */
+    const void *q, *k_pers, *v_pers;
+    void* o;
+    int64_t q_stride[2], o_stride[2];
+    const int32_t* pos;
+} tmw_paged_attention_desc;
+
+TMW_API size_t tmw_paged_attention_scratch_bytes(const tmw_paged_attention_desc* desc);
+TMW_API int tmw_paged_attention(const tmw_paged_attention_desc* desc, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * What a row of logits says of a token: logprobs[r] = log softmax(logits[r])[targets[r]] (targets: int64; -100: none, the value is
+ * 0), entropy[r] = -sum p log p, and the `top` most likely ids with their log-probabilities (top_ids int64, top_logprobs, both
+ * [rows, top]; among equal logits the lower id first; top at most 32 and at most vocab).  Rows are (b, t): row b * tokens + t of
+ * the outputs, at logits + b * stride[0] + t * stride[1]; any address that the element type allows.  lse[r] (optional, with the
+ * entropy what the backward needs): largest logit, and the logarithm of the sum of exponentials below it, [rows, 2].
+ * All outputs are fp32 (ids apart).  A logit of -inf has probability 0.  A row without a distribution (a NaN, +inf, or nothing but
+ * -inf) has NaN everywhere (but for the 0 of a target of -100) and ids of -1; a target outside the vocabulary has NaN and is
+ * reported by tmw_poll_status.  vocab at most 2^26.
+ *
+ * Backward: d_logits (rows like logits, through d_stride; must not overlap them) from the gradients of logprobs, entropy and
+ * top_logprobs, each NULL where there is none (contiguous fp32), and the forward's entropy, lse and top_ids.  A row to which
+ * nothing but zeros comes back has a gradient of zeros.  Extends the loss of titanmac.py:674-684 (its mean cross-entropy is minus
+ * the mean of logprobs).
+ */
+typedef struct tmw_logprobs_desc {
+    int32_t dtype;
+    int32_t batch, tokens, vocab, top;
+    int32_t reserved; /* 0 */
+    const void* logits;
+    int64_t stride[2];
+    const int64_t* targets;
+    float *logprobs, *entropy, *lse, *top_logprobs;
+    int64_t* top_ids;
+} tmw_logprobs_desc;
+
+TMW_API int tmw_token_logprobs(const tmw_logprobs_desc* desc, void* stream);
+TMW_API int tmw_token_logprobs_backward(const tmw_logprobs_desc* desc, const float* d_logprobs, const float* d_entropy,
+                                        const float* d_top, void* d_logits, const int64_t d_stride[2], void* stream);
+
+/*
  * One decode step of the whole model: token_ids [batch] int64 and pos [batch] int32 (device) -> logits [batch, vocab].
  * Every block runs RMSNorm -> QKV -> tmw_decode on its ring -> output projection + residual -> RMSNorm -> MLP + residual
  * (titan_block.py:92-100, blocks/mlp.py:58-65), then the final norm and the head; what the reference's generation

@@ -6,8 +6,10 @@ from .attn.block_sparse_attention import BlockSparseAttention, create_block_spar
 from .blocks.titan_block import MLPBlock, RMSNorm, TitanBlock
 from .models.titanmac import TitanMAC
 from .host_pipeline import HostPipeline
+from .paged_cache import PagedCache, paged_append, paged_attention
+from .logprobs import TokenLogprobs, token_logprobs
 from . import _native
 
 __all__ = ["TitanMACConfig", "WindowConfig", "WindowedAttention", "BlockSparseAttention",
            "create_block_sparse_attention", "TitanBlock", "RMSNorm", "MLPBlock", "TitanMAC",
-           "HostPipeline", "_native"]
+           "HostPipeline", "PagedCache", "paged_append", "paged_attention", "TokenLogprobs", "token_logprobs", "_native"]

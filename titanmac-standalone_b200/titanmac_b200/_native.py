@@ -278,6 +278,15 @@ SIGNATURES = {
         [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
     ),
+    # (descriptions packed by paged_cache and logprobs: filling a ctypes structure field by field takes longer than the calls)
+    "tmw_paged_append": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "tmw_paged_attention_scratch_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
+    "tmw_paged_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tmw_token_logprobs": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "tmw_token_logprobs_backward": (
+        ctypes.c_int,
+        [ctypes.c_char_p] + [ctypes.c_void_p] * 4 + [ctypes.c_char_p, ctypes.c_void_p],
+    ),
 }
 
 MAX_DECODE_SPLITS = 16

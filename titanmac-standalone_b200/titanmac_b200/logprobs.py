@@ -1,0 +1,121 @@
+"""What rows of logits say of tokens: their log-probabilities, the entropy, the most likely alternatives (``tmw_token_logprobs``).
+
+The model's own loss is the mean of the first with the opposite sign; here every token's value is kept, and all three can be
+trained on.
+"""
+
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_DESC = struct.Struct("@6iQ2q6Q")  # tmw_logprobs_desc
+_STRIDES = struct.Struct("@2q")
+MAX_TOP = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprobs`` and ``entropy`` of the shape of the targets, ``top_ids`` (int64) and ``top_logprobs`` with one more axis of the
+    alternatives, the most likely first and the lower id first among equals (None without alternatives).  fp32."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+
+
+def _rows(t: torch.Tensor):
+    """``(tensor with the same values, batch, tokens, strides)`` of ``[.., V]``: rows in two steps, one behind the other inside."""
+    shape, strides = t.shape, t.stride()
+    if (strides[-1] != 1 and shape[-1] != 1) or t.dim() > 3:
+        t = t.contiguous()
+        strides = t.stride()
+    if t.dim() == 3:
+        return t, shape[0], shape[1], strides[:2]
+    if t.dim() == 1:
+        return t, 1, 1, (0, 0)
+    if t.dim() == 2:
+        return t, shape[0], 1, (strides[0], 0)
+    return t, t.numel() // shape[-1], 1, (shape[-1], 0)
+
+
+def _pack(rows, vocab: int, n_top: int, dtype: torch.dtype, targets, logprobs, entropy, lse, top_logprobs, top_ids):
+    t, batch, tokens, strides = rows
+    return _DESC.pack(_native._DTYPES[dtype], batch, tokens, vocab, n_top, 0, t.data_ptr(), *strides, targets.data_ptr(), logprobs,
+                      entropy.data_ptr(), lse.data_ptr() if lse is not None else 0, top_logprobs,
+                      top_ids.data_ptr() if top_ids is not None else 0)
+
+
+def _forward(logits: torch.Tensor, targets: torch.Tensor, n_top: int, with_lse: bool):
+    """``(logprobs, entropy, top_ids, top_logprobs, lse)``; without alternatives the ids and their values are None."""
+    device, shape = logits.device, targets.shape
+    logprobs, entropy = torch.empty((2, *shape), dtype=torch.float32, device=device)
+    lse = torch.empty((*shape, 2), dtype=torch.float32, device=device) if with_lse else None
+    top_ids = top_logprobs = None
+    if n_top:
+        top_ids = torch.empty((*shape, n_top), dtype=torch.int64, device=device)
+        top_logprobs = torch.empty((*shape, n_top), dtype=torch.float32, device=device)
+    if targets.numel():
+        rows = _rows(logits)
+        desc = _pack(rows, logits.shape[-1], n_top, logits.dtype, targets, logprobs.data_ptr(), entropy, lse,
+                     top_logprobs.data_ptr() if n_top else 0, top_ids)
+        with _native._on(device):
+            _native.check(_native.lib().tmw_token_logprobs(desc, _native._stream_ptr(device)))
+    return logprobs, entropy, top_ids, top_logprobs, lse
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits: torch.Tensor, targets: torch.Tensor, n_top: int):
+        logprobs, entropy, top_ids, top_logprobs, lse = _forward(logits, targets, n_top, True)
+        ctx.n_top = n_top
+        ctx.set_materialize_grads(False)
+        if n_top:
+            ctx.mark_non_differentiable(top_ids)
+        ctx.save_for_backward(logits, targets, lse, entropy, top_ids)
+        return logprobs, entropy, top_ids, top_logprobs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_logprobs, d_entropy, _, d_top):
+        logits, targets, lse, entropy, top_ids = ctx.saved_tensors
+        device = logits.device
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        given = [None if g is None else g.contiguous() for g in (d_logprobs, d_entropy, d_top)]
+        if targets.numel():
+            rows = _rows(logits)  # (held: it may be a copy)
+            desc = _pack(rows, logits.shape[-1], ctx.n_top, logits.dtype, targets, 0, entropy, lse, 0, top_ids)
+            with _native._on(device):
+                _native.check(_native.lib().tmw_token_logprobs_backward(
+                    desc, *(None if g is None else g.data_ptr() for g in given), d_logits.data_ptr(),
+                    _STRIDES.pack(*_rows(d_logits)[3]), _native._stream_ptr(device)))
+        return d_logits, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_top: int = 0) -> TokenLogprobs:
+    """Log-probabilities of ``targets [..]`` (int64) under ``logits [.., V]``, the entropy of every row, and its ``n_top`` (at most
+    32) most likely ids.  Differentiable in the logits.
+
+    A target of -100 counts as none: its value is 0 and no gradient comes from it.  A target outside the vocabulary has NaN and
+    ``_native.poll_status`` raises.  A row without a distribution (a NaN, +inf or nothing but -inf among its logits) has NaN, and
+    ids of -1."""
+    _native._require_cuda(logits, targets)
+    if logits.dtype not in _native._DTYPES:
+        raise TypeError("token_logprobs: logits in fp32, bf16 or fp16 expected")
+    if targets.dtype != torch.int64:
+        raise TypeError("token_logprobs: targets must be int64")
+    if logits.dim() < 1 or logits.shape[:-1] != targets.shape or logits.shape[-1] == 0:
+        raise ValueError("token_logprobs: logits [.., vocabulary] and targets [..] must agree in the axes in front")
+    if targets.device != logits.device:
+        raise ValueError("token_logprobs: logits and targets must be on one device")
+    if not 0 <= n_top <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: n_top must be in 0 .. {min(MAX_TOP, logits.shape[-1])}, got {n_top}")
+    targets = targets.contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, n_top))
+    return TokenLogprobs(*_forward(logits, targets, n_top, False)[:4])

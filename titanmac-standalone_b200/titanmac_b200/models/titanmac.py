@@ -24,7 +24,7 @@ re-forward would return for its last row.
 
 from __future__ import annotations
 
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Union
 
 import torch
 import torch.nn as nn
@@ -32,6 +32,8 @@ import torch.nn.functional as F
 
 from .. import _native, _stack, _train
 from ..blocks.titan_block import RMSNorm, TitanBlock
+from ..paged_cache import PagedCache
+from ..logprobs import TokenLogprobs, token_logprobs
 
 
 class TitanMAC(nn.Module):
@@ -114,6 +116,16 @@ class TitanMAC(nn.Module):
             out["loss"] = loss
         return out
 
+    def token_logprobs(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None, n_top: int = 0) -> TokenLogprobs:
+        """What the model says of every next token: entry ``[b, t]`` is the log-probability of ``labels[b, t + 1]`` (default: the
+        ids themselves; -100: none) behind the tokens ``0 .. t``, with the entropy and the ``n_top`` most likely ids there.  The
+        last column has no next token: its log-probability is 0, its alternatives are what comes next.  ``forward``'s loss is minus
+        the mean of the counted entries; gradients flow as they do there."""
+        labels = input_ids if labels is None else labels
+        targets = torch.full_like(labels, -100)
+        targets[:, :-1] = labels[:, 1:]
+        return token_logprobs(self.forward(input_ids)["logits"], targets, n_top)
+
     def _forward_modules(self, input_ids: torch.Tensor) -> torch.Tensor:
         """Logits of every row, persistent rows first, module by module."""
         x = self._embed(input_ids)
@@ -147,8 +159,18 @@ class TitanMAC(nn.Module):
         storage = torch.zeros((len(self.layers), _native.RingCache.elements(*geometry)), dtype=dtype, device=device)
         return [_native.RingCache(*geometry, dtype, device, storage=storage[i]) for i in range(len(self.layers))]
 
+    def new_paged_caches(self, page_table: torch.Tensor, pages: int, page_size: int, dtype) -> List[PagedCache]:
+        """Caches for ``prefill`` and ``decode_step`` whose sequences live in pages: ``page_table [B, columns]`` (int32, on the
+        device, shared by the layers), a pool of ``pages`` pages of ``page_size`` tokens per layer.  ``prefill`` fills every
+        sequence's pages with the whole prompt it is given; ``decode_step`` takes positions of -1 for rows without a sequence
+        (their logits mean nothing)."""
+        self._need_windowed()
+        c = self.config
+        return [PagedCache(page_table, pages, page_size, c.n_heads, c.d_head, c.window_size, c.n_persistent, dtype)
+                for _ in self.layers]
+
     @torch.no_grad()
-    def prefill(self, input_ids: torch.Tensor, caches: Optional[List[_native.RingCache]] = None):
+    def prefill(self, input_ids: torch.Tensor, caches: Optional[List[Union[_native.RingCache, PagedCache]]] = None):
         """Run the prompt ``[B, T]`` once; returns (logits of the last prompt token ``[B, V]``, caches)."""
         self._need_windowed()
         B, T = input_ids.shape
@@ -188,7 +210,8 @@ class TitanMAC(nn.Module):
         return logits, caches
 
     @torch.no_grad()
-    def decode_step(self, token_ids: torch.Tensor, pos: torch.Tensor, caches: List[_native.RingCache]) -> torch.Tensor:
+    def decode_step(self, token_ids: torch.Tensor, pos: torch.Tensor,
+                    caches: List[Union[_native.RingCache, PagedCache]]) -> torch.Tensor:
         """One new token per sequence.  ``token_ids [B]``, ``pos [B] int32`` = its index in the sequence
         (the prompt occupied 0..T-1).  Returns logits ``[B, V]``; ``pos`` is not modified."""
         self._need_windowed()
@@ -199,7 +222,10 @@ class TitanMAC(nn.Module):
                 return logits
         c = self.config
         B = token_ids.shape[0]
-        x = self.embed_tokens(token_ids) + self.embed_positions(pos.long())
+        at = pos.long()
+        if any(isinstance(cache, PagedCache) for cache in caches):  # (a row without a sequence is at -1)
+            at = at.clamp(min=0)
+        x = self.embed_tokens(token_ids) + self.embed_positions(at)
         pending = None
         for layer, cache in zip(self.layers, caches):
             attn = layer.attention
