@@ -13,6 +13,8 @@
 // scratch memory, and a second kernel, launched under the first, joins them in the order of the CTAs.
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace tmw {
@@ -33,6 +35,7 @@ struct PagedAttention {
     int items;        // of a sequence
     float scale;      // times log2(e)
     int row_bytes;
+    bool q_pairs;  // queries can be read two at a time
     float* partial;  // [CTA][2][rows][head_dim]: of the item that a CTA begins with, of the one that it ends with
     float2* sums;    // [CTA][2][rows]: maximum, sum
     int4* joins;     // [CTA]: the item cut at the CTA's end that begins in it - sequence, item, last CTA, which of the two parts
@@ -328,11 +331,218 @@ struct SimtCore {
     }
 };
 
+// ---- the core on tensor cores: 16-bit types, head_dim 32, 64, 96, 128 or 256 -------------------------------------------------
+// mma.sync with the query heads as the sixteen rows of a tile (tcgen05's 64 or 128 would multiply a group of at most sixteen
+// for nothing, and the step is bound by HBM long before): scores 16 x 16 keys, their exponentials straight from the accumulators
+// to the operand of the second product.  The weights go in as two 16-bit numbers each, a value and what it lacks: one alone would
+// put up to 2^-9 of itself on the output, the two 2^-16.  (The first is cut off and the second is never zero: both positive,
+// they take an infinite value to infinity, as the weight itself would.)  In fp16 they are raised by 2^12, as far as the largest allows, so
+// that those below 2^-14 of it keep their bits.  Up to eight heads: the tile's upper eight rows are zeros and have no registers.
+template <int DH>
+struct MmaLayout {
+    int bytes;
+    __host__ __device__ static constexpr int pitch() { return DH * 2; }
+    __host__ __device__ static constexpr int chunks() { return DH / 8; }
+    // a chunk's place in its row keeps eight rows' same chunk on different banks
+    __device__ __forceinline__ static int offset(int r, int c) {
+        const int turn = chunks() % 8 == 0 ? r & 7 : r >> 1 & 3;
+        return r * pitch() + ((c ^ turn) << 4);
+    }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// the same cut off instead of rounded
+template <typename T>
+__device__ __forceinline__ uint32_t cut2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t cut2<__nv_bfloat16>(float a, float b) {
+    uint32_t w;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
+}
+template <>
+__device__ __forceinline__ uint32_t cut2<__half>(float a, float b) {
+    uint32_t w;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
+}
+// no number below the smallest that a product takes (2^-126, 2^-24)
+template <typename T>
+__device__ __forceinline__ uint32_t positive2(uint32_t w);
+template <>
+__device__ __forceinline__ uint32_t positive2<__nv_bfloat16>(uint32_t w) {
+    const uint32_t least = 0x00800080u;
+    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&least));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t positive2<__half>(uint32_t w) {
+    const uint32_t least = 0x00010001u;
+    const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&least));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+template <typename T, int DH, bool WIDE>
+struct MmaCore {
+    static constexpr int kRows = kMaxRows;
+    static constexpr int kHalves = WIDE ? 2 : 1;  // of the sixteen rows
+    static constexpr float kRaise = std::is_same<T, __half>::value ? 12.f : 0.f;
+    using Layout = MmaLayout<DH>;
+    const PagedAttention& p;
+    uint32_t q[DH / 16][2 * kHalves];  // a0, a2 (, a1, a3)
+    float m[kHalves], l[kHalves];      // of rows lane / 4 and 8 + lane / 4; l: this lane's columns
+    float o[DH / 8][2 * kHalves];
+
+    static __host__ __device__ int extra(int) { return 0; }
+
+    __device__ MmaCore(const PagedAttention& p, unsigned char*) : p(p) {}
+    __device__ __forceinline__ void begin(int b, int first, int rows) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            const int r = h * 8 + lane / 4;
+            const T* from = static_cast<const T*>(p.q) + b * p.qs[0] + (first + r) * p.qs[1] + lane % 4 * 2;
+#pragma unroll
+            for (int k = 0; k < DH / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t w = 0;
+                    if (r < rows) {
+                        const T* at = from + k * 16 + i * 8;
+                        if (p.q_pairs) w = *reinterpret_cast<const uint32_t*>(at);
+                        else w = *reinterpret_cast<const uint16_t*>(at) | (uint32_t)*reinterpret_cast<const uint16_t*>(at + 1) << 16;
+                    }
+                    q[k][h * 2 + i] = w;
+                }
+            m[h] = -CUDART_INF_F;
+            l[h] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < DH / 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 2 * kHalves; ++i) o[j][i] = 0.f;
+    }
+    // c += a b, a the rows' two halves (the upper one zero where there is none)
+    __device__ __forceinline__ static void product(float* c, const uint32_t (&a)[2 * kHalves], uint32_t b0, uint32_t b1) {
+        float d[4] = {c[0], c[1], WIDE ? c[2] : 0.f, WIDE ? c[3] : 0.f};
+        mma_16816<T>(d, a[0], WIDE ? a[2] : 0u, a[1], WIDE ? a[3] : 0u, b0, b1);
+        c[0] = d[0];
+        c[1] = d[1];
+        if (WIDE) c[2] = d[2], c[3] = d[3];
+    }
+    __device__ __forceinline__ void tile(const unsigned char* tile, uint32_t marks, const Layout& lay) {
+        const int lane = threadIdx.x & 31;
+        const uint32_t keys = (uint32_t)__cvta_generic_to_shared(tile), values = keys + kTile * Layout::pitch();
+        float s[2][2 * kHalves] = {};  // eight keys each
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k) {
+            uint32_t b[4];
+            ldmatrix4(b, keys + lay.offset((lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)));
+            product(s[0], q[k], b[0], b[1]);
+            product(s[1], q[k], b[2], b[3]);
+        }
+        uint32_t hi[2 * kHalves], lo[2 * kHalves];  // a0, a2 (, a1, a3) of the weights
+        float keep[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            float top = -CUDART_INF_F;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = j * 8 + lane % 4 * 2 + e;
+                    float& x = s[j][h * 2 + e];
+                    x = marks >> (16 + key) & 1 ? CUDART_NAN_F : marks >> key & 1 ? x * p.scale : -CUDART_INF_F;
+                    top = fmaxf(top, x);
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float now = fmaxf(m[h], top), base = now == -CUDART_INF_F ? 0.f : now;
+            keep[h] = m[h] == -CUDART_INF_F ? 1.f : ex2_ftz(m[h] - base);  // (nothing to keep, or NaN)
+            m[h] = now;
+            l[h] *= keep[h];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float w[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    w[e] = ex2_ftz(s[j][h * 2 + e] - base + kRaise);
+                    l[h] += w[e];
+                }
+                hi[h * 2 + j] = cut2<T>(w[0], w[1]);
+                const float2 there = unpack2<T>(hi[h * 2 + j]);
+                lo[h * 2 + j] = positive2<T>(pack2<T>(w[0] - there.x, w[1] - there.y));
+            }
+        }
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[kHalves - 1] != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < DH / 8; ++j)
+#pragma unroll
+                for (int i = 0; i < 2 * kHalves; ++i) o[j][i] *= keep[i / 2];
+        }
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, values + lay.offset((lane >> 3 & 1) * 8 + (lane & 7), k * 2 + (lane >> 4)));
+            product(o[2 * k], hi, b[0], b[1]);
+            product(o[2 * k + 1], hi, b[2], b[3]);
+            product(o[2 * k], lo, b[0], b[1]);
+            product(o[2 * k + 1], lo, b[2], b[3]);
+        }
+    }
+    __device__ __forceinline__ void leave(float2* sums, float* out, int rows) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            const int r = h * 8 + lane / 4;
+            float t = l[h];
+            t += __shfl_xor_sync(0xffffffffu, t, 1);
+            t += __shfl_xor_sync(0xffffffffu, t, 2);
+            if (r >= rows) continue;
+            if (lane % 4 == 0) sums[r] = make_float2(m[h], t);
+#pragma unroll
+            for (int j = 0; j < DH / 8; ++j)
+                *reinterpret_cast<float2*>(out + r * DH + j * 8 + lane % 4 * 2) = make_float2(o[j][h * 2], o[j][h * 2 + 1]);
+        }
+    }
+};
+
 // ---- the line of tiles ------------------------------------------------------------------------------------------------------
 
 // weight of a part whose maximum is m under the common one (base: that, or 0 where it is -inf): a part of hidden scores alone
 // holds zeros, or NaN that has to stay
 __device__ __forceinline__ float part_weight(float m, float base) { return m == -CUDART_INF_F ? 1.f : exp2f(m - base); }
+
+// (the largest score's weight is 1 or more: no sum at all is that of scores of -inf)
+__device__ __forceinline__ float quotient(float o, float l) { return l == 0.f ? CUDART_NAN_F : o / l; }
 
 template <typename T, typename Core, int W, int S>
 __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_constant__ PagedAttention p) {
@@ -416,7 +626,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
                 o = fmaf(x, outs[w * p.rows * dim + i], o);
             }
             if (whole) {
-                static_cast<T*>(p.o)[at.b * p.os[0] + (head + r) * p.os[1] + (i - r * dim)] = from_f32<T>(o / l);
+                static_cast<T*>(p.o)[at.b * p.os[0] + (head + r) * p.os[1] + (i - r * dim)] = from_f32<T>(quotient(o, l));
             } else {
                 p.partial[slot * p.rows * dim + i] = o;
                 if (i == r * dim) p.sums[slot * p.rows + r] = make_float2(m, l);
@@ -480,7 +690,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
         out += outs[w][tid];
     }
     const int head = join.y / p.parts * p.group + first + r;
-    static_cast<T*>(p.o)[join.x * p.os[0] + head * p.os[1] + tid] = from_f32<T>(out / sum);
+    static_cast<T*>(p.o)[join.x * p.os[0] + head * p.os[1] + tid] = from_f32<T>(quotient(out, sum));
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -542,11 +752,28 @@ int with_simt(const tmw_paged_attention_desc& d, F&& use) {
     return use(Kernel<T, SimtCore<T>, 2, 3>());
 }
 
+template <typename T, int DH, typename F>
+int with_mma(const tmw_paged_attention_desc& d, F&& use) {
+    if (d.heads / d.at.kv_heads <= 8) return use(Kernel<T, MmaCore<T, DH, false>, 4, 3>());
+    return use(Kernel<T, MmaCore<T, DH, true>, (DH > 128 ? 2 : 4), 3>());
+}
+template <typename T, typename F>
+int with_16_bits(const tmw_paged_attention_desc& d, F&& use) {
+    switch (d.at.head_dim) {
+        case 32: return with_mma<T, 32>(d, use);
+        case 64: return with_mma<T, 64>(d, use);
+        case 96: return with_mma<T, 96>(d, use);
+        case 128: return with_mma<T, 128>(d, use);
+        case 256: return with_mma<T, 256>(d, use);
+        default: return with_simt<T>(d, use);
+    }
+}
+
 // `use` with the Kernel that takes the call
 template <typename F>
 int with_kernel(const tmw_paged_attention_desc& d, F&& use) {
     if (d.at.dtype == TMW_F32) return with_simt<float>(d, use);
-    return d.at.dtype == TMW_BF16 ? with_simt<__nv_bfloat16>(d, use) : with_simt<__half>(d, use);
+    return d.at.dtype == TMW_BF16 ? with_16_bits<__nv_bfloat16>(d, use) : with_16_bits<__half>(d, use);
 }
 
 int validate(const tmw_paged_attention_desc* d, bool& used) {
@@ -607,6 +834,7 @@ extern "C" int tmw_paged_attention(const tmw_paged_attention_desc* d, void* scra
     p.group = d->heads / d->at.kv_heads;
     p.scale = (d->scale > 0.f ? d->scale : 1.0f / sqrtf((float)d->at.head_dim)) * 1.4426950408889634f;
     p.row_bytes = d->at.head_dim * (int)size;
+    p.q_pairs = bits(d->q) % 4 == 0 && (d->q_stride[0] | d->q_stride[1]) % 2 == 0;
     p.status = device_status_word();
     if (p.status == nullptr) return TMW_ERR_CUDA;
     return with_kernel(*d, [&](auto kernel) {
