@@ -6,11 +6,12 @@
 // handful of keys, launch and latency.
 //
 // The lengths are on the device and may differ by any factor, so the host cannot cut the work up.  The keys of an item - a
-// sequence and the heads of one key head, at most kMaxRows of them - come in tiles of 16, the tiles of all items in one line, and
-// CTA c takes the tiles [c, c + 1) * per of it: every CTA the same number, whatever the lengths.  Its warps take every
-// W-th tile, each with its own ring of tiles in shared memory (cp.async, no barrier in the loop) and its own maximum and
-// sums, and join them where an item ends.  An item that lies in one CTA is stored at once; the parts of one that was cut go to
-// scratch memory, and a second kernel, launched under the first, joins them in the order of the CTAs.
+// sequence and the heads of one key head, at most kMaxRows of them - come in tiles of 32 or 16, the tiles of all items in one line, and
+// every warp of the grid takes an equal piece of the line, whatever the lengths.  A warp has its own ring of tiles in shared
+// memory (cp.async), its own running maximum and sums, and meets no barrier on its way: an item that lies in its piece is stored
+// from its registers.  Of an item that was cut, the warps of a CTA join their parts through shared memory when all of them are
+// done; what was cut between CTAs goes to scratch memory, and a second kernel, launched under the first, joins it in the order of
+// the CTAs.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -20,7 +21,6 @@
 namespace tmw {
 namespace {
 
-constexpr int kTile = 16;   // keys
 constexpr int kMaxRows = 16;
 
 struct PagedAttention {
@@ -30,120 +30,126 @@ struct PagedAttention {
     long long qs[2], os[2];
     const int32_t* pos;
     int batch, np, window;
+    int pers_tiles;    // of the persistent keys
+    bool whole_runs;   // sixteen tokens from a multiple of sixteen on lie in one page
     int group;        // query heads of a key head
     int rows, parts;  // query heads of an item at most; items of a key head
     int items;        // of a sequence
     float scale;      // times log2(e)
     int row_bytes;
     bool q_pairs;  // queries can be read two at a time
-    float* partial;  // [CTA][2][rows][head_dim]: of the item that a CTA begins with, of the one that it ends with
+    float* partial;  // [CTA][2][rows][head_dim]: of the item that a CTA begins in, of the one that begins in it
     float2* sums;    // [CTA][2][rows]: maximum, sum
-    int4* joins;     // [CTA]: the item cut at the CTA's end that begins in it - sequence, item, last CTA, which of the two parts
+    float* firsts;   // [CTA][warp][rows][head_dim]: what a warp has of the item that its piece begins in
+    int4* joins;     // [CTA]: the item that begins in it and ends in another one - sequence (-1: none), item, last CTA
     int* status;
 };
 
-// Tiles of sequence b's items; lo, pos: its first and last token seen (lo > pos: none).  0 with bad: no such position.
+// Tiles, of KT keys, of sequence b's items; lo, pos: its first and last token seen (lo > pos: none).  0 with bad: no such position.
+template <int KT>
 __device__ __forceinline__ int tiles_of(const PagedAttention& p, int b, int& lo, int& pos, bool& bad) {
     pos = __ldg(p.pos + b);
     bad = pos < -1 || pos >= p.map.capacity;
     lo = 0;
     if (bad) return 0;
-    const int pers = (p.np + kTile - 1) / kTile;
-    if (pos < 0) return pers;
+    if (pos < 0) return p.pers_tiles;
     if (p.window >= 0 && pos > p.window) lo = pos - p.window;
-    return pers + pos / kTile - lo / kTile + 1;
+    return p.pers_tiles + pos / KT - lo / KT + 1;
 }
 
-// A place in the line of tiles.
+// A place in the line.  An item takes kItemCost more units of it than it has tiles, ahead of them: loading the queries and
+// storing the output hold a warp up for about that long, and pieces of equal length are to take equal time.
+constexpr int kItemCost = 1;
+template <int KT>
 struct Cursor {
     int b, item;  // sequence, item of it
-    int t, n;     // tile of the item, of so many
+    int head;     // the item's key head
+    int t, n;     // unit of the item; units of an item
     int lo, pos;
     __device__ __forceinline__ void sequence(const PagedAttention& p) {
         bool bad;
-        n = tiles_of(p, b, lo, pos, bad);
+        n = tiles_of<KT>(p, b, lo, pos, bad);
+        if (n > 0) n += kItemCost;
     }
-    // k tiles on; not past the end of the line
-    __device__ __forceinline__ void advance(const PagedAttention& p, int k) {
-        t += k;
-        while (t >= n) {
-            t -= n;
-            if (++item == p.items) {
-                item = 0;
-                do {
-                    ++b;
-                    sequence(p);
-                } while (n == 0);
-            }
+    __device__ __forceinline__ int tile() const { return t - kItemCost; }
+    // the next item's first unit; not past the end of the line
+    __device__ __forceinline__ void next_item(const PagedAttention& p) {
+        t = 0;
+        if (++item < p.items) {
+            head = item / p.parts;
+            return;
         }
+        item = head = 0;
+        do {
+            ++b;
+            sequence(p);
+        } while (n == 0);
     }
 };
 
-// This CTA's part of the line, and the place where it begins.  Every thread of the CTA.
+__device__ __forceinline__ long long scan(long long x) {  // sums up to each lane
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// This warp's piece of the line: units [first, end), of pieces of `per` units, `warps` of which go to a CTA; and the place where it
+// begins.
 struct Share {
     long long first, end, per;
+    int warps;
 };
-template <int W>
-__device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor& at) {
-    __shared__ long long warp_sum[W];
-    __shared__ long long found_before;
-    __shared__ int found_b;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int lo, pos;
-    bool bad;
-    // tiles of all sequences
-    long long sum = 0;
-    for (int b = tid; b < p.batch; b += (W * 32)) sum += tiles_of(p, b, lo, pos, bad);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) warp_sum[warp] = sum;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) total += warp_sum[w];
-    total *= p.items;
+template <int KT>
+__device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT>& at) {
+    const int lane = threadIdx.x & 31;
+    auto units = [&](int b) -> long long {
+        if (b >= p.batch) return 0;
+        int lo, pos;
+        bool bad;
+        const int n = tiles_of<KT>(p, b, lo, pos, bad);
+        return n > 0 ? (long long)(n + kItemCost) * p.items : 0;
+    };
+    // each lane sums up a run of sequences
+    const int run = (p.batch + 31) / 32;
+    long long mine = 0;
+    for (int i = 0; i < run; ++i) mine += units(lane * run + i);
+    const long long upto = scan(mine), total = __shfl_sync(0xffffffffu, upto, 31);
     Share s;
-    // (below a tile for every warp, a CTA more costs more to join than it saves)
-    s.per = (total + gridDim.x - 1) / gridDim.x;
-    if (s.per < W) s.per = W;
-    s.first = s.per * blockIdx.x;
-    s.end = s.first + s.per < total ? s.first + s.per : total;
-    if (s.first >= s.end) return s;
-    // the sequence that holds the first tile
-    long long before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += (W * 32)) {
-        const int b = b0 + tid;
-        const long long mine = b < p.batch ? (long long)tiles_of(p, b, lo, pos, bad) * p.items : 0;
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
-        }
-        __syncthreads();
-        if (lane == 31) warp_sum[warp] = upto;
-        if (tid == 0) found_b = -1;
-        __syncthreads();
-        long long all = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) upto += warp_sum[w];
-            all += warp_sum[w];
-        }
-        upto += before;
-        if (upto - mine <= s.first && s.first < upto) {
-            found_b = b;
-            found_before = upto - mine;
-        }
-        __syncthreads();
-        if (found_b >= 0) break;
-        before += all;
+    const int most = blockDim.x / 32, warp = threadIdx.x / 32;
+    s.warps = most;
+    s.per = (total + (long long)gridDim.x * most - 1) / ((long long)gridDim.x * most);
+    if (s.per <= kItemCost) {  // a tile at least, and with less than that for every warp all SMs rather than all warps of some
+        s.per = kItemCost + 1;
+        s.warps = (int)((total + gridDim.x * s.per - 1) / (gridDim.x * s.per));
+        s.warps = max(min(s.warps, most), 1);
     }
-    at.b = found_b;
+    s.first = s.per * (blockIdx.x * (long long)s.warps + warp);
+    s.end = warp >= s.warps ? s.first : s.first + s.per < total ? s.first + s.per : total;
+    if (s.first >= s.end) return s;
+    // the run that holds the first unit, and the sequence in it
+    const int owner = __ffs(__ballot_sync(0xffffffffu, upto > s.first)) - 1;
+    long long before = __shfl_sync(0xffffffffu, upto - mine, owner);
+    for (int i = 0;; i += 32) {
+        const int b = owner * run + i + lane;
+        const long long own = i + lane < run ? units(b) : 0, sum = scan(own) + before;
+        const uint32_t there = __ballot_sync(0xffffffffu, sum > s.first);
+        if (there != 0) {
+            const int l = __ffs(there) - 1;
+            at.b = owner * run + i + l;
+            before = __shfl_sync(0xffffffffu, sum - own, l);
+            break;
+        }
+        before = __shfl_sync(0xffffffffu, sum, 31);
+    }
     at.sequence(p);
-    const long long inside = s.first - found_before;
+    const long long inside = s.first - before;
     at.item = (int)(inside / at.n);
     at.t = (int)(inside - (long long)at.item * at.n);
+    at.head = at.item / p.parts;
     return s;
 }
 
@@ -151,52 +157,100 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-// A warp's ring: tiles of keys, as many of values, and what of them counts (bits 0-15: seen, 16-31: without a page).
+// A warp's ring: tiles of keys, as many of values, and which of their rows are seen and which have no page.
 struct Ring {
     unsigned char* tiles;
-    uint32_t* marks;
+    uint2* marks;
 };
 
-// Tile `at` of keys and values into a stage of the ring.  Rows that do not count become zeros: whatever stands in a page behind a
-// sequence's end, infinities and NaN among them, reaches no product.
-template <typename T, typename Layout>
-__device__ __forceinline__ void load_tile(const PagedAttention& p, const Ring& ring, const Layout& lay, const Cursor& at, int stage) {
-    const int lane = threadIdx.x & 31, r = lane & (kTile - 1);
-    const int head = at.item / p.parts;
-    const int pers = (p.np + kTile - 1) / kTile;
-    const unsigned char *k = static_cast<const unsigned char*>(p.k_pages), *v = static_cast<const unsigned char*>(p.v_pages);
-    long long row = -1;
-    bool seen;
-    if (at.t < pers) {
-        k = static_cast<const unsigned char*>(p.k_pers);
-        v = static_cast<const unsigned char*>(p.v_pers);
-        const int j = at.t * kTile + r;
-        seen = j < p.np;
-        if (seen) row = ((long long)head * p.np + j) * p.map.head_dim;
-    } else {
-        const int j = (at.lo / kTile + at.t - pers) * kTile + r;
-        seen = j >= at.lo && j <= at.pos;
-        if (seen) {
-            row = p.map.token(at.b, j);
-            if (row >= 0) row += head * p.map.head_step();
+// Brings a warp's tiles into its ring, one after the other.  Rows that do not count become zeros: whatever stands in a page behind
+// a sequence's end, infinities and NaN among them, reaches no product.  A lane looks its row's page up a tile ahead of the copies
+// that need it.  Where pages are made of sixteens, so are the tiles' runs of memory; else every row is found by itself.
+template <typename T, int KT, typename Layout>
+struct Loader {
+    const PagedAttention& p;
+    const Ring& ring;
+    const Layout& lay;
+    Cursor<KT> at;
+    int j0, first, last;  // of the tile: its first key; rows first .. last are seen
+    int slot, page;       // of this lane's row
+
+    __device__ __forceinline__ bool persistent() const { return at.tile() < p.pers_tiles; }
+    __device__ __forceinline__ int row_of_lane() const { return threadIdx.x & (KT - 1) & 31; }
+    __device__ __forceinline__ void look() {
+        const bool pers = persistent();
+        const int r = row_of_lane();
+        j0 = (pers ? at.tile() : at.lo / KT + at.tile() - p.pers_tiles) * KT;
+        first = pers ? 0 : max(at.lo - j0, 0);
+        last = min(pers ? p.np - 1 - j0 : at.pos - j0, KT - 1);
+        if (!pers && r >= first && r <= last) {
+            const uint32_t column = p.map.page.div((uint32_t)(j0 + r));
+            slot = j0 + r - (int)(column * p.map.page.d);
+            page = __ldg(p.map.table + at.b * p.map.table_stride + column);
         }
     }
-    const uint32_t bits = __ballot_sync(0xffffffffu, lane < kTile ? seen : row < 0 && seen);
-    if (lane == 0) ring.marks[stage] = bits;
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring.tiles) + stage * 2 * kTile * lay.pitch();
-    const int chunks = lay.chunks(), n = kTile * chunks;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = min(i0 + lane, n - 1), rr = i / chunks, c = i - rr * chunks;
-        const long long at_row = __shfl_sync(0xffffffffu, row, rr);
-        if (i0 + lane >= n) continue;
-        const bool there = at_row >= 0;
-        const long long off = at_row * (long long)sizeof(T) + c * 16;
-        const uint32_t dst = to + lay.offset(rr, c);
-        copy16(dst, there ? static_cast<const void*>(k + off) : p.sums, there);  // (no byte is read where there is none)
-        copy16(dst + kTile * lay.pitch(), there ? static_cast<const void*>(v + off) : p.sums, there);
+    __device__ __forceinline__ void issue(int stage) {
+        const int lane = threadIdx.x & 31, r = row_of_lane();
+        const bool pers = persistent(), mine = r >= first && r <= last;
+        const unsigned char *k, *v;
+        long long row = -1;  // where this lane's row is, in elements
+        if (pers) {
+            k = static_cast<const unsigned char*>(p.k_pers);
+            v = static_cast<const unsigned char*>(p.v_pers);
+            if (mine) row = ((long long)at.head * p.np + j0 + r) * p.map.head_dim;
+        } else {
+            k = static_cast<const unsigned char*>(p.k_pages);
+            v = static_cast<const unsigned char*>(p.v_pages);
+            if (mine && (uint32_t)page < (uint32_t)p.map.pages)
+                row = (((long long)page * p.map.kv_heads + at.head) * p.map.page.d + slot) * p.map.head_dim;
+        }
+        const uint32_t seen = (2u << last) - (1u << first), lost = __ballot_sync(0xffffffffu, mine && row < 0) & (0xffffffffu >> (32 - KT));
+        if (lane == 0) ring.marks[stage] = make_uint2(seen, lost);
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring.tiles) + stage * 2 * KT * lay.pitch();
+        const int chunks = lay.chunks();
+        if (pers || p.whole_runs) {
+#pragma unroll
+            for (int h = 0; h < KT / 16; ++h) {
+                const int from = min(max(first, h * 16), KT - 1);  // a row that has the run's page, if any has
+                const long long off = (__shfl_sync(0xffffffffu, row, from) - (from - h * 16) * p.map.head_dim) * (long long)sizeof(T) + lane * 16;
+                const unsigned char *kr = k + off, *vr = v + off;
+                const int n = 16 * chunks;
+                const uint32_t want = seen >> (h * 16) & 0xffffu & ~(lost >> (h * 16));
+                if (want == 0xffffu) {
+#pragma unroll
+                    for (int i0 = 0; i0 < n; i0 += 32) {
+                        const int i = i0 + lane, rr = i / chunks;
+                        if (n % 32 != 0 && i >= n) break;
+                        const uint32_t dst = to + lay.offset(h * 16 + rr, i - rr * chunks);
+                        copy16(dst, kr + i0 * 16, true);
+                        copy16(dst + KT * lay.pitch(), vr + i0 * 16, true);
+                    }
+                } else {
+                    for (int i0 = 0; i0 < n; i0 += 32) {
+                        const int i = i0 + lane, rr = i / chunks;
+                        if (n % 32 != 0 && i >= n) break;
+                        const uint32_t dst = to + lay.offset(h * 16 + rr, i - rr * chunks);
+                        const bool there = want >> rr & 1;  // (no byte is read where not: any address will do)
+                        copy16(dst, there ? static_cast<const void*>(kr + i0 * 16) : p.sums, there);
+                        copy16(dst + KT * lay.pitch(), there ? static_cast<const void*>(vr + i0 * 16) : p.sums, there);
+                    }
+                }
+            }
+        } else {
+            const int n = KT * chunks;
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int i = min(i0 + lane, n - 1), rr = i / chunks, c = i - rr * chunks;
+                const long long at_row = __shfl_sync(0xffffffffu, row, rr);
+                if (i0 + lane >= n) continue;
+                const bool there = at_row >= 0;
+                const long long off = at_row * (long long)sizeof(T) + c * 16;
+                const uint32_t dst = to + lay.offset(rr, c);
+                copy16(dst, there ? static_cast<const void*>(k + off) : p.sums, there);
+                copy16(dst + KT * lay.pitch(), there ? static_cast<const void*>(v + off) : p.sums, there);
+            }
+        }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-}
+};
 
 // ---- the core on CUDA cores: every type, head_dim a multiple of 8 --------------------------------------------------------
 // Lane l has key l % 16 of a tile and one half of the head's dimensions of its scores; then the four dimensions from 4 l on (and
@@ -237,35 +291,40 @@ constexpr int kSimtRows = 4;
 
 template <typename T>
 struct SimtCore {
-    static constexpr int kRows = kSimtRows;
+    static constexpr int kRows = kSimtRows, KT = 16;
     using Layout = SimtLayout<T>;
     const PagedAttention& p;
     float* q;        // [kRows][head_dim], of the CTA's warp
-    float* weights;  // [kTile][kRows]
+    float* weights;  // [KT][kRows]
     float m[kRows], l[kRows];
     float4 o[kRows][2];
 
     // shared memory of a warp besides its ring
-    static __host__ __device__ int extra(int head_dim) { return (kRows * head_dim + kTile * kRows) * (int)sizeof(float); }
+    static __host__ __device__ int extra(int head_dim) { return (kRows * head_dim + KT * kRows) * (int)sizeof(float); }
 
     __device__ SimtCore(const PagedAttention& p, unsigned char* mine) : p(p), q(reinterpret_cast<float*>(mine)) {
         weights = q + kRows * p.map.head_dim;
     }
-    __device__ __forceinline__ void begin(int b, int first, int rows) {
+    __device__ __forceinline__ void load_queries(int b, int first, int rows) {
         const int lane = threadIdx.x & 31, dim = p.map.head_dim;
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const T* from = static_cast<const T*>(p.q) + b * p.qs[0] + (first + r) * p.qs[1];
             for (int i = lane; i < dim; i += 32) q[r * dim + i] = r < rows ? to_f32<T>(from[i]) : 0.f;
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
             m[r] = -CUDART_INF_F;
             l[r] = 0.f;
             o[r][0] = o[r][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        __syncwarp();
     }
-    __device__ __forceinline__ void tile(const unsigned char* tile, uint32_t marks, const Layout& lay) {
-        const int lane = threadIdx.x & 31, key = lane & (kTile - 1), dim = p.map.head_dim, half = dim / 2;
+    __device__ __forceinline__ void tile(const unsigned char* tile, uint2 marks, const Layout& lay) {
+        const int lane = threadIdx.x & 31, key = lane & (KT - 1), dim = p.map.head_dim, half = dim / 2;
         const unsigned char* row = tile + key * lay.pitch();
         float s[kRows] = {};
         for (int i = (lane >> 4) * half; i < (lane >> 4) * half + half; i += 4) {
@@ -276,7 +335,7 @@ struct SimtCore {
                 s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
             }
         }
-        const bool seen = marks >> key & 1, bad = marks >> (16 + key) & 1;
+        const bool seen = marks.x >> key & 1, bad = marks.y >> key & 1;
         float w[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
@@ -295,15 +354,15 @@ struct SimtCore {
                 o[r][h].x *= keep; o[r][h].y *= keep; o[r][h].z *= keep; o[r][h].w *= keep;
             }
         }
-        if (lane < kTile) *reinterpret_cast<float4*>(weights + key * kRows) = make_float4(w[0], w[1], w[2], w[3]);
+        if (lane < KT) *reinterpret_cast<float4*>(weights + key * kRows) = make_float4(w[0], w[1], w[2], w[3]);
         __syncwarp();
-        const unsigned char* values = tile + kTile * lay.pitch();
+        const unsigned char* values = tile + KT * lay.pitch();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int i = h * 128 + lane * 4;
             if (i >= dim) break;
 #pragma unroll 4
-            for (int j = 0; j < kTile; ++j) {
+            for (int j = 0; j < KT; ++j) {
                 const float4 v4 = load4<T>(values + j * lay.pitch() + i * sizeof(T));
                 const float4 w4 = *reinterpret_cast<const float4*>(weights + j * kRows);
                 add_product(o[0][h], w4.x, v4);
@@ -314,8 +373,9 @@ struct SimtCore {
         }
         __syncwarp();
     }
-    // this warp's part of the item: sums [rows], outputs [rows][head_dim]
-    __device__ __forceinline__ void leave(float2* sums, float* out, int rows) {
+    // use(row, its maximum, its sum, first dimension, up to four numbers of the output), from every lane that has some
+    template <typename F>
+    __device__ __forceinline__ void results(int rows, F&& use) {
         const int lane = threadIdx.x & 31, dim = p.map.head_dim;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
@@ -323,18 +383,19 @@ struct SimtCore {
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
             if (r >= rows) continue;
-            if (lane == 0) sums[r] = make_float2(m[r], t);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (h * 128 + lane * 4 < dim) *reinterpret_cast<float4*>(out + r * dim + h * 128 + lane * 4) = o[r][h];
+            for (int h = 0; h < 2; ++h) {
+                const float x[4] = {o[r][h].x, o[r][h].y, o[r][h].z, o[r][h].w};
+                if (h * 128 + lane * 4 < dim) use(r, m[r], t, h * 128 + lane * 4, x);
+            }
         }
     }
 };
 
 // ---- the core on tensor cores: 16-bit types, head_dim 32, 64, 96, 128 or 256 -------------------------------------------------
-// mma.sync with the query heads as the sixteen rows of a tile (tcgen05's 64 or 128 would multiply a group of at most sixteen
-// for nothing, and the step is bound by HBM long before): scores 16 x 16 keys, their exponentials straight from the accumulators
-// to the operand of the second product.  The weights go in as two 16-bit numbers each, a value and what it lacks: one alone would
+// mma.sync with the keys, then the dimensions of the values, as the sixteen rows of a tile and eight query heads as its columns
+// (tcgen05's 64 or 128 rows would wait for as many keys per step, and the step is bound by HBM long before the tensor cores): the
+// scores are K Q^T, their exponentials, turned over eight by eight (movmatrix), are the operand of V^T W^T.  The weights go in as two 16-bit numbers each, a value and what it lacks: one alone would
 // put up to 2^-9 of itself on the output, the two 2^-16.  (The first is cut off and the second is never zero: both positive,
 // they take an infinite value to infinity, as the weight itself would.)  In fp16 they are raised by 2^12, as far as the largest allows, so
 // that those below 2^-14 of it keep their bits.  Up to eight heads: the tile's upper eight rows are zeros and have no registers.
@@ -410,24 +471,31 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-template <typename T, int DH, bool WIDE>
+// an 8 x 8 matrix of 16-bit numbers, two of a row to a lane, with rows and columns exchanged
+__device__ __forceinline__ uint32_t turned(uint32_t w) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
+}
+
+// EIGHTS: of query heads; lane l has heads l % 4 * 2 and the next one of each eight
+template <typename T, int DH, int EIGHTS>
 struct MmaCore {
-    static constexpr int kRows = kMaxRows;
-    static constexpr int kHalves = WIDE ? 2 : 1;  // of the sixteen rows
+    static constexpr int kRows = kMaxRows, KT = DH > 128 ? 16 : 32;
     static constexpr float kRaise = std::is_same<T, __half>::value ? 12.f : 0.f;
     using Layout = MmaLayout<DH>;
     const PagedAttention& p;
-    uint32_t q[DH / 16][2 * kHalves];  // a0, a2 (, a1, a3)
-    float m[kHalves], l[kHalves];      // of rows lane / 4 and 8 + lane / 4; l: this lane's columns
-    float o[DH / 8][2 * kHalves];
+    uint32_t q[EIGHTS][DH / 16][2];
+    float m[EIGHTS][2], l[EIGHTS][2];  // l: of this lane's keys
+    float o[EIGHTS][DH / 16][4];       // dimension 16 k + lane / 4 of both heads, 16 k + 8 + lane / 4 of both
 
     static __host__ __device__ int extra(int) { return 0; }
 
     __device__ MmaCore(const PagedAttention& p, unsigned char*) : p(p) {}
-    __device__ __forceinline__ void begin(int b, int first, int rows) {
+    __device__ __forceinline__ void load_queries(int b, int first, int rows) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
+        for (int h = 0; h < EIGHTS; ++h) {
             const int r = h * 8 + lane / 4;
             const T* from = static_cast<const T*>(p.q) + b * p.qs[0] + (first + r) * p.qs[1] + lane % 4 * 2;
 #pragma unroll
@@ -440,98 +508,126 @@ struct MmaCore {
                         if (p.q_pairs) w = *reinterpret_cast<const uint32_t*>(at);
                         else w = *reinterpret_cast<const uint16_t*>(at) | (uint32_t)*reinterpret_cast<const uint16_t*>(at + 1) << 16;
                     }
-                    q[k][h * 2 + i] = w;
+                    q[h][k][i] = w;
                 }
-            m[h] = -CUDART_INF_F;
-            l[h] = 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < DH / 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 2 * kHalves; ++i) o[j][i] = 0.f;
     }
-    // c += a b, a the rows' two halves (the upper one zero where there is none)
-    __device__ __forceinline__ static void product(float* c, const uint32_t (&a)[2 * kHalves], uint32_t b0, uint32_t b1) {
-        float d[4] = {c[0], c[1], WIDE ? c[2] : 0.f, WIDE ? c[3] : 0.f};
-        mma_16816<T>(d, a[0], WIDE ? a[2] : 0u, a[1], WIDE ? a[3] : 0u, b0, b1);
-        c[0] = d[0];
-        c[1] = d[1];
-        if (WIDE) c[2] = d[2], c[3] = d[3];
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int h = 0; h < EIGHTS; ++h) {
+            m[h][0] = m[h][1] = -CUDART_INF_F;
+            l[h][0] = l[h][1] = 0.f;
+#pragma unroll
+            for (int k = 0; k < DH / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[h][k][i] = 0.f;
+        }
     }
-    __device__ __forceinline__ void tile(const unsigned char* tile, uint32_t marks, const Layout& lay) {
+    __device__ __forceinline__ void tile(const unsigned char* tile, uint2 marks, const Layout& lay) {
         const int lane = threadIdx.x & 31;
-        const uint32_t keys = (uint32_t)__cvta_generic_to_shared(tile), values = keys + kTile * Layout::pitch();
-        float s[2][2 * kHalves] = {};  // eight keys each
+        const uint32_t keys = (uint32_t)__cvta_generic_to_shared(tile), values = keys + KT * Layout::pitch();
+        float s[EIGHTS][KT / 16][4];  // of each sixteen: keys lane / 4 and 8 + lane / 4, both heads each
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k) {
-            uint32_t b[4];
-            ldmatrix4(b, keys + lay.offset((lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)));
-            product(s[0], q[k], b[0], b[1]);
-            product(s[1], q[k], b[2], b[3]);
-        }
-        uint32_t hi[2 * kHalves], lo[2 * kHalves];  // a0, a2 (, a1, a3) of the weights
-        float keep[kHalves];
+        for (int h = 0; h < EIGHTS; ++h)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            float top = -CUDART_INF_F;
+            for (int g = 0; g < KT / 16; ++g)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int i = 0; i < 4; ++i) s[h][g][i] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int key = j * 8 + lane % 4 * 2 + e;
-                    float& x = s[j][h * 2 + e];
-                    x = marks >> (16 + key) & 1 ? CUDART_NAN_F : marks >> key & 1 ? x * p.scale : -CUDART_INF_F;
-                    top = fmaxf(top, x);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float now = fmaxf(m[h], top), base = now == -CUDART_INF_F ? 0.f : now;
-            keep[h] = m[h] == -CUDART_INF_F ? 1.f : ex2_ftz(m[h] - base);  // (nothing to keep, or NaN)
-            m[h] = now;
-            l[h] *= keep[h];
+        for (int k = 0; k < DH / 16; ++k)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float w[2];
+            for (int g = 0; g < KT / 16; ++g) {
+                uint32_t a[4];
+                ldmatrix4(a, keys + lay.offset(g * 16 + (lane & 15), k * 2 + (lane >> 4)));
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    w[e] = ex2_ftz(s[j][h * 2 + e] - base + kRaise);
-                    l[h] += w[e];
-                }
-                hi[h * 2 + j] = cut2<T>(w[0], w[1]);
-                const float2 there = unpack2<T>(hi[h * 2 + j]);
-                lo[h * 2 + j] = positive2<T>(pack2<T>(w[0] - there.x, w[1] - there.y));
+                for (int h = 0; h < EIGHTS; ++h) mma_16816<T>(s[h][g], a[0], a[1], a[2], a[3], q[h][k][0], q[h][k][1]);
             }
-        }
-        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[kHalves - 1] != 1.f)) {
+        uint32_t hi[EIGHTS][KT / 16][2], lo[EIGHTS][KT / 16][2];
+        float keep[EIGHTS][2];
+        bool moved = false;
 #pragma unroll
-            for (int j = 0; j < DH / 8; ++j)
+        for (int h = 0; h < EIGHTS; ++h) {
+            float base[2];
 #pragma unroll
-                for (int i = 0; i < 2 * kHalves; ++i) o[j][i] *= keep[i / 2];
+            for (int e = 0; e < 2; ++e) {
+                float top = -CUDART_INF_F;
+#pragma unroll
+                for (int g = 0; g < KT / 16; ++g)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = g * 16 + i * 8 + lane / 4;
+                        float& x = s[h][g][i * 2 + e];
+                        x *= p.scale;
+                        if (marks.x != 0xffffffffu >> (32 - KT) || marks.y != 0)
+                            x = marks.y >> key & 1 ? CUDART_NAN_F : marks.x >> key & 1 ? x : -CUDART_INF_F;
+                        top = fmaxf(top, x);
+                    }
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float now = fmaxf(m[h][e], top);
+                base[e] = now == -CUDART_INF_F ? 0.f : now;
+                keep[h][e] = m[h][e] == -CUDART_INF_F ? 1.f : ex2_ftz(m[h][e] - base[e]);  // (nothing to keep, or NaN)
+                moved |= keep[h][e] != 1.f;
+                m[h][e] = now;
+                l[h][e] *= keep[h][e];
+            }
+#pragma unroll
+            for (int g = 0; g < KT / 16; ++g)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        w[e] = ex2_ftz(s[h][g][i * 2 + e] - base[e] + kRaise);
+                        l[h][e] += w[e];
+                    }
+                    const uint32_t cut = cut2<T>(w[0], w[1]);
+                    const float2 there = unpack2<T>(cut);
+                    hi[h][g][i] = turned(cut);
+                    lo[h][g][i] = turned(positive2<T>(pack2<T>(w[0] - there.x, w[1] - there.y)));
+                }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int h = 0; h < EIGHTS; ++h)
+#pragma unroll
+                for (int k = 0; k < DH / 16; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[h][k][i] *= keep[h][i & 1];
         }
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k) {
-            uint32_t b[4];
-            ldmatrix4_trans(b, values + lay.offset((lane >> 3 & 1) * 8 + (lane & 7), k * 2 + (lane >> 4)));
-            product(o[2 * k], hi, b[0], b[1]);
-            product(o[2 * k + 1], hi, b[2], b[3]);
-            product(o[2 * k], lo, b[0], b[1]);
-            product(o[2 * k + 1], lo, b[2], b[3]);
-        }
+        for (int k = 0; k < DH / 16; ++k)
+#pragma unroll
+            for (int g = 0; g < KT / 16; ++g) {
+                uint32_t a[4];
+                ldmatrix4_trans(a, values + lay.offset(g * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)));
+#pragma unroll
+                for (int h = 0; h < EIGHTS; ++h) {
+                    mma_16816<T>(o[h][k], a[0], a[1], a[2], a[3], hi[h][g][0], hi[h][g][1]);
+                    mma_16816<T>(o[h][k], a[0], a[1], a[2], a[3], lo[h][g][0], lo[h][g][1]);
+                }
+            }
     }
-    __device__ __forceinline__ void leave(float2* sums, float* out, int rows) {
+    template <typename F>
+    __device__ __forceinline__ void results(int rows, F&& use) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            const int r = h * 8 + lane / 4;
-            float t = l[h];
-            t += __shfl_xor_sync(0xffffffffu, t, 1);
-            t += __shfl_xor_sync(0xffffffffu, t, 2);
-            if (r >= rows) continue;
-            if (lane % 4 == 0) sums[r] = make_float2(m[h], t);
+        for (int h = 0; h < EIGHTS; ++h)
 #pragma unroll
-            for (int j = 0; j < DH / 8; ++j)
-                *reinterpret_cast<float2*>(out + r * DH + j * 8 + lane % 4 * 2) = make_float2(o[j][h * 2], o[j][h * 2 + 1]);
-        }
+            for (int e = 0; e < 2; ++e) {
+                const int r = h * 8 + lane % 4 * 2 + e;
+                float t = l[h][e];
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) t += __shfl_xor_sync(0xffffffffu, t, d);
+                if (r >= rows) continue;
+#pragma unroll
+                for (int k = 0; k < DH / 16; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float x[1] = {o[h][k][i * 2 + e]};
+                        use(r, m[h][e], t, k * 16 + i * 8 + lane / 4, x);
+                    }
+            }
     }
 };
 
@@ -544,101 +640,173 @@ __device__ __forceinline__ float part_weight(float m, float base) { return m == 
 // (the largest score's weight is 1 or more: no sum at all is that of scores of -inf)
 __device__ __forceinline__ float quotient(float o, float l) { return l == 0.f ? CUDART_NAN_F : o / l; }
 
-template <typename T, typename Core, int W, int S>
+// A warp's part of an item that was cut: of the one that its piece begins in (0), of the one that begins in it (1).
+struct Part {
+    int there, b, item, starts, ends;
+    long long item_end;
+};
+
+template <typename T, typename Core, int W, int S>  // up to W warps
 __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_constant__ PagedAttention p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ uint32_t marks[W][S];
-    __shared__ float2 warp_sums[W][kMaxRows];
+    constexpr int KT = Core::KT;
+    __shared__ uint2 marks[W][S];
+    __shared__ Part parts[2 * W];
     pdl_trigger();
-    const int tid = threadIdx.x, warp = tid >> 5, dim = p.map.head_dim;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x / 32, dim = p.map.head_dim;
     const typename Core::Layout lay{p.row_bytes};
-    const int ring_bytes = S * 2 * kTile * lay.pitch(), extra = Core::extra(dim);
+    const int ring_bytes = S * 2 * KT * lay.pitch(), extra = Core::extra(dim);
     unsigned char* mine = smem + warp * (ring_bytes + extra);
     const Ring ring{mine, marks[warp]};
-    float* outs = reinterpret_cast<float*>(smem + W * (ring_bytes + extra));  // [warp][rows][head_dim]
+    float2* part_sums = reinterpret_cast<float2*>(smem + warps * (ring_bytes + extra));  // [2 * warps][rows]
+    // a warp's first part [rows][head_dim] goes through memory; its second one, made when all its tiles are done, where they were
+    auto part_out = [&](int w, int which) {
+        return which == 0 ? p.firsts + (blockIdx.x * warps + w) * (long long)p.rows * dim
+                          : reinterpret_cast<float*>(smem + w * (ring_bytes + extra));
+    };
 
     // sequences without a key to see, or without a place
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
         int lo, pos;
         bool bad;
-        if (tiles_of(p, b, lo, pos, bad) > 0) continue;
+        if (tiles_of<KT>(p, b, lo, pos, bad) > 0) continue;
         if (bad && tid == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
         const int heads = p.group * p.map.kv_heads;
-        for (int i = tid; i < heads * dim; i += W * 32)
+        for (int i = tid; i < heads * dim; i += blockDim.x)
             static_cast<T*>(p.o)[b * p.os[0] + (i / dim) * p.os[1] + i % dim] = from_f32<T>(bad ? CUDART_NAN_F : 0.f);
     }
     if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    Cursor at;
-    const Share share = find_share<W>(p, at);
-    if (share.first >= share.end) return;
+    if (lane < 2) parts[2 * warp + lane].there = 0;
+    __syncwarp();
 
-    Cursor ahead = at;  // the tile to load next
-    long long load = share.first + warp;
-    if (load < share.end) ahead.advance(p, warp);
-    int stage_in = 0, stage_out = 0;
-    auto fetch = [&]() {
-        if (load < share.end) {
-            load_tile<T>(p, ring, lay, ahead, stage_in);
-            load += W;
-            if (load < share.end) ahead.advance(p, W);
-        } else {
+    Cursor<KT> at;
+    const Share share = find_share<KT>(p, at);
+    if (share.first < share.end) {
+        Loader<T, KT, typename Core::Layout> ahead{p, ring, lay, at};  // of the tile to load next, unit `load` of the line
+        long long load = share.first;
+        int stage_in = 0, stage_out = 0;
+        auto look = [&]() {
+            if (load < share.end && ahead.at.t < kItemCost) {
+                load += kItemCost - ahead.at.t;
+                ahead.at.t = kItemCost;
+            }
+            if (load < share.end) ahead.look();
+        };
+        auto fetch = [&]() {
+            if (load < share.end) {
+                ahead.issue(stage_in);
+                if (++load < share.end && ++ahead.at.t == ahead.at.n) ahead.at.next_item(p);
+                look();
+            }
             asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        stage_in = stage_in + 1 == S ? 0 : stage_in + 1;
-    };
+            stage_in = stage_in + 1 == S ? 0 : stage_in + 1;
+        };
+        look();
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) fetch();
+        for (int s = 0; s < S - 1; ++s) fetch();
 
-    Core core(p, mine + ring_bytes);
-    long long u = share.first + warp, begin = share.first;
-    bool bad_page = false;
-    while (begin < share.end) {
-        const long long item_end = begin + (at.n - at.t), end = item_end < share.end ? item_end : share.end;
-        const int first = at.item % p.parts * p.rows, rows = min(p.rows, p.group - first);
-        const int head = at.item / p.parts * p.group + first;
-        core.begin(at.b, head, rows);
-        for (; u < end; u += W) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-            __syncwarp();
-            fetch();
-            const uint32_t mark = ring.marks[stage_out];
-            bad_page |= mark >> 16 != 0;
-            core.tile(ring.tiles + stage_out * 2 * kTile * lay.pitch(), mark, lay);
-            stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
-        }
-        // (a warp without a tile leaves a maximum of -inf and zeros)
-        core.leave(warp_sums[warp], outs + warp * p.rows * dim, rows);
-        __syncthreads();
-        const bool whole = at.t == 0 && end == item_end;
-        const int part = begin == share.first ? 0 : 1;
-        const long long slot = (long long)blockIdx.x * 2 + part;
-        for (int i = tid; i < rows * dim; i += W * 32) {
-            const int r = i / dim;
-            float m = warp_sums[0][r].x;
-#pragma unroll
-            for (int w = 1; w < W; ++w) m = fmaxf(m, warp_sums[w][r].x);
-            const float base = m == -CUDART_INF_F ? 0.f : m;
-            float l = 0.f, o = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float x = part_weight(warp_sums[w][r].x, base);
-                l = fmaf(x, warp_sums[w][r].y, l);
-                o = fmaf(x, outs[w * p.rows * dim + i], o);
+        Core core(p, mine + ring_bytes);
+        auto queries = [&](const Cursor<KT>& c, int& head, int& rows) {  // the item's first head, and how many
+            const int first = (c.item - c.head * p.parts) * p.rows;
+            rows = min(p.rows, p.group - first);
+            head = c.head * p.group + first;
+            core.load_queries(c.b, head, rows);
+        };
+        long long begin = share.first;
+        bool bad_page = false;
+        int head, rows;
+        queries(at, head, rows);
+        while (begin < share.end) {
+            const long long item_end = begin + (at.n - at.t), end = item_end < share.end ? item_end : share.end;
+            const int tiles = (int)(end - begin) - max(kItemCost - at.t, 0);
+            core.reset();
+            for (int i = 0; i < tiles; ++i) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+                __syncwarp();
+                fetch();
+                const uint2 mark = ring.marks[stage_out];
+                bad_page |= mark.y != 0;
+                core.tile(ring.tiles + stage_out * 2 * KT * lay.pitch(), mark, lay);
+                stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
             }
-            if (whole) {
-                static_cast<T*>(p.o)[at.b * p.os[0] + (head + r) * p.os[1] + (i - r * dim)] = from_f32<T>(quotient(o, l));
+            const Cursor<KT> done = at;
+            const int done_head = head, done_rows = rows;
+            if (item_end < share.end) {  // the next item's queries load while this one's results are stored
+                at.next_item(p);
+                queries(at, head, rows);
+            }
+            begin = end;
+            if (tiles <= 0) continue;
+            const bool starts = done.t <= kItemCost, ends = end == item_end;
+            if (starts && ends) {
+                T* to = static_cast<T*>(p.o) + done.b * p.os[0] + done_head * p.os[1];
+                core.results(done_rows, [&](int r, float, float sum, int d, const auto& x) {
+                    constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) to[r * p.os[1] + d + e] = from_f32<T>(quotient(x[e], sum));
+                });
             } else {
-                p.partial[slot * p.rows * dim + i] = o;
-                if (i == r * dim) p.sums[slot * p.rows + r] = make_float2(m, l);
+                const int which = starts ? 1 : 0;
+                __syncwarp();
+                float* to = part_out(warp, which);
+                float2* sums = part_sums + (2 * warp + which) * p.rows;
+                core.results(done_rows, [&](int r, float top, float sum, int d, const auto& x) {
+                    constexpr int N = sizeof(x) / sizeof(float);
+                    if (d == 0) sums[r] = make_float2(top, sum);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) to[r * dim + d + e] = x[e];
+                });
+                if (lane == 0) parts[2 * warp + which] = {1, done.b, done.item, starts, ends, item_end};
             }
         }
-        if (at.t == 0 && end < item_end && tid == 0)  // begins here, ends in another CTA
-            p.joins[blockIdx.x] = make_int4(at.b, at.item, (int)((item_end - 1) / share.per), part);
-        __syncthreads();
-        if (item_end < share.end) at.advance(p, at.n - at.t);
-        begin = end;
+        if (bad_page && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
     }
-    if (__any_sync(0xffffffffu, bad_page) && (tid & 31) == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+    __syncthreads();
+
+    // The CTA's parts of one item are neighbours: one that begins here, or that the CTA begins in, and those that go on with it.
+    // Each item's numbers, four to a thread, begin with the thread behind the last one's.
+    const uint32_t there = __ballot_sync(0xffffffffu, lane < 2 * warps && parts[lane].there);
+    int turn = 0;
+    for (uint32_t todo = there & (0xaaaaaaaau | 1u); todo != 0; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1;
+        const uint32_t rest = todo & (todo - 1), members = there & ~((1u << i) - 1) & (rest != 0 ? (rest & (0u - rest)) - 1 : 0xffffffffu);
+        const Part part = parts[i];
+        const bool starts = part.starts, ends = parts[31 - __clz(members)].ends;
+        const int first = part.item % p.parts * p.rows, rows = min(p.rows, p.group - first);
+        const int head = part.item / p.parts * p.group + first;
+        const long long slot = (blockIdx.x * 2 + (starts ? 1 : 0)) * (long long)p.rows;
+        const int units = rows * dim / 4;
+        int x = tid - turn;
+        if (x < 0) x += blockDim.x;
+        for (; x < units; x += blockDim.x) {
+            const int r = x * 4 / dim;
+            float m = -CUDART_INF_F, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t j = members; j != 0; j &= j - 1) m = fmaxf(m, part_sums[(__ffs(j) - 1) * p.rows + r].x);
+            const float base = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll 4
+            for (uint32_t j = members; j != 0; j &= j - 1) {
+                const int at = __ffs(j) - 1;
+                const float2 sum = part_sums[at * p.rows + r];
+                const float w = part_weight(sum.x, base);
+                l = fmaf(w, sum.y, l);
+                add_product(o, w, reinterpret_cast<const float4*>(part_out(at >> 1, at & 1))[x]);
+            }
+            if (starts && ends) {
+                T* to = static_cast<T*>(p.o) + part.b * p.os[0] + (head + r) * p.os[1] + (x * 4 - r * dim);
+                to[0] = from_f32<T>(quotient(o.x, l));
+                to[1] = from_f32<T>(quotient(o.y, l));
+                to[2] = from_f32<T>(quotient(o.z, l));
+                to[3] = from_f32<T>(quotient(o.w, l));
+            } else {
+                reinterpret_cast<float4*>(p.partial + slot * dim)[x] = o;
+                if (x * 4 == r * dim) p.sums[slot + r] = make_float2(m, l);
+            }
+        }
+        turn = (turn + units) % blockDim.x;
+        if (starts && !ends && tid == 0)
+            p.joins[blockIdx.x] = make_int4(part.b, part.item, (int)((part.item_end - 1) / (share.per * share.warps)), 0);
+    }
 }
 
 // The parts of an item that was cut: CTA (c, r) joins row r of the one that begins in CTA c.  Its warps take every
@@ -655,7 +823,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     const int first = join.y % p.parts * p.rows;
     if (r >= min(p.rows, p.group - first)) return;
     const int n = join.z - (int)blockIdx.x + 1;
-    auto slot = [&](int i) { return (2LL * (blockIdx.x + i) + (i == 0 ? join.w : 0)) * p.rows + r; };
+    auto slot = [&](int i) { return (2LL * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * p.rows + r; };
     float m = -CUDART_INF_F;
     for (int i = tid; i < n; i += kJoinWarps * 32) m = fmaxf(m, __ldcg(p.sums + slot(i)).x);
 #pragma unroll
@@ -695,47 +863,51 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
-constexpr int kMostShared = 226 * 1024;  // of a CTA, beside what the kernel declares
+// Shared memory of a CTA, one to an SM: with more than this, or more than 196 KB in all, what is left of the SM's memory as L1 is
+// too little for the copies on their way, and they come from L2 twice (32 heads on 4, 545,000 tokens: 231 us, with this 189).
+constexpr int kMostShared = 193 * 1024 + 512;
 
 struct Plan {
-    int rows, parts, grid, smem;
-    size_t sums_at, partial_at, bytes;
+    int rows, parts, warps, grid, smem;
+    size_t sums_at, partial_at, firsts_at, bytes;
 };
 
 template <typename T, typename Core, int W, int S>
 struct Kernel {
-    static constexpr int kMostCtas = 4;  // to an SM
+    static constexpr int KT = Core::KT;
     static Plan plan(const tmw_paged_attention_desc& d, int row_bytes) {
         Plan n;
         const int group = d.heads / d.at.kv_heads;
         n.parts = (group + Core::kRows - 1) / Core::kRows;
         n.rows = (group + n.parts - 1) / n.parts;
-        const int pitch = typename Core::Layout{row_bytes}.pitch();
-        n.smem = W * (S * 2 * kTile * pitch + Core::extra(d.at.head_dim) + n.rows * d.at.head_dim * (int)sizeof(float));
-        int ctas = 228 * 1024 / (n.smem + 2048);
-        ctas = ctas < 1 ? 1 : ctas > kMostCtas ? kMostCtas : ctas;
+        const int warp = S * 2 * KT * typename Core::Layout{row_bytes}.pitch() + Core::extra(d.at.head_dim) + 2 * n.rows * (int)sizeof(float2);
+        n.warps = kMostShared / warp < W ? kMostShared / warp : W;
+        n.smem = n.warps * warp;
         // no more CTAs than the longest sequences could have work for
         const long long capacity = (long long)d.at.columns * d.at.page_size;
         const long long keys = d.window >= 0 && d.window + 1LL < capacity ? d.window + 1LL : capacity;
-        const long long tiles = ((d.n_persistent + kTile - 1) / kTile + keys / kTile + 2) * (long long)d.at.kv_heads * n.parts;
-        const long long most = (tiles * d.at.batch + W - 1) / W;
-        n.grid = (int)(most < (long long)ctas * sm_count() ? most : (long long)ctas * sm_count());
+        const long long tiles = ((d.n_persistent + KT - 1) / KT + keys / KT + 2) * (long long)d.at.kv_heads * n.parts * d.at.batch;
+        n.grid = (int)(tiles < sm_count() ? tiles : sm_count());
+        const size_t out = (size_t)n.rows * d.at.head_dim * sizeof(float);
         n.sums_at = (size_t)n.grid * sizeof(int4);
         n.partial_at = (n.sums_at + (size_t)n.grid * 2 * n.rows * sizeof(float2) + 15) & ~(size_t)15;
-        n.bytes = n.partial_at + (size_t)n.grid * 2 * n.rows * d.at.head_dim * sizeof(float);
+        n.firsts_at = n.partial_at + n.grid * 2 * out;
+        n.bytes = n.firsts_at + (size_t)n.grid * n.warps * out;
         return n;
     }
     static int launch(PagedAttention& p, const Plan& n, unsigned char* scratch, cudaStream_t stream) {
         p.rows = n.rows;
         p.parts = n.parts;
         p.items = p.map.kv_heads * n.parts;
+        p.pers_tiles = (p.np + KT - 1) / KT;
         p.joins = reinterpret_cast<int4*>(scratch);
         p.sums = reinterpret_cast<float2*>(scratch + n.sums_at);
         p.partial = reinterpret_cast<float*>(scratch + n.partial_at);
+        p.firsts = reinterpret_cast<float*>(scratch + n.firsts_at);
         auto kern = paged_attention_kernel<T, Core, W, S>;
         const int rc = allow_shared_memory(reinterpret_cast<const void*>(kern), n.smem);
         if (rc != TMW_OK) return rc;
-        kern<<<n.grid, W * 32, n.smem, stream>>>(p);
+        kern<<<n.grid, n.warps * 32, n.smem, stream>>>(p);
         TMW_CUDA_TRY(cudaGetLastError());
         if (n.grid > 1)
             TMW_CUDA_TRY(launch_ex(paged_join_kernel<T>, dim3((unsigned)n.grid - 1, (unsigned)n.rows), dim3(kJoinWarps * 32), 0, stream, true,
@@ -744,18 +916,11 @@ struct Kernel {
     }
 };
 
-// four warps to a CTA, or two where the rings of four would not fit
-template <typename T, typename F>
-int with_simt(const tmw_paged_attention_desc& d, F&& use) {
-    using Four = Kernel<T, SimtCore<T>, 4, 3>;
-    if (Four::plan(d, d.at.head_dim * (int)sizeof(T)).smem <= kMostShared) return use(Four());
-    return use(Kernel<T, SimtCore<T>, 2, 3>());
-}
-
 template <typename T, int DH, typename F>
 int with_mma(const tmw_paged_attention_desc& d, F&& use) {
-    if (d.heads / d.at.kv_heads <= 8) return use(Kernel<T, MmaCore<T, DH, false>, 4, 3>());
-    return use(Kernel<T, MmaCore<T, DH, true>, (DH > 128 ? 2 : 4), 3>());
+    constexpr int W = DH >= 128 ? 6 : DH > 64 ? 8 : 12;
+    if (d.heads / d.at.kv_heads <= 8) return use(Kernel<T, MmaCore<T, DH, 1>, W, 2>());
+    return use(Kernel<T, MmaCore<T, DH, 2>, W, 2>());
 }
 template <typename T, typename F>
 int with_16_bits(const tmw_paged_attention_desc& d, F&& use) {
@@ -765,14 +930,14 @@ int with_16_bits(const tmw_paged_attention_desc& d, F&& use) {
         case 96: return with_mma<T, 96>(d, use);
         case 128: return with_mma<T, 128>(d, use);
         case 256: return with_mma<T, 256>(d, use);
-        default: return with_simt<T>(d, use);
+        default: return use(Kernel<T, SimtCore<T>, 12, 2>());
     }
 }
 
 // `use` with the Kernel that takes the call
 template <typename F>
 int with_kernel(const tmw_paged_attention_desc& d, F&& use) {
-    if (d.at.dtype == TMW_F32) return with_simt<float>(d, use);
+    if (d.at.dtype == TMW_F32) return use(Kernel<float, SimtCore<float>, 12, 2>());
     return d.at.dtype == TMW_BF16 ? with_16_bits<__nv_bfloat16>(d, use) : with_16_bits<__half>(d, use);
 }
 
@@ -831,6 +996,7 @@ extern "C" int tmw_paged_attention(const tmw_paged_attention_desc* d, void* scra
     }
     p.pos = d->pos;
     p.batch = d->at.batch; p.np = d->n_persistent; p.window = d->window;
+    p.whole_runs = d->at.page_size % 16 == 0;
     p.group = d->heads / d->at.kv_heads;
     p.scale = (d->scale > 0.f ? d->scale : 1.0f / sqrtf((float)d->at.head_dim)) * 1.4426950408889634f;
     p.row_bytes = d->at.head_dim * (int)size;
