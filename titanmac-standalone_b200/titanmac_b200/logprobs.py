@@ -32,38 +32,31 @@ class TokenLogprobs(NamedTuple):
 def _rows(t: torch.Tensor):
     """``(tensor with the same values, batch, tokens, strides)`` of ``[.., V]``: rows in two steps, one behind the other inside."""
     shape, strides = t.shape, t.stride()
-    if (strides[-1] != 1 and shape[-1] != 1) or t.dim() > 3:
+    if (strides[-1] != 1 and shape[-1] != 1) or len(shape) > 3:
         t = t.contiguous()
         strides = t.stride()
-    if t.dim() == 3:
-        return t, shape[0], shape[1], strides[:2]
-    if t.dim() == 1:
-        return t, 1, 1, (0, 0)
-    if t.dim() == 2:
-        return t, shape[0], 1, (strides[0], 0)
-    return t, t.numel() // shape[-1], 1, (shape[-1], 0)
-
-
-def _pack(rows, vocab: int, n_top: int, dtype: torch.dtype, targets, logprobs, entropy, lse, top_logprobs, top_ids):
-    t, batch, tokens, strides = rows
-    return _DESC.pack(_native._DTYPES[dtype], batch, tokens, vocab, n_top, 0, t.data_ptr(), *strides, targets.data_ptr(), logprobs,
-                      entropy.data_ptr(), lse.data_ptr() if lse is not None else 0, top_logprobs,
-                      top_ids.data_ptr() if top_ids is not None else 0)
+    if len(shape) == 3:
+        return t, shape[0], shape[1], strides[0], strides[1]
+    if len(shape) == 2:
+        return t, shape[0], 1, strides[0], 0
+    return t, t.numel() // shape[-1], 1, shape[-1], 0
 
 
 def _forward(logits: torch.Tensor, targets: torch.Tensor, n_top: int, with_lse: bool):
     """``(logprobs, entropy, top_ids, top_logprobs, lse)``; without alternatives the ids and their values are None."""
     device, shape = logits.device, targets.shape
-    logprobs, entropy = torch.empty((2, *shape), dtype=torch.float32, device=device)
-    lse = torch.empty((*shape, 2), dtype=torch.float32, device=device) if with_lse else None
+    logprobs = torch.empty_like(targets, dtype=torch.float32)
+    entropy = torch.empty_like(logprobs)
+    lse = torch.empty(*shape, 2, dtype=torch.float32, device=device) if with_lse else None
     top_ids = top_logprobs = None
     if n_top:
-        top_ids = torch.empty((*shape, n_top), dtype=torch.int64, device=device)
-        top_logprobs = torch.empty((*shape, n_top), dtype=torch.float32, device=device)
+        top_ids = torch.empty(*shape, n_top, dtype=torch.int64, device=device)
+        top_logprobs = torch.empty(*shape, n_top, dtype=torch.float32, device=device)
     if targets.numel():
-        rows = _rows(logits)
-        desc = _pack(rows, logits.shape[-1], n_top, logits.dtype, targets, logprobs.data_ptr(), entropy, lse,
-                     top_logprobs.data_ptr() if n_top else 0, top_ids)
+        t, batch, tokens, s0, s1 = _rows(logits)
+        desc = _DESC.pack(_native._DTYPES[t.dtype], batch, tokens, t.shape[-1], n_top, 0, t.data_ptr(), s0, s1, targets.data_ptr(),
+                          logprobs.data_ptr(), entropy.data_ptr(), lse.data_ptr() if with_lse else 0,
+                          top_logprobs.data_ptr() if n_top else 0, top_ids.data_ptr() if n_top else 0)
         with _native._on(device):
             _native.check(_native.lib().tmw_token_logprobs(desc, _native._stream_ptr(device)))
     return logprobs, entropy, top_ids, top_logprobs, lse
@@ -73,7 +66,6 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, targets: torch.Tensor, n_top: int):
         logprobs, entropy, top_ids, top_logprobs, lse = _forward(logits, targets, n_top, True)
-        ctx.n_top = n_top
         ctx.set_materialize_grads(False)
         if n_top:
             ctx.mark_non_differentiable(top_ids)
@@ -85,15 +77,17 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, d_logprobs, d_entropy, _, d_top):
         logits, targets, lse, entropy, top_ids = ctx.saved_tensors
         device = logits.device
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        d_logits = torch.empty(*logits.shape, dtype=logits.dtype, device=device)
         given = [None if g is None else g.contiguous() for g in (d_logprobs, d_entropy, d_top)]
         if targets.numel():
-            rows = _rows(logits)  # (held: it may be a copy)
-            desc = _pack(rows, logits.shape[-1], ctx.n_top, logits.dtype, targets, 0, entropy, lse, 0, top_ids)
+            t, batch, tokens, s0, s1 = _rows(logits)
+            n_top = 0 if top_ids is None else top_ids.shape[-1]
+            desc = _DESC.pack(_native._DTYPES[t.dtype], batch, tokens, t.shape[-1], n_top, 0, t.data_ptr(), s0, s1, targets.data_ptr(),
+                              0, entropy.data_ptr(), lse.data_ptr(), 0, top_ids.data_ptr() if n_top else 0)
             with _native._on(device):
                 _native.check(_native.lib().tmw_token_logprobs_backward(
-                    desc, *(None if g is None else g.data_ptr() for g in given), d_logits.data_ptr(),
-                    _STRIDES.pack(*_rows(d_logits)[3]), _native._stream_ptr(device)))
+                    desc, *[None if g is None else g.data_ptr() for g in given], d_logits.data_ptr(),
+                    _STRIDES.pack(*_rows(d_logits)[3:]), _native._stream_ptr(device)))
         return d_logits, None, None
 
 
@@ -104,18 +98,17 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_top: int = 0) 
     A target of -100 counts as none: its value is 0 and no gradient comes from it.  A target outside the vocabulary has NaN and
     ``_native.poll_status`` raises.  A row without a distribution (a NaN, +inf or nothing but -inf among its logits) has NaN, and
     ids of -1."""
-    _native._require_cuda(logits, targets)
-    if logits.dtype not in _native._DTYPES:
-        raise TypeError("token_logprobs: logits in fp32, bf16 or fp16 expected")
-    if targets.dtype != torch.int64:
-        raise TypeError("token_logprobs: targets must be int64")
-    if logits.dim() < 1 or logits.shape[:-1] != targets.shape or logits.shape[-1] == 0:
-        raise ValueError("token_logprobs: logits [.., vocabulary] and targets [..] must agree in the axes in front")
-    if targets.device != logits.device:
+    if not logits.is_cuda or targets.get_device() != logits.get_device():
+        _native._require_cuda(logits, targets)
         raise ValueError("token_logprobs: logits and targets must be on one device")
-    if not 0 <= n_top <= min(MAX_TOP, logits.shape[-1]):
-        raise ValueError(f"token_logprobs: n_top must be in 0 .. {min(MAX_TOP, logits.shape[-1])}, got {n_top}")
+    if logits.dtype not in _native._DTYPES or targets.dtype is not torch.int64:
+        raise TypeError("token_logprobs: logits in fp32, bf16 or fp16 and targets in int64 expected")
+    shape = logits.shape
+    if not shape or shape[:-1] != targets.shape or shape[-1] == 0:
+        raise ValueError("token_logprobs: logits [.., vocabulary] and targets [..] must agree in the axes in front")
+    if not 0 <= n_top <= min(MAX_TOP, shape[-1]):
+        raise ValueError(f"token_logprobs: n_top must be in 0 .. {min(MAX_TOP, shape[-1])}, got {n_top}")
     targets = targets.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, n_top))
     return TokenLogprobs(*_forward(logits, targets, n_top, False)[:4])

@@ -25,32 +25,26 @@ _APPEND = struct.Struct("@8iq3Q 4i 4Q 12q 3Q")
 _ATTENTION = struct.Struct("@8iq3Q 3if 4Q 4q Q")
 
 
-def _check_pages(k_pages, v_pages, page_table, batch: int, name: str):
+def _refuse_devices(name: str, like: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
+    _native._require_cuda(like, *(t for t in tensors if t is not None))
+    raise ValueError(f"{name}: every tensor must be on {like.device}")
+
+
+def _page_numbers(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, batch: int):
     """``(dtype number, kv_heads, head_dim, page_size, pages, columns)`` of a pool and its table."""
-    dtype = _native._DTYPES.get(k_pages.dtype)
-    if dtype is None or v_pages.dtype != k_pages.dtype:
-        raise TypeError(f"{name}: k_pages and v_pages must share one dtype out of float32, bfloat16, float16")
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+    shape, table = k_pages.shape, page_table.shape
+    if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise ValueError(f"{name}: k_pages and v_pages must be contiguous [pages, kv_heads, page_size, head_dim]")
-    if page_table.dtype != torch.int32:
-        raise TypeError(f"{name}: page_table must be int32")
-    if page_table.dim() != 2 or page_table.shape[0] != batch or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+    if len(table) != 2 or table[0] != batch or (table[1] > 1 and page_table.stride(1) != 1):
         raise ValueError(f"{name}: page_table must be [batch, columns] with contiguous rows")
-    pages, kv_heads, page_size, head_dim = k_pages.shape
-    return dtype, kv_heads, head_dim, page_size, pages, page_table.shape[1]
+    dtype = _native._DTYPES.get(k_pages.dtype)
+    if dtype is None:
+        raise TypeError(f"{name}: pages in float32, bfloat16 or float16 expected")
+    return dtype, shape[1], shape[3], shape[2], shape[0], table[1]
 
 
-def _check_numbers(t: torch.Tensor, batch: int, name: str) -> None:
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be int32")
-    if t.shape != (batch,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous vector of one number per sequence")
-
-
-def _check_heads(t: torch.Tensor, shape, like: torch.Tensor, name: str):
-    """Strides in front of the last axis."""
-    if t.dtype != like.dtype:
-        raise TypeError(f"{name} must have the dtype of the pages")
+def _strides(name: str, t: torch.Tensor, shape):
+    """In front of the last axis, which is contiguous."""
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     strides = t.stride()
@@ -59,12 +53,9 @@ def _check_heads(t: torch.Tensor, shape, like: torch.Tensor, name: str):
     return strides[:-1]
 
 
-def _check_devices(name: str, device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            if not t.is_cuda:
-                raise RuntimeError("libtmw works on CUDA tensors only; there is no CPU path")
-            raise ValueError(f"{name}: every tensor must be on {device}")
+def _check_numbers(name: str, t: torch.Tensor, batch: int) -> None:
+    if t.shape != (batch,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of one number per sequence")
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -79,43 +70,57 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     ``(2 i, 2 i + 1)``.  ``q [B, heads, rows, dh]`` is rotated likewise into ``q_out`` (may be ``q``; made if None), which is
     returned; its rows that are no new token's are left as they are.  Writes of the same slot twice in one call are the caller's
     to avoid."""
-    device = k_pages.device
-    _native._require_cuda(k_pages)
-    _check_devices("paged_append", device, k, v, v_pages, page_table, start, counts, q, q_out, inv_freq)
-    if k.dim() != 4:
+    index = k_pages.get_device()
+    if not 0 <= index == k.get_device() == v.get_device() == v_pages.get_device() == page_table.get_device() == start.get_device():
+        _refuse_devices("paged_append", k_pages, k, v, v_pages, page_table, start)
+    dtype = k_pages.dtype
+    if not (dtype is v_pages.dtype is k.dtype is v.dtype and torch.int32 is page_table.dtype is start.dtype):
+        raise TypeError("paged_append: k, v and the pages must share one dtype; page_table and start must be int32")
+    shape = k.shape
+    if len(shape) != 4:
         raise ValueError("paged_append: k and v must be [batch, kv_heads, rows, head_dim]")
-    B, _, rows, _ = k.shape
-    dtype, kv_heads, head_dim, page_size, pages, columns = _check_pages(k_pages, v_pages, page_table, B, "paged_append")
-    shape = (B, kv_heads, rows, head_dim)
-    ks, vs = _check_heads(k, shape, k_pages, "k"), _check_heads(v, shape, k_pages, "v")
-    _check_numbers(start, B, "start")
+    B, rows = shape[0], shape[2]
+    dtype_number, kv_heads, head_dim, page_size, pages, columns = _page_numbers("paged_append", k_pages, v_pages, page_table, B)
+    ks, vs = _strides("k", k, (B, kv_heads, rows, head_dim)), _strides("v", v, shape)
+    _check_numbers("start", start, B)
     if counts is not None:
-        _check_numbers(counts, B, "counts")
+        if counts.get_device() != index:
+            _refuse_devices("paged_append", k_pages, counts)
+        if counts.dtype is not torch.int32:
+            raise TypeError("counts must be int32")
+        _check_numbers("counts", counts, B)
     rotated = 0
     if inv_freq is not None:
-        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        if inv_freq.get_device() != index:
+            _refuse_devices("paged_append", k_pages, inv_freq)
+        if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
             raise TypeError("inv_freq must be a contiguous fp32 vector")
         rotated = 2 * inv_freq.shape[0]
         if rotated > head_dim:
             raise ValueError("inv_freq has more than head_dim / 2 numbers")
     heads, qs, os_ = 0, (0, 0, 0), (0, 0, 0)
     if q is not None:
+        if q.get_device() != index or (q_out is not None and q_out.get_device() != index):
+            _refuse_devices("paged_append", k_pages, q, q_out)
+        if q.dtype is not dtype or (q_out is not None and q_out.dtype is not dtype):
+            raise TypeError("q and q_out must have the dtype of the pages")
         if q.dim() != 4:
             raise ValueError("q must be [batch, heads, rows, head_dim]")
         heads = q.shape[1]
         q_shape = (B, heads, rows, head_dim)
-        qs = _check_heads(q, q_shape, k_pages, "q")
+        qs = _strides("q", q, q_shape)
         if q_out is None:
-            q_out = torch.empty((B, rows, heads, head_dim), dtype=q.dtype, device=device).permute(0, 2, 1, 3)
-        os_ = _check_heads(q_out, q_shape, k_pages, "q_out")
+            q_out = torch.empty(B, rows, heads, head_dim, dtype=dtype, device=k_pages.device).permute(0, 2, 1, 3)
+        os_ = _strides("q_out", q_out, q_shape)
     elif q_out is not None:
         raise ValueError("q_out goes with q")
     if B == 0 or rows == 0:
         return q_out
-    desc = _APPEND.pack(dtype, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0), k_pages.data_ptr(),
+    desc = _APPEND.pack(dtype_number, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0), k_pages.data_ptr(),
                         v_pages.data_ptr(), page_table.data_ptr(), rows, heads, rotated, interleaved, k.data_ptr(), v.data_ptr(),
                         q.data_ptr() if heads else 0, q_out.data_ptr() if heads else 0, *ks, *vs, *qs, *os_, start.data_ptr(),
                         counts.data_ptr() if counts is not None else 0, inv_freq.data_ptr() if rotated else 0)
+    device = k_pages.device
     with _native._on(device):
         _native.check(_native.lib().tmw_paged_append(desc, _native._stream_ptr(device)))
     return q_out
@@ -128,17 +133,21 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     have been appended: over tokens ``pos - window .. pos`` (None: all up to ``pos``) and the persistent keys
     ``k_pers, v_pers [kv_heads, Np, dh]``.  ``heads`` is a multiple of the pages' ``kv_heads``.  ``pos`` of -1: a sequence without
     tokens; it sees the persistent keys, and is zero without them."""
-    device = k_pages.device
-    _native._require_cuda(k_pages)
-    _check_devices("paged_attention", device, q, v_pages, page_table, pos, k_pers, v_pers, out)
-    if q.dim() != 3:
+    index = k_pages.get_device()
+    if not 0 <= index == q.get_device() == v_pages.get_device() == page_table.get_device() == pos.get_device():
+        _refuse_devices("paged_attention", k_pages, q, v_pages, page_table, pos)
+    dtype = k_pages.dtype
+    if not (dtype is v_pages.dtype is q.dtype and torch.int32 is page_table.dtype is pos.dtype):
+        raise TypeError("paged_attention: q and the pages must share one dtype; page_table and pos must be int32")
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError("paged_attention: q must be [batch, heads, head_dim]")
-    B, heads, _ = q.shape
-    dtype, kv_heads, head_dim, page_size, pages, columns = _check_pages(k_pages, v_pages, page_table, B, "paged_attention")
+    B, heads, _ = shape
+    dtype_number, kv_heads, head_dim, page_size, pages, columns = _page_numbers("paged_attention", k_pages, v_pages, page_table, B)
     if kv_heads == 0 or heads % kv_heads != 0:
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-    qs = _check_heads(q, (B, heads, head_dim), k_pages, "q")
-    _check_numbers(pos, B, "pos")
+    qs = _strides("q", q, (B, heads, head_dim))
+    _check_numbers("pos", pos, B)
     if window is None:
         window = -1
     elif window < 0:
@@ -146,24 +155,33 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif window > 0x7FFFFFFF:
         window = -1  # (no sequence is longer)
     n_persistent = 0
-    if (k_pers is None) != (v_pers is None):
+    if k_pers is not None and v_pers is not None:
+        if not index == k_pers.get_device() == v_pers.get_device():
+            _refuse_devices("paged_attention", k_pages, k_pers, v_pers)
+        if not dtype is k_pers.dtype is v_pers.dtype:
+            raise TypeError("k_pers and v_pers must have the dtype of the pages")
+        pers = k_pers.shape
+        if len(pers) != 3 or pers[0] != kv_heads or pers[2] != head_dim or v_pers.shape != pers or not k_pers.is_contiguous() \
+                or not v_pers.is_contiguous():
+            raise ValueError("k_pers and v_pers must be contiguous [kv_heads, n_persistent, head_dim]")
+        n_persistent = pers[1]
+    elif k_pers is not None or v_pers is not None:
         raise ValueError("k_pers and v_pers go together")
-    if k_pers is not None:
-        n_persistent = k_pers.shape[1] if k_pers.dim() == 3 else -1
-        for t, name in ((k_pers, "k_pers"), (v_pers, "v_pers")):
-            _check_heads(t, (kv_heads, n_persistent, head_dim), k_pages, name)
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
     if out is None:
-        out = torch.empty((B, heads, head_dim), dtype=q.dtype, device=device)
-    os_ = _check_heads(out, (B, heads, head_dim), k_pages, "out")
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(B, heads, head_dim, dtype=dtype, device=q.device)
+    else:
+        if out.get_device() != index:
+            _refuse_devices("paged_attention", k_pages, out)
+        if out.dtype is not dtype:
+            raise TypeError("out must have the dtype of the pages")
+    os_ = _strides("out", out, shape)
     if B == 0 or heads == 0:
         return out
-    desc = _ATTENTION.pack(dtype, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0), k_pages.data_ptr(),
-                           v_pages.data_ptr(), page_table.data_ptr(), heads, n_persistent, window, scale, q.data_ptr(),
-                           k_pers.data_ptr() if n_persistent else 0, v_pers.data_ptr() if n_persistent else 0, out.data_ptr(),
-                           *qs, *os_, pos.data_ptr())
-    lib = _native.lib()
+    desc = _ATTENTION.pack(dtype_number, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0),
+                           k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), heads, n_persistent, window, scale,
+                           q.data_ptr(), k_pers.data_ptr() if n_persistent else 0, v_pers.data_ptr() if n_persistent else 0,
+                           out.data_ptr(), *qs, *os_, pos.data_ptr())
+    lib, device = _native.lib(), k_pages.device
     with _native._on(device):
         nbytes = lib.tmw_paged_attention_scratch_bytes(desc)
         # of this call alone: calls on two streams, or of two captured graphs, have nothing in common
