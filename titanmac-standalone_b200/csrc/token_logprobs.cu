@@ -7,16 +7,19 @@
 //   dx_i = g [i = t] + sum_j a_j [i = i_j] - p_i (g + sum_j a_j + h (log p_i + H)).
 // Both are bound by HBM: the logits once, and once more with their gradient on the way back.
 //
-// The most likely ids, the lower one first among equals: the k best of a row lie with the k threads whose own best are the k best
-// of all threads' (any other thread's logits have k ahead of them).  So the threads' bests, of which the pass has kept value and
-// vector, are ranked first, and then only those k threads' logits are looked at again (from L2).  Ranking is merging of sorted
-// lists of 32, one key to a lane: (value, index) in 64 bits, so there are no equals and no order of arrival.
+// The most likely ids, the lower one first among equals: if every warp knows r logits, of different threads, at or above a bound,
+// and r times the warps is k, then the k best of the row are at or above the bound.  The pass leaves every thread's best, so the
+// bound costs r maxima in each warp and the least of them all; then only the threads whose best reaches it look at their logits
+// again (from L2).  What they find - some dozens - is ranked by counting what is ahead of each: (value, index) in 64 bits, so there
+// are no equals, and the order of arrival does not matter.  Where it is more than fits (long runs of equal logits), every warp
+// keeps a sorted list of 32 keys, one to a lane, and the lists are merged.
 //
 // A row goes to a CTA, or, where there are few, to a cluster of them that joins through distributed shared memory.
 #include <cooperative_groups.h>
 #include <float.h>
 #include <math_constants.h>
 
+#include "tc_ptx.cuh"
 #include "tmw_common.cuh"
 
 namespace tmw {
@@ -83,13 +86,50 @@ __device__ __forceinline__ void unpack<__half>(const uint4& raw, float (&f)[8]) 
     load8<__half>(reinterpret_cast<const __half*>(&raw), f);
 }
 
-// ---- ranking ------------------------------------------------------------------------------------------------------------------
-// value in the high word, in an order that unsigned numbers have; the complement of the index in the low one; 0: none
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
-    const uint32_t bits = __float_as_uint(x + 0.0f);  // (-0 is 0)
-    const uint32_t order = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-    return (uint64_t)order << 32 | (uint32_t)~index;
+template <typename T>
+__device__ __forceinline__ void pack(const float (&f)[16 / sizeof(T)], uint4& raw);
+template <>
+__device__ __forceinline__ void pack<float>(const float (&f)[4], uint4& raw) {
+    raw = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
+template <>
+__device__ __forceinline__ void pack<__nv_bfloat16>(const float (&f)[8], uint4& raw) {
+    store8<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16*>(&raw), f);
+}
+template <>
+__device__ __forceinline__ void pack<__half>(const float (&f)[8], uint4& raw) { store8<__half>(reinterpret_cast<__half*>(&raw), f); }
+
+// the largest of a vector's elements (NaN aside) - for 16-bit types two at a time
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& raw);
+template <>
+__device__ __forceinline__ float largest<float>(const uint4& raw) {
+    return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+}
+template <>
+__device__ __forceinline__ float largest<__nv_bfloat16>(const uint4& raw) {
+    const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(__bfloat162float(m.x), __bfloat162float(m.y));
+}
+template <>
+__device__ __forceinline__ float largest<__half>(const uint4& raw) {
+    const __half2* v = reinterpret_cast<const __half2*>(&raw);
+    const __half2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(__half2float(m.x), __half2float(m.y));
+}
+
+// ---- ranking ------------------------------------------------------------------------------------------------------------------
+// an order of unsigned numbers that is the values' (-0 is 0; 0: none), and back
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t bits = __float_as_uint(x + 0.0f);
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+// value above index, the lower index first
+__device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t index) { return (uint64_t)order << 32 | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
 
 // one step of a bitonic network over the lanes: the larger key of a pair to the lower lane (down), or to the upper one
@@ -114,7 +154,7 @@ __device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b) {
     for (int apart = 16; apart > 0; apart /= 2) key = exchange(key, apart, true);
     return key;
 }
-// The 32 largest of n lists in shared memory (n a power of two, at most the CTA's warps times two), in the first one.  All threads.
+// The 32 largest of n sorted lists (n a power of two, at most twice the CTA's warps), in the first one.  All threads.
 __device__ __forceinline__ void merge_lists(uint64_t (*lists)[32], int n) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (; n > 1; n /= 2) {
@@ -131,106 +171,171 @@ __device__ __forceinline__ void merge_lists(uint64_t (*lists)[32], int n) {
 struct Sums {
     float m, s, t;
 };
-// (a difference of -inf weighs nothing: the bound keeps infinity times zero out)
-__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -1e30f); }
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    Sums r;
-    r.m = fmaxf(a.m, b.m);
-    const float da = (a.m - r.m) * kLog2e, db = (b.m - r.m) * kLog2e, wa = exp2f(da), wb = exp2f(db);
-    r.s = wa * a.s + wb * b.s;
-    r.t = wa * (a.t + bounded(da) * a.s) + wb * (b.t + bounded(db) * b.s);
-    return r;
+// A logarithm below which a weight is zero (2^-150, flushed): the bound keeps infinity times zero out of the sums.
+__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -150.f); }
+// the same under a larger maximum
+__device__ __forceinline__ void raise(Sums& a, float m) {
+    const float d = bounded((a.m - m) * kLog2e), w = ex2_ftz(d);
+    a.t = w * fmaf(d, a.s, a.t);
+    a.s *= w;
+    a.m = m;
+}
+__device__ __forceinline__ float warp_max(float x) { return value_of(__reduce_max_sync(0xffffffffu, order_of(x))); }
+// all lanes' together, on every lane
+__device__ __forceinline__ Sums warp_sums(Sums a) {
+    raise(a, warp_max(a.m));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
+    return a;
 }
 
+constexpr int kKeys = 256;  // that are ranked by counting
+
 template <typename T, int W>
-__global__ void __launch_bounds__(W * 32) logprobs_kernel(const __grid_constant__ Logprobs p, int ctas) {
-    constexpr int THREADS = W * 32, E = RowView<T>::E, AHEAD = 4, LISTS = W > 8 ? W : 8;
-    __shared__ Sums warp_sums[W];
-    __shared__ Sums part;                // this CTA's
-    __shared__ uint64_t lists[LISTS][32];
+__global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_constant__ Logprobs p, int ctas) {
+    constexpr int THREADS = W * 32, E = RowView<T>::E, AHEAD = 4;
+    __shared__ Sums sums[W];
+    __shared__ uint32_t low[W];
+    __shared__ Sums part;  // this CTA's
+    __shared__ __align__(16) uint64_t keys[kKeys / 32][32];
+    __shared__ uint64_t tops[kMostTop];  // the likely ids' keys in order
+    __shared__ int found;
+    __shared__ unsigned char chosen[W][32];
     __shared__ Sums whole_row;
     namespace cg = cooperative_groups;
     const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const RowView<T> x(row_of(p, row, sizeof(T)), p.vocab);
     const int per = (x.vectors + ctas - 1) / ctas, v_first = min(rank * per, x.vectors), v_end = min(v_first + per, x.vectors);
+    long long y = kNoTarget;
+    float picked = 0.f;
+    if (tid == 0 && rank == 0) {
+        y = p.targets[row];
+        if (y >= 0 && y < p.vocab) picked = to_f32<T>(x.x[y]);
+    }
+    if (tid == 0) found = 0;
+    if (tid < kMostTop) tops[tid] = 0;
 
-    // best: this thread's largest logit, best_at: the first vector that has it
-    float best = -CUDART_INF_F, base = -FLT_MAX, s = 0.f, t = 0.f;
-    int best_at = -1;
-    for (int v0 = v_first + tid; v0 < v_end; v0 += THREADS * AHEAD) {
+    // best: this thread's largest logit; a zero order where it has none
+    float best = -CUDART_INF_F, base = -FLT_MAX;
+    bool any = false;
+    uint64_t s2 = ptx::pack2(0.f, 0.f), t2 = s2, base2 = ptx::pack2(FLT_MAX, FLT_MAX);
+    const uint64_t log2e2 = ptx::pack2(kLog2e, kLog2e);
+    auto take = [&](const uint4& raw) {
+        const float top = largest<T>(raw);
+        if (top > best) {
+            best = top;
+            Sums a, b;
+            a.m = b.m = base;
+            ptx::unpack2(s2, a.s, b.s);
+            ptx::unpack2(t2, a.t, b.t);
+            const float m = fmaxf(top, base);
+            raise(a, m);
+            raise(b, m);
+            base = m;
+            s2 = ptx::pack2(a.s, b.s);
+            t2 = ptx::pack2(a.t, b.t);
+            base2 = ptx::pack2(-m, -m);
+        }
+        float f[E];
+        unpack<T>(raw, f);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            float da, db;
+            ptx::unpack2(ptx::mul2(ptx::add2(ptx::pack2(f[e], f[e + 1]), base2), log2e2), da, db);
+            const uint64_t w = ptx::pack2(ex2_ftz(da), ex2_ftz(db));  // (not of the bounded one: that would drop a NaN)
+            s2 = ptx::add2(s2, w);
+            t2 = ptx::fma2(w, ptx::pack2(bounded(da), bounded(db)), t2);
+        }
+    };
+    int v = v_first + tid;
+    for (; v + (AHEAD - 1) * THREADS < v_end; v += THREADS * AHEAD) {
         uint4 raw[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (v0 + u * THREADS < v_end) raw[u] = x.load(v0 + u * THREADS);
+        for (int u = 0; u < AHEAD; ++u) raw[u] = x.load(v + u * THREADS);
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = v0 + u * THREADS;
-            if (v >= v_end) break;
-            float f[E];
-            unpack<T>(raw[u], f);
-            float top = f[0];
-#pragma unroll
-            for (int e = 1; e < E; ++e) top = fmaxf(top, f[e]);
-            if (top > best || best_at < 0) {
-                best = top;
-                best_at = v;
-                if (top > base) {
-                    const float d = (base - top) * kLog2e, w = exp2f(d);
-                    t = w * (t + bounded(d) * s);
-                    s *= w;
-                    base = top;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float d = (f[e] - base) * kLog2e, w = ex2_ftz(d);
-                s += w;
-                t = fmaf(w, bounded(d), t);
-            }
+        for (int u = 0; u < AHEAD; ++u) take(raw[u]);
+        any = true;
+    }
+    for (; v < v_end; v += THREADS) {
+        take(x.load(v));
+        any = true;
+    }
+    float sa, sb, ta, tb;
+    ptx::unpack2(s2, sa, sb);
+    ptx::unpack2(t2, ta, tb);
+    const Sums of_warp = warp_sums({base, sa + sb, ta + tb});
+    const uint32_t best_order = any ? order_of(best) : 0;
+    if (lane == 0) sums[warp] = of_warp;
+    // the r-th best of every warp whose threads all have logits; with less than one such warp, everything fits
+    const int full = min(v_end - v_first, THREADS) / 32;
+    if (p.top > 0 && warp < full) {
+        uint32_t left = best_order, top = 0;
+        for (int r = (p.top + full - 1) / full; r > 0; --r) {
+            top = __reduce_max_sync(0xffffffffu, left);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, left == top)) - 1) left = 0;
         }
+        if (lane == 0) low[warp] = top;
     }
-    Sums mine{base, s, t};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Sums other{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o),
-                         __shfl_xor_sync(0xffffffffu, mine.t, o)};
-        mine = lane & o ? joined(other, mine) : joined(mine, other);  // (the same order on both sides)
-    }
-    if (lane == 0) warp_sums[warp] = mine;
     __syncthreads();
-    if (tid == 0) {
-        Sums all = warp_sums[0];
-        for (int w = 1; w < W; ++w) all = joined(all, warp_sums[w]);
-        part = all;
+    if (warp == 0) {
+        const Sums all = warp_sums(lane < W ? sums[lane] : Sums{-FLT_MAX, 0.f, 0.f});
+        if (lane == 0) part = all;
     }
 
     if (p.top > 0) {
-        // the threads whose best are among the k best: `least` and above
-        lists[warp][lane] = sorted(best_at < 0 ? 0 : key_of(best, (uint32_t)best_at * E));
-        merge_lists(lists, W);
-        const uint64_t least = lists[0][p.top - 1];
-        const bool look = best_at >= 0 && key_of(best, (uint32_t)best_at * E) >= least;
-        // (the best's own place in its vector is not known: the vector's last one stands for it)
-        const uint64_t floor = least == 0 ? 0 : least - (E - 1);
-        __syncthreads();
-        uint64_t top = 0;
-        for (uint32_t todo = __ballot_sync(0xffffffffu, look); todo != 0; todo &= todo - 1) {
-            const int from = v_first + warp * 32 + __ffs(todo) - 1;
-            for (int v0 = from; v0 < v_end; v0 += 32 * THREADS) {
-                const int v = v0 + lane * THREADS;
-                float f[E];
-                if (v < v_end) unpack<T>(x.load(v), f);
+        uint32_t least = full > 0 ? 0xffffffffu : 0;
+        for (int w = 0; w < full; ++w) least = min(least, low[w]);
+        const bool look = any && best_order >= least;
+        const uint32_t todo = __ballot_sync(0xffffffffu, look);
+        const int looking = __popc(todo), rounds = (v_end - v_first + THREADS - 1) / THREADS;
+        if (look) chosen[warp][__popc(todo & ((1u << lane) - 1))] = (unsigned char)lane;
+        __syncwarp();
+        for (int i = lane; i < looking * rounds; i += 32) {
+            const int c = i / rounds, at = v_first + warp * 32 + chosen[warp][c] + (i - c * rounds) * THREADS;
+            if (at >= v_end) continue;
+            float f[E];
+            unpack<T>(x.load(at), f);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const uint64_t key = v < v_end && x.has(v, e) ? key_of(f[e], (uint32_t)(v * E + e)) : 0;
-                    const uint64_t last = __shfl_sync(0xffffffffu, top, p.top - 1);
-                    const bool in = key >= floor && key > last;
-                    if (__any_sync(0xffffffffu, in)) top = merged(top, sorted(in ? key : 0));
-                }
+            for (int e = 0; e < E; ++e) {
+                const uint32_t order = order_of(f[e]);
+                if (order < least || !x.has(at, e)) continue;
+                const int n = atomicAdd(&found, 1);
+                if (n < kKeys) keys[n / 32][n % 32] = key_of(order, (uint32_t)(at * E + e));
             }
         }
-        lists[warp][lane] = top;
-        merge_lists(lists, W);
+        __syncthreads();
+        const int n = found;
+        if (n <= kKeys) {
+            for (int i = tid; i < n; i += THREADS) {
+                const uint64_t key = keys[i / 32][i % 32];
+                int ahead = 0;
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) ahead += keys[j / 32][j % 32] > key;
+                if (ahead < p.top) tops[ahead] = key;
+            }
+        } else {
+            uint64_t top = 0;
+            for (int i0 = 0; i0 < looking * rounds; i0 += 32) {
+                const int i = i0 + lane, c = min(i / rounds, looking - 1);
+                const int at = v_first + warp * 32 + chosen[warp][c] + (i - c * rounds) * THREADS;
+                const bool there = i < looking * rounds && at < v_end;
+                float f[E];
+                if (there) unpack<T>(x.load(at), f);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const uint64_t key = there && x.has(at, e) ? key_of(order_of(f[e]), (uint32_t)(at * E + e)) : 0;
+                    const uint64_t last = __shfl_sync(0xffffffffu, top, p.top - 1);
+                    if (__any_sync(0xffffffffu, key > last)) top = merged(top, sorted(key > last ? key : 0));
+                }
+            }
+            __syncthreads();
+            keys[warp][lane] = top;
+            merge_lists(keys, W);
+            if (tid < p.top) tops[tid] = keys[0][tid];
+        }
     }
     __syncthreads();
 
@@ -238,17 +343,14 @@ __global__ void __launch_bounds__(W * 32) logprobs_kernel(const __grid_constant_
         auto cluster = cg::this_cluster();
         cluster.sync();
         if (rank == 0) {
-            if (tid == 0) {
-                Sums all = part;
-                for (int c = 1; c < ctas; ++c) all = joined(all, *cluster.map_shared_rank(&part, c));
-                whole_row = all;
+            if (warp == 0) {
+                const Sums all = warp_sums(lane < ctas ? *cluster.map_shared_rank(&part, lane) : Sums{-FLT_MAX, 0.f, 0.f});
+                if (lane == 0) whole_row = all;
             }
-            uint64_t key = 0;
-            if (p.top > 0 && warp < ctas) key = cluster.map_shared_rank(&lists[0][0], warp)[lane];
-            __syncthreads();  // (list 0 is this CTA's own)
             if (p.top > 0) {
-                if (warp < ctas) lists[warp][lane] = key;
-                merge_lists(lists, ctas);
+                for (int c = warp; c < ctas; c += W) keys[c][lane] = cluster.map_shared_rank(tops, c)[lane];
+                merge_lists(keys, ctas);
+                if (tid < p.top) tops[tid] = keys[0][tid];
             }
         }
         cluster.sync();
@@ -262,11 +364,10 @@ __global__ void __launch_bounds__(W * 32) logprobs_kernel(const __grid_constant_
     const bool fine = all.s > 0.f;  // (NaN: a NaN or +inf among the logits; 0: nothing but -inf)
     const float log_sum = logf(all.s);
     if (tid == 0) {
-        const long long y = p.targets[row];
         float lp = CUDART_NAN_F;
         if (y == kNoTarget) lp = 0.f;
         else if (y < 0 || y >= p.vocab) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
-        else if (fine) lp = (to_f32<T>(x.x[y]) - all.m) - log_sum;
+        else if (fine) lp = (picked - all.m) - log_sum;
         p.logprobs[row] = lp;
         p.entropy[row] = fine ? log_sum - kLn2 * (all.t / all.s) : CUDART_NAN_F;
         if (p.lse != nullptr) {
@@ -276,9 +377,9 @@ __global__ void __launch_bounds__(W * 32) logprobs_kernel(const __grid_constant_
     }
     if (tid < p.top) {
         const long long at = (long long)row * p.top + tid;
-        const uint32_t i = index_of(lists[0][tid]) - (uint32_t)x.shift;
-        p.top_ids[at] = fine ? (int64_t)i : -1;
-        p.top_logprobs[at] = fine ? (to_f32<T>(x.x[i]) - all.m) - log_sum : CUDART_NAN_F;
+        const uint64_t key = tops[tid];
+        p.top_ids[at] = fine ? (int64_t)(index_of(key) - (uint32_t)x.shift) : -1;
+        p.top_logprobs[at] = fine ? (value_of((uint32_t)(key >> 32)) - all.m) - log_sum : CUDART_NAN_F;
     }
 }
 
@@ -292,41 +393,62 @@ struct LogprobsBackward {
 
 constexpr int kBackThreads = 256, kBackVectors = 8;  // vectors of a thread
 
-// VEC: whole vectors; else (logits and gradient begin at different places of their vectors) one element at a time
-template <typename T, bool VEC>
+// VEC: whole vectors; else (logits and gradient begin at different places of their vectors) one element at a time.
+// H: the entropy has a gradient.
+template <typename T, bool VEC, bool H>
 __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const __grid_constant__ LogprobsBackward p) {
-    constexpr int E = VEC ? RowView<T>::E : 1;
-    const int row = blockIdx.x, tid = threadIdx.x;
+    constexpr int E = VEC ? RowView<T>::E : 1, AHEAD = kBackVectors / 2;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     const RowView<T> x(row_of(p.f, row, sizeof(T)), p.f.vocab);
     const int b = row / p.f.tokens;
     T* d = static_cast<T*>(p.d_logits) + b * p.stride[0] + (row - b * p.f.tokens) * p.stride[1];
-    const float m = p.f.lse[2LL * row], log_sum = p.f.lse[2LL * row + 1], entropy = p.f.entropy[row];
-    const long long y = p.f.targets[row];
-    const float h = p.d_entropy != nullptr ? p.d_entropy[row] : 0.f;
-    float g = p.d_logprobs != nullptr && y != kNoTarget ? p.d_logprobs[row] : 0.f;
-    if (y != kNoTarget && (y < 0 || y >= p.f.vocab)) g = CUDART_NAN_F;
-    float pulled = g;
-    const int top = p.d_top != nullptr ? p.f.top : 0;
-    for (int j = 0; j < top; ++j) pulled += p.d_top[(long long)row * top + j];
-    const float at_zero = pulled + h * entropy;  // - dx_i / p_i = pulled + h (log p_i + H)
-    // nothing comes back to the row: nothing goes on, whatever its logits are
-    const bool none = g == 0.f && h == 0.f && pulled == 0.f;
-    auto gradient = [&](float v) {
-        if (none) return 0.f;
-        const float lp = (v - m) - log_sum;
-        return -exp2f(lp * kLog2e) * fmaf(h, fmaxf(lp, -200.f), at_zero);  // (e^-200 is zero: the bound keeps infinity out)
-    };
-
     const int shift = VEC ? x.shift : 0, n = VEC ? x.vectors : p.f.vocab;
     const int first = blockIdx.y * (kBackThreads * kBackVectors), end = min(first + kBackThreads * kBackVectors, n);
+
+    const float m = p.f.lse[2LL * row], log_sum = p.f.lse[2LL * row + 1];
+    const long long y = p.f.targets[row];
+    const float h = H ? p.d_entropy[row] : 0.f;
+    float g = p.d_logprobs != nullptr && y != kNoTarget ? p.d_logprobs[row] : 0.f;
+    if (y != kNoTarget && (y < 0 || y >= p.f.vocab)) g = CUDART_NAN_F;
+    const int top = p.d_top != nullptr ? p.f.top : 0;
+    float pulled = top > 0 && lane < top ? p.d_top[(long long)row * top + lane] : 0.f;
+    bool none = true;  // nothing comes back to the row: nothing goes on, whatever its logits are
+    if (top > 0) {
+        none = __all_sync(0xffffffffu, pulled == 0.f);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) pulled += __shfl_xor_sync(0xffffffffu, pulled, o);
+    }
+    none = none && g == 0.f && h == 0.f;
+    pulled += g;
+    // dx_i = p_i (-pulled - h H - h log p_i)
+    const float at_zero = H ? -fmaf(h, p.f.entropy[row], pulled) : -pulled;
+    auto gradient = [&](float v) {
+        const float lp = (v - m) - log_sum;
+        return ex2_ftz(lp * kLog2e) * (H ? fmaf(-h, fmaxf(lp, -200.f), at_zero) : at_zero);  // (e^-200 is zero: infinity stays out)
+    };
+    const uint64_t m2 = ptx::pack2(-m, -m), log_sum2 = ptx::pack2(-log_sum, -log_sum), log2e2 = ptx::pack2(kLog2e, kLog2e),
+                   h2 = ptx::pack2(-h, -h), zero2 = ptx::pack2(at_zero, at_zero);
+    auto gradients = [&](float va, float vb, float& ra, float& rb) {
+        const uint64_t lp = ptx::add2(ptx::add2(ptx::pack2(va, vb), m2), log_sum2);
+        float ea, eb;
+        ptx::unpack2(ptx::mul2(lp, log2e2), ea, eb);
+        uint64_t c = zero2;
+        if (H) {
+            float la, lb;
+            ptx::unpack2(lp, la, lb);
+            c = ptx::fma2(h2, ptx::pack2(fmaxf(la, -200.f), fmaxf(lb, -200.f)), zero2);
+        }
+        ptx::unpack2(ptx::mul2(ptx::pack2(ex2_ftz(ea), ex2_ftz(eb)), c), ra, rb);
+    };
+    const int y_vector = y >= 0 && y < p.f.vocab ? (int)((y + shift) / E) : -1, y_element = (int)((y + shift) % E);
+
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        constexpr int AHEAD = kBackVectors / 2;
         uint4 raw[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int v = first + tid + (half * AHEAD + u) * kBackThreads;
-            if (v >= end) continue;
+            if (v >= end || none) continue;
             if (VEC) raw[u] = x.load(v);
             else *reinterpret_cast<T*>(&raw[u]) = x.x[v];
         }
@@ -335,26 +457,39 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const _
             const int v = first + tid + (half * AHEAD + u) * kBackThreads;
             if (v >= end) continue;
             float f[E];
-            if constexpr (VEC) unpack<T>(raw[u], f);
-            else f[0] = to_f32<T>(*reinterpret_cast<T*>(&raw[u]));
-            T out[E];
+            if (none) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                float r = gradient(f[e]);
-                if (v * E + e - shift == y) r += g;
-                out[e] = from_f32<T>(r);
-            }
-            if (!VEC || x.whole(v)) {
-                if constexpr (VEC) *reinterpret_cast<uint4*>(d + (long long)v * E - shift) = *reinterpret_cast<const uint4*>(out);
-                else d[v] = out[0];
+                for (int e = 0; e < E; ++e) f[e] = 0.f;
             } else {
+                if constexpr (VEC) {
+                    unpack<T>(raw[u], f);
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (x.has(v, e)) d[v * E + e - shift] = out[e];
+                    for (int e = 0; e < E; e += 2) gradients(f[e], f[e + 1], f[e], f[e + 1]);
+                } else {
+                    f[0] = gradient(to_f32<T>(*reinterpret_cast<T*>(&raw[u])));
+                }
+                if (v == y_vector) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (e == y_element) f[e] += g;
+                }
+            }
+            if constexpr (VEC) {
+                uint4 out;
+                pack<T>(f, out);
+                if (x.whole(v)) {
+                    *reinterpret_cast<uint4*>(d + (long long)v * E - shift) = out;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (x.has(v, e)) d[v * E + e - shift] = reinterpret_cast<const T*>(&out)[e];
+                }
+            } else {
+                d[v] = from_f32<T>(f[0]);
             }
         }
     }
-    if (top == 0) return;
+    if (top == 0 || none) return;
     __syncthreads();  // the likely ids' own gradients, over what the pass has written
     if (tid < top) {
         const long long id = p.f.top_ids[(long long)row * top + tid];
@@ -385,8 +520,9 @@ int launch_backward(const LogprobsBackward& p, cudaStream_t stream) {
                      (p.f.stride[0] - p.stride[0]) % E == 0 && (p.f.stride[1] - p.stride[1]) % E == 0;
     const long long n = vec ? ((long long)p.f.vocab + 2 * E - 2) / E : p.f.vocab;
     const dim3 grid((unsigned)p.f.rows, (unsigned)((n + kBackThreads * kBackVectors - 1) / (kBackThreads * kBackVectors)));
-    if (vec) logprobs_backward_kernel<T, true><<<grid, kBackThreads, 0, stream>>>(p);
-    else logprobs_backward_kernel<T, false><<<grid, kBackThreads, 0, stream>>>(p);
+    const auto run = [&](auto kern) { kern<<<grid, kBackThreads, 0, stream>>>(p); };
+    if (vec) p.d_entropy != nullptr ? run(logprobs_backward_kernel<T, true, true>) : run(logprobs_backward_kernel<T, true, false>);
+    else p.d_entropy != nullptr ? run(logprobs_backward_kernel<T, false, true>) : run(logprobs_backward_kernel<T, false, false>);
     TMW_CUDA_TRY(cudaGetLastError());
     return TMW_OK;
 }
