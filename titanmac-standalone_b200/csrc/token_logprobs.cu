@@ -220,7 +220,6 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
 
     // best: this thread's largest logit; a zero order where it has none
     float best = -CUDART_INF_F, base = -FLT_MAX;
-    bool any = false;
     uint64_t s2 = ptx::pack2(0.f, 0.f), t2 = s2, base2 = ptx::pack2(FLT_MAX, FLT_MAX);
     const uint64_t log2e2 = ptx::pack2(kLog2e, kLog2e);
     auto take = [&](const uint4& raw) {
@@ -251,18 +250,42 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
         }
     };
     int v = v_first + tid;
-    for (; v + (AHEAD - 1) * THREADS < v_end; v += THREADS * AHEAD) {
-        uint4 raw[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) raw[u] = x.load(v + u * THREADS);
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) take(raw[u]);
-        any = true;
-    }
-    for (; v < v_end; v += THREADS) {
+    const bool any = v < v_end;
+    if (any && !x.whole(v)) {  // (the row's first vector, or its only one)
         take(x.load(v));
-        any = true;
+        v += THREADS;
     }
+    // whole vectors, the next batch on its way under this one
+    const int stop = v_end > v_first && !x.whole(v_end - 1) ? v_end - 1 : v_end;
+    const uint4* at = reinterpret_cast<const uint4*>(x.x - x.shift) + v;
+    uint4 now[AHEAD], next[AHEAD];
+    auto fetch = [&](uint4 (&raw)[AHEAD]) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) raw[u] = at[u * THREADS];
+        at += AHEAD * THREADS;
+    };
+    int batches = v < stop ? ((stop - v - 1) / THREADS + 1) / AHEAD : 0;
+    v += batches * AHEAD * THREADS;
+    if (batches > 0) fetch(now);
+    for (; batches > 1; --batches) {
+        fetch(next);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) take(now[u]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) now[u] = next[u];
+    }
+    // the rest, fewer than a batch, under the last one
+#pragma unroll
+    for (int u = 0; u < AHEAD - 1; ++u)
+        if (v + u * THREADS < v_end) next[u] = x.load(v + u * THREADS);
+    if (batches > 0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) take(now[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD - 1; ++u)
+        if (v + u * THREADS < v_end) take(next[u]);
+    if (AHEAD > 1 && v + (AHEAD - 1) * THREADS < v_end) take(x.load(v + (AHEAD - 1) * THREADS));  // (the row's last, in part)
     float sa, sb, ta, tb;
     ptx::unpack2(s2, sa, sb);
     ptx::unpack2(t2, ta, tb);
@@ -288,7 +311,8 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     if (p.top > 0) {
         uint32_t least = full > 0 ? 0xffffffffu : 0;
         for (int w = 0; w < full; ++w) least = min(least, low[w]);
-        const bool look = any && best_order >= least;
+        const float floor = least == 0 ? -CUDART_INF_F : value_of(least);
+        const bool look = any && best >= floor;
         const uint32_t todo = __ballot_sync(0xffffffffu, look);
         const int looking = __popc(todo), rounds = (v_end - v_first + THREADS - 1) / THREADS;
         if (look) chosen[warp][__popc(todo & ((1u << lane) - 1))] = (unsigned char)lane;
@@ -300,10 +324,9 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
             unpack<T>(x.load(at), f);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const uint32_t order = order_of(f[e]);
-                if (order < least || !x.has(at, e)) continue;
+                if (!(f[e] >= floor) || !x.has(at, e)) continue;
                 const int n = atomicAdd(&found, 1);
-                if (n < kKeys) keys[n / 32][n % 32] = key_of(order, (uint32_t)(at * E + e));
+                if (n < kKeys) keys[n / 32][n % 32] = key_of(order_of(f[e]), (uint32_t)(at * E + e));
             }
         }
         __syncthreads();
@@ -391,19 +414,30 @@ struct LogprobsBackward {
     long long stride[2];
 };
 
-constexpr int kBackThreads = 256, kBackVectors = 8;  // vectors of a thread
+constexpr int kBackThreads = 256, kBackVectors = 16;  // vectors of a thread
 
 // VEC: whole vectors; else (logits and gradient begin at different places of their vectors) one element at a time.
 // H: the entropy has a gradient.
 template <typename T, bool VEC, bool H>
 __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const __grid_constant__ LogprobsBackward p) {
-    constexpr int E = VEC ? RowView<T>::E : 1, AHEAD = kBackVectors / 2;
+    constexpr int E = VEC ? RowView<T>::E : 1, AHEAD = 2;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     const RowView<T> x(row_of(p.f, row, sizeof(T)), p.f.vocab);
     const int b = row / p.f.tokens;
     T* d = static_cast<T*>(p.d_logits) + b * p.stride[0] + (row - b * p.f.tokens) * p.stride[1];
     const int shift = VEC ? x.shift : 0, n = VEC ? x.vectors : p.f.vocab;
     const int first = blockIdx.y * (kBackThreads * kBackVectors), end = min(first + kBackThreads * kBackVectors, n);
+
+    // the first logits are on their way while the row's numbers are, and then AHEAD vectors always
+    uint4 raw[AHEAD];
+    auto fetch = [&](int i) {
+        const int v = first + tid + i * kBackThreads;
+        if (v >= end) return;
+        if (VEC) raw[i % AHEAD] = x.load(v);
+        else *reinterpret_cast<T*>(&raw[i % AHEAD]) = x.x[v];
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(i);
 
     const float m = p.f.lse[2LL * row], log_sum = p.f.lse[2LL * row + 1];
     const long long y = p.f.targets[row];
@@ -443,50 +477,41 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const _
     const int y_vector = y >= 0 && y < p.f.vocab ? (int)((y + shift) / E) : -1, y_element = (int)((y + shift) % E);
 
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint4 raw[AHEAD];
+    for (int i = 0; i < kBackVectors; ++i) {
+        const int v = first + tid + i * kBackThreads;
+        if (v >= end) break;
+        const uint4 now = raw[i % AHEAD];
+        if (i + AHEAD < kBackVectors) fetch(i + AHEAD);
+        float f[E];
+        if (none) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = first + tid + (half * AHEAD + u) * kBackThreads;
-            if (v >= end || none) continue;
-            if (VEC) raw[u] = x.load(v);
-            else *reinterpret_cast<T*>(&raw[u]) = x.x[v];
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = first + tid + (half * AHEAD + u) * kBackThreads;
-            if (v >= end) continue;
-            float f[E];
-            if (none) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) f[e] = 0.f;
-            } else {
-                if constexpr (VEC) {
-                    unpack<T>(raw[u], f);
-#pragma unroll
-                    for (int e = 0; e < E; e += 2) gradients(f[e], f[e + 1], f[e], f[e + 1]);
-                } else {
-                    f[0] = gradient(to_f32<T>(*reinterpret_cast<T*>(&raw[u])));
-                }
-                if (v == y_vector) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (e == y_element) f[e] += g;
-                }
-            }
+            for (int e = 0; e < E; ++e) f[e] = 0.f;
+        } else {
             if constexpr (VEC) {
-                uint4 out;
-                pack<T>(f, out);
-                if (x.whole(v)) {
-                    *reinterpret_cast<uint4*>(d + (long long)v * E - shift) = out;
-                } else {
+                unpack<T>(now, f);
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (x.has(v, e)) d[v * E + e - shift] = reinterpret_cast<const T*>(&out)[e];
-                }
+                for (int e = 0; e < E; e += 2) gradients(f[e], f[e + 1], f[e], f[e + 1]);
             } else {
-                d[v] = from_f32<T>(f[0]);
+                f[0] = gradient(to_f32<T>(*reinterpret_cast<const T*>(&now)));
             }
+            if (v == y_vector) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e == y_element) f[e] += g;
+            }
+        }
+        if constexpr (VEC) {
+            uint4 out;
+            pack<T>(f, out);
+            if (x.whole(v)) {
+                *reinterpret_cast<uint4*>(d + (long long)v * E - shift) = out;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (x.has(v, e)) d[v * E + e - shift] = reinterpret_cast<const T*>(&out)[e];
+            }
+        } else {
+            d[v] = from_f32<T>(f[0]);
         }
     }
     if (top == 0 || none) return;
