@@ -192,6 +192,7 @@ __device__ __forceinline__ Sums warp_sums(Sums a) {
     return a;
 }
 
+constexpr float kSlack = 30.f;  // e^30 times the vocabulary's largest size is far from an fp32 number's end
 constexpr int kKeys = 256;  // that are ranked by counting
 
 template <typename T, int W>
@@ -218,25 +219,27 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     if (tid == 0) found = 0;
     if (tid < kMostTop) tops[tid] = 0;
 
-    // best: this thread's largest logit; a zero order where it has none
-    float best = -CUDART_INF_F, base = -FLT_MAX;
+    // best: this thread's largest logit.  Its sums stand under a base that follows only a logit more than kSlack above it: some
+    // lane of a warp meets a new largest logit at most steps (3000 rows of 49999 with it followed each time: 89 us, 190 for 4096 of
+    // 128000).
+    float best = -CUDART_INF_F, base = -FLT_MAX, limit = -FLT_MAX;
     uint64_t s2 = ptx::pack2(0.f, 0.f), t2 = s2, base2 = ptx::pack2(FLT_MAX, FLT_MAX);
     const uint64_t log2e2 = ptx::pack2(kLog2e, kLog2e);
     auto take = [&](const uint4& raw) {
         const float top = largest<T>(raw);
-        if (top > best) {
-            best = top;
+        best = fmaxf(best, top);
+        if (top > limit) {
             Sums a, b;
             a.m = b.m = base;
             ptx::unpack2(s2, a.s, b.s);
             ptx::unpack2(t2, a.t, b.t);
-            const float m = fmaxf(top, base);
-            raise(a, m);
-            raise(b, m);
-            base = m;
+            base = fmaxf(top, base);
+            limit = base + kSlack;
+            raise(a, base);
+            raise(b, base);
             s2 = ptx::pack2(a.s, b.s);
             t2 = ptx::pack2(a.t, b.t);
-            base2 = ptx::pack2(-m, -m);
+            base2 = ptx::pack2(-base, -base);
         }
         float f[E];
         unpack<T>(raw, f);
@@ -289,7 +292,9 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     float sa, sb, ta, tb;
     ptx::unpack2(s2, sa, sb);
     ptx::unpack2(t2, ta, tb);
-    const Sums of_warp = warp_sums({base, sa + sb, ta + tb});
+    Sums mine{base, sa + sb, ta + tb};
+    raise(mine, fmaxf(best, base));
+    const Sums of_warp = warp_sums(mine);
     const uint32_t best_order = any ? order_of(best) : 0;
     if (lane == 0) sums[warp] = of_warp;
     // the r-th best of every warp whose threads all have logits; with less than one such warp, everything fits
