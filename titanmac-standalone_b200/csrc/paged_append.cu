@@ -18,40 +18,130 @@ struct PagedAppend {
     const int32_t *start, *counts;
     const float* inv_freq;
     int rows, heads, half;
-    FastDiv units, slots;  // vector pairs of a head; heads of a token, queries' first
+    int step_r, step_slot, step_u;  // from a thread's pair of vectors to its next one: tokens, heads, pairs
     int* status;
 };
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendTokens = 4;   // tokens of a CTA
-constexpr int kAppendAhead = 2;    // vector pairs that a thread loads before it stores the first
+constexpr int kAppendTokens = 4;  // tokens of a CTA
 
 template <typename T, int E>
 struct alignas(sizeof(T) * E) Pack {
     T x[E];
 };
 
+// x c + y s, in one way for every layout: the same bits wherever a row begins
+__device__ __forceinline__ float turned(float x, float y, float c, float s) { return fmaf(x, c, __fmul_rn(y, s)); }
+
 // E: elements of a vector, 16 bytes or (rows at any address, pairs that fit no vector) one element
 template <typename T, int E, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppend p) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ PagedAppend p) {
+    using V = Pack<T, E>;
     extern __shared__ float2 turn[];  // [token][half] cosine and sine
     __shared__ long long place[kAppendTokens];
     const int b = blockIdx.y, r0 = blockIdx.x * kAppendTokens, tid = threadIdx.x;
     const int start = p.start[b];
     int count = p.counts != nullptr ? p.counts[b] : p.rows;
     if (start == -1) return;
-    if (start < -1 || count < 0 || count > p.rows) {  // the sequence has no place: every row that it may have is NaN
-        count = start < -1 && count >= 0 && count <= p.rows ? count : p.rows;
-        if (tid < kAppendTokens) place[tid] = -1;
-        if (tid == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
-    } else if (tid < kAppendTokens && r0 + tid < count) {
+    const bool nowhere = start < -1 || count < 0 || count > p.rows;  // every row that the sequence may have is NaN
+    if (nowhere && (count < 0 || count > p.rows)) count = p.rows;
+    const int tokens = min(kAppendTokens, count - r0);
+    if (tokens <= 0) return;
+
+    // A pair of vectors of a head of a token; a thread takes every kAppendThreads-th one of the CTA's.
+    struct Item {
+        int r, slot, u;  // token, head (queries, keys, values), pair of the head
+    };
+    const int units = p.map.head_dim / (2 * E), slots = p.heads + 2 * p.map.kv_heads;
+    auto after = [&](Item w) {
+        w.u += p.step_u;
+        w.slot += p.step_slot;
+        w.r += p.step_r;
+        if (w.u >= units) w.u -= units, ++w.slot;
+        if (w.slot >= slots) w.slot -= slots, ++w.r;
+        return w;
+    };
+    // first elements of the two: rotated halves face each other, everything else lies side by side
+    auto ends = [&](int u, int& ia, int& ib) {
+        const bool facing = (!INTERLEAVED || E == 1) && u * E < p.half;
+        if (INTERLEAVED && E == 1) ia = 2 * u, ib = 2 * u + 1;
+        else if (facing) ia = u * E, ib = u * E + p.half;
+        else ia = 2 * u * E, ib = ia + E;
+    };
+    const T *q = static_cast<const T*>(p.q) + b * p.qs[0] + r0 * p.qs[2], *k = static_cast<const T*>(p.k) + b * p.ks[0] + r0 * p.ks[2],
+            *v = static_cast<const T*>(p.v) + b * p.vs[0] + r0 * p.vs[2];
+    T* q_out = static_cast<T*>(p.q_out) + b * p.os[0] + r0 * p.os[2];
+    auto load = [&](const Item& w, V& va, V& vb) {
+        if (w.r >= tokens) return;
+        int ia, ib;
+        ends(w.u, ia, ib);
+        const int of_kv = w.slot - p.heads;
+        const T* from;
+        if (of_kv < 0) from = q + w.slot * p.qs[1] + w.r * p.qs[2];
+        else if (of_kv < p.map.kv_heads) from = k + of_kv * p.ks[1] + w.r * p.ks[2];
+        else from = v + (of_kv - p.map.kv_heads) * p.vs[1] + w.r * p.vs[2];
+        va = *reinterpret_cast<const V*>(from + ia);
+        vb = *reinterpret_cast<const V*>(from + ib);
+    };
+    auto store = [&](const Item& w, V& va, V& vb) {
+        int ia, ib;
+        ends(w.u, ia, ib);
+        const int of_kv = w.slot - p.heads;
+        const bool query = of_kv < 0, value = of_kv >= p.map.kv_heads;
+        const long long at = place[w.r];
+        T* to;
+        if (query) to = q_out + w.slot * p.os[1] + w.r * p.os[2];
+        else if (at < 0) return;
+        else if (value) to = static_cast<T*>(p.v_pages) + at + (of_kv - p.map.kv_heads) * p.map.head_step();
+        else to = static_cast<T*>(p.k_pages) + at + of_kv * p.map.head_step();
+        const float2* t = turn + w.r * p.half;
+        if (query && at < 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) va.x[e] = vb.x[e] = from_f32<T>(__int_as_float(0x7fffffff));
+        } else if (!value && INTERLEAVED && E > 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                V& v = h ? vb : va;
+                const int first = h ? ib : ia;
+                if (first >= 2 * p.half) continue;
+#pragma unroll
+                for (int e = 0; e + 1 < E; e += 2) {
+                    const float2 cs = t[(first + e) / 2];
+                    const float x = to_f32<T>(v.x[e]), y = to_f32<T>(v.x[e + 1]);
+                    v.x[e] = from_f32<T>(turned(x, y, cs.x, -cs.y));
+                    v.x[e + 1] = from_f32<T>(turned(y, x, cs.x, cs.y));
+                }
+            }
+        } else if (!value) {
+            const int pair = INTERLEAVED ? ia / 2 : ia;
+            if (pair < p.half && ib < 2 * p.half) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float2 cs = t[pair + e];
+                    const float x = to_f32<T>(va.x[e]), y = to_f32<T>(vb.x[e]);
+                    va.x[e] = from_f32<T>(turned(x, y, cs.x, -cs.y));
+                    vb.x[e] = from_f32<T>(turned(y, x, cs.x, cs.y));
+                }
+            }
+        }
+        *reinterpret_cast<V*>(to + ia) = va;
+        *reinterpret_cast<V*>(to + ib) = vb;
+    };
+
+    Item now;
+    now.slot = tid / units;
+    now.u = tid - now.slot * units;
+    now.r = now.slot / slots;
+    now.slot -= now.r * slots;
+    V va, vb;
+    load(now, va, vb);
+    // under the first loads: the tokens' places, and their angles
+    if (tid < tokens) {
         const long long t = (long long)start + r0 + tid;
-        const long long at = t < p.map.capacity ? p.map.token(b, (int)t) : -1;
+        const long long at = !nowhere && t < p.map.capacity ? p.map.token(b, (int)t) : -1;
         if (at < 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
         place[tid] = at;
     }
-    const int tokens = min(kAppendTokens, count - r0);
-    if (tokens <= 0) return;
     for (int i = tid; i < tokens * p.half; i += kAppendThreads) {
         const int r = i / p.half;
         // turns instead of radians: the whole ones fall away exactly
@@ -62,88 +152,23 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Page
         turn[i] = make_float2(c, s);
     }
     __syncthreads();
-
-    using V = Pack<T, E>;
-    const int n = tokens * (int)(p.units.d * p.slots.d);
-    for (int first = tid; first < n; first += kAppendThreads * kAppendAhead) {
-        V va[kAppendAhead], vb[kAppendAhead];
-        T* to[kAppendAhead];
-        int ia[kAppendAhead], ib[kAppendAhead], row[kAppendAhead], kind[kAppendAhead];  // kind: 0 query, 1 key, 2 value
-#pragma unroll
-        for (int j = 0; j < kAppendAhead; ++j) {
-            const int i = first + j * kAppendThreads;
-            to[j] = nullptr;
-            if (i >= n) continue;
-            const int head = (int)p.units.div(i), u = i - head * (int)p.units.d;
-            const int r = (int)p.slots.div(head);
-            int slot = head - r * (int)p.slots.d;
-            row[j] = r;
-            // the pair of vectors: rotated halves face each other, everything else lies side by side
-            const int facing = INTERLEAVED && E > 1 ? 0 : p.half / E;
-            if (INTERLEAVED && E == 1) ia[j] = 2 * u, ib[j] = 2 * u + 1;
-            else if (u < facing) ia[j] = u * E, ib[j] = u * E + p.half;
-            else ia[j] = 2 * u * E, ib[j] = (2 * u + 1) * E;
-            const T* from;
-            const long long at = place[r];
-            if (slot < p.heads) {
-                kind[j] = 0;
-                from = static_cast<const T*>(p.q) + b * p.qs[0] + slot * p.qs[1] + (r0 + r) * p.qs[2];
-                to[j] = static_cast<T*>(p.q_out) + b * p.os[0] + slot * p.os[1] + (r0 + r) * p.os[2];
-            } else {
-                if (at < 0) continue;
-                slot -= p.heads;
-                const bool value = slot >= p.map.kv_heads;
-                if (value) slot -= p.map.kv_heads;
-                kind[j] = value ? 2 : 1;
-                const long long* s = value ? p.vs : p.ks;
-                from = static_cast<const T*>(value ? p.v : p.k) + b * s[0] + slot * s[1] + (r0 + r) * s[2];
-                to[j] = static_cast<T*>(value ? p.v_pages : p.k_pages) + at + slot * p.map.head_step();
-            }
-            va[j] = *reinterpret_cast<const V*>(from + ia[j]);
-            vb[j] = *reinterpret_cast<const V*>(from + ib[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < kAppendAhead; ++j) {
-            if (to[j] == nullptr) continue;
-            const float2* t = turn + row[j] * p.half;
-            if (kind[j] == 0 && place[row[j]] < 0) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) va[j].x[e] = vb[j].x[e] = from_f32<T>(__int_as_float(0x7fffffff));
-            } else if (kind[j] != 2) {
-                if (INTERLEAVED && E > 1) {
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        V& v = w ? vb[j] : va[j];
-                        const int at = w ? ib[j] : ia[j];
-                        if (at < 2 * p.half) {
-#pragma unroll
-                            for (int e = 0; e + 1 < E; e += 2) {
-                                const float2 cs = t[(at + e) / 2];
-                                const float x = to_f32<T>(v.x[e]), y = to_f32<T>(v.x[e + 1]);
-                                v.x[e] = from_f32<T>(x * cs.x - y * cs.y);
-                                v.x[e + 1] = from_f32<T>(y * cs.x + x * cs.y);
-                            }
-                        }
-                    }
-                } else if ((INTERLEAVED ? ia[j] / 2 : ia[j]) < p.half && ib[j] < 2 * p.half) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float2 cs = t[(INTERLEAVED ? ia[j] / 2 : ia[j]) + e];
-                        const float x = to_f32<T>(va[j].x[e]), y = to_f32<T>(vb[j].x[e]);
-                        va[j].x[e] = from_f32<T>(x * cs.x - y * cs.y);
-                        vb[j].x[e] = from_f32<T>(y * cs.x + x * cs.y);
-                    }
-                }
-            }
-            *reinterpret_cast<V*>(to[j] + ia[j]) = va[j];
-            *reinterpret_cast<V*>(to[j] + ib[j]) = vb[j];
-        }
+    while (now.r < tokens) {  // the next pair loads under this one
+        const Item next = after(now);
+        V na, nb;
+        load(next, na, nb);
+        store(now, va, vb);
+        va = na;
+        vb = nb;
+        now = next;
     }
 }
 
 template <typename T, int E>
 int launch_append(PagedAppend& p, bool interleaved, int batch, cudaStream_t stream) {
-    p.units = FastDiv((uint32_t)(p.map.head_dim / (2 * E)));
+    const int units = p.map.head_dim / (2 * E), slots = p.heads + 2 * p.map.kv_heads;
+    p.step_u = kAppendThreads % units;
+    p.step_slot = kAppendThreads / units % slots;
+    p.step_r = kAppendThreads / units / slots;
     const dim3 grid((unsigned)((p.rows + kAppendTokens - 1) / kAppendTokens), (unsigned)batch), block(kAppendThreads);
     const int smem = kAppendTokens * p.half * (int)sizeof(float2);
     if (interleaved) paged_append_kernel<T, E, true><<<grid, block, smem, stream>>>(p);
@@ -197,7 +222,6 @@ extern "C" int tmw_paged_append(const tmw_paged_append_desc* d, void* stream) {
     }
     p.start = d->start; p.counts = d->counts; p.inv_freq = d->inv_freq;
     p.rows = d->rows; p.heads = d->heads; p.half = d->rotated / 2;
-    p.slots = FastDiv((uint32_t)(d->heads + 2 * d->at.kv_heads));
     p.status = device_status_word();
     if (p.status == nullptr) return TMW_ERR_CUDA;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

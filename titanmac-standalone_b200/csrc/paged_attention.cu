@@ -116,6 +116,7 @@ __device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT>&
     // each lane sums up a run of sequences
     const int run = (p.batch + 31) / 32;
     long long mine = 0;
+#pragma unroll 8
     for (int i = 0; i < run; ++i) mine += units(lane * run + i);
     const long long upto = scan(mine), total = __shfl_sync(0xffffffffu, upto, 31);
     Share s;
@@ -665,16 +666,6 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
                           : reinterpret_cast<float*>(smem + w * (ring_bytes + extra));
     };
 
-    // sequences without a key to see, or without a place
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        int lo, pos;
-        bool bad;
-        if (tiles_of<KT>(p, b, lo, pos, bad) > 0) continue;
-        if (bad && tid == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
-        const int heads = p.group * p.map.kv_heads;
-        for (int i = tid; i < heads * dim; i += blockDim.x)
-            static_cast<T*>(p.o)[b * p.os[0] + (i / dim) * p.os[1] + i % dim] = from_f32<T>(bad ? CUDART_NAN_F : 0.f);
-    }
     if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (lane < 2) parts[2 * warp + lane].there = 0;
     __syncwarp();
@@ -807,6 +798,17 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
         if (starts && !ends && tid == 0)
             p.joins[blockIdx.x] = make_int4(part.b, part.item, (int)((part.item_end - 1) / (share.per * share.warps)), 0);
     }
+
+    // sequences without a key to see, or without a place
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        int lo, pos;
+        bool bad;
+        if (tiles_of<KT>(p, b, lo, pos, bad) > 0) continue;
+        if (bad && tid == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+        const int heads = p.group * p.map.kv_heads;
+        for (int i = tid; i < heads * dim; i += blockDim.x)
+            static_cast<T*>(p.o)[b * p.os[0] + (i / dim) * p.os[1] + i % dim] = from_f32<T>(bad ? CUDART_NAN_F : 0.f);
+    }
 }
 
 // The parts of an item that was cut: CTA (c, r) joins row r of the one that begins in CTA c.  Its warps take every
@@ -814,7 +816,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttention p) {
-    __shared__ float warp_max[kJoinWarps], warp_sum[kJoinWarps];
+    __shared__ float2 warp_sums[kJoinWarps];
     __shared__ float outs[kJoinWarps][256];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = p.map.head_dim, r = blockIdx.y;
     pdl_wait();
@@ -824,38 +826,40 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     if (r >= min(p.rows, p.group - first)) return;
     const int n = join.z - (int)blockIdx.x + 1;
     auto slot = [&](int i) { return (2LL * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * p.rows + r; };
-    float m = -CUDART_INF_F;
-    for (int i = tid; i < n; i += kJoinWarps * 32) m = fmaxf(m, __ldcg(p.sums + slot(i)).x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) warp_max[warp] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, warp_max[w]);
-    const float base = m == -CUDART_INF_F ? 0.f : m;
-    float l = 0.f;
+    float m = -CUDART_INF_F, l = 0.f;
     float4 o[2] = {};
 #pragma unroll 4
     for (int i = warp; i < n; i += kJoinWarps) {
         const float2 ml = __ldcg(p.sums + slot(i));
-        const float x = part_weight(ml.x, base);
-        l = fmaf(x, ml.y, l);
         const float* from = p.partial + slot(i) * dim;
+        float4 part[2] = {};
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            if (h * 128 + lane * 4 < dim) add_product(o[h], x, __ldcg(reinterpret_cast<const float4*>(from + h * 128 + lane * 4)));
+            if (h * 128 + lane * 4 < dim) part[h] = __ldcg(reinterpret_cast<const float4*>(from + h * 128 + lane * 4));
+        const float now = fmaxf(m, ml.x), base = now == -CUDART_INF_F ? 0.f : now, keep = part_weight(m, base), w = part_weight(ml.x, base);
+        m = now;
+        l = fmaf(w, ml.y, l * keep);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            o[h].x *= keep; o[h].y *= keep; o[h].z *= keep; o[h].w *= keep;
+            add_product(o[h], w, part[h]);
+        }
     }
-    if (lane == 0) warp_sum[warp] = l;
+    if (lane == 0) warp_sums[warp] = make_float2(m, l);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
         if (h * 128 + lane * 4 < dim) *reinterpret_cast<float4*>(&outs[warp][h * 128 + lane * 4]) = o[h];
     __syncthreads();
     if (tid >= dim) return;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, warp_sums[w].x);
+    const float base = m == -CUDART_INF_F ? 0.f : m;
     float sum = 0.f, out = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) {
-        sum += warp_sum[w];
-        out += outs[w][tid];
+        const float x = part_weight(warp_sums[w].x, base);
+        sum = fmaf(x, warp_sums[w].y, sum);
+        out = fmaf(x, outs[w][tid], out);
     }
     const int head = join.y / p.parts * p.group + first + r;
     static_cast<T*>(p.o)[join.x * p.os[0] + head * p.os[1] + tid] = from_f32<T>(quotient(out, sum));
