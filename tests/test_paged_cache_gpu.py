@@ -67,6 +67,13 @@ def check(got, want, bound):
     ([70, 5], 3, 1, 8, 5, 30, 0),
     ([70, 5], 4, 2, 40, 16, None, 2),                    # a head size of no tile
     ([33, 12], 5, 5, 200, 48, None, 0),
+    ([45, 100], 8, 2, 80, 16, None, 3),
+    ([45, 100], 12, 1, 80, 9, 60, 0),
+    ([45, 100], 3, 1, 192, 32, None, 0),
+    ([70, 45], 20, 1, 192, 16, None, 1),
+    ([70, 45], 2, 2, 144, 16, None, 1),                  # one head on one, wide, of no tile
+    ([70, 45], 5, 1, 24, 16, None, 1),                   # five heads on one, on CUDA cores in every type
+    ([70, 45], 18, 2, 16, 16, 20, 1),
 ])
 def test_attention_against_64_bits(lengths, heads, kv_heads, dh, page, window, n_p, dtype):
     check(*attend(lengths, heads, kv_heads, dh, page, dtype, window, n_p, seed=len(lengths) * dh + page))

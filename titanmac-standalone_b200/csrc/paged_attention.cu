@@ -255,7 +255,7 @@ struct Loader {
 
 // ---- the core on CUDA cores: every type, head_dim a multiple of 8 --------------------------------------------------------
 // Lane l has key l % 16 of a tile and one half of the head's dimensions of its scores; then the four dimensions from 4 l on (and
-// from 128 + 4 l) of the outputs.  kRows query heads, their numbers as fp32 in shared memory.
+// from 128 + 4 l, with QUADS 2) of the outputs.  kRows query heads, their numbers as fp32 in shared memory.
 template <typename T>
 struct SimtLayout {
     int bytes;  // of a row; 16 more keep the rows of 8 lanes off each other's banks
@@ -288,17 +288,15 @@ __device__ __forceinline__ void add_product(float4& acc, float w, const float4& 
     acc.w = fmaf(w, x.w, acc.w);
 }
 
-constexpr int kSimtRows = 4;
-
-template <typename T>
+template <typename T, int ROWS, int QUADS>
 struct SimtCore {
-    static constexpr int kRows = kSimtRows, KT = 16;
+    static constexpr int kRows = ROWS, KT = 16;
     using Layout = SimtLayout<T>;
     const PagedAttention& p;
     float* q;        // [kRows][head_dim], of the CTA's warp
     float* weights;  // [KT][kRows]
     float m[kRows], l[kRows];
-    float4 o[kRows][2];
+    float4 o[kRows][QUADS];
 
     // shared memory of a warp besides its ring
     static __host__ __device__ int extra(int head_dim) { return (kRows * head_dim + KT * kRows) * (int)sizeof(float); }
@@ -321,7 +319,8 @@ struct SimtCore {
         for (int r = 0; r < kRows; ++r) {
             m[r] = -CUDART_INF_F;
             l[r] = 0.f;
-            o[r][0] = o[r][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int h = 0; h < QUADS; ++h) o[r][h] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
     __device__ __forceinline__ void tile(const unsigned char* tile, uint2 marks, const Layout& lay) {
@@ -351,25 +350,31 @@ struct SimtCore {
             w[r] = seen ? exp2f(x - base) : 0.f;
             l[r] = l[r] * keep + w[r];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < QUADS; ++h) {
                 o[r][h].x *= keep; o[r][h].y *= keep; o[r][h].z *= keep; o[r][h].w *= keep;
             }
         }
-        if (lane < KT) *reinterpret_cast<float4*>(weights + key * kRows) = make_float4(w[0], w[1], w[2], w[3]);
+        if (lane < KT) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) weights[key * kRows + r] = w[r];
+        }
         __syncwarp();
         const unsigned char* values = tile + KT * lay.pitch();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < QUADS; ++h) {
             const int i = h * 128 + lane * 4;
             if (i >= dim) break;
 #pragma unroll 4
             for (int j = 0; j < KT; ++j) {
                 const float4 v4 = load4<T>(values + j * lay.pitch() + i * sizeof(T));
-                const float4 w4 = *reinterpret_cast<const float4*>(weights + j * kRows);
-                add_product(o[0][h], w4.x, v4);
-                add_product(o[1][h], w4.y, v4);
-                add_product(o[2][h], w4.z, v4);
-                add_product(o[3][h], w4.w, v4);
+                float wj[kRows];
+#pragma unroll
+                for (int r = 0; r < kRows; r += 4) {
+                    if constexpr (kRows >= 4) *reinterpret_cast<float4*>(wj + r) = *reinterpret_cast<const float4*>(weights + j * kRows + r);
+                    else wj[r] = weights[j * kRows + r];
+                }
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) add_product(o[r][h], wj[r], v4);
             }
         }
         __syncwarp();
@@ -385,7 +390,7 @@ struct SimtCore {
             for (int d = 8; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
             if (r >= rows) continue;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < QUADS; ++h) {
                 const float x[4] = {o[r][h].x, o[r][h].y, o[r][h].z, o[r][h].w};
                 if (h * 128 + lane * 4 < dim) use(r, m[r], t, h * 128 + lane * 4, x);
             }
@@ -393,7 +398,7 @@ struct SimtCore {
     }
 };
 
-// ---- the core on tensor cores: 16-bit types, head_dim 32, 64, 96, 128 or 256 -------------------------------------------------
+// ---- the core on tensor cores: 16-bit types, head_dim 16, 32, 64, 80, 96, 128, 192 or 256 -------------------------------------------------
 // mma.sync with the keys, then the dimensions of the values, as the sixteen rows of a tile and eight query heads as its columns
 // (tcgen05's 64 or 128 rows would wait for as many keys per step, and the step is bound by HBM long before the tensor cores): the
 // scores are K Q^T, their exponentials, turned over eight by eight (movmatrix), are the operand of V^T W^T.  The weights go in as two 16-bit numbers each, a value and what it lacks: one alone would
@@ -403,11 +408,12 @@ struct SimtCore {
 template <int DH>
 struct MmaLayout {
     int bytes;
-    __host__ __device__ static constexpr int pitch() { return DH * 2; }
+    static constexpr bool kTurned = DH / 8 % 4 == 0;
+    __host__ __device__ static constexpr int pitch() { return DH * 2 + (kTurned ? 0 : 16); }
     __host__ __device__ static constexpr int chunks() { return DH / 8; }
-    // a chunk's place in its row keeps eight rows' same chunk on different banks
+    // eight rows' same chunk stands on different banks: by its place in the row, or by rows of an odd number of chunks
     __device__ __forceinline__ static int offset(int r, int c) {
-        const int turn = chunks() % 8 == 0 ? r & 7 : r >> 1 & 3;
+        const int turn = !kTurned ? 0 : chunks() % 8 == 0 ? r & 7 : r >> 1 & 3;
         return r * pitch() + ((c ^ turn) << 4);
     }
 };
@@ -920,6 +926,14 @@ struct Kernel {
     }
 };
 
+// as many query heads at once as a group has, up to four, or eight where a lane has four dimensions of each
+template <typename T, typename F>
+int with_simt(const tmw_paged_attention_desc& d, F&& use) {
+    const int group = d.heads / d.at.kv_heads;
+    if (d.at.head_dim > 128) return group == 1 ? use(Kernel<T, SimtCore<T, 1, 2>, 12, 2>()) : use(Kernel<T, SimtCore<T, 4, 2>, 12, 2>());
+    if (group == 1) return use(Kernel<T, SimtCore<T, 1, 1>, 12, 2>());
+    return group <= 4 ? use(Kernel<T, SimtCore<T, 4, 1>, 12, 2>()) : use(Kernel<T, SimtCore<T, 8, 1>, 12, 2>());
+}
 template <typename T, int DH, typename F>
 int with_mma(const tmw_paged_attention_desc& d, F&& use) {
     constexpr int W = DH >= 128 ? 6 : DH > 64 ? 8 : 12;
@@ -929,19 +943,22 @@ int with_mma(const tmw_paged_attention_desc& d, F&& use) {
 template <typename T, typename F>
 int with_16_bits(const tmw_paged_attention_desc& d, F&& use) {
     switch (d.at.head_dim) {
+        case 16: return with_mma<T, 16>(d, use);
         case 32: return with_mma<T, 32>(d, use);
         case 64: return with_mma<T, 64>(d, use);
+        case 80: return with_mma<T, 80>(d, use);
         case 96: return with_mma<T, 96>(d, use);
         case 128: return with_mma<T, 128>(d, use);
+        case 192: return with_mma<T, 192>(d, use);
         case 256: return with_mma<T, 256>(d, use);
-        default: return use(Kernel<T, SimtCore<T>, 12, 2>());
+        default: return with_simt<T>(d, use);
     }
 }
 
 // `use` with the Kernel that takes the call
 template <typename F>
 int with_kernel(const tmw_paged_attention_desc& d, F&& use) {
-    if (d.at.dtype == TMW_F32) return use(Kernel<float, SimtCore<float>, 12, 2>());
+    if (d.at.dtype == TMW_F32) return with_simt<float>(d, use);
     return d.at.dtype == TMW_BF16 ? with_16_bits<__nv_bfloat16>(d, use) : with_16_bits<__half>(d, use);
 }
 

@@ -297,8 +297,9 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     const Sums of_warp = warp_sums(mine);
     const uint32_t best_order = any ? order_of(best) : 0;
     if (lane == 0) sums[warp] = of_warp;
-    // the r-th best of every warp whose threads all have logits; with less than one such warp, everything fits
-    const int full = min(v_end - v_first, THREADS) / 32;
+    // the r-th best of every warp whose threads all have logits (a warp alone: of as many as have some, if those are enough); with
+    // less than one such warp, everything fits
+    const int n_vectors = v_end - v_first, full = W == 1 ? (n_vectors >= p.top ? 1 : 0) : min(n_vectors, THREADS) / 32;
     if (p.top > 0 && warp < full) {
         uint32_t left = best_order, top = 0;
         for (int r = (p.top + full - 1) / full; r > 0; --r) {
@@ -327,11 +328,14 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
             if (at >= v_end) continue;
             float f[E];
             unpack<T>(x.load(at), f);
+            uint32_t hits = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (!(f[e] >= floor) || !x.has(at, e)) continue;
+            for (int e = 0; e < E; ++e) hits |= (f[e] >= floor ? 1u : 0u) << e;
+            for (; hits != 0; hits &= hits - 1) {
+                const int e = __ffs(hits) - 1;
+                if (!x.has(at, e)) continue;
                 const int n = atomicAdd(&found, 1);
-                if (n < kKeys) keys[n / 32][n % 32] = key_of(order_of(f[e]), (uint32_t)(at * E + e));
+                if (n < kKeys) keys[n / 32][n % 32] = key_of(order_of(to_f32<T>(x.x[at * E + e - x.shift])), (uint32_t)(at * E + e));
             }
         }
         __syncthreads();
@@ -530,17 +534,31 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const _
     }
 }
 
+template <typename T, int W>
+int launch_forward(const Logprobs& p, int ctas, cudaStream_t stream) {
+    TMW_CUDA_TRY(launch_ex(logprobs_kernel<T, W>, dim3((unsigned)p.rows * ctas), dim3(W * 32), 0, stream, false, ctas, p, ctas));
+    return TMW_OK;
+}
 template <typename T>
 int launch_forward(const Logprobs& p, cudaStream_t stream) {
-    // Eight warps to a row, four for short ones.  Few rows: clusters, while every thread of them has a vector or more.
+    // Few rows: eight warps each, and clusters while every thread of them has a vector or more.  With rows enough to keep kWarpsBusy
+    // warps to an SM, a row has fewer warps - no barrier to wait at, more rows at once: 4096 rows of 8000, us, without alternatives 20.7
+    // with one warp and 43 with four - unless a thread's part of it, or what the likely ids make it read again, top / (32 warps) of the
+    // row, became long: 3000 rows of 49999 with 5 ids 98 with two warps, 81 with four, 86 with eight; 4096 of 128000 530 with one
+    // (and the backward), 521 with eight.
+    constexpr int kWarpsBusy = 20, kMostAgain = 2048, kMostOfThread = 64;
     const int vectors = (int)(((long long)p.vocab * sizeof(T) + 15) / 16);
-    const bool narrow = vectors <= 512;
+    int warps = 8;
+    while (warps > 1 && (vectors <= warps * 16 || ((long long)p.rows * (warps / 2) >= (long long)kWarpsBusy * sm_count() &&
+                                                   vectors <= warps * 16 * kMostOfThread &&
+                                                   (long long)p.top * vectors <= (long long)kMostAgain * (warps / 2) * (warps / 2))))
+        warps /= 2;
+    if (warps == 1) return launch_forward<T, 1>(p, 1, stream);
+    if (warps == 2) return launch_forward<T, 2>(p, 1, stream);
+    if (warps == 4) return launch_forward<T, 4>(p, 1, stream);
     int ctas = 1;
     while (ctas < 8 && (long long)p.rows * ctas * 2 <= 4LL * sm_count() && vectors / (ctas * 2) >= 256) ctas *= 2;
-    const dim3 grid((unsigned)p.rows * ctas);
-    if (narrow) TMW_CUDA_TRY(launch_ex(logprobs_kernel<T, 4>, grid, dim3(128), 0, stream, false, ctas, p, ctas));
-    else TMW_CUDA_TRY(launch_ex(logprobs_kernel<T, 8>, grid, dim3(256), 0, stream, false, ctas, p, ctas));
-    return TMW_OK;
+    return launch_forward<T, 8>(p, ctas, stream);
 }
 
 template <typename T>
