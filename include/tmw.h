@@ -495,8 +495,8 @@ TMW_API int tmw_paged_append(const tmw_paged_append_desc* desc, void* stream);
  * Attention of one new token per sequence over its pages: o[b, h] = softmax(q[b, h] kᵀ · scale) v over the persistent keys
  * (k_pers, v_pers: [kv_heads, n_persistent, head_dim] contiguous, shared by the batch) and the sequence's tokens
  * max(0, pos[b] - window) .. pos[b] (window -1: all of them), the new one at pos[b] among them: it has been appended before.
- * q, o: [batch, heads, head_dim] through {batch, head} strides; heads is a multiple of kv_heads, and head h reads the keys of
- * head h / (heads / kv_heads).  pos[b] = -1: a sequence without tokens; it sees the persistent keys, and without these its output
+ * q, o: [batch, heads, head_dim] through {batch, head} strides, not overlapping; heads is a multiple of kv_heads, and head h reads
+ * the keys of head h / (heads / kv_heads).  pos[b] = -1: a sequence without tokens; it sees the persistent keys, and without these its output
  * is zero.  A position or a page outside the table or the pool makes the sequence's output NaN and is reported by
  * tmw_poll_status (TMW_ERR_INVALID_ARGUMENT).
  *

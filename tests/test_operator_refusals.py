@@ -17,7 +17,7 @@ PAGES = dict(dtype=1, batch=2, kv_heads=2, head_dim=64, page_size=16, pages=8, c
              v_pages=FAKE, page_table=FAKE)
 APPEND = dict(PAGES, rows=3, heads=4, rotated=64, interleaved=0, k=FAKE, v=FAKE, q=FAKE, q_out=FAKE,
               **{f"{n}{i}": 64 for n in ("ks", "vs", "qs", "os") for i in range(3)}, start=FAKE, counts=0, inv_freq=FAKE)
-ATTENTION = dict(PAGES, heads=4, n_persistent=1, window=-1, scale=0.0, q=FAKE, k_pers=FAKE, v_pers=FAKE, o=FAKE, qs0=64, qs1=64,
+ATTENTION = dict(PAGES, heads=4, n_persistent=1, window=-1, scale=0.0, q=FAKE, k_pers=FAKE, v_pers=FAKE, o=0x2000, qs0=64, qs1=64,
                  os0=64, os1=64, pos=FAKE)
 LOGPROBS = dict(dtype=1, batch=2, tokens=3, vocab=100, top=4, reserved=0, logits=FAKE, s0=300, s1=100, targets=FAKE, logprobs=FAKE,
                 entropy=FAKE, lse=FAKE, top_logprobs=FAKE, top_ids=FAKE)
@@ -79,7 +79,8 @@ def test_append_refuses(change, status):
 @pytest.mark.parametrize("change,status", PAGES_REFUSED + [
     (dict(heads=3), BAD), (dict(heads=-2), BAD), (dict(n_persistent=-1), BAD), (dict(window=-2), BAD), (dict(scale=-1.0), BAD),
     (dict(scale=float("nan")), BAD), (dict(heads=70000), LARGE), (dict(n_persistent=1 << 25), LARGE), (dict(q=0), BAD), (dict(o=0), BAD),
-    (dict(pos=0), BAD), (dict(k_pers=0), BAD), (dict(v_pers=0x1008), BAD), (dict(q=0x1001), BAD), (dict(qs1=-1), BAD), (dict(os0=-1), BAD)])
+    (dict(pos=0), BAD), (dict(k_pers=0), BAD), (dict(v_pers=0x1008), BAD), (dict(q=0x1001), BAD), (dict(qs1=-1), BAD), (dict(os0=-1), BAD),
+    (dict(o=FAKE), BAD)])
 def test_attention_refuses(change, status):
     lib, desc = _native.lib(), packed(paged_cache._ATTENTION, ATTENTION, **change)
     assert lib.tmw_paged_attention(desc, FAKE, 1 << 30, None) == status

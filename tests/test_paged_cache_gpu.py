@@ -86,6 +86,35 @@ def test_attention_of_many_short_sequences(dtype):
     check(*attend(lengths, 4, 2, 64, 16, dtype, seed=5))
 
 
+def test_attention_of_a_large_batch():
+    """Thousands of sequences: each lane of a warp counts the tiles of many, and most of the line lies in other CTAs."""
+    g = torch.Generator().manual_seed(8)
+    lengths = (torch.randint(0, 9, (5000,), generator=g) * (torch.rand(5000, generator=g) < 0.3)).tolist()
+    lengths[777], lengths[4999] = 3000, 500
+    check(*attend(lengths, 2, 1, 32, 16, BF, seed=6))
+
+
+def test_calls_on_two_streams_at_once():
+    """Different batches on two streams without a wait between them: nothing is shared but the pool."""
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    cases = []
+    for i, lengths in enumerate(([700, 3, 90], [40] * 30)):
+        k, v, table = pr.pool(lengths, 16, 2, 64, BF, i)
+        q = torch.randn(len(lengths), 6, 64, generator=torch.Generator().manual_seed(i)).to(BF)
+        pos = torch.tensor(lengths) - 1
+        cases.append((dev(q, k, v, table) + [pos.to(torch.int32).to(DEV)], pr.attention(q, k, v, table, pos)))
+    torch.cuda.synchronize(DEV)
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(paged_attention(*cases[i][0]))
+    torch.cuda.synchronize(DEV)
+    for results, (_, want) in zip(got, cases):
+        check(results[0], *want)
+        assert all(torch.equal(r, results[0]) for r in results)
+
+
 @pytest.mark.parametrize("dtype,dh,heads", [(BF, 128, 8), (HF, 64, 3), (FF, 64, 2)])
 def test_attention_of_one_long_sequence(dtype, dh, heads):
     """Every CTA has a part of the same item."""
@@ -442,6 +471,7 @@ def test_refusals():
     refused(ValueError, 0, q, k_pers=k_pages[0])
     refused(ValueError, 0, q, k_pers=k_pages[0, :1], v_pers=k_pages[0, :1])
     refused(_native.TmwError, 0, q, scale=-1.0)
+    refused(ValueError, 0, q, out=q)
     with pytest.raises(_native.TmwError):  # head_dim 12
         paged_attention(q[..., :12].contiguous(), k_pages[..., :12].contiguous(), v_pages[..., :12].contiguous(), table, pos)
     k = torch.zeros(2, 2, 3, 64, dtype=BF, device=DEV)

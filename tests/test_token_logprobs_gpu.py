@@ -149,6 +149,32 @@ def test_far_apart_and_large_logits():
     check(x, y, 5)
 
 
+@pytest.mark.parametrize("rows", [1, 100, 700, 4000])
+@pytest.mark.parametrize("V,n_top", [(300, 7), (1030, 32), (5001, 1), (16500, 20), (40000, 32)])
+def test_every_number_of_warps(V, n_top, rows):
+    """One to eight warps to a row, clusters of them, by the number of rows and their length."""
+    if rows * V > 3e7:
+        rows = int(3e7 / V)
+    check(*data((rows,), V, BF, seed=rows), n_top)
+
+
+def test_more_than_2_to_the_31_logits():
+    x = torch.zeros(67200, 32003, dtype=BF, device=DEV)
+    last = data((3,), 32003, BF)[0]
+    x[-3:] = last
+    y = torch.zeros(67200, dtype=torch.int64, device=DEV)
+    y[-3:] = torch.tensor([5, 32002, 77])
+    a = x.requires_grad_(True)
+    out = token_logprobs(a, y, 4)
+    picked, entropy, ids, top, _ = reference(last, y[-3:], 4)
+    assert torch.equal(out.top_ids[-3:], ids) and torch.equal(out.top_ids[:2], torch.arange(4, device=DEV).expand(2, -1))
+    assert ((out.logprobs[-3:].double() - picked).abs() <= allowed(last, picked)).all()
+    (g,) = torch.autograd.grad(out.logprobs[-3:].sum(), a)
+    want = -torch.softmax(last.double(), -1)
+    want[torch.arange(3), y[-3:]] += 1
+    assert ((g[-3:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 5e-5).all() and (g[:67197:999] == 0).all()
+
+
 # ---- gradients ---------------------------------------------------------------------------------------------------------------------
 
 

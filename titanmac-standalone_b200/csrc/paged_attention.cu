@@ -327,6 +327,7 @@ struct SimtCore {
         const int lane = threadIdx.x & 31, key = lane & (KT - 1), dim = p.map.head_dim, half = dim / 2;
         const unsigned char* row = tile + key * lay.pitch();
         float s[kRows] = {};
+#pragma unroll 4
         for (int i = (lane >> 4) * half; i < (lane >> 4) * half + half; i += 4) {
             const float4 k4 = load4<T>(row + i * sizeof(T));
 #pragma unroll
@@ -364,7 +365,7 @@ struct SimtCore {
         for (int h = 0; h < QUADS; ++h) {
             const int i = h * 128 + lane * 4;
             if (i >= dim) break;
-#pragma unroll 4
+#pragma unroll
             for (int j = 0; j < KT; ++j) {
                 const float4 v4 = load4<T>(values + j * lay.pitch() + i * sizeof(T));
                 float wj[kRows];
@@ -997,6 +998,10 @@ extern "C" int tmw_paged_attention(const tmw_paged_attention_desc* d, void* scra
     const int rc = validate(d, used);
     if (rc != TMW_OK || !used) return rc;
     const size_t size = dtype_size(d->at.dtype);
+    if (d->o == d->q) {
+        set_error_text("tmw_paged_attention: o must not be q (other CTAs may still read it)");
+        return TMW_ERR_INVALID_ARGUMENT;
+    }
     if (d->q == nullptr || d->o == nullptr || d->pos == nullptr || scratch == nullptr ||
         (d->n_persistent > 0 && (d->k_pers == nullptr || d->v_pers == nullptr)))
         return TMW_ERR_INVALID_ARGUMENT;

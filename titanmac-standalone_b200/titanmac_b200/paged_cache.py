@@ -132,7 +132,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Attention of the newest token of every sequence, ``q [B, heads, dh]`` at ``pos[b]`` (int32 ``[B]``), whose keys and values
     have been appended: over tokens ``pos - window .. pos`` (None: all up to ``pos``) and the persistent keys
     ``k_pers, v_pers [kv_heads, Np, dh]``.  ``heads`` is a multiple of the pages' ``kv_heads``.  ``pos`` of -1: a sequence without
-    tokens; it sees the persistent keys, and is zero without them."""
+    tokens; it sees the persistent keys, and is zero without them.  ``out`` must not overlap ``q``."""
     index = k_pages.get_device()
     if not 0 <= index == q.get_device() == v_pages.get_device() == page_table.get_device() == pos.get_device():
         _refuse_devices("paged_attention", k_pages, q, v_pages, page_table, pos)
@@ -174,6 +174,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             _refuse_devices("paged_attention", k_pages, out)
         if out.dtype is not dtype:
             raise TypeError("out must have the dtype of the pages")
+        if out.data_ptr() == q.data_ptr() and q.numel():
+            raise ValueError("out must not be q")
     os_ = _strides("out", out, shape)
     if B == 0 or heads == 0:
         return out
