@@ -350,6 +350,18 @@ def _on(device: torch.device):
     return _no_guard if device.index == _raw_device() else torch.cuda.device(device)
 
 
+def launch(index: int, fn, *args) -> None:
+    """``fn(*args, current stream of device index)`` with that device current; raises what its status says.  (The same as ``_on``,
+    ``_stream_ptr`` and ``check`` around the call, in half their time: it counts where a call's kernels take a few microseconds.)"""
+    if _raw_stream is not None and index == _raw_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if status:
+        check(status)
+
+
 def _bhrd_strides(t: torch.Tensor) -> Sequence[int]:
     if t.stride(3) != 1:
         raise ValueError("the head_dim axis must be contiguous")

@@ -51,14 +51,13 @@ def _forward(logits: torch.Tensor, targets: torch.Tensor, n_top: int, with_lse: 
     top_ids = top_logprobs = None
     if n_top:
         top_ids = torch.empty(*shape, n_top, dtype=torch.int64, device=device)
-        top_logprobs = torch.empty(*shape, n_top, dtype=torch.float32, device=device)
+        top_logprobs = torch.empty_like(top_ids, dtype=torch.float32)
     if targets.numel():
         t, batch, tokens, s0, s1 = _rows(logits)
         desc = _DESC.pack(_native._DTYPES[t.dtype], batch, tokens, t.shape[-1], n_top, 0, t.data_ptr(), s0, s1, targets.data_ptr(),
                           logprobs.data_ptr(), entropy.data_ptr(), lse.data_ptr() if with_lse else 0,
                           top_logprobs.data_ptr() if n_top else 0, top_ids.data_ptr() if n_top else 0)
-        with _native._on(device):
-            _native.check(_native.lib().tmw_token_logprobs(desc, _native._stream_ptr(device)))
+        _native.launch(t.get_device(), _native.lib().tmw_token_logprobs, desc)
     return logprobs, entropy, top_ids, top_logprobs, lse
 
 
@@ -84,10 +83,9 @@ class _TokenLogprobs(torch.autograd.Function):
             n_top = 0 if top_ids is None else top_ids.shape[-1]
             desc = _DESC.pack(_native._DTYPES[t.dtype], batch, tokens, t.shape[-1], n_top, 0, t.data_ptr(), s0, s1, targets.data_ptr(),
                               0, entropy.data_ptr(), lse.data_ptr(), 0, top_ids.data_ptr() if n_top else 0)
-            with _native._on(device):
-                _native.check(_native.lib().tmw_token_logprobs_backward(
-                    desc, *[None if g is None else g.data_ptr() for g in given], d_logits.data_ptr(),
-                    _STRIDES.pack(*_rows(d_logits)[3:]), _native._stream_ptr(device)))
+            _native.launch(t.get_device(), _native.lib().tmw_token_logprobs_backward, desc,
+                           *[None if g is None else g.data_ptr() for g in given], d_logits.data_ptr(),
+                           _STRIDES.pack(*_rows(d_logits)[3:]))
         return d_logits, None, None
 
 

@@ -43,14 +43,10 @@ def _page_numbers(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_
     return dtype, shape[1], shape[3], shape[2], shape[0], table[1]
 
 
-def _strides(name: str, t: torch.Tensor, shape):
-    """In front of the last axis, which is contiguous."""
+def _refuse_shape(name: str, t: torch.Tensor, shape) -> None:
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    strides = t.stride()
-    if strides[-1] != 1:
-        raise ValueError("the head_dim axis must be contiguous")
-    return strides[:-1]
+    raise ValueError("the head_dim axis must be contiguous")
 
 
 def _check_numbers(name: str, t: torch.Tensor, batch: int) -> None:
@@ -81,7 +77,11 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         raise ValueError("paged_append: k and v must be [batch, kv_heads, rows, head_dim]")
     B, rows = shape[0], shape[2]
     dtype_number, kv_heads, head_dim, page_size, pages, columns = _page_numbers("paged_append", k_pages, v_pages, page_table, B)
-    ks, vs = _strides("k", k, (B, kv_heads, rows, head_dim)), _strides("v", v, shape)
+    ks, vs = k.stride(), v.stride()
+    if shape[1] != kv_heads or shape[3] != head_dim or ks[3] != 1:
+        _refuse_shape("k", k, (B, kv_heads, rows, head_dim))
+    if v.shape != shape or vs[3] != 1:
+        _refuse_shape("v", v, shape)
     _check_numbers("start", start, B)
     if counts is not None:
         if counts.get_device() != index:
@@ -98,31 +98,33 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         rotated = 2 * inv_freq.shape[0]
         if rotated > head_dim:
             raise ValueError("inv_freq has more than head_dim / 2 numbers")
-    heads, qs, os_ = 0, (0, 0, 0), (0, 0, 0)
+    heads, qs, os_ = 0, (0, 0, 0, 1), (0, 0, 0, 1)
     if q is not None:
         if q.get_device() != index or (q_out is not None and q_out.get_device() != index):
             _refuse_devices("paged_append", k_pages, q, q_out)
         if q.dtype is not dtype or (q_out is not None and q_out.dtype is not dtype):
             raise TypeError("q and q_out must have the dtype of the pages")
-        if q.dim() != 4:
+        q_shape, qs = q.shape, q.stride()
+        if len(q_shape) != 4:
             raise ValueError("q must be [batch, heads, rows, head_dim]")
-        heads = q.shape[1]
-        q_shape = (B, heads, rows, head_dim)
-        qs = _strides("q", q, q_shape)
+        heads = q_shape[1]
+        if q_shape[0] != B or q_shape[2] != rows or q_shape[3] != head_dim or qs[3] != 1:
+            _refuse_shape("q", q, (B, heads, rows, head_dim))
         if q_out is None:
             q_out = torch.empty(B, rows, heads, head_dim, dtype=dtype, device=k_pages.device).permute(0, 2, 1, 3)
-        os_ = _strides("q_out", q_out, q_shape)
+        os_ = q_out.stride()
+        if q_out.shape != q_shape or os_[3] != 1:
+            _refuse_shape("q_out", q_out, q_shape)
     elif q_out is not None:
         raise ValueError("q_out goes with q")
     if B == 0 or rows == 0:
         return q_out
     desc = _APPEND.pack(dtype_number, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0), k_pages.data_ptr(),
                         v_pages.data_ptr(), page_table.data_ptr(), rows, heads, rotated, interleaved, k.data_ptr(), v.data_ptr(),
-                        q.data_ptr() if heads else 0, q_out.data_ptr() if heads else 0, *ks, *vs, *qs, *os_, start.data_ptr(),
+                        q.data_ptr() if heads else 0, q_out.data_ptr() if heads else 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0],
+                        qs[1], qs[2], os_[0], os_[1], os_[2], start.data_ptr(),
                         counts.data_ptr() if counts is not None else 0, inv_freq.data_ptr() if rotated else 0)
-    device = k_pages.device
-    with _native._on(device):
-        _native.check(_native.lib().tmw_paged_append(desc, _native._stream_ptr(device)))
+    _native.launch(index, _native.lib().tmw_paged_append, desc)
     return q_out
 
 
@@ -146,7 +148,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     dtype_number, kv_heads, head_dim, page_size, pages, columns = _page_numbers("paged_attention", k_pages, v_pages, page_table, B)
     if kv_heads == 0 or heads % kv_heads != 0:
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-    qs = _strides("q", q, (B, heads, head_dim))
+    qs = q.stride()
+    if shape[2] != head_dim or qs[2] != 1:
+        _refuse_shape("q", q, (B, heads, head_dim))
     _check_numbers("pos", pos, B)
     if window is None:
         window = -1
@@ -176,19 +180,21 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise TypeError("out must have the dtype of the pages")
         if out.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("out must not be q")
-    os_ = _strides("out", out, shape)
+    os_ = out.stride()
+    if out.shape != shape or os_[2] != 1:
+        _refuse_shape("out", out, shape)
     if B == 0 or heads == 0:
         return out
     desc = _ATTENTION.pack(dtype_number, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0),
                            k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), heads, n_persistent, window, scale,
                            q.data_ptr(), k_pers.data_ptr() if n_persistent else 0, v_pers.data_ptr() if n_persistent else 0,
-                           out.data_ptr(), *qs, *os_, pos.data_ptr())
+                           out.data_ptr(), qs[0], qs[1], os_[0], os_[1], pos.data_ptr())
     lib, device = _native.lib(), k_pages.device
-    with _native._on(device):
+    with _native._on(device):  # (how much depends on the device's SMs)
         nbytes = lib.tmw_paged_attention_scratch_bytes(desc)
-        # of this call alone: calls on two streams, or of two captured graphs, have nothing in common
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _native.check(lib.tmw_paged_attention(desc, scratch.data_ptr() or None, nbytes, _native._stream_ptr(device)))
+    # of this call alone: calls on two streams, or of two captured graphs, have nothing in common
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _native.launch(index, lib.tmw_paged_attention, desc, scratch.data_ptr() or None, nbytes)
     return out
 
 
