@@ -209,6 +209,17 @@ struct Loader {
         if (lane == 0) ring.marks[stage] = make_uint2(seen, lost);
         const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring.tiles) + stage * 2 * KT * lay.pitch();
         const int chunks = lay.chunks();
+        // a lane's chunks, every 32nd one: chunk c of row rr (by steps: chunks is not always a constant)
+        struct Chunk {
+            int rr, c;
+        };
+        const Chunk start{lane / chunks, lane % chunks};
+        auto after = [&](Chunk x) {
+            x.rr += 32 / chunks;
+            x.c += 32 % chunks;
+            if (x.c >= chunks) x.c -= chunks, ++x.rr;
+            return x;
+        };
         if (pers || p.whole_runs) {
 #pragma unroll
             for (int h = 0; h < KT / 16; ++h) {
@@ -217,35 +228,33 @@ struct Loader {
                 const unsigned char *kr = k + off, *vr = v + off;
                 const int n = 16 * chunks;
                 const uint32_t want = seen >> (h * 16) & 0xffffu & ~(lost >> (h * 16));
+                Chunk x = start;
                 if (want == 0xffffu) {
 #pragma unroll
-                    for (int i0 = 0; i0 < n; i0 += 32) {
-                        const int i = i0 + lane, rr = i / chunks;
-                        if (n % 32 != 0 && i >= n) break;
-                        const uint32_t dst = to + lay.offset(h * 16 + rr, i - rr * chunks);
+                    for (int i0 = 0; i0 < n; i0 += 32, x = after(x)) {
+                        if (n % 32 != 0 && x.rr >= 16) break;
+                        const uint32_t dst = to + lay.offset(h * 16 + x.rr, x.c);
                         copy16(dst, kr + i0 * 16, true);
                         copy16(dst + KT * lay.pitch(), vr + i0 * 16, true);
                     }
                 } else {
-                    for (int i0 = 0; i0 < n; i0 += 32) {
-                        const int i = i0 + lane, rr = i / chunks;
-                        if (n % 32 != 0 && i >= n) break;
-                        const uint32_t dst = to + lay.offset(h * 16 + rr, i - rr * chunks);
-                        const bool there = want >> rr & 1;  // (no byte is read where not: any address will do)
+                    for (int i0 = 0; i0 < n; i0 += 32, x = after(x)) {
+                        if (n % 32 != 0 && x.rr >= 16) break;
+                        const uint32_t dst = to + lay.offset(h * 16 + x.rr, x.c);
+                        const bool there = want >> x.rr & 1;  // (no byte is read where not: any address will do)
                         copy16(dst, there ? static_cast<const void*>(kr + i0 * 16) : p.sums, there);
                         copy16(dst + KT * lay.pitch(), there ? static_cast<const void*>(vr + i0 * 16) : p.sums, there);
                     }
                 }
             }
         } else {
-            const int n = KT * chunks;
-            for (int i0 = 0; i0 < n; i0 += 32) {
-                const int i = min(i0 + lane, n - 1), rr = i / chunks, c = i - rr * chunks;
-                const long long at_row = __shfl_sync(0xffffffffu, row, rr);
-                if (i0 + lane >= n) continue;
+            Chunk x = start;
+            for (int i0 = 0; i0 < KT * chunks; i0 += 32, x = after(x)) {
+                const long long at_row = __shfl_sync(0xffffffffu, row, x.rr & (KT - 1));
+                if (x.rr >= KT) continue;
                 const bool there = at_row >= 0;
-                const long long off = at_row * (long long)sizeof(T) + c * 16;
-                const uint32_t dst = to + lay.offset(rr, c);
+                const long long off = at_row * (long long)sizeof(T) + x.c * 16;
+                const uint32_t dst = to + lay.offset(x.rr, x.c);
                 copy16(dst, there ? static_cast<const void*>(k + off) : p.sums, there);
                 copy16(dst + KT * lay.pitch(), there ? static_cast<const void*>(v + off) : p.sums, there);
             }
