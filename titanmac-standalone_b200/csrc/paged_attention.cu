@@ -41,7 +41,7 @@ struct PagedAttention {
     int items;        // of a sequence
     float scale;      // times log2(e)
     int row_bytes;
-    bool q_pairs;  // queries can be read two at a time
+    bool q_pairs, o_pairs;  // queries can be read, outputs stored two at a time
     float* partial;  // [CTA][2][rows][head_dim]: of the item that a CTA begins in, of the one that begins in it
     float2* sums;    // [CTA][2][rows]: maximum, sum
     float* firsts;   // [CTA][warp][rows][head_dim]: what a warp has of the item that its piece begins in
@@ -80,7 +80,7 @@ struct Cursor {
     __device__ __forceinline__ void next_item(const PagedAttention& p) {
         t = 0;
         if (++item < p.items) {
-            head = item / p.parts;
+            head = p.parts == 1 ? item : item / p.parts;
             return;
         }
         item = head = 0;
@@ -157,6 +157,9 @@ __device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT>&
     at.head = at.item / p.parts;
     return s;
 }
+
+// 1 / l, what a sum of weights turns into (the largest score's weight is 1 or more: no sum at all is that of scores of -inf)
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? CUDART_NAN_F : 1.0f / l; }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
@@ -242,6 +245,7 @@ struct Loader {
                         copy16(dst + KT * lay.pitch(), vr + i0 * 16, true);
                     }
                 } else {
+#pragma unroll 4
                     for (int i0 = 0; i0 < n; i0 += 32, x = after(x)) {
                         if (n % 32 != 0 && x.rr >= 16) break;
                         const uint32_t dst = to + lay.offset(h * 16 + x.rr, x.c);
@@ -409,6 +413,14 @@ struct SimtCore {
                 if (h * 128 + lane * 4 < dim) use(r, m[r], t, h * 128 + lane * 4, x);
             }
         }
+    }
+    __device__ __forceinline__ void store(T* to, int rows) {
+        results(rows, [&](int r, float, float sum, int d, const float (&x)[4]) {
+            const float scale = inverse(sum);
+            T* at = to + r * p.os[1] + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) at[e] = from_f32<T>(x[e] * scale);
+        });
     }
 };
 
@@ -650,6 +662,36 @@ struct MmaCore {
                     }
             }
     }
+    // rounded, and turned over eight by eight so that a lane has two neighbouring dimensions of one head
+    __device__ __forceinline__ void store(T* to, int rows) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int h = 0; h < EIGHTS; ++h) {
+            float scale[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float t = l[h][e];
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) t += __shfl_xor_sync(0xffffffffu, t, d);
+                scale[e] = inverse(t);
+            }
+            const int r = h * 8 + lane / 4;
+            T* at = to + r * p.os[1] + lane % 4 * 2;
+#pragma unroll
+            for (int k = 0; k < DH / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t w = turned(pack2<T>(o[h][k][i * 2] * scale[0], o[h][k][i * 2 + 1] * scale[1]));
+                    if (r >= rows) continue;
+                    if (p.o_pairs) {
+                        *reinterpret_cast<uint32_t*>(at + k * 16 + i * 8) = w;
+                    } else {
+                        reinterpret_cast<uint16_t*>(at)[k * 16 + i * 8] = (uint16_t)w;
+                        reinterpret_cast<uint16_t*>(at)[k * 16 + i * 8 + 1] = (uint16_t)(w >> 16);
+                    }
+                }
+        }
+    }
 };
 
 // ---- the line of tiles ------------------------------------------------------------------------------------------------------
@@ -657,9 +699,6 @@ struct MmaCore {
 // weight of a part whose maximum is m under the common one (base: that, or 0 where it is -inf): a part of hidden scores alone
 // holds zeros, or NaN that has to stay
 __device__ __forceinline__ float part_weight(float m, float base) { return m == -CUDART_INF_F ? 1.f : exp2f(m - base); }
-
-// (the largest score's weight is 1 or more: no sum at all is that of scores of -inf)
-__device__ __forceinline__ float quotient(float o, float l) { return l == 0.f ? CUDART_NAN_F : o / l; }
 
 // A warp's part of an item that was cut: of the one that its piece begins in (0), of the one that begins in it (1).
 struct Part {
@@ -751,11 +790,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
             const bool starts = done.t <= kItemCost, ends = end == item_end;
             if (starts && ends) {
                 T* to = static_cast<T*>(p.o) + done.b * p.os[0] + done_head * p.os[1];
-                core.results(done_rows, [&](int r, float, float sum, int d, const auto& x) {
-                    constexpr int N = sizeof(x) / sizeof(float);
-#pragma unroll
-                    for (int e = 0; e < N; ++e) to[r * p.os[1] + d + e] = from_f32<T>(quotient(x[e], sum));
-                });
+                core.store(to, done_rows);
             } else {
                 const int which = starts ? 1 : 0;
                 __syncwarp();
@@ -805,10 +840,11 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
             }
             if (starts && ends) {
                 T* to = static_cast<T*>(p.o) + part.b * p.os[0] + (head + r) * p.os[1] + (x * 4 - r * dim);
-                to[0] = from_f32<T>(quotient(o.x, l));
-                to[1] = from_f32<T>(quotient(o.y, l));
-                to[2] = from_f32<T>(quotient(o.z, l));
-                to[3] = from_f32<T>(quotient(o.w, l));
+                const float scale = inverse(l);
+                to[0] = from_f32<T>(o.x * scale);
+                to[1] = from_f32<T>(o.y * scale);
+                to[2] = from_f32<T>(o.z * scale);
+                to[3] = from_f32<T>(o.w * scale);
             } else {
                 reinterpret_cast<float4*>(p.partial + slot * dim)[x] = o;
                 if (x * 4 == r * dim) p.sums[slot + r] = make_float2(m, l);
@@ -890,11 +926,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
         sum = fmaf(x, warp_sums[w].y, sum);
         add_product(out, x, outs[w][lane]);
     }
+    const float scale = inverse(sum);
     T* to = static_cast<T*>(p.o) + join.x * p.os[0] + (join.y / p.parts * p.group + first + r) * p.os[1] + d;
-    to[0] = from_f32<T>(quotient(out.x, sum));
-    to[1] = from_f32<T>(quotient(out.y, sum));
-    to[2] = from_f32<T>(quotient(out.z, sum));
-    to[3] = from_f32<T>(quotient(out.w, sum));
+    to[0] = from_f32<T>(out.x * scale);
+    to[1] = from_f32<T>(out.y * scale);
+    to[2] = from_f32<T>(out.z * scale);
+    to[3] = from_f32<T>(out.w * scale);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -1052,6 +1089,7 @@ extern "C" int tmw_paged_attention(const tmw_paged_attention_desc* d, void* scra
     p.scale = (d->scale > 0.f ? d->scale : 1.0f / sqrtf((float)d->at.head_dim)) * 1.4426950408889634f;
     p.row_bytes = d->at.head_dim * (int)size;
     p.q_pairs = bits(d->q) % 4 == 0 && (d->q_stride[0] | d->q_stride[1]) % 2 == 0;
+    p.o_pairs = bits(d->o) % 4 == 0 && (d->o_stride[0] | d->o_stride[1]) % 2 == 0;
     p.status = device_status_word();
     if (p.status == nullptr) return TMW_ERR_CUDA;
     return with_kernel(*d, [&](auto kernel) {

@@ -7,6 +7,8 @@ graph); entries that no token needs may hold anything.  Sequences may share page
 without a sequence (``start`` / ``pos`` of -1), query heads may share key heads, and keys and queries can be rotated by their
 positions on the way into the cache.
 
+Serving only: no gradient flows through these calls.
+
 What the device finds wrong - a position or a page outside the table or the pool - makes NaN of what depends on it, touches nothing
 else and is raised by ``_native.poll_status``.
 """
