@@ -13,9 +13,8 @@
 // done; what was cut between CTAs goes to scratch memory, and a second kernel, launched under the first, joins it in the order of
 // the CTAs.
 //
-// bf16, 545,000 tokens of 12 sequences, 32 heads of 128 on 4: 185 us, 6.1 TB/s (one CTA per piece of fixed length would have left
-// the shorter sequences' SMs idle; warps of a CTA on neighbouring tiles, joined at every item's end: 192).  48 sequences of 1 to
-// 16384 tokens, 32 heads on 8: 118 us, 5.8 TB/s (joined at every item's end: 202).
+// bf16, 545,000 tokens of 12 sequences, 32 heads of 128 on 4: 187 us, 6.1 TB/s (warps of a CTA on neighbouring tiles, joined at every
+// item's end: 192).  48 sequences of 1 to 16384 tokens, 32 heads on 8, fp16: 118 us, 5.8 TB/s (joined at every item's end: 202).
 #include <math_constants.h>
 
 #include <type_traits>
@@ -34,14 +33,14 @@ struct PagedAttention {
     long long qs[2], os[2];
     const int32_t* pos;
     int batch, np, window;
-    int pers_tiles;    // of the persistent keys
-    bool whole_runs;   // sixteen tokens from a multiple of sixteen on lie in one page
-    int group;        // query heads of a key head
-    int rows, parts;  // query heads of an item at most; items of a key head
-    int items;        // of a sequence
-    float scale;      // times log2(e)
-    int row_bytes;
+    int pers_tiles;         // of the persistent keys
+    bool whole_runs;        // sixteen tokens from a multiple of sixteen on lie in one page
     bool q_pairs, o_pairs;  // queries can be read, outputs stored two at a time
+    int group;              // query heads of a key head
+    int rows, parts;        // query heads of an item at most; items of a key head
+    int items;              // of a sequence
+    float scale;            // times log2(e)
+    int row_bytes;
     float* partial;  // [CTA][2][rows][head_dim]: of the item that a CTA begins in, of the one that begins in it
     float2* sums;    // [CTA][2][rows]: maximum, sum
     float* firsts;   // [CTA][warp][rows][head_dim]: what a warp has of the item that its piece begins in
