@@ -33,16 +33,16 @@ def _refuse_devices(name: str, like: torch.Tensor, *tensors: Optional[torch.Tens
 
 
 def _page_numbers(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, batch: int):
-    """``(dtype number, kv_heads, head_dim, page_size, pages, columns)`` of a pool and its table."""
-    shape, table = k_pages.shape, page_table.shape
+    """``(dtype number, kv_heads, head_dim, page_size, pages, columns, row stride of the table)`` of a pool and its table."""
+    shape, table, strides = k_pages.shape, page_table.shape, page_table.stride()
     if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise ValueError(f"{name}: k_pages and v_pages must be contiguous [pages, kv_heads, page_size, head_dim]")
-    if len(table) != 2 or table[0] != batch or (table[1] > 1 and page_table.stride(1) != 1):
+    if len(table) != 2 or table[0] != batch or (strides[1] != 1 and table[1] > 1):
         raise ValueError(f"{name}: page_table must be [batch, columns] with contiguous rows")
     dtype = _native._DTYPES.get(k_pages.dtype)
     if dtype is None:
         raise TypeError(f"{name}: pages in float32, bfloat16 or float16 expected")
-    return dtype, shape[1], shape[3], shape[2], shape[0], table[1]
+    return dtype, shape[1], shape[3], shape[2], shape[0], table[1], strides[0]
 
 
 def _refuse_shape(name: str, t: torch.Tensor, shape) -> None:
@@ -78,7 +78,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if len(shape) != 4:
         raise ValueError("paged_append: k and v must be [batch, kv_heads, rows, head_dim]")
     B, rows = shape[0], shape[2]
-    dtype_number, kv_heads, head_dim, page_size, pages, columns = _page_numbers("paged_append", k_pages, v_pages, page_table, B)
+    number, kv_heads, head_dim, page_size, pages, columns, table_stride = _page_numbers("paged_append", k_pages, v_pages, page_table,
+                                                                                        B)
     ks, vs = k.stride(), v.stride()
     if shape[1] != kv_heads or shape[3] != head_dim or ks[3] != 1:
         _refuse_shape("k", k, (B, kv_heads, rows, head_dim))
@@ -121,7 +122,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         raise ValueError("q_out goes with q")
     if B == 0 or rows == 0:
         return q_out
-    desc = _APPEND.pack(dtype_number, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0), k_pages.data_ptr(),
+    desc = _APPEND.pack(number, B, kv_heads, head_dim, page_size, pages, columns, 0, table_stride, k_pages.data_ptr(),
                         v_pages.data_ptr(), page_table.data_ptr(), rows, heads, rotated, interleaved, k.data_ptr(), v.data_ptr(),
                         q.data_ptr() if heads else 0, q_out.data_ptr() if heads else 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0],
                         qs[1], qs[2], os_[0], os_[1], os_[2], start.data_ptr(),
@@ -147,7 +148,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if len(shape) != 3:
         raise ValueError("paged_attention: q must be [batch, heads, head_dim]")
     B, heads, _ = shape
-    dtype_number, kv_heads, head_dim, page_size, pages, columns = _page_numbers("paged_attention", k_pages, v_pages, page_table, B)
+    number, kv_heads, head_dim, page_size, pages, columns, table_stride = _page_numbers("paged_attention", k_pages, v_pages, page_table,
+                                                                                        B)
     if kv_heads == 0 or heads % kv_heads != 0:
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
     qs = q.stride()
@@ -187,7 +189,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _refuse_shape("out", out, shape)
     if B == 0 or heads == 0:
         return out
-    desc = _ATTENTION.pack(dtype_number, B, kv_heads, head_dim, page_size, pages, columns, 0, page_table.stride(0),
+    desc = _ATTENTION.pack(number, B, kv_heads, head_dim, page_size, pages, columns, 0, table_stride,
                            k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), heads, n_persistent, window, scale,
                            q.data_ptr(), k_pers.data_ptr() if n_persistent else 0, v_pers.data_ptr() if n_persistent else 0,
                            out.data_ptr(), qs[0], qs[1], os_[0], os_[1], pos.data_ptr())
