@@ -449,7 +449,8 @@ TMW_API int tmw_cross_entropy(int32_t dtype, int32_t batch, int32_t tokens, int3
  * k_pages, v_pages : [pages, kv_heads, page_size, head_dim] contiguous, on a 16-byte boundary.
  * page_table       : [batch, columns] int32 (device), rows table_stride elements apart: token t of sequence b lives in slot
  *                    t % page_size of page page_table[b][t / page_size].  Entries that no token of a call needs are not read.
- * Sequences may share pages that no call writes.  head_dim: a multiple of 8, at most 256.  columns * page_size < 2^31.
+ * Sequences may share pages that no call writes.  head_dim: a multiple of 8, at most 256; batch, kv_heads and a call's heads: at
+ * most 65535; columns * page_size < 2^31.
  */
 typedef struct tmw_pages {
     int32_t dtype; /* tmw_dtype of the pages and of every q, k, v and o that goes with them */
