@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import paged_reference as pr
-from titanmac_b200 import PagedCache, TitanMAC, TitanMACConfig, _native, paged_append, paged_attention
+from titanmac_b200 import PagedCache, TitanMAC, TitanMACConfig, _native, paged_append, paged_attention, token_logprobs
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -406,6 +406,49 @@ def test_model_decodes_from_pages():
         both = model.decode_step(token, torch.tensor([70, 70], dtype=torch.int32, device=DEV), paged)
         assert torch.equal(alone[0], both[0])
     _native.poll_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", [FF, BF])
+def test_serving_loop_says_what_the_whole_sequence_says(dtype):
+    """Prompt into pages, then token by token: append, attend, logits, log-probabilities with alternatives - against
+    TitanMAC.token_logprobs of the finished sequences."""
+    cfg = TitanMACConfig(vocab_size=96, d_model=128, n_heads=2, n_layers=2, d_ff=256, max_seq_len=64, window_size=16, n_persistent=3,
+                         use_block_sparse=False)
+    torch.manual_seed(2)
+    model = TitanMAC(cfg).to(device=DEV, dtype=dtype).eval()
+    B, T, new = 3, 21, 12
+    ids = torch.randint(0, 96, (B, T), device=DEV)
+    table = torch.randperm(B * 5, device=DEV).view(B, 5).to(torch.int32)
+    with torch.no_grad():
+        logits, caches = model.prefill(ids, model.new_paged_caches(table, B * 5, 7, dtype))
+        said, entropies = [], []
+        for i in range(new):
+            token = logits.argmax(-1)
+            out = token_logprobs(logits, token, n_top=4)
+            assert torch.equal(out.top_ids[:, 0], token) and torch.equal(out.top_logprobs[:, 0], out.logprobs)
+            said.append(out.logprobs), entropies.append(out.entropy)
+            ids = torch.cat((ids, token[:, None]), 1)
+            logits = model.decode_step(token, torch.full((B,), T + i, dtype=torch.int32, device=DEV), caches)
+        whole = model.token_logprobs(ids)
+    _native.poll_status(DEV)
+    # fp32: sums of some hundred terms in another order, twice over.  bf16: some 24 roundings of half a step on a token's way
+    # through two layers, of logits below 2, and as many again on the other side
+    most = 2e-5 if dtype == FF else 2 * 24 * 2.0 ** -8 * 2.0
+    for got, want in ((said, whole.logprobs), (entropies, whole.entropy)):
+        assert (torch.stack(got, 1) - want[:, T - 1:T - 1 + new]).abs().max() <= most
+
+
+def test_filling_in_pieces():
+    """A prompt in two pieces at any place is the prompt at once."""
+    k, v = (torch.randn(2, 2, 50, 64, device=DEV).to(BF) for _ in range(2))
+    table = torch.randperm(8, device=DEV).view(2, 4).to(torch.int32)
+    caches = [PagedCache(table, 8, 13, 2, 64, None, 0, BF, inv_freq=(10.0 ** -torch.linspace(0, 4, 32)).to(DEV)) for _ in range(2)]
+    caches[0].fill(k, v)
+    caches[1].fill(k[:, :, 29:], v[:, :, 29:], t0=29)
+    caches[1].fill(k[:, :, :29], v[:, :, :29])
+    assert torch.equal(caches[0].k_pages, caches[1].k_pages) and torch.equal(caches[0].v_pages, caches[1].v_pages)
+    with pytest.raises(ValueError):
+        caches[0].fill(k, v, t0=-1)
 
 
 def test_two_captured_steps_replay_together():
