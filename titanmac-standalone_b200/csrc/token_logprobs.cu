@@ -438,13 +438,19 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const _
     const int shift = VEC ? x.shift : 0, n = VEC ? x.vectors : p.f.vocab;
     const int first = blockIdx.y * (kBackThreads * kBackVectors), end = min(first + kBackThreads * kBackVectors, n);
 
+    // this thread's vectors, every kBackThreads-th one of the CTA's; the row's first and last may be there in part and go by
+    // themselves
+    const int count = first + tid < end ? (end - first - tid + kBackThreads - 1) / kBackThreads : 0;
+    int from = 0, to = count;  // the whole ones
+    if (VEC && count > 0) {
+        if (!x.whole(first + tid)) from = 1;
+        if (!x.whole(first + tid + (count - 1) * kBackThreads)) to = count - 1;
+    }
     // the first logits are on their way while the row's numbers are, and then AHEAD vectors always
+    const uint4* in = reinterpret_cast<const uint4*>(x.x - x.shift) + first + tid;
     uint4 raw[AHEAD];
     auto fetch = [&](int i) {
-        const int v = first + tid + i * kBackThreads;
-        if (v >= end) return;
-        if (VEC) raw[i % AHEAD] = x.load(v);
-        else *reinterpret_cast<T*>(&raw[i % AHEAD]) = x.x[v];
+        if (VEC && i >= from && i < to) raw[i % AHEAD] = in[i * kBackThreads];
     };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) fetch(i);
@@ -484,55 +490,52 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const _
         }
         ptx::unpack2(ptx::mul2(ptx::pack2(ex2_ftz(ea), ex2_ftz(eb)), c), ra, rb);
     };
-    const int y_vector = y >= 0 && y < p.f.vocab ? (int)((y + shift) / E) : -1, y_element = (int)((y + shift) % E);
-
+    auto one = [&](int v, int e) {  // an element by itself
+        const int i = v * E + e - shift;
+        if (VEC && !x.has(v, e)) return;
+        d[i] = from_f32<T>(none ? 0.f : gradient(to_f32<T>(x.x[i])));
+    };
+    if constexpr (VEC) {
+        uint4* out = reinterpret_cast<uint4*>(d - shift) + first + tid;
 #pragma unroll
-    for (int i = 0; i < kBackVectors; ++i) {
-        const int v = first + tid + i * kBackThreads;
-        if (v >= end) break;
-        const uint4 now = raw[i % AHEAD];
-        if (i + AHEAD < kBackVectors) fetch(i + AHEAD);
-        float f[E];
-        if (none) {
+        for (int i = 0; i < kBackVectors; ++i) {
+            if (i >= to) break;
+            const uint4 now = raw[i % AHEAD];
+            if (i + AHEAD < kBackVectors) fetch(i + AHEAD);
+            if (i < from) continue;
+            float f[E];
+            unpack<T>(now, f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = 0.f;
-        } else {
-            if constexpr (VEC) {
-                unpack<T>(now, f);
-#pragma unroll
-                for (int e = 0; e < E; e += 2) gradients(f[e], f[e + 1], f[e], f[e + 1]);
-            } else {
-                f[0] = gradient(to_f32<T>(*reinterpret_cast<const T*>(&now)));
-            }
-            if (v == y_vector) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e == y_element) f[e] += g;
-            }
+            for (int e = 0; e < E; e += 2) gradients(f[e], f[e + 1], f[e], f[e + 1]);
+            uint4 result;
+            pack<T>(f, result);
+            out[i * kBackThreads] = none ? make_uint4(0, 0, 0, 0) : result;
         }
-        if constexpr (VEC) {
-            uint4 out;
-            pack<T>(f, out);
-            if (x.whole(v)) {
-                *reinterpret_cast<uint4*>(d + (long long)v * E - shift) = out;
-            } else {
+        if (from > 0) {
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (x.has(v, e)) d[v * E + e - shift] = reinterpret_cast<const T*>(&out)[e];
-            }
-        } else {
-            d[v] = from_f32<T>(f[0]);
+            for (int e = 0; e < E; ++e) one(first + tid, e);
         }
+        if (to < count && count - 1 >= from) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) one(first + tid + (count - 1) * kBackThreads, e);
+        }
+    } else {
+        for (int i = 0; i < count; ++i) one(first + tid + i * kBackThreads, 0);
     }
-    if (top == 0 || none) return;
-    __syncthreads();  // the likely ids' own gradients, over what the pass has written
-    if (tid < top) {
-        const long long id = p.f.top_ids[(long long)row * top + tid];
-        if (id < 0 || (id + shift) / E < first || (id + shift) / E >= end) return;
-        float r = gradient(to_f32<T>(x.x[id])) + p.d_top[(long long)row * top + tid];
-        if (id == y) r += g;
-        d[id] = from_f32<T>(r);
+    if (none) return;
+    __syncthreads();  // over what the pass has written: the target and the likely ids, whose gradients are more
+    if (tid >= 32) return;
+    long long id = tid < top ? p.f.top_ids[(long long)row * top + tid] : -1;
+    float more = tid < top ? p.d_top[(long long)row * top + tid] : 0.f;
+    if (id == y && id >= 0) more += g;
+    if (!__any_sync(0xffffffffu, id == y && id >= 0)) {  // a lane without a likely id takes the target; else the last one, in turn
+        const bool spare = top < 32 ? tid == top : tid == 31;
+        if (spare && top < 32) id = y, more = g;
+        if (spare && top == 32 && y >= 0 && y < p.f.vocab && (y + shift) / E >= first && (y + shift) / E < end)
+            d[y] = from_f32<T>(gradient(to_f32<T>(x.x[y])) + g);
     }
+    if (id < 0 || id >= p.f.vocab || (id + shift) / E < first || (id + shift) / E >= end) return;
+    d[id] = from_f32<T>(gradient(to_f32<T>(x.x[id])) + more);
 }
 
 template <typename T, int W>
