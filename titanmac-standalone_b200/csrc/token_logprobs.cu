@@ -6,7 +6,7 @@
 // The gradient, for the gradients g of log p_t, h of H and a_j of the log-probability of the j-th likely id i_j:
 //   dx_i = g [i = t] + sum_j a_j [i = i_j] - p_i (g + sum_j a_j + h (log p_i + H)).
 // Both are bound by HBM: the logits once, and once more with their gradient on the way back (bf16, 4096 rows of 128000: 178 us, 5.9
-// TB/s, with the exponentials at 73 % of their pipe; 337 us, 6.2 TB/s).
+// TB/s, with the exponentials at 73 % of their pipe; 319 us, 6.6 TB/s).
 //
 // The most likely ids, the lower one first among equals: if every warp knows r logits, of different threads, at or above a bound,
 // and r times the warps is k, then the k best of the row are at or above the bound.  The pass leaves every thread's best, so the
