@@ -1,5 +1,7 @@
 """Token log-probabilities, entropy and alternatives against 64 bits, and their gradients against the formula and differences."""
 
+import math
+
 import pytest
 import torch
 
@@ -173,6 +175,21 @@ def test_more_than_2_to_the_31_logits():
     want = -torch.softmax(last.double(), -1)
     want[torch.arange(3), y[-3:]] += 1
     assert ((g[-3:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 5e-5).all() and (g[:67197:999] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, FF])
+@pytest.mark.parametrize("rows,V", [((5,), 60), ((3,), 40000), ((1,), 128000), ((2000,), 900), ((900,), 5000)])
+def test_tokens_that_are_nearly_certain(rows, V, dtype):
+    """Log-probabilities and entropies of almost nothing, to their own size: ln(1 + rest) with the rest summed up by itself, weights to
+    2^-22 and their arguments, below 100, to 2^-23 of themselves, chains of at most 512 sums.  (The 64-bit reference sums V weights
+    up next to 1, each sum off by 2^-53 at most: V 2^-53 is what its own logarithm may be off by.)"""
+    x, y = data(rows, V, dtype, seed=3, spread=2.0)
+    ahead = torch.linspace(8.0, 20.0, x.shape[0], device=DEV) + math.log(V)
+    x.scatter_(1, y[:, None], (x.float().amax(-1) + ahead).to(dtype)[:, None])
+    got, (picked, entropy, _, _, _) = run(x, y), reference(x, y, 1)
+    most = 100 * 2.0 ** -23 + 512 * 2.0 ** -24 + 2.0 ** -21
+    assert ((got.logprobs.double() - picked).abs() <= most * picked.abs() + V * 2.0 ** -53).all(), ((got.logprobs.double() / picked) - 1).abs().max()
+    assert ((got.entropy.double() - entropy).abs() <= 2 * most * entropy + V * 2.0 ** -53).all(), ((got.entropy.double() / entropy) - 1).abs().max()
 
 
 # ---- gradients ---------------------------------------------------------------------------------------------------------------------

@@ -193,7 +193,7 @@ __device__ __forceinline__ Sums warp_sums(Sums a) {
     return a;
 }
 
-constexpr float kSlack = 30.f;  // e^30 times the vocabulary's largest size is far from an fp32 number's end
+constexpr float kSlack = 8.f;  // (each unit is one of 2^-23 on the entropy, where the sums are brought under the largest logit)
 constexpr int kKeys = 256;  // that are ranked by counting
 
 template <typename T, int W>
@@ -201,12 +201,14 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     constexpr int THREADS = W * 32, E = RowView<T>::E, AHEAD = 4;
     __shared__ Sums sums[W];
     __shared__ uint32_t low[W];
-    __shared__ Sums part;  // this CTA's
+    __shared__ Sums part;   // this CTA's
+    __shared__ float rest;  // S without the largest logit's own 1
     __shared__ __align__(16) uint64_t keys[kKeys / 32][32];
     __shared__ uint64_t tops[kMostTop];  // the likely ids' keys in order
     __shared__ int found;
     __shared__ unsigned char chosen[W][32];
     __shared__ Sums whole_row;
+    __shared__ float whole_rest;
     namespace cg = cooperative_groups;
     const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const RowView<T> x(row_of(p, row, sizeof(T)), p.vocab);
@@ -312,7 +314,10 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     __syncthreads();
     if (warp == 0) {
         const Sums all = warp_sums(lane < W ? sums[lane] : Sums{-FLT_MAX, 0.f, 0.f});
-        if (lane == 0) part = all;
+        if (lane == 0) {
+            part = all;
+            rest = all.s - 1.f;
+        }
     }
 
     if (p.top > 0) {
@@ -372,13 +377,57 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
     }
     __syncthreads();
 
+    // A row whose largest logit has nearly all of it: ln S = ln(1 + rest) is as exact as the rest is, and in fp32 a sum that holds the 1
+    // would leave a rest of 2^-10 with 14 bits.  The one thread that has that logit leaves its sums to its warp, without it.
+    if (part.s >= 1.f && part.s < 1.f + 1.f / 64) {
+        const bool has_largest = any && best == part.m;
+        Sums others = mine;
+        raise(others, part.m);
+        if (has_largest) others.s = others.t = 0.f;
+        const uint32_t owner = __ballot_sync(0xffffffffu, has_largest);
+        for (int at = v_first + warp * 32 + __ffs(owner) - 1 + lane * THREADS; owner != 0 && at < v_end; at += 32 * THREADS) {
+            float f[E];
+            unpack<T>(x.load(at), f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = (f[e] - part.m) * kLog2e, w = f[e] < part.m ? ex2_ftz(d) : 0.f;
+                others.s += w;
+                others.t = fmaf(w, bounded(d), others.t);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            others.s += __shfl_xor_sync(0xffffffffu, others.s, o);
+            others.t += __shfl_xor_sync(0xffffffffu, others.t, o);
+        }
+        if (lane == 0) sums[warp] = others;
+        __syncthreads();
+        if (tid == 0) {
+            rest = part.t = 0.f;
+            for (int w = 0; w < W; ++w) {
+                rest += sums[w].s;
+                part.t += sums[w].t;
+            }
+        }
+        __syncthreads();
+    }
+
     if (ctas > 1) {  // the first CTA of the cluster takes the others' parts
         auto cluster = cg::this_cluster();
         cluster.sync();
         if (rank == 0) {
             if (warp == 0) {
-                const Sums all = warp_sums(lane < ctas ? *cluster.map_shared_rank(&part, lane) : Sums{-FLT_MAX, 0.f, 0.f});
-                if (lane == 0) whole_row = all;
+                const Sums its = lane < ctas ? *cluster.map_shared_rank(&part, lane) : Sums{-FLT_MAX, 0.f, 0.f}, all = warp_sums(its);
+                // the rest: of the first part with the largest logit, and all of the others
+                const int owner = __ffs(__ballot_sync(0xffffffffu, its.m == all.m)) - 1;
+                float others = its.s * ex2_ftz((its.m - all.m) * kLog2e);
+                if (lane == owner) others = *cluster.map_shared_rank(&rest, lane);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
+                if (lane == 0) {
+                    whole_row = all;
+                    whole_rest = others;
+                }
             }
             if (p.top > 0) {
                 for (int c = warp; c < ctas; c += W) keys[c][lane] = cluster.map_shared_rank(tops, c)[lane];
@@ -390,12 +439,13 @@ __global__ void __launch_bounds__(W * 32, 32 / W) logprobs_kernel(const __grid_c
         if (rank != 0) return;
     } else if (tid == 0) {
         whole_row = part;
+        whole_rest = rest;
     }
     __syncthreads();
 
     const Sums all = whole_row;
     const bool fine = all.s > 0.f;  // (NaN: a NaN or +inf among the logits; 0: nothing but -inf)
-    const float log_sum = logf(all.s);
+    const float log_sum = log1pf(whole_rest);
     if (tid == 0) {
         float lp = CUDART_NAN_F;
         if (y == kNoTarget) lp = 0.f;
