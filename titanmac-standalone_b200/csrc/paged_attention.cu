@@ -426,10 +426,11 @@ struct SimtCore {
 // ---- the core on tensor cores: 16-bit types, head_dim 16, 32, 64, 80, 96, 128, 192 or 256 -------------------------------------------------
 // mma.sync with the keys, then the dimensions of the values, as the sixteen rows of a tile and eight query heads as its columns
 // (tcgen05's 64 or 128 rows would wait for as many keys per step, and the step is bound by HBM long before the tensor cores): the
-// scores are K Q^T, their exponentials, turned over eight by eight (movmatrix), are the operand of V^T W^T.  The weights go in as two 16-bit numbers each, a value and what it lacks: one alone would
-// put up to 2^-9 of itself on the output, the two 2^-16.  (The first is cut off and the second is never zero: both positive,
-// they take an infinite value to infinity, as the weight itself would.)  In fp16 they are raised by 2^12, as far as the largest allows, so
-// that those below 2^-14 of it keep their bits.  Up to eight heads: the tile's upper eight rows are zeros and have no registers.
+// scores are K Q^T, their exponentials, turned over eight by eight (movmatrix), are the operand of V^T W^T.  A weight goes in as several
+// 16-bit numbers that add up to it - three in bf16, all 24 bits; two in fp16, 22 bits, what the exponential itself has -: one alone
+// would put up to 2^-8 of itself on the output, two in bf16 2^-16, which shows where values cancel.  In fp16 they are raised by 2^12, as far as
+// the largest allows, so that those below 2^-14 of it keep their bits.  Up to eight heads: the tile's upper eight rows are zeros and have
+// no registers.
 template <int DH>
 struct MmaLayout {
     int bytes;
@@ -479,21 +480,6 @@ __device__ __forceinline__ uint32_t cut2<__half>(float a, float b) {
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
     return w;
 }
-// no number below the smallest that a product takes (2^-126, 2^-24)
-template <typename T>
-__device__ __forceinline__ uint32_t positive2(uint32_t w);
-template <>
-__device__ __forceinline__ uint32_t positive2<__nv_bfloat16>(uint32_t w) {
-    const uint32_t least = 0x00800080u;
-    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&least));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t positive2<__half>(uint32_t w) {
-    const uint32_t least = 0x00010001u;
-    const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&least));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <>
@@ -502,6 +488,36 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 }
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// Two weights as so many 16-bit numbers each: a weight cut off, what that lacks, cut off too but for the last one.  None of them is
+// below the smallest number that a product takes (2^-126, 2^-24), so that an infinite value stays one; a weight of nothing is nothing
+// in bf16.
+constexpr int kMostTerms = 3;
+template <typename T>
+constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 3;
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&terms)[kMostTerms]);
+template <>
+__device__ __forceinline__ void split2<__nv_bfloat16>(float a, float b, uint32_t (&terms)[kMostTerms]) {
+    const auto as_pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const auto bits = [](__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); };
+    terms[0] = cut2<__nv_bfloat16>(a, b);
+    const __nv_bfloat162 least = __hmin2(as_pair(terms[0]), as_pair(0x00800080u));
+    const float2 first = unpack2<__nv_bfloat16>(terms[0]);
+    a -= first.x, b -= first.y;
+    terms[1] = bits(__hmax2(as_pair(cut2<__nv_bfloat16>(a, b)), least));
+    const float2 second = unpack2<__nv_bfloat16>(terms[1]);
+    terms[2] = bits(__hmax2(as_pair(pack2<__nv_bfloat16>(a - second.x, b - second.y)), least));
+}
+template <>
+__device__ __forceinline__ void split2<__half>(float a, float b, uint32_t (&terms)[kMostTerms]) {
+    const uint32_t least = 0x00010001u;
+    terms[0] = cut2<__half>(a, b);
+    const float2 first = unpack2<__half>(terms[0]);
+    const uint32_t rest = pack2<__half>(a - first.x, b - first.y);
+    const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&rest), *reinterpret_cast<const __half2*>(&least));
+    terms[1] = *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // an 8 x 8 matrix of 16-bit numbers, two of a row to a lane, with rows and columns exchanged
 __device__ __forceinline__ uint32_t turned(uint32_t w) {
@@ -574,7 +590,7 @@ struct MmaCore {
 #pragma unroll
                 for (int h = 0; h < EIGHTS; ++h) mma_16816<T>(s[h][g], a[0], a[1], a[2], a[3], q[h][k][0], q[h][k][1]);
             }
-        uint32_t hi[EIGHTS][KT / 16][2], lo[EIGHTS][KT / 16][2];
+        uint32_t weights[EIGHTS][KT / 16][2][kMostTerms];
         float keep[EIGHTS][2];
         bool moved = false;
 #pragma unroll
@@ -613,10 +629,9 @@ struct MmaCore {
                         w[e] = ex2_ftz(s[h][g][i * 2 + e] - base[e] + kRaise);
                         l[h][e] += w[e];
                     }
-                    const uint32_t cut = cut2<T>(w[0], w[1]);
-                    const float2 there = unpack2<T>(cut);
-                    hi[h][g][i] = turned(cut);
-                    lo[h][g][i] = turned(positive2<T>(pack2<T>(w[0] - there.x, w[1] - there.y)));
+                    split2<T>(w[0], w[1], weights[h][g][i]);
+#pragma unroll
+                    for (int t = 0; t < kTerms<T>; ++t) weights[h][g][i][t] = turned(weights[h][g][i][t]);
                 }
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -634,10 +649,10 @@ struct MmaCore {
                 uint32_t a[4];
                 ldmatrix4_trans(a, values + lay.offset(g * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)));
 #pragma unroll
-                for (int h = 0; h < EIGHTS; ++h) {
-                    mma_16816<T>(o[h][k], a[0], a[1], a[2], a[3], hi[h][g][0], hi[h][g][1]);
-                    mma_16816<T>(o[h][k], a[0], a[1], a[2], a[3], lo[h][g][0], lo[h][g][1]);
-                }
+                for (int h = 0; h < EIGHTS; ++h)
+#pragma unroll
+                    for (int t = 0; t < kTerms<T>; ++t)
+                        mma_16816<T>(o[h][k], a[0], a[1], a[2], a[3], weights[h][g][0][t], weights[h][g][1][t]);
             }
     }
     template <typename F>
