@@ -42,3 +42,43 @@ def test_weights_are_held_in_32_bits(heads, kv_heads, dh, dtype):
     allowed = bound + step * (want + bound) + (2.0 ** -25 if dtype == HF else 0.0)  # (fp16 has steps of 2^-24 below 2^-14)
     off = (got.double().cpu() - want).abs()
     assert (off <= allowed).all(), (off / allowed).max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,dh", [(8, 64), (1, 128), (16, 128), (4, 256)])
+def test_long_sums_are_rounded_not_cut_off(heads, dh, dtype):
+    """One key of value -1 against 65,000 of value 1 with as much weight together: the sum of the many passes through hundreds of
+    additions in each warp, and what is left of the output, nearly nothing, shows what they lost.
+
+    Relative to the weights A on either side: the scores are below 18 in powers of two and rounded three times, 3 * 18 * 2^-24 ln 2,
+    the exponential is off by 2^-22; a tile's sum of at most six cut-off products by 8 * 2^-23; each of a warp's tiles is added with
+    2^-24 of the sum before; joining parts costs 2^-22.  The output is half of the difference.  (All products cut off in one chain:
+    6e-5 to 1.3e-4 towards the single key.)"""
+    page, n, B, pages = 128, 65536, 384, 8
+    g = torch.Generator().manual_seed(dh)
+    k, v = torch.zeros(pages + 1, 1, page, dh, dtype=dtype), torch.ones(pages + 1, 1, page, dh, dtype=dtype)
+    k[:pages, 0, :, 0] = (8 * torch.randn(pages, page, generator=g)).to(dtype)
+    k[pages, 0, :, 0] = torch.tensor([64.0] + [-6e4] * (page - 1), dtype=dtype)
+    v[pages, 0, 1:], v[pages, 0, 0] = 0, -1
+    columns = torch.arange(n // page - 1) % pages
+    many = k[:pages, 0, :, 0].double()[columns]
+
+    def sides(scale):  # over e^(64 scale)
+        return torch.exp((many - 64) * scale).sum().item()
+
+    low, high = 0.01, 1.0
+    for _ in range(60):
+        low, high = ((low + high) / 2, high) if sides((low + high) / 2) > 1 else (low, (low + high) / 2)
+    scale = torch.tensor(low, dtype=torch.float32).item()
+    A = sides(scale)
+    want = (A - 1) / (A + 1)
+    assert abs(want) < 1e-5 and 64 * scale * math.log2(math.e) < 18
+    q = torch.zeros(B, heads, dh, dtype=dtype)
+    q[..., 0] = 1
+    table = torch.cat((torch.tensor([pages]), columns)).to(torch.int32).expand(B, -1).contiguous()
+    got = paged_attention(*[t.to(DEV) for t in (q, k, v, table)], torch.full((B,), n - 1, dtype=torch.int32, device=DEV), scale=scale)
+    _native.poll_status(DEV)
+    tiles = B * n / (16 if dh > 128 else 32) / torch.cuda.get_device_properties(DEV).multi_processor_count / 6  # of a warp, six to an SM
+    allowed = 0.5 * (3 * 18 * 2.0 ** -24 * math.log(2) + 2 * 2.0 ** -22 + 8 * 2.0 ** -23 + tiles * 2.0 ** -24) + 1e-5 * torch.finfo(dtype).eps
+    off = (got.double() - want).abs().max().item()
+    assert off <= allowed + 2.0 ** -25, (off, allowed)
