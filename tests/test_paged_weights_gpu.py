@@ -82,3 +82,33 @@ def test_long_sums_are_rounded_not_cut_off(heads, dh, dtype):
     allowed = 0.5 * (3 * 18 * 2.0 ** -24 * math.log(2) + 2 * 2.0 ** -22 + 8 * 2.0 ** -23 + tiles * 2.0 ** -24) + 1e-5 * torch.finfo(dtype).eps
     off = (got.double() - want).abs().max().item()
     assert off <= allowed + 2.0 ** -25, (off, allowed)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF])
+@pytest.mark.parametrize("heads,dh", [(2, 64), (12, 64), (4, 256), (4, 40)])
+@pytest.mark.parametrize("behind", [0.0, 5.0, 17.0, 25.0, 30.0, 60.0, 85.0])
+def test_an_infinite_value_behind_the_largest_score(behind, heads, dh, dtype):
+    """Its weight, e^-behind, is a normal number of fp32: the output is that infinity in its dimension, and nothing else changes.  A
+    key of no weight at all, a score of -inf, makes it NaN (0 times infinity)."""
+    n = 40
+    k, v, table = pr.pool([n, n], 16, 1, dh, dtype, 3)
+    q = torch.zeros(2, heads, dh, dtype=dtype)
+    q[..., 0] = 1
+    k[..., 0] = 0
+    for t in (3, 21):  # one value in each direction, of different dimensions
+        k[table[0, t // 16], 0, t % 16, 0] = -behind
+        v[table[0, t // 16], 0, t % 16, t] = math.inf if t == 3 else -math.inf
+    k[table[1, 0], 0, 7, 0] = -math.inf
+    v[table[1, 0], 0, 7, 5] = math.inf
+    got = paged_attention(*[t.to(DEV) for t in (q, k, v, table)], torch.full((2,), n - 1, dtype=torch.int32, device=DEV), scale=1.0)
+    _native.poll_status(DEV)
+    got = got.double().cpu()
+    v[v.isinf()] = 0
+    k[k.isinf()] = -1000  # (no weight in 64 bits either)
+    want, bound = pr.attention(q, k, v, table, torch.tensor([n - 1] * 2), scale=1.0)
+    assert (got[0, :, 3] == math.inf).all() and (got[0, :, 21] == -math.inf).all() and torch.isnan(got[1, :, 5]).all()
+    got[0, :, [3, 21]], got[1, :, 5] = want[0, :, [3, 21]], want[1, :, 5]
+    step = torch.finfo(dtype).eps / 2
+    off = (got - want).abs()
+    bound = 2 * v.double().abs().max() * (n + 8 + 85) * 2.0 ** -23  # (the scores are exact, their multiples below 85 / ln 2 rounded)
+    assert (off <= bound + step * (want.abs() + bound)).all(), off.max()

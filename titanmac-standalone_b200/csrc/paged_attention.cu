@@ -490,9 +490,9 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// Two weights as so many 16-bit numbers each: a weight cut off, what that lacks, cut off too but for the last one.  None of them is
-// below the smallest number that a product takes (2^-126, 2^-24), so that an infinite value stays one; a weight of nothing is nothing
-// in bf16.
+// Two weights as so many 16-bit numbers each: a weight cut off, what that lacks, cut off too but for the last one.  Of a weight that
+// is not zero none is below the smallest number that a product takes (2^-126; 2^-24 under the raise, 2^-36 of the largest weight), so
+// that all of them take an infinite value to the same infinity; of one that is zero all are.
 constexpr int kMostTerms = 3;
 template <typename T>
 constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 3;
@@ -512,12 +512,13 @@ __device__ __forceinline__ void split2<__nv_bfloat16>(float a, float b, uint32_t
 }
 template <>
 __device__ __forceinline__ void split2<__half>(float a, float b, uint32_t (&terms)[kMostTerms]) {
-    const uint32_t least = 0x00010001u;
-    terms[0] = cut2<__half>(a, b);
+    const auto as_pair = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
+    const auto bits = [](__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); };
+    // (whether a weight is zero, from its upper sixteen bits: those of a positive number are in order in every format)
+    const __half2 least = __hmin2(as_pair(cut2<__nv_bfloat16>(a, b)), as_pair(0x00010001u));
+    terms[0] = bits(__hmax2_nan(as_pair(cut2<__half>(a, b)), least));
     const float2 first = unpack2<__half>(terms[0]);
-    const uint32_t rest = pack2<__half>(a - first.x, b - first.y);
-    const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&rest), *reinterpret_cast<const __half2*>(&least));
-    terms[1] = *reinterpret_cast<const uint32_t*>(&v);
+    terms[1] = bits(__hmax2(as_pair(pack2<__half>(a - first.x, b - first.y)), least));
 }
 
 // an 8 x 8 matrix of 16-bit numbers, two of a row to a lane, with rows and columns exchanged
