@@ -36,6 +36,13 @@ from ..paged_cache import PagedCache
 from ..logprobs import TokenLogprobs, token_logprobs
 
 
+def _in_table(embedding: nn.Module, ids: torch.Tensor):
+    """``(ids that can be looked up, which of them are not the ones given)``."""
+    rows = getattr(embedding, "num_embeddings", None)  # (another kind of embedding: whatever is not negative)
+    known = ids.clamp(0, None if rows is None else rows - 1)
+    return known, known != ids
+
+
 class TitanMAC(nn.Module):
     def __init__(self, config):
         super().__init__()
@@ -85,7 +92,8 @@ class TitanMAC(nn.Module):
 
         An id or label outside the vocabulary is met on the device: in 16-bit types its sequence's logits, or the loss and
         the gradients, are NaN, and ``_native.poll_status`` (which synchronises) raises; otherwise PyTorch's own device-side
-        check ends the process's CUDA context.  ``decode_step`` likewise, for its positions too."""
+        check ends the process's CUDA context.  ``decode_step`` likewise, for its positions too; with paged caches ``prefill``
+        and ``decode_step`` meet them on the device in every type."""
         Np = self.config.n_persistent
         rows = logits = held = None  # logits of every row, persistent rows first; of the sequence rows; what holds both
         if torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()):
@@ -162,8 +170,13 @@ class TitanMAC(nn.Module):
     def new_paged_caches(self, page_table: torch.Tensor, pages: int, page_size: int, dtype) -> List[PagedCache]:
         """Caches for ``prefill`` and ``decode_step`` whose sequences live in pages: ``page_table [B, columns]`` (int32, on the
         device, shared by the layers), a pool of ``pages`` pages of ``page_size`` tokens per layer.  ``prefill`` fills every
-        sequence's pages with the whole prompt it is given; ``decode_step`` takes positions of -1 for rows without a sequence
-        (their logits mean nothing)."""
+        sequence's pages with the whole prompt it is given, all prompts of one length; ``decode_step`` takes positions of -1 for
+        rows without a sequence (their logits mean nothing).
+
+        An id outside the vocabulary, a position of ``decode_step`` outside the model's or the pages' table: that row's logits are
+        NaN, what it adds to its pages is too (steps that see it are NaN again), the other rows are as they would be, and
+        ``_native.poll_status`` raises.  ``prefill`` raises a ValueError for a prompt longer than the model's positions; what of
+        it has no place in the pages is left out and reported."""
         self._need_windowed()
         c = self.config
         return [PagedCache(page_table, pages, page_size, c.n_heads, c.d_head, c.window_size, c.n_persistent, dtype)
@@ -182,6 +195,12 @@ class TitanMAC(nn.Module):
             logits = _stack.forward(table, input_ids, caches)
             if logits is not None:
                 return logits, caches
+        bad = None  # sequences with an id outside the vocabulary
+        if caches is not None and any(isinstance(cache, PagedCache) for cache in caches) and self._embeds():
+            if T > getattr(self.embed_positions, "num_embeddings", T):
+                raise ValueError(f"a prompt of {T} tokens exceeds max_seq_len (the position-embedding table)")
+            input_ids, bad = _in_table(self.embed_tokens, input_ids)
+            bad = bad.any(dim=1)
         x = self._embed(input_ids)
         if caches is None:  # (the keys' type is that of the embedded rows, not of one table)
             caches = self.new_caches(B, x.device, x.dtype)
@@ -202,12 +221,16 @@ class TitanMAC(nn.Module):
             # hand the keys/values over: the persistent rows are the same for every sequence
             if Np > 0:
                 cache.set_persistent(k[0, :, :Np], v[0, :, :Np])
-            cache.fill(k[:, :, Np:], v[:, :, Np:], t0=0)
+            k, v = k[:, :, Np:], v[:, :, Np:]
+            if bad is not None and isinstance(cache, PagedCache):
+                v = v.masked_fill(bad[:, None, None, None], float("nan"))
+                cache.append(k[:, :, :1], v[:, :, :1], torch.where(bad, -2, -1).to(torch.int32))  # (stores nothing: it reports)
+            cache.fill(k, v, t0=0)
             x, h = layer.norm_mlp.add_forward(x, _native.project(attn.out_proj, o.view(B, L, -1)), inplace=True)
             pending = layer.mlp(h)
         last = self.norm(x[:, -1]) if pending is None else self.norm.add_forward(x[:, -1], pending[:, -1])[1]
         logits = self.lm_head(last)
-        return logits, caches
+        return logits if bad is None else logits.masked_fill(bad[:, None], float("nan")), caches
 
     @torch.no_grad()
     def decode_step(self, token_ids: torch.Tensor, pos: torch.Tensor,
@@ -222,10 +245,15 @@ class TitanMAC(nn.Module):
                 return logits
         c = self.config
         B = token_ids.shape[0]
-        at = pos.long()
-        if any(isinstance(cache, PagedCache) for cache in caches):  # (a row without a sequence is at -1)
-            at = at.clamp(min=0)
+        at, seen = pos.long(), None
+        if any(isinstance(cache, PagedCache) for cache in caches):
+            token_ids, unknown = _in_table(self.embed_tokens, token_ids)
+            at, outside = _in_table(self.embed_positions, at)
+            bad = (unknown | outside) & (pos != -1)  # (-1: a row without a sequence)
+            seen = pos.masked_fill(bad, -2)  # where no sequence is: the attention's output is NaN, and it reports
         x = self.embed_tokens(token_ids) + self.embed_positions(at)
+        if seen is not None:
+            x = x.masked_fill(bad[:, None], float("nan"))
         pending = None
         for layer, cache in zip(self.layers, caches):
             attn = layer.attention
@@ -234,7 +262,8 @@ class TitanMAC(nn.Module):
             else:
                 x, h = layer.norm_attn.add_forward(x, pending, inplace=True)
             qkv = attn.qkv_proj(h).view(B, 3, c.n_heads, c.d_head)
-            o = cache.decode(qkv[:, 0], qkv[:, 1], qkv[:, 2], pos)
+            at_pages = (seen,) if isinstance(cache, PagedCache) else ()
+            o = cache.decode(qkv[:, 0], qkv[:, 1], qkv[:, 2], pos, None, *at_pages)
             x, h = layer.norm_mlp.add_forward(x, attn.out_proj(o.view(B, -1)), inplace=True)
             pending = layer.mlp(h)
         h = self.norm(x) if pending is None else self.norm.add_forward(x, pending, inplace=True)[1]

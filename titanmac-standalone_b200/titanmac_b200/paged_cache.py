@@ -249,9 +249,10 @@ class PagedCache:
         self.append(k, v, torch.full((k.shape[0],), t0, dtype=torch.int32, device=self.device), counts)
 
     def decode(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pos: torch.Tensor,
-               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               out: Optional[torch.Tensor] = None, seen: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One step: ``q [B, heads, dh]``, ``k_new, v_new [B, kv_heads, dh]``, ``pos [B] int32`` (index of the new token; -1: no
-        sequence in this row).  Appends, rotates if the cache does, and attends."""
+        sequence in this row).  Appends, rotates if the cache does, and attends, at ``seen [B]`` instead of ``pos`` if it is
+        given (the caller's way of declaring a row wrong: -2)."""
         if self.inv_freq is None:
             self.append(k_new.unsqueeze(2), v_new.unsqueeze(2), pos)
         else:
@@ -259,4 +260,4 @@ class PagedCache:
             turned = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
             self.append(k_new.unsqueeze(2), v_new.unsqueeze(2), pos, q=q.unsqueeze(2), q_out=turned.unsqueeze(2))
             q = turned
-        return self.attend(q, pos, out)
+        return self.attend(q, pos if seen is None else seen, out)
