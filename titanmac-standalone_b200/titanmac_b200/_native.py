@@ -14,6 +14,7 @@ import os
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtmw.so")
@@ -360,6 +361,15 @@ def launch(index: int, fn, *args) -> None:
             status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
     if status:
         check(status)
+
+
+def refuse_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises where a tensor carries a forward-mode derivative: the call would drop it without a word.  (Outside every dual level,
+    as almost always, one comparison.)"""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name}: no forward-mode derivative")
 
 
 def _bhrd_strides(t: torch.Tensor) -> Sequence[int]:

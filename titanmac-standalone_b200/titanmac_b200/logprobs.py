@@ -91,7 +91,7 @@ class _TokenLogprobs(torch.autograd.Function):
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_top: int = 0) -> TokenLogprobs:
     """Log-probabilities of ``targets [..]`` (int64) under ``logits [.., V]``, the entropy of every row, and its ``n_top`` (at most
-    32) most likely ids.  Differentiable in the logits.
+    32) most likely ids.  Differentiable in the logits, backwards and once; a forward-mode derivative is refused.
 
     A target of -100 counts as none: its value is 0 and no gradient comes from it.  A target outside the vocabulary has NaN and
     ``_native.poll_status`` raises.  A row without a distribution (a NaN, +inf or nothing but -inf among its logits) has NaN, and
@@ -106,6 +106,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_top: int = 0) 
         raise ValueError("token_logprobs: logits [.., vocabulary] and targets [..] must agree in the axes in front")
     if not 0 <= n_top <= min(MAX_TOP, shape[-1]):
         raise ValueError(f"token_logprobs: n_top must be in 0 .. {min(MAX_TOP, shape[-1])}, got {n_top}")
+    _native.refuse_tangents("token_logprobs", logits)
     targets = targets.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, n_top))

@@ -7,7 +7,8 @@ graph); entries that no token needs may hold anything.  Sequences may share page
 without a sequence (``start`` / ``pos`` of -1), query heads may share key heads, and keys and queries can be rotated by their
 positions on the way into the cache.
 
-Serving only: no gradient flows through these calls.
+Serving only: no gradient flows through these calls (inputs that require one are taken as they are; forward-mode derivatives are
+refused).
 
 What the device finds wrong - a position or a page outside the table or the pool - makes NaN of what depends on it, touches nothing
 else and is raised by ``_native.poll_status``.
@@ -67,13 +68,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     pair ``i`` by ``t * inv_freq[i]`` at token ``t``; the pairs are ``(i, i + len(inv_freq))`` or, ``interleaved``,
     ``(2 i, 2 i + 1)``.  ``q [B, heads, rows, dh]`` is rotated likewise into ``q_out`` (may be ``q``; made if None), which is
     returned; its rows that are no new token's are left as they are.  Writes of the same slot twice in one call are the caller's
-    to avoid."""
+    to avoid.  Serving only: nothing that is returned or written carries a gradient."""
     index = k_pages.get_device()
     if not 0 <= index == k.get_device() == v.get_device() == v_pages.get_device() == page_table.get_device() == start.get_device():
         _refuse_devices("paged_append", k_pages, k, v, v_pages, page_table, start)
     dtype = k_pages.dtype
     if not (dtype is v_pages.dtype is k.dtype is v.dtype and torch.int32 is page_table.dtype is start.dtype):
         raise TypeError("paged_append: k, v and the pages must share one dtype; page_table and start must be int32")
+    _native.refuse_tangents("paged_append", k, v, k_pages, v_pages, q)
     shape = k.shape
     if len(shape) != 4:
         raise ValueError("paged_append: k and v must be [batch, kv_heads, rows, head_dim]")
@@ -137,13 +139,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Attention of the newest token of every sequence, ``q [B, heads, dh]`` at ``pos[b]`` (int32 ``[B]``), whose keys and values
     have been appended: over tokens ``pos - window .. pos`` (None: all up to ``pos``) and the persistent keys
     ``k_pers, v_pers [kv_heads, Np, dh]``.  ``heads`` is a multiple of the pages' ``kv_heads``.  ``pos`` of -1: a sequence without
-    tokens; it sees the persistent keys, and is zero without them.  ``out`` must not overlap ``q``."""
+    tokens; it sees the persistent keys, and is zero without them.  ``out`` must not overlap ``q``.  Serving only: the output carries
+    no gradient."""
     index = k_pages.get_device()
     if not 0 <= index == q.get_device() == v_pages.get_device() == page_table.get_device() == pos.get_device():
         _refuse_devices("paged_attention", k_pages, q, v_pages, page_table, pos)
     dtype = k_pages.dtype
     if not (dtype is v_pages.dtype is q.dtype and torch.int32 is page_table.dtype is pos.dtype):
         raise TypeError("paged_attention: q and the pages must share one dtype; page_table and pos must be int32")
+    _native.refuse_tangents("paged_attention", q, k_pages, v_pages, k_pers, v_pers)
     shape = q.shape
     if len(shape) != 3:
         raise ValueError("paged_attention: q must be [batch, heads, head_dim]")
