@@ -576,17 +576,34 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(const _
     if (none) return;
     __syncthreads();  // over what the pass has written: the target and the likely ids, whose gradients are more
     if (tid >= 32) return;
+    // With `more` its own incoming gradient and `others` the rest of the row's: more (1 - p) - p (others + h (log p + H)).  1 - p
+    // comes from log p, and the others are added up without `more`: where an id has nearly all of its row, more - p (more + others) by
+    // a subtraction would leave little of it (nothing from log p = -2e-8 on), and the forward has log p to 1e-5 of itself.
+    auto of_one = [&](long long i, float more, float others) {
+        const float lp = (to_f32<T>(x.x[i]) - m) - log_sum;
+        if (H) others = fmaf(h, fmaxf(lp, -200.f) + p.f.entropy[row], others);
+        return fmaf(-ex2_ftz(lp * kLog2e), others, -more * expm1f(lp));
+    };
     long long id = tid < top ? p.f.top_ids[(long long)row * top + tid] : -1;
-    float more = tid < top ? p.d_top[(long long)row * top + tid] : 0.f;
-    if (id == y && id >= 0) more += g;
-    if (!__any_sync(0xffffffffu, id == y && id >= 0)) {  // a lane without a likely id takes the target; else the last one, in turn
+    float more = tid < top ? p.d_top[(long long)row * top + tid] : 0.f, others = 0.f;
+    for (int l = 0; l < top; ++l) {
+        const float its = __shfl_sync(0xffffffffu, more, l);
+        if (l != lane) others += its;
+    }
+    const bool is_target = id == y && id >= 0;
+    if (!__any_sync(0xffffffffu, is_target)) {  // a lane without a likely id takes the target; else the last one, in turn
         const bool spare = top < 32 ? tid == top : tid == 31;
-        if (spare && top < 32) id = y, more = g;
         if (spare && top == 32 && y >= 0 && y < p.f.vocab && (y + shift) / E >= first && (y + shift) / E < end)
-            d[y] = from_f32<T>(gradient(to_f32<T>(x.x[y])) + g);
+            d[y] = from_f32<T>(of_one(y, g, others + more));
+        if (spare && top < 32) id = y, more = g;
+        else others += g;
+    } else if (is_target) {
+        more += g;
+    } else {
+        others += g;
     }
     if (id < 0 || id >= p.f.vocab || (id + shift) / E < first || (id + shift) / E >= end) return;
-    d[id] = from_f32<T>(gradient(to_f32<T>(x.x[id])) + more);
+    d[id] = from_f32<T>(of_one(id, more, others));
 }
 
 template <typename T, int W>
