@@ -472,7 +472,7 @@ typedef struct tmw_pages {
  * pair i by the angle t * inv_freq[i] (inv_freq: rotated / 2 fp32 numbers, device), pairs being (i, i + rotated / 2) or, with
  * interleaved, (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin), with the angle in 64 bits and one rounding at the end.
  * q (may be NULL): [batch, heads, rows, head_dim], turned likewise into q_out, which may be q itself with the same strides; rows
- * behind a sequence's last new token stay as they are.  Buffers must not overlap otherwise.
+ * behind a sequence's last new token stay as they are.  Buffers must not overlap otherwise, nor rows of an output one another.
  *
  * The device checks what the host cannot see: a token without a place (a position or a page outside the table or the pool, or a
  * count outside 0 .. rows, a start below -1, which takes the whole sequence) is not stored, its q_out is NaN, and tmw_poll_status
@@ -496,9 +496,9 @@ TMW_API int tmw_paged_append(const tmw_paged_append_desc* desc, void* stream);
  * Attention of one new token per sequence over its pages: o[b, h] = softmax(q[b, h] kᵀ · scale) v over the persistent keys
  * (k_pers, v_pers: [kv_heads, n_persistent, head_dim] contiguous, shared by the batch) and the sequence's tokens
  * max(0, pos[b] - window) .. pos[b] (window -1: all of them), the new one at pos[b] among them: it has been appended before.
- * q, o: [batch, heads, head_dim] through {batch, head} strides, not overlapping; heads is a multiple of kv_heads, and head h reads
- * the keys of head h / (heads / kv_heads).  pos[b] = -1: a sequence without tokens; it sees the persistent keys, and without these its output
- * is zero.  A position or a page outside the table or the pool makes the sequence's output NaN and is reported by
+ * q, o: [batch, heads, head_dim] through {batch, head} strides, not overlapping, nor o's rows one another; heads is a multiple of
+ * kv_heads, and head h reads the keys of head h / (heads / kv_heads).  pos[b] = -1: a sequence without tokens; it sees the
+ * persistent keys, and without these its output is zero.  A position or a page outside the table or the pool makes the sequence's output NaN and is reported by
  * tmw_poll_status (TMW_ERR_INVALID_ARGUMENT).
  *
  * The keys of all sequences are shared out evenly over the GPU, however long each sequence is; the parts of one that came to

@@ -1,6 +1,8 @@
 // What the kernels over paged keys and values share (internal): where a token lives.
 #pragma once
 
+#include <initializer_list>
+
 #include "tmw_common.cuh"
 
 namespace tmw {
@@ -56,6 +58,13 @@ inline int validate_pages(const tmw_pages& p, bool used) {
     if (p.pages > 0 && (p.k_pages == nullptr || p.v_pages == nullptr)) return TMW_ERR_INVALID_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages)) & 15u) return TMW_ERR_INVALID_ARGUMENT;
     return TMW_OK;
+}
+
+// Whether an output's strides bring its rows to places of their own, as far as a stride of 0 tells.
+inline bool rows_apart(const int64_t* strides, std::initializer_list<int> extents) {
+    for (int n : extents)
+        if (*strides++ == 0 && n > 1) return false;
+    return true;
 }
 
 }  // namespace tmw

@@ -211,6 +211,15 @@ extern "C" int tmw_paged_append(const tmw_paged_append_desc* d, void* stream) {
         !add(d->q_out, d->q_out_stride, d->heads > 0))
         return TMW_ERR_INVALID_ARGUMENT;
     if (d->heads > 65535) return TMW_ERR_TOO_LARGE;
+    if (d->heads > 0) {
+        const int extents[3] = {d->at.batch, d->heads, d->rows};
+        bool same = true;
+        for (int i = 0; i < 3; ++i) same = same && (extents[i] == 1 || d->q_stride[i] == d->q_out_stride[i]);
+        if ((d->q == d->q_out && !same) || !rows_apart(d->q_out_stride, {d->at.batch, d->heads, d->rows})) {
+            set_error_text("tmw_paged_append: q_out must have places of its own, or be q with q's strides");
+            return TMW_ERR_INVALID_ARGUMENT;
+        }
+    }
 
     PagedAppend p = {};
     p.map = PageMap(d->at);

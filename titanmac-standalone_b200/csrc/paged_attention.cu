@@ -1092,6 +1092,10 @@ extern "C" int tmw_paged_attention(const tmw_paged_attention_desc* d, void* scra
         return TMW_ERR_INVALID_ARGUMENT;
     for (int i = 0; i < 2; ++i)
         if (d->q_stride[i] < 0 || d->o_stride[i] < 0) return TMW_ERR_INVALID_ARGUMENT;
+    if (!rows_apart(d->o_stride, {d->at.batch, d->heads})) {
+        set_error_text("tmw_paged_attention: every output must have a place of its own");
+        return TMW_ERR_INVALID_ARGUMENT;
+    }
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     if ((bits(d->k_pers) | bits(d->v_pers) | bits(scratch)) % 16 != 0 || (bits(d->q) | bits(d->o)) % size != 0)
         return TMW_ERR_INVALID_ARGUMENT;

@@ -694,6 +694,7 @@ extern "C" int tmw_token_logprobs_backward(const tmw_logprobs_desc* d, const flo
     const int rc = checked(d, p.f);
     if (rc != TMW_OK || p.f.rows == 0) return rc;
     if (p.f.lse == nullptr || d_logits == nullptr || d_logits == d->logits || d_stride == nullptr || d_stride[0] < 0 || d_stride[1] < 0 ||
+        (d_stride[0] == 0 && d->batch > 1) || (d_stride[1] == 0 && d->tokens > 1) ||
         (d_top != nullptr && p.f.top > 0 && p.f.top_ids == nullptr) || reinterpret_cast<uintptr_t>(d_logits) % dtype_size(d->dtype) != 0)
         return TMW_ERR_INVALID_ARGUMENT;
     p.d_logprobs = d_logprobs;
