@@ -195,12 +195,13 @@ class TitanMAC(nn.Module):
             logits = _stack.forward(table, input_ids, caches)
             if logits is not None:
                 return logits, caches
-        bad = None  # sequences with an id outside the vocabulary
+        bad = wrong = None  # sequences with an id outside the vocabulary
         if caches is not None and any(isinstance(cache, PagedCache) for cache in caches) and self._embeds():
             if T > getattr(self.embed_positions, "num_embeddings", T):
                 raise ValueError(f"a prompt of {T} tokens exceeds max_seq_len (the position-embedding table)")
             input_ids, bad = _in_table(self.embed_tokens, input_ids)
             bad = bad.any(dim=1)
+            wrong = bad.to(torch.int32)
         x = self._embed(input_ids)
         if caches is None:  # (the keys' type is that of the embedded rows, not of one table)
             caches = self.new_caches(B, x.device, x.dtype)
@@ -221,11 +222,12 @@ class TitanMAC(nn.Module):
             # hand the keys/values over: the persistent rows are the same for every sequence
             if Np > 0:
                 cache.set_persistent(k[0, :, :Np], v[0, :, :Np])
-            k, v = k[:, :, Np:], v[:, :, Np:]
-            if bad is not None and isinstance(cache, PagedCache):
-                v = v.masked_fill(bad[:, None, None, None], float("nan"))
-                cache.append(k[:, :, :1], v[:, :, :1], torch.where(bad, -2, -1).to(torch.int32))  # (stores nothing: it reports)
-            cache.fill(k, v, t0=0)
+            cache.fill(k[:, :, Np:], v[:, :, Np:], t0=0)
+            if wrong is not None and isinstance(cache, PagedCache):  # (one layer's keys are enough: the step's others see its NaN)
+                nan = torch.full(k.shape[-1:], float("nan"), dtype=k.dtype, device=k.device).expand(B, k.shape[1], T, -1)
+                cache.append(nan, nan, wrong - 1)  # over the wrong sequences' tokens; -1: the others are not there
+                cache.append(nan[:, :, :1], nan[:, :, :1], -1 - wrong)  # (-2 stores nothing: it reports)
+                wrong = None
             x, h = layer.norm_mlp.add_forward(x, _native.project(attn.out_proj, o.view(B, L, -1)), inplace=True)
             pending = layer.mlp(h)
         last = self.norm(x[:, -1]) if pending is None else self.norm.add_forward(x[:, -1], pending[:, -1])[1]
