@@ -13,8 +13,8 @@
 // done; what was cut between CTAs goes to scratch memory, and a second kernel, launched under the first, joins it in the order of
 // the CTAs.
 //
-// bf16, 545,000 tokens of 12 sequences, 32 heads of 128 on 4: 187 us, 6.1 TB/s (warps of a CTA on neighbouring tiles, joined at every
-// item's end: 192).  48 sequences of 1 to 16384 tokens, 32 heads on 8, fp16: 118 us, 5.8 TB/s (joined at every item's end: 202).
+// bf16, 553,000 tokens of 12 sequences, 32 heads of 128 on 4: 191 us, 5.9 TB/s; 48 sequences of 1 to 16384 tokens, 32 heads on 8, fp16:
+// 119 us, 5.7 TB/s.  (Warps of a CTA on neighbouring tiles, joined at every item's end: 192 and 202 when this took 187 and 118.)
 #include <math_constants.h>
 
 #include <type_traits>
@@ -427,11 +427,12 @@ struct SimtCore {
 // mma.sync with the keys, then the dimensions of the values, as the sixteen rows of a tile and eight query heads as its columns
 // (tcgen05's 64 or 128 rows would wait for as many keys per step, and the step is bound by HBM long before the tensor cores): the
 // scores are K Q^T, their exponentials, turned over eight by eight (movmatrix), are the operand of V^T W^T.  A weight goes in as several
-// 16-bit numbers that add up to it - three in bf16, all 24 bits; two in fp16, 22 bits, what the exponential itself has -: one alone
-// would put up to 2^-8 of itself on the output, two in bf16 2^-16, which shows where values cancel.  In fp16 they are raised by 2^12, as far as
-// the largest allows, so that those below 2^-14 of it keep their bits.  The products cut their sums off instead of rounding them, so a
-// tile's begin at zero and are added to the outputs by themselves: all in one, a warp's 900 tiles brought its part 2^-12 nearer to zero.  Up to eight heads: the tile's upper eight rows are zeros and have
-// no registers.
+// 16-bit numbers that add up to it: three in bf16, all 24 bits; two in fp16, 22 bits, what the exponential itself has.  One alone
+// would put up to 2^-8 of itself on the output, two in bf16 2^-16, which shows where values cancel.  In fp16 they are raised by
+// 2^12, as far as the largest allows, so that those below 2^-14 of it keep their bits.  The products cut their sums off instead of
+// rounding them, so a tile's begin at zero and are added to the outputs by themselves (all in one chain, a warp's 900 tiles brought
+// its part 2^-12 nearer to zero), one chain for each sixteen keys (one for all 32: 12.4 us for 700 tokens instead of 10.9).  Up to
+// eight heads: the tile's upper eight rows are zeros and have no registers.
 template <int DH>
 struct MmaLayout {
     int bytes;
@@ -892,8 +893,8 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
 
 // The parts of an item that was cut: CTA (c, .) joins 128 dimensions of a row of the one that begins in CTA c.  Its warps take every
 // kJoinWarps-th part each, a lane four dimensions, kJoinAhead parts on their way at once.  The first two parts, mostly all there are,
-// load before it is known whether there is an item (one sequence of 65536 tokens in 148 parts: 22.7 us the two kernels, one part at
-// a time; 700 tokens: 12.4).
+// load before it is known whether there is an item (one sequence of 65536 tokens in 148 parts: 20.7 us the two kernels, with one part
+// at a time 22.7; 700 tokens: 10.9, 12.4).
 constexpr int kJoinWarps = 8, kJoinAhead = 6;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttention p) {
@@ -959,8 +960,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
-// Shared memory of a CTA, one to an SM: with more than this, or more than 196 KB in all, what is left of the SM's memory as L1 is
-// too little for the copies on their way, and they come from L2 twice (32 heads on 4, 545,000 tokens: 231 us, with this 189).
+// Shared memory of a CTA, one to an SM: with much more, what is left of the SM's memory as L1 is too little for the copies on their
+// way, and they come from L2 twice (32 heads on 4, 553,000 tokens, rings of three tiles in 226 KB: 231 us when this took 189).  Head
+// size 64 has eleven warps here; with twelve its 256 windows of 512 take the same 68.5 us.
 constexpr int kMostShared = 193 * 1024 + 512;
 
 struct Plan {

@@ -474,7 +474,8 @@ struct LogprobsBackward {
     long long stride[2];
 };
 
-// (4096 rows of 128000, us, with 4, 8, 16 and 32 vectors to a thread: 387, 351, 339, 371)
+// (us with 4, 8, 16 and 32 vectors to a thread, bf16: 4096 rows of 128000 without the entropy 361, 326, 325, 327, with it 322, 325, 326,
+// 329; 4096 of 50264 135, 136, 133, 136; 4 of 128000 4.2, 5.3, 6.3, 8.4.  2048 of 32000 in fp32, and of 1000 and 8000, the same with all.)
 constexpr int kBackThreads = 256, kBackVectors = 16;  // vectors of a thread
 
 // VEC: whole vectors; else (logits and gradient begin at different places of their vectors) one element at a time.
@@ -614,10 +615,16 @@ int launch_forward(const Logprobs& p, int ctas, cudaStream_t stream) {
 template <typename T>
 int launch_forward(const Logprobs& p, cudaStream_t stream) {
     // Few rows: eight warps each, and clusters while every thread of them has a vector or more.  With rows enough to keep kWarpsBusy
-    // warps to an SM, a row has fewer warps - no barrier to wait at, more rows at once: 4096 rows of 8000, us, without alternatives 20.7
-    // with one warp and 43 with four - unless a thread's part of it, or what the likely ids make it read again, top / (32 warps) of the
-    // row, became long: 3000 rows of 49999 with 5 ids 98 with two warps, 81 with four, 86 with eight; 4096 of 128000 with a
-    // backward of 339 530 with one, 521 with eight.
+    // warps to an SM, a row has fewer warps - no barrier to wait at, more rows at once - unless a thread's part of it, or what the
+    // likely ids make it read again, top / (32 warps) of the row, became long.  Measured, us, bf16:
+    //                                     1 warp   2      4      8 warps
+    //   16384 rows of 1000, no ids         21.5   28.5   43.1   76.9
+    //   4096 rows of 8000, no ids          19.7   20.6   24.7   33.3
+    //   3000 rows of 50000, no ids         67.6   66.2   61.2   64.6   (four here: kMostOfThread)
+    //   4096 rows of 128000, no ids       178.4  173.2  168.8  171.0   (eight here)
+    //   3000 rows of 49999, 5 ids, fp16           98.3   81.3   83.4   (four here: kMostAgain)
+    // kMostAgain, us with 512 | 2048 | 8192: 4096 rows of 16000 with 5 ids 59.6 | 47.2 | 47.2, with 20 70 | 70 | 55; 4096 of 8000 with 20 54 | 39 |
+    // 38; 4096 of 32000 with 10 88 | 88 | 78; 2048 of 50257 with 20 73 | 73 | 76; 2048 of 32000 with 5 in fp32 65 | 66 | 72: no one number is best for all.
     constexpr int kWarpsBusy = 20, kMostAgain = 2048, kMostOfThread = 64;
     const int vectors = (int)(((long long)p.vocab * sizeof(T) + 15) / 16);
     int warps = 8;
