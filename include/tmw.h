@@ -519,6 +519,94 @@ TMW_API size_t tmw_paged_attention_scratch_bytes(const tmw_paged_attention_desc*
 TMW_API int tmw_paged_attention(const tmw_paged_attention_desc* desc, void* scratch, size_t scratch_bytes, void* stream);
 
 /*
+ * Pages of 8-bit numbers, with an fp32 scale for every token and key head: half the memory of 16-bit pages and half the traffic of a
+ * step.  k_pages and v_pages of tmw_pages then hold codes, one byte each; dtype stays that of q, k, v and o.  A code stands for
+ * itself times its row's scale.  k_scales, v_scales: [pages, kv_heads, page_size] contiguous; k_pers_scales, v_pers_scales:
+ * [kv_heads, n_persistent] contiguous, of persistent keys in the same form.  head_dim: a multiple of 16.
+ *
+ * A row x of head_dim numbers (a key rotated already) is written as scale = max(max |x| / largest, 2^-100), largest being 127 or 448,
+ * and the codes nearest to x / scale, halves to the even one.  A row with a NaN or an infinity has a scale of NaN and codes of 0: it
+ * reads as NaN.  Scales that the caller writes are positive; what is below 2^-100 counts as that under a value.
+ */
+enum { TMW_PAGES_SAME = 0, TMW_PAGES_INT8 = 1, TMW_PAGES_E4M3 = 2 };
+typedef struct tmw_page_scales {
+    int32_t format; /* TMW_PAGES_SAME: pages in dtype, no scales */
+    int32_t reserved; /* 0 */
+    float *k_scales, *v_scales;
+    const float *k_pers_scales, *v_pers_scales;
+} tmw_page_scales;
+
+/*
+ * tmw_paged_append into pages of either form (scales NULL: pages in dtype).  positions (may be NULL): [batch, rows] int32, the
+ * positions that the rows are rotated by instead of those of their slots: drafted tokens of a tree lie one behind the other, several
+ * of them at one depth.  Any number will do.
+ */
+TMW_API int tmw_paged_append_scaled(const tmw_paged_append_desc* desc, const tmw_page_scales* scales, const int32_t* positions,
+                                    void* stream);
+
+/*
+ * Keys and values of tokens back from their pages: row r of sequence b of k and v, [batch, kv_heads, rows, head_dim] in dtype through
+ * {batch, head, row} strides, is token start[b] + r (from 8 bits: the product in fp32, rounded to dtype) for r < counts[b] (counts NULL: every row); the others are left
+ * as they are, all of them with start[b] = -1.  What has no place reads as NaN and is reported, as tmw_paged_append does.
+ */
+typedef struct tmw_paged_read_desc {
+    tmw_pages at;
+    int32_t rows, reserved; /* reserved: 0 */
+    void *k, *v;
+    int64_t k_stride[3], v_stride[3];
+    const int32_t* start;
+    const int32_t* counts;
+} tmw_paged_read_desc;
+
+TMW_API int tmw_paged_read(const tmw_paged_read_desc* desc, const tmw_page_scales* scales, void* stream);
+
+/* tmw_paged_attention over pages of 8 bits (persistent keys in the same form). */
+TMW_API size_t tmw_paged_attention_scaled_scratch_bytes(const tmw_paged_attention_desc* desc, const tmw_page_scales* scales);
+TMW_API int tmw_paged_attention_scaled(const tmw_paged_attention_desc* desc, const tmw_page_scales* scales, void* scratch,
+                                       size_t scratch_bytes, void* stream);
+
+/*
+ * Attention of the drafted tokens of a tree over the cache: sequence b has start[b] tokens and, behind them in its pages (appended
+ * before), counts[b] drafted ones (counts NULL: nodes), its nodes, at most 64.  q, o: [batch, heads, nodes, head_dim] through
+ * {batch, head, node} strides.  Node i sees the persistent keys, the tokens max(0, positions[b][i] - window) .. start[b] - 1 (window
+ * -1: all of them, and positions may be NULL; a position below start[b] counts as that), and every node j < counts[b] whose bit j of
+ * seen[b][i] is set - with a tree its ancestors and itself.  positions int32, seen int64: [batch, nodes] contiguous.  A node
+ * that sees nothing has an output of zero.  What it does not see does not matter, infinities and NaN included.  Rows of o from counts[b] on are left as they
+ * are, and with start[b] = -1 all of them.  A count outside 0 .. nodes, a start below -1 or nodes behind the table's end make the
+ * sequence's outputs NaN (with such a count all nodes'), a page outside the pool those of the nodes that see it; tmw_poll_status reports
+ * it.  Pages of either form (scales NULL: in dtype).  The rest is as with tmw_paged_attention.
+ */
+typedef struct tmw_paged_tree_desc {
+    tmw_pages at;
+    int32_t heads, nodes, n_persistent, window;
+    float scale; /* 0 selects 1/sqrt(head_dim) */
+    int32_t reserved; /* 0 */
+    const void *q, *k_pers, *v_pers;
+    void* o;
+    int64_t q_stride[3], o_stride[3];
+    const int32_t *start, *counts, *positions;
+    const int64_t* seen;
+} tmw_paged_tree_desc;
+
+TMW_API size_t tmw_paged_tree_attention_scratch_bytes(const tmw_paged_tree_desc* desc, const tmw_page_scales* scales);
+TMW_API int tmw_paged_tree_attention(const tmw_paged_tree_desc* desc, const tmw_page_scales* scales, void* scratch, size_t scratch_bytes,
+                                     void* stream);
+
+/*
+ * Tokens moved towards the front of their sequence, as the accepted path of a drafted tree: token start[b] + kept[b][i] becomes token
+ * start[b] + i for i < counts[b], keys, values and scales.  kept: [batch, rows] int32, contiguous, rising, none below its place
+ * (i <= kept[b][i] < kept[b][i + 1]); counts at most rows, rows at most 64.  start[b] = -1: nothing is touched.  A sequence whose kept does not rise, whose tokens have no
+ * place, or whose count is outside 0 .. rows is left as it is and reported.  No two sequences may move tokens of one page.
+ */
+typedef struct tmw_paged_keep_desc {
+    tmw_pages at;
+    int32_t rows, reserved; /* reserved: 0 */
+    const int32_t *start, *kept, *counts;
+} tmw_paged_keep_desc;
+
+TMW_API int tmw_paged_keep(const tmw_paged_keep_desc* desc, const tmw_page_scales* scales, void* stream);
+
+/*
  * What a row of logits says of a token: logprobs[r] = log softmax(logits[r])[targets[r]] (targets: int64; -100: none, the value is
  * 0), entropy[r] = -sum p log p, and the `top` most likely ids with their log-probabilities (top_ids int64, top_logprobs, both
  * [rows, top]; among equal logits the lower id first; top at most 32 and at most vocab).  Rows are (b, t): row b * tokens + t of

@@ -39,9 +39,26 @@ struct PageMap {
         if ((uint32_t)at >= (uint32_t)pages) return -1;
         return ((long long)at * kv_heads * page.d + (t - column * page.d)) * head_dim;
     }
+    // the same counted in rows
+    __device__ __forceinline__ long long row(int b, int t) const {
+        const uint32_t column = page.div((uint32_t)t);
+        const int at = __ldg(table + b * table_stride + column);
+        if ((uint32_t)at >= (uint32_t)pages) return -1;
+        return (long long)at * kv_heads * page.d + (t - column * page.d);
+    }
     // from one head's rows to the next one's
     __device__ __forceinline__ long long head_step() const { return (long long)page.d * head_dim; }
 };
+
+// Pages in 8 bits: a code of four exponent and three fraction bits.
+struct E4m3 {
+    uint8_t bits;
+};
+__device__ __forceinline__ __half2 from_e4m3(uint32_t two) {  // the lower two codes
+    uint32_t w;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(w) : "h"((uint16_t)two));
+    return *reinterpret_cast<const __half2*>(&w);
+}
 
 // TMW_OK, or what is wrong with the description (the pointers only where there is something to do)
 inline int validate_pages(const tmw_pages& p, bool used) {
@@ -57,6 +74,22 @@ inline int validate_pages(const tmw_pages& p, bool used) {
     if (p.columns > 0 && p.page_table == nullptr) return TMW_ERR_INVALID_ARGUMENT;
     if (p.pages > 0 && (p.k_pages == nullptr || p.v_pages == nullptr)) return TMW_ERR_INVALID_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages)) & 15u) return TMW_ERR_INVALID_ARGUMENT;
+    return TMW_OK;
+}
+
+// The same of the scales, with as many pointers as a call needs.
+inline int validate_scales(const tmw_pages& p, const tmw_page_scales& s, bool used, bool persistent) {
+    if (s.format != TMW_PAGES_SAME && s.format != TMW_PAGES_INT8 && s.format != TMW_PAGES_E4M3) return TMW_ERR_UNSUPPORTED;
+    if (s.format == TMW_PAGES_SAME) return TMW_OK;
+    if (p.head_dim % 16 != 0) {
+        set_error_text("paged cache: head_dim must be a multiple of 16 with pages in 8 bits");
+        return TMW_ERR_UNSUPPORTED;
+    }
+    if (!used) return TMW_OK;
+    if (p.pages > 0 && (s.k_scales == nullptr || s.v_scales == nullptr)) return TMW_ERR_INVALID_ARGUMENT;
+    if (persistent && (s.k_pers_scales == nullptr || s.v_pers_scales == nullptr)) return TMW_ERR_INVALID_ARGUMENT;
+    const auto bits = [](const float* x) { return reinterpret_cast<uintptr_t>(x); };
+    if ((bits(s.k_scales) | bits(s.v_scales) | bits(s.k_pers_scales) | bits(s.v_pers_scales)) % 4 != 0) return TMW_ERR_INVALID_ARGUMENT;
     return TMW_OK;
 }
 

@@ -7,22 +7,10 @@
 // that hold both ends of their pairs, the next two on their way under them (with four on their way half as many warps find room:
 // 8 prompts, 453 MB in and out, 111 us against 80; nothing on its way 92).  Bound by HBM, 5.7 TB/s there; a decode step by its launch
 // (64 tokens: 5.2 us).  t f goes through 64 bits: in fp32 the angle of token 100,000 would be off by 0.004.
-#include "paged.cuh"
+#include "paged_append.cuh"
 
 namespace tmw {
 namespace {
-
-struct PagedAppend {
-    PageMap map;
-    const void *k, *v, *q;
-    void *k_pages, *v_pages, *q_out;
-    long long ks[3], vs[3], qs[3], os[3];  // {batch, head, row}
-    const int32_t *start, *counts;
-    const float* inv_freq;
-    int rows, heads, half;
-    int step_r, step_slot, step_u;  // from a thread's pair of vectors to its next one: tokens, heads, pairs
-    int* status;
-};
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 4;  // tokens of a CTA
@@ -147,7 +135,8 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     for (int i = tid; i < tokens * p.half; i += kAppendThreads) {
         const int r = i / p.half;
         // turns instead of radians: the whole ones fall away exactly
-        double x = (double)((long long)start + r0 + r) * (double)p.inv_freq[i - r * p.half] * 0.15915494309189533577;
+        const long long t = p.positions != nullptr ? p.positions[(long long)b * p.rows + r0 + r] : (long long)start + r0 + r;
+        double x = (double)t * (double)p.inv_freq[i - r * p.half] * 0.15915494309189533577;
         x -= rint(x);
         float s, c;
         sincospif(2.0f * (float)x, &s, &c);
@@ -180,68 +169,21 @@ int launch_append(PagedAppend& p, bool interleaved, int batch, cudaStream_t stre
 }
 
 }  // namespace
+
+int append_same(PagedAppend& p, const tmw_paged_append_desc& d, uintptr_t bits, long long strides, cudaStream_t stream) {
+    const int e = 16 / (int)dtype_size(d.at.dtype);
+    // Whole vectors where every row begins on 16 bytes and no pair is cut; single elements otherwise.
+    const bool whole = bits % 16 == 0 && strides % e == 0 && d.at.head_dim % (2 * e) == 0 &&
+                       (d.interleaved ? d.rotated : d.rotated / 2) % e == 0;
+    const bool il = d.interleaved != 0;
+    if (d.at.dtype == TMW_F32) return whole ? launch_append<float, 4>(p, il, d.at.batch, stream) : launch_append<float, 1>(p, il, d.at.batch, stream);
+    if (d.at.dtype == TMW_BF16)
+        return whole ? launch_append<__nv_bfloat16, 8>(p, il, d.at.batch, stream) : launch_append<__nv_bfloat16, 1>(p, il, d.at.batch, stream);
+    return whole ? launch_append<__half, 8>(p, il, d.at.batch, stream) : launch_append<__half, 1>(p, il, d.at.batch, stream);
+}
+
 }  // namespace tmw
 
 extern "C" int tmw_paged_append(const tmw_paged_append_desc* d, void* stream) {
-    using namespace tmw;
-    if (d == nullptr) return TMW_ERR_INVALID_ARGUMENT;
-    const bool used = d->at.batch > 0 && d->rows > 0;
-    const int rc = validate_pages(d->at, used);
-    if (rc != TMW_OK) return rc;
-    if (d->rows < 0 || d->heads < 0 || d->rotated < 0 || d->rotated % 2 != 0 || d->rotated > d->at.head_dim)
-        return TMW_ERR_INVALID_ARGUMENT;
-    if (!used) return TMW_OK;
-    if (d->k == nullptr || d->v == nullptr || d->start == nullptr || (d->rotated > 0 && d->inv_freq == nullptr) ||
-        (d->heads > 0 && (d->q == nullptr || d->q_out == nullptr)))
-        return TMW_ERR_INVALID_ARGUMENT;
-    const size_t size = dtype_size(d->at.dtype);
-    const int e = 16 / (int)size;
-    uintptr_t bits = 0;     // of every address
-    long long strides = 0;  // and stride
-    auto add = [&](const void* x, const int64_t* s, bool with) {
-        if (!with) return true;
-        bits |= reinterpret_cast<uintptr_t>(x);
-        for (int i = 0; i < 3; ++i) {
-            if (s[i] < 0) return false;
-            strides |= s[i];
-        }
-        return reinterpret_cast<uintptr_t>(x) % size == 0;
-    };
-    if (!add(d->k, d->k_stride, true) || !add(d->v, d->v_stride, true) || !add(d->q, d->q_stride, d->heads > 0) ||
-        !add(d->q_out, d->q_out_stride, d->heads > 0))
-        return TMW_ERR_INVALID_ARGUMENT;
-    if (d->heads > 65535) return TMW_ERR_TOO_LARGE;
-    if (d->heads > 0) {
-        const int extents[3] = {d->at.batch, d->heads, d->rows};
-        bool same = true;
-        for (int i = 0; i < 3; ++i) same = same && (extents[i] == 1 || d->q_stride[i] == d->q_out_stride[i]);
-        if ((d->q == d->q_out && !same) || !rows_apart(d->q_out_stride, {d->at.batch, d->heads, d->rows})) {
-            set_error_text("tmw_paged_append: q_out must have places of its own, or be q with q's strides");
-            return TMW_ERR_INVALID_ARGUMENT;
-        }
-    }
-
-    PagedAppend p = {};
-    p.map = PageMap(d->at);
-    p.k = d->k; p.v = d->v; p.q = d->q;
-    p.k_pages = d->at.k_pages; p.v_pages = d->at.v_pages; p.q_out = d->q_out;
-    for (int i = 0; i < 3; ++i) {
-        p.ks[i] = d->k_stride[i];
-        p.vs[i] = d->v_stride[i];
-        p.qs[i] = d->q_stride[i];
-        p.os[i] = d->q_out_stride[i];
-    }
-    p.start = d->start; p.counts = d->counts; p.inv_freq = d->inv_freq;
-    p.rows = d->rows; p.heads = d->heads; p.half = d->rotated / 2;
-    p.status = device_status_word();
-    if (p.status == nullptr) return TMW_ERR_CUDA;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // Whole vectors where every row begins on 16 bytes and no pair is cut; single elements otherwise.
-    const bool whole = bits % 16 == 0 && strides % e == 0 && d->at.head_dim % (2 * e) == 0 &&
-                       (d->interleaved ? d->rotated : d->rotated / 2) % e == 0;
-    const bool il = d->interleaved != 0;
-    if (d->at.dtype == TMW_F32) return whole ? launch_append<float, 4>(p, il, d->at.batch, s) : launch_append<float, 1>(p, il, d->at.batch, s);
-    if (d->at.dtype == TMW_BF16)
-        return whole ? launch_append<__nv_bfloat16, 8>(p, il, d->at.batch, s) : launch_append<__nv_bfloat16, 1>(p, il, d->at.batch, s);
-    return whole ? launch_append<__half, 8>(p, il, d->at.batch, s) : launch_append<__half, 1>(p, il, d->at.batch, s);
+    return tmw_paged_append_scaled(d, nullptr, nullptr, stream);
 }

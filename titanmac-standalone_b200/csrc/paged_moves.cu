@@ -1,0 +1,238 @@
+// Tokens out of their pages and from place to place in them: tmw_paged_read, tmw_paged_keep.
+//
+// Both move bytes: bound by HBM, or for a few tokens by launch and latency.
+#include "paged.cuh"
+
+namespace tmw {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct PagedRead {
+    PageMap map;
+    const void *k_pages, *v_pages;
+    const float *k_scales, *v_scales;
+    void *k, *v;
+    long long ks[3], vs[3];  // {batch, head, row}
+    const int32_t *start, *counts;
+    int rows;
+    int* status;
+};
+
+template <typename T, typename P>
+__device__ __forceinline__ void read8(const P* from, float scale, T (&x)[8]) {
+    if constexpr (sizeof(P) == 1) {
+        const uint2 w = *reinterpret_cast<const uint2*>(from);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t two = (i < 2 ? w.x : w.y) >> i % 2 * 16;
+            float2 c;
+            if constexpr (std::is_same<P, E4m3>::value) c = __half22float2(from_e4m3(two));
+            else c = make_float2((float)(int8_t)two, (float)(int8_t)(two >> 8));
+            x[2 * i] = from_f32<T>(c.x * scale);
+            x[2 * i + 1] = from_f32<T>(c.y * scale);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(x) / 16; ++i) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(from)[i];
+    }
+}
+
+// A CTA has kReadTokens tokens of a sequence, all heads of theirs; a thread eight numbers at a time.
+constexpr int kReadTokens = 8;
+template <typename T, typename P, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) paged_read_kernel(const __grid_constant__ PagedRead p) {
+    __shared__ long long place[kReadTokens];
+    const int b = blockIdx.y, r0 = blockIdx.x * kReadTokens, tid = threadIdx.x;
+    const int start = p.start[b];
+    int count = p.counts != nullptr ? p.counts[b] : p.rows;
+    if (start == -1) return;
+    const bool nowhere = start < -1 || count < 0 || count > p.rows;
+    if (count < 0 || count > p.rows) count = p.rows;
+    const int tokens = min(kReadTokens, count - r0);
+    if (tokens <= 0) return;
+    if (tid < tokens) {
+        const long long t = (long long)start + r0 + tid;
+        const long long at = !nowhere && t < p.map.capacity ? p.map.row(b, (int)t) : -1;
+        if (at < 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+        place[tid] = at;
+    }
+    __syncthreads();
+    const int units = p.map.head_dim / 8, slots = 2 * p.map.kv_heads;
+    for (int i = tid; i < tokens * slots * units; i += kThreads) {
+        const int row = i / units, d = (i - row * units) * 8, r = row / slots, slot = row - r * slots;
+        const bool value = slot >= p.map.kv_heads;
+        const int head = value ? slot - p.map.kv_heads : slot;
+        alignas(16) T x[8];
+        if (place[r] >= 0) {
+            const long long at = place[r] + (long long)head * p.map.page.d;
+            float scale = 1.f;
+            if constexpr (sizeof(P) == 1) scale = __ldg((value ? p.v_scales : p.k_scales) + at);
+            read8<T, P>(static_cast<const P*>(value ? p.v_pages : p.k_pages) + at * p.map.head_dim + d, scale, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = from_f32<T>(__int_as_float(0x7fffffff));
+        }
+        const long long(&s)[3] = value ? p.vs : p.ks;
+        T* to = static_cast<T*>(value ? p.v : p.k) + b * s[0] + head * s[1] + (r0 + r) * s[2] + d;
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int e = 0; e < (int)sizeof(x) / 16; ++e) reinterpret_cast<uint4*>(to)[e] = reinterpret_cast<const uint4*>(x)[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = x[e];
+        }
+    }
+}
+
+template <typename T>
+int launch_read(const PagedRead& p, int format, int batch, bool whole, cudaStream_t stream) {
+    const dim3 grid((unsigned)((p.rows + kReadTokens - 1) / kReadTokens), (unsigned)batch);
+    auto with = [&](auto page) {
+        using P = decltype(page);
+        if (whole) paged_read_kernel<T, P, true><<<grid, kThreads, 0, stream>>>(p);
+        else paged_read_kernel<T, P, false><<<grid, kThreads, 0, stream>>>(p);
+    };
+    if (format == TMW_PAGES_INT8) with(int8_t{});
+    else if (format == TMW_PAGES_E4M3) with(E4m3{});
+    else with(T{});
+    TMW_CUDA_TRY(cudaGetLastError());
+    return TMW_OK;
+}
+
+constexpr int kMostKept = 64;
+struct PagedKeep {
+    PageMap map;
+    unsigned char *k_pages, *v_pages;
+    float *k_scales, *v_scales;  // NULL: none
+    const int32_t *start, *kept, *counts;
+    int rows, vectors;  // vectors: of 16 bytes, in a row
+    int* status;
+};
+
+// A CTA has the keys, or the values, of one head of a sequence.  Tokens come from further back than they go to, in the order of both,
+// so a batch of them is read, and when every thread has its part, written: no later token has been written over by then.
+__global__ void __launch_bounds__(kThreads) paged_keep_kernel(const __grid_constant__ PagedKeep p) {
+    __shared__ long long from[kMostKept], to[kMostKept];
+    constexpr int kAhead = 4;
+    const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const bool value = blockIdx.z != 0;
+    const int start = p.start[b], count = p.counts[b];
+    if (start == -1) return;
+    bool bad = start < -1 || count < 0 || count > p.rows;
+    if (!bad && tid < count) {
+        const int32_t* kept = p.kept + (long long)b * p.rows;
+        const int j = kept[tid];
+        bad = j < tid || (tid > 0 && j <= kept[tid - 1]) || (long long)start + j >= p.map.capacity;
+        if (!bad) {
+            const long long source = p.map.row(b, start + j), target = p.map.row(b, start + tid);
+            bad = source < 0 || target < 0;
+            from[tid] = source + (long long)head * p.map.page.d;
+            to[tid] = target + (long long)head * p.map.page.d;
+        }
+    }
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+        return;
+    }
+    uint4* pages = reinterpret_cast<uint4*>(value ? p.v_pages : p.k_pages);
+    float* scales = value ? p.v_scales : p.k_scales;
+    float scale = 0.f;
+    if (scales != nullptr && tid < count) scale = scales[from[tid]];
+    const int n = count * p.vectors;
+    for (int i0 = 0; i0 < n; i0 += kThreads * kAhead) {
+        uint4 x[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = i0 + a * kThreads + tid, t = i / p.vectors;
+            if (i < n && from[t] != to[t]) x[a] = pages[from[t] * p.vectors + (i - t * p.vectors)];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = i0 + a * kThreads + tid, t = i / p.vectors;
+            if (i < n && from[t] != to[t]) pages[to[t] * p.vectors + (i - t * p.vectors)] = x[a];
+        }
+    }
+    if (scales != nullptr && tid < count) scales[to[tid]] = scale;
+}
+
+}  // namespace
+}  // namespace tmw
+
+extern "C" int tmw_paged_read(const tmw_paged_read_desc* d, const tmw_page_scales* scales, void* stream) {
+    using namespace tmw;
+    if (d == nullptr) return TMW_ERR_INVALID_ARGUMENT;
+    const bool used = d->at.batch > 0 && d->rows > 0;
+    int rc = validate_pages(d->at, used);
+    if (rc != TMW_OK) return rc;
+    const tmw_page_scales s = scales != nullptr ? *scales : tmw_page_scales{};
+    rc = validate_scales(d->at, s, used, false);
+    if (rc != TMW_OK) return rc;
+    if (d->rows < 0) return TMW_ERR_INVALID_ARGUMENT;
+    if (!used) return TMW_OK;
+    if (d->k == nullptr || d->v == nullptr || d->start == nullptr) return TMW_ERR_INVALID_ARGUMENT;
+    const size_t size = dtype_size(d->at.dtype);
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v);
+    long long strides = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (d->k_stride[i] < 0 || d->v_stride[i] < 0) return TMW_ERR_INVALID_ARGUMENT;
+        strides |= d->k_stride[i] | d->v_stride[i];
+    }
+    if (bits % size != 0) return TMW_ERR_INVALID_ARGUMENT;
+    if (d->k == d->v || !rows_apart(d->k_stride, {d->at.batch, d->at.kv_heads, d->rows}) ||
+        !rows_apart(d->v_stride, {d->at.batch, d->at.kv_heads, d->rows})) {
+        set_error_text("tmw_paged_read: every output must have a place of its own");
+        return TMW_ERR_INVALID_ARGUMENT;
+    }
+    PagedRead p = {};
+    p.map = PageMap(d->at);
+    p.k_pages = d->at.k_pages; p.v_pages = d->at.v_pages;
+    p.k_scales = s.k_scales; p.v_scales = s.v_scales;
+    p.k = d->k; p.v = d->v;
+    for (int i = 0; i < 3; ++i) {
+        p.ks[i] = d->k_stride[i];
+        p.vs[i] = d->v_stride[i];
+    }
+    p.start = d->start; p.counts = d->counts;
+    p.rows = d->rows;
+    p.status = device_status_word();
+    if (p.status == nullptr) return TMW_ERR_CUDA;
+    const bool whole = bits % 16 == 0 && strides % (16 / (long long)size) == 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (d->at.dtype == TMW_F32) return launch_read<float>(p, s.format, d->at.batch, whole, st);
+    return d->at.dtype == TMW_BF16 ? launch_read<__nv_bfloat16>(p, s.format, d->at.batch, whole, st)
+                                   : launch_read<__half>(p, s.format, d->at.batch, whole, st);
+}
+
+extern "C" int tmw_paged_keep(const tmw_paged_keep_desc* d, const tmw_page_scales* scales, void* stream) {
+    using namespace tmw;
+    if (d == nullptr) return TMW_ERR_INVALID_ARGUMENT;
+    const bool used = d->at.batch > 0 && d->rows > 0;
+    int rc = validate_pages(d->at, used);
+    if (rc != TMW_OK) return rc;
+    const tmw_page_scales s = scales != nullptr ? *scales : tmw_page_scales{};
+    rc = validate_scales(d->at, s, used, false);
+    if (rc != TMW_OK) return rc;
+    if (d->rows < 0) return TMW_ERR_INVALID_ARGUMENT;
+    if (d->rows > kMostKept) {
+        set_error_text("tmw_paged_keep: at most 64 tokens of a sequence");
+        return TMW_ERR_TOO_LARGE;
+    }
+    if (!used) return TMW_OK;
+    if (d->start == nullptr || d->kept == nullptr || d->counts == nullptr) return TMW_ERR_INVALID_ARGUMENT;
+    PagedKeep p = {};
+    p.map = PageMap(d->at);
+    p.k_pages = static_cast<unsigned char*>(d->at.k_pages); p.v_pages = static_cast<unsigned char*>(d->at.v_pages);
+    if (s.format != TMW_PAGES_SAME) p.k_scales = s.k_scales, p.v_scales = s.v_scales;
+    p.start = d->start; p.kept = d->kept; p.counts = d->counts;
+    p.rows = d->rows;
+    const int bytes = d->at.head_dim * (s.format == TMW_PAGES_SAME ? (int)dtype_size(d->at.dtype) : 1);
+    p.vectors = bytes / 16;  // (head_dim is a multiple of 8, of 16 in 8 bits)
+    p.status = device_status_word();
+    if (p.status == nullptr) return TMW_ERR_CUDA;
+    const dim3 grid((unsigned)d->at.kv_heads, (unsigned)d->at.batch, 2);
+    paged_keep_kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    TMW_CUDA_TRY(cudaGetLastError());
+    return TMW_OK;
+}

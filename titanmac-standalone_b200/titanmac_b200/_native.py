@@ -283,6 +283,13 @@ SIGNATURES = {
     "tmw_paged_append": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "tmw_paged_attention_scratch_bytes": (ctypes.c_size_t, [ctypes.c_char_p]),
     "tmw_paged_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tmw_paged_append_scaled": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "tmw_paged_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p]),
+    "tmw_paged_attention_scaled_scratch_bytes": (ctypes.c_size_t, [ctypes.c_char_p, ctypes.c_char_p]),
+    "tmw_paged_attention_scaled": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tmw_paged_tree_attention_scratch_bytes": (ctypes.c_size_t, [ctypes.c_char_p, ctypes.c_char_p]),
+    "tmw_paged_tree_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tmw_paged_keep": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p]),
     "tmw_token_logprobs": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "tmw_token_logprobs_backward": (
         ctypes.c_int,
