@@ -17,6 +17,10 @@ namespace {
 // any factor: x_j = s_j + e_j takes the score's place under the running maximum, u_j = 2^(x_j - m) f_j are the weights of the
 // codes, and u_j / scale_j = 2^(x_j - m) 2^-e_j those that are summed up for the denominator; both with one exponential and no
 // logarithm, and a token whose values are small counts as much in the sum as any other.
+//
+// HEADS: of an item at most, 1, 2, 4, 8 or 16.  With fewer than eight the columns hold them several times over, and each of the 8 / HEADS
+// copies deals with its own share of the tile's keys: its weights are zero in the rows of the others', its running maximum
+// is its own, and the copies are added up when the item ends.  So a lane has KT HEADS / 32 exponentials to a tile instead of KT / 4.
 template <int DH>
 struct Mma8Layout {
     int bytes;
@@ -53,9 +57,13 @@ __device__ __forceinline__ void to_pairs<E4m3>(uint32_t w, uint32_t& even, uint3
     odd = *reinterpret_cast<const uint32_t*>(&b);
 }
 
-template <typename T, typename P, int DH, int EIGHTS>
+template <typename T, typename P, int DH, int HEADS>
 struct Mma8Core {
-    static constexpr int kRows = kMaxRows, KT = 32, kChunks = DH / 16;
+    static constexpr int kRows = HEADS, KT = 32, kChunks = DH / 16;
+    static constexpr int EIGHTS = HEADS > 8 ? 2 : 1, kCopies = HEADS < 8 ? 8 / HEADS : 1;
+    static constexpr int kKeys = kCopies == 1 ? 4 : kCopies == 2 ? 2 : 1;  // of a lane
+    static constexpr int kOfLane = HEADS == 1 ? 1 : 2;                     // heads of each eight
+    static constexpr int kTerms8 = HEADS == 1 ? 1 : 2;  // products of a weight with the values
     static constexpr float kRaise = 12.f;  // as far as fp16 allows: a weight is at most 2^13
     using Layout = Mma8Layout<DH>;
     const PagedAttention& p;
@@ -71,7 +79,7 @@ struct Mma8Core {
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int h = 0; h < EIGHTS; ++h) {
-            const int r = h * 8 + lane / 4;
+            const int r = h * 8 + lane / 4 % HEADS;
             const T* from = static_cast<const T*>(p.q) + row_at<false>(p, p.qs, of, r) + lane % 4 * 4;
             uint32_t raw[kChunks][2];
             float top = 0.f;
@@ -151,63 +159,95 @@ struct Mma8Core {
                     for (int h = 0; h < EIGHTS; ++h) mma_16816<__half>(s[h][g], even[0], even[1], odd[0], odd[1], q[h][k + c][0], q[h][k + c][1]);
                 }
             }
-        // of this lane's keys: the values' scales in their two parts
-        float e[KT / 16][2], f[KT / 16][2], back[KT / 16][2], ks[KT / 16][2];
+        // this lane's keys, with the values' scales in their two parts
+        const int t = lane % 4;
+        const auto key_of = [&](int j) { return kCopies == 1 ? j * 8 : kCopies == 2 ? (t >> 1) * 16 + j * 8 : t * 8; };
+        float e[kKeys], f[kKeys], back[kKeys], ks[kKeys];
 #pragma unroll
-        for (int g = 0; g < KT / 16; ++g)
+        for (int j = 0; j < kKeys; ++j) {
+            ks[j] = scales[key_of(j)];
+            const float vs = scales[KT + key_of(j)];
+            const int bits = __float_as_int(fmaxf(vs, 0x1p-100f));
+            e[j] = __int_as_float(0x4b000000 | (bits >> 23)) - (8388608.f + 127.f) + (vs - vs);  // (NaN stays that)
+            f[j] = __int_as_float((bits & 0x007fffff) | 0x3f800000);
+            back[j] = __int_as_float(0x7f000000 - (bits & 0x7f800000));
+        }
+        // all heads side by side: their chains of shuffles and exponentials overlap
+        uint32_t weights[EIGHTS][KT / 16][2][kTerms8];
+        float keep[EIGHTS][2], base[EIGHTS][2], top[EIGHTS][2], w[EIGHTS][kKeys][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int key = g * 16 + i * 8;
-                ks[g][i] = scales[key];
-                const float vs = scales[KT + key];
-                const int bits = __float_as_int(fmaxf(vs, 0x1p-100f));
-                e[g][i] = __int_as_float(0x4b000000 | (bits >> 23)) - (8388608.f + 127.f) + (vs - vs);  // (NaN stays that)
-                f[g][i] = __int_as_float((bits & 0x007fffff) | 0x3f800000);
-                back[g][i] = __int_as_float(0x7f000000 - (bits & 0x7f800000));
-            }
-        uint32_t weights[EIGHTS][KT / 16][2][2];
-        float keep[EIGHTS][2];
+        for (int h = 0; h < EIGHTS; ++h)
 #pragma unroll
-        for (int h = 0; h < EIGHTS; ++h) {
-            float base[2];
+            for (int a = 0; a < kOfLane; ++a) {
+                top[h][a] = -CUDART_INF_F;
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                float top = -CUDART_INF_F;
-#pragma unroll
-                for (int g = 0; g < KT / 16; ++g)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = g * 16 + i * 8 + lane / 4;
-                        float& x = s[h][g][i * 2 + a];
-                        x = fmaf(x * ks[g][i], q_scale[h][a], e[g][i]);
-                        if (marks.x != 0xffffffffu || marks.y != 0) x = marks.y >> key & 1 ? CUDART_NAN_F : marks.x >> key & 1 ? x : -CUDART_INF_F;
-                        top = fmaxf(top, x);
+                for (int j = 0; j < kKeys; ++j) {
+                    float x;
+                    if constexpr (kCopies == 1) x = s[h][j / 2][j % 2 * 2 + a];
+                    else if constexpr (kCopies == 2) x = t < 2 ? s[h][0][j * 2 + a] : s[h][1][j * 2 + a];
+                    else x = t < 2 ? (t == 0 ? s[h][0][a] : s[h][0][2 + a]) : (t == 2 ? s[h][1][a] : s[h][1][2 + a]);
+                    x = fmaf(x * ks[j], q_scale[h][a], e[j]);
+                    if (marks.x != 0xffffffffu || marks.y != 0) {
+                        const int key = key_of(j) + lane / 4;
+                        x = marks.y >> key & 1 ? CUDART_NAN_F : marks.x >> key & 1 ? x : -CUDART_INF_F;
                     }
+                    w[h][j][a] = x;
+                    top[h][a] = fmaxf(top[h][a], x);
+                }
+            }
 #pragma unroll
-                for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                const float now = fmaxf(m[h][a], top);
-                base[a] = now == -CUDART_INF_F ? 0.f : now;
-                keep[h][a] = m[h][a] == -CUDART_INF_F ? 1.f : ex2_ftz(m[h][a] - base[a]);  // (nothing to keep, or NaN)
+        for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+            for (int h = 0; h < EIGHTS; ++h)
+#pragma unroll
+                for (int a = 0; a < kOfLane; ++a) top[h][a] = fmaxf(top[h][a], __shfl_xor_sync(0xffffffffu, top[h][a], d));
+#pragma unroll
+        for (int h = 0; h < EIGHTS; ++h)
+#pragma unroll
+            for (int a = 0; a < kOfLane; ++a) {
+                const float now = fmaxf(m[h][a], top[h][a]);
+                base[h][a] = now == -CUDART_INF_F ? 0.f : now;
+                keep[h][a] = m[h][a] == -CUDART_INF_F ? 1.f : ex2_ftz(m[h][a] - base[h][a]);  // (nothing to keep, or NaN)
                 m[h][a] = now;
                 l[h][a] *= keep[h][a];
+                base[h][a] -= kRaise;
+            }
+#pragma unroll
+        for (int h = 0; h < EIGHTS; ++h) {
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j)
+#pragma unroll
+                for (int a = 0; a < kOfLane; ++a) {
+                    const float x = ex2_ftz(w[h][j][a] - base[h][a]);
+                    l[h][a] = fmaf(x, back[j], l[h][a]);
+                    w[h][j][a] = x * f[j];
+                }
+            if (kOfLane == 1) keep[h][1] = keep[h][0];
+            // weights as two numbers each, 22 bits: two registers, or (one head) its two columns
+            uint32_t parts[kKeys][kTerms8];
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j) {
+                if constexpr (kOfLane == 1) {
+                    const float first = __half2float(__float2half_rz(w[h][j][0]));
+                    parts[j][0] = pack2<__half>(first, w[h][j][0] - first);
+                } else {
+                    parts[j][0] = cut2<__half>(w[h][j][0], w[h][j][1]);
+                    const float2 had = unpack2<__half>(parts[j][0]);
+                    parts[j][1] = pack2<__half>(w[h][j][0] - had.x, w[h][j][1] - had.y);
+                }
             }
 #pragma unroll
             for (int g = 0; g < KT / 16; ++g)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float w[2];
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        w[a] = ex2_ftz(s[h][g][i * 2 + a] - base[a] + kRaise);
-                        l[h][a] = fmaf(w[a], back[g][i], l[h][a]);
-                        w[a] *= f[g][i];
+                    for (int n = 0; n < kTerms8; ++n) {
+                        uint32_t x;
+                        if constexpr (kCopies == 1) x = parts[g * 2 + i][n];
+                        else if constexpr (kCopies == 2) x = (t >> 1) == g ? parts[i][n] : 0;
+                        else x = t == g * 2 + i ? parts[0][n] : 0;
+                        weights[h][g][i][n] = turned(x);
                     }
-                    // as two numbers each, 22 bits
-                    const uint32_t first = cut2<__half>(w[0], w[1]);
-                    const float2 had = unpack2<__half>(first);
-                    weights[h][g][i][0] = turned(first);
-                    weights[h][g][i][1] = turned(pack2<__half>(w[0] - had.x, w[1] - had.y));
-                }
         }
 #pragma unroll
         for (int k = 0; k < kChunks; k += 2) {
@@ -227,8 +267,8 @@ struct Mma8Core {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) sum[g][h][i] = 0.f;
 #pragma unroll
-                        for (int t = 0; t < 2; ++t)
-                            mma_16816<__half>(sum[g][h], even[0], odd[0], even[1], odd[1], weights[h][g][0][t], weights[h][g][1][t]);
+                        for (int n = 0; n < kTerms8; ++n)
+                            mma_16816<__half>(sum[g][h], even[0], odd[0], even[1], odd[1], weights[h][g][0][n], weights[h][g][1][n]);
                     }
                 }
 #pragma unroll
@@ -250,16 +290,33 @@ struct Mma8Core {
 #pragma unroll
         for (int h = 0; h < EIGHTS; ++h)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int r = h * 8 + lane % 4 * 2 + a;
-                float t = l[h][a];
+            for (int a = 0; a < kOfLane; ++a) {
+                float total = l[h][a], top = m[h][a];
 #pragma unroll
-                for (int d = 4; d < 32; d *= 2) t += __shfl_xor_sync(0xffffffffu, t, d);
-                if (r >= rows.n) continue;
+                for (int d = 4; d < 32; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+                float weight = 1.f;
+                if constexpr (kCopies > 1) {  // copies of a head lie HEADS columns apart, two columns to a lane
+#pragma unroll
+                    for (int d = HEADS < 4 ? 1 : 2; d < 4; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    weight = part_weight(m[h][a], top == -CUDART_INF_F ? 0.f : top);
+                    total *= weight;
+#pragma unroll
+                    for (int d = HEADS < 4 ? 1 : 2; d < 4; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+                }
+                const int r = h * 8 + lane % 4 * 2 + a;
 #pragma unroll
                 for (int k = 0; k < kChunks; ++k) {
-                    const float x[2] = {o[h][k][a], o[h][k][2 + a]};
-                    use(r, m[h][a], t, k * 16 + lane / 4 * 2, x);
+                    float x[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[i] = kOfLane == 1 ? o[h][k][2 * i] + o[h][k][2 * i + 1] : o[h][k][2 * i + a];
+                        if constexpr (kCopies > 1) {
+                            x[i] *= weight;
+#pragma unroll
+                            for (int d = HEADS < 4 ? 1 : 2; d < 4; d *= 2) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
+                        }
+                    }
+                    if (r < rows.n && r < HEADS && (HEADS > 1 || a == 0)) use(r, top, total, k * 16 + lane / 4 * 2, x);
                 }
             }
     }
@@ -277,11 +334,16 @@ struct Mma8Core {
     }
 };
 
+// as many heads as a group has, the next power of two of them
 template <typename T, typename P, int DH, typename F>
 int with_mma(const tmw_paged_attention_desc& d, F&& use) {
-    constexpr int W = DH > 128 ? 6 : 12;
-    if (d.heads / d.at.kv_heads <= 8) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 1>, W, 2>());
-    return use(Kernel<T, P, false, Mma8Core<T, P, DH, 2>, W, 2>());
+    constexpr int W = DH > 128 ? 6 : DH > 64 ? 12 : 16;
+    const int group = d.heads / d.at.kv_heads;
+    if (group == 1) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 1>, W, 2>());
+    if (group == 2) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 2>, W, 2>());
+    if (group <= 4) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 4>, W, 2>());
+    if (group <= 8) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 8>, W, 2>());
+    return use(Kernel<T, P, false, Mma8Core<T, P, DH, 16>, (DH > 64 ? W : 12), 2>());
 }
 template <typename T, typename P, typename F>
 int with_16_bits(const tmw_paged_attention_desc& d, F&& use) {
