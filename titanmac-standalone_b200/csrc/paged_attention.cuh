@@ -23,6 +23,8 @@
 #include <type_traits>
 
 #include "paged.cuh"
+#include "tc_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace tmw {
 namespace {
@@ -42,6 +44,8 @@ struct PagedAttention {
     int batch, np, window;
     int pers_tiles;         // of the persistent keys
     bool whole_runs;        // sixteen tokens from a multiple of sixteen on lie in one page
+    int run;                // as many from a multiple of that on do, 16, 8 or none
+    bool bf16;              // of two types with 16 bits
     bool q_pairs, o_pairs;  // queries can be read, outputs stored two at a time
     int group;              // query heads of a key head
     int rows, parts;        // query heads of an item at most; items of a key head
@@ -78,15 +82,14 @@ __device__ __forceinline__ int tiles_of(const PagedAttention& p, int b, int& lo,
     return p.pers_tiles + pos / KT - lo / KT + 1;
 }
 
-// A place in the line.  An item takes kItemCost more units of it than it has tiles, ahead of them: loading the queries and
+// A place in the line.  An item takes COST more units of it than it has tiles, ahead of them: loading the queries and
 // storing the output hold a warp up for about that long, and pieces of equal length are to take equal time.
-constexpr int kItemCost = 1;
 // items of a key head's query rows: of a sequence with so many nodes
 template <bool TREE>
 __device__ __forceinline__ int parts_of(const PagedAttention& p, int count) {
     return TREE ? (count * p.group + p.rows - 1) / p.rows : p.parts;
 }
-template <int KT, bool TREE>
+template <int KT, bool TREE, int COST>
 struct Cursor {
     int b, item;  // sequence, item of it
     int head;     // the item's key head
@@ -95,10 +98,10 @@ struct Cursor {
     __device__ __forceinline__ void sequence(const PagedAttention& p) {
         bool bad;
         n = tiles_of<KT, TREE>(p, b, lo, pos, count, bad);
-        if (n > 0) n += kItemCost;
+        if (n > 0) n += COST;
     }
     __device__ __forceinline__ int parts(const PagedAttention& p) const { return parts_of<TREE>(p, count); }
-    __device__ __forceinline__ int tile() const { return t - kItemCost; }
+    __device__ __forceinline__ int tile() const { return t - COST; }
     // the next item's first unit; not past the end of the line
     __device__ __forceinline__ void next_item(const PagedAttention& p) {
         t = 0;
@@ -125,14 +128,14 @@ __device__ __forceinline__ long long scan(long long x) {  // sums up to each lan
     return x;
 }
 
-// This warp's piece of the line: units [first, end), of pieces of `per` units, `warps` of which go to a CTA; and the place where it
-// begins.
+// The piece of the line of the CTA's `warp` of `most`: units [first, end), of pieces of `per` units, `warps` of which go to a CTA; and the
+// place where it begins.
 struct Share {
     long long first, end, per;
     int warps;
 };
-template <int KT, bool TREE>
-__device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT, TREE>& at) {
+template <int KT, bool TREE, int COST>
+__device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT, TREE, COST>& at, int warp, int most) {
     const int lane = threadIdx.x & 31;
     auto units = [&](int b) -> long long {
         if (b >= p.batch) return 0;
@@ -140,7 +143,7 @@ __device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT, 
         bool bad;
         const int n = tiles_of<KT, TREE>(p, b, lo, pos, count, bad);
         const int items = TREE ? p.map.kv_heads * parts_of<TREE>(p, count) : p.items;
-        return n > 0 ? (long long)(n + kItemCost) * items : 0;
+        return n > 0 ? (long long)(n + COST) * items : 0;
     };
     // each lane sums up a run of sequences
     const int run = (p.batch + 31) / 32;
@@ -149,11 +152,10 @@ __device__ __forceinline__ Share find_share(const PagedAttention& p, Cursor<KT, 
     for (int i = 0; i < run; ++i) mine += units(lane * run + i);
     const long long upto = scan(mine), total = __shfl_sync(0xffffffffu, upto, 31);
     Share s;
-    const int most = blockDim.x / 32, warp = threadIdx.x / 32;
     s.warps = most;
     s.per = (total + (long long)gridDim.x * most - 1) / ((long long)gridDim.x * most);
-    if (s.per <= kItemCost) {  // a tile at least, and with less than that for every warp all SMs rather than all warps of some
-        s.per = kItemCost + 1;
+    if (s.per <= COST) {  // a tile at least, and with less than that for every warp all SMs rather than all warps of some
+        s.per = COST + 1;
         s.warps = (int)((total + gridDim.x * s.per - 1) / (gridDim.x * s.per));
         s.warps = max(min(s.warps, most), 1);
     }
@@ -230,6 +232,11 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there)
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
 
+// The same where tiles come by TMA: of the pages and the persistent keys as rows of 16-bit pairs.
+struct alignas(64) PagedAttentionBulk : PagedAttention {
+    CUtensorMap k_map, v_map, k_pers_map, v_pers_map;
+};
+
 // A warp's ring: tiles of keys, as many of values, and which of their rows are seen and which have no page; the first key's token (-1:
 // persistent ones); with pages in 8 bits the rows' scales, of the keys and of the values.
 struct Ring {
@@ -237,6 +244,7 @@ struct Ring {
     uint2* marks;
     int* places;
     float* scales;
+    uint32_t arrived;  // with TMA: a barrier for each stage
 };
 template <typename P>
 constexpr bool kScaled = sizeof(P) == 1;
@@ -244,12 +252,13 @@ constexpr bool kScaled = sizeof(P) == 1;
 // Brings a warp's tiles into its ring, one after the other.  Rows that do not count become zeros: whatever stands in a page behind
 // a sequence's end, infinities and NaN among them, reaches no product.  A lane looks its row's page up a tile ahead of the copies
 // that need it.  Where pages are made of sixteens, so are the tiles' runs of memory; else every row is found by itself.
-template <typename P, int KT, bool TREE, typename Layout>
+template <typename P, int KT, bool TREE, int COST, typename Layout>
 struct Loader {
+    static constexpr bool kBulk = false;
     const PagedAttention& p;
     const Ring& ring;
     const Layout& lay;
-    Cursor<KT, TREE> at;
+    Cursor<KT, TREE, COST> at;
     int j0, first, last;  // of the tile: its first key; rows first .. last are seen
     int slot, page;       // of this lane's row
 
@@ -352,6 +361,129 @@ struct Loader {
     }
 };
 
+// The same by TMA, a run of rows at a time: pages made of sixteens, or of eights, hold as many neighbouring tokens as one run of memory, and the
+// hardware puts the chunks of a row where the layout has them.  Where the next 32 runs are every lane finds out for one of them,
+// so a tile costs a handful of instructions of one lane and two shuffles instead of an address and a copy for every sixteen bytes
+// (heads of 64, int8: 311 instructions to a tile of 32 keys with every tile's rows looked up for itself).  What is not seen in a run is
+// brought too: a core has to see to it that it does no harm.
+template <typename P, int KT, bool TREE, int COST, typename Layout>
+struct BulkLoader {
+    static constexpr bool kBulk = true;
+    static_assert(KT == 32, "marks are a word");
+    const PagedAttentionBulk& p;
+    const Ring& ring;
+    const Layout& lay;
+    Cursor<KT, TREE, COST> at;
+    int planned = 1 << 30, page = -1;  // tile of the item whose first run is lane 0's; this lane's page
+    int row = -1;                      // this lane's run among the rows of the pool (of the persistent keys); -1: not wanted, -2: nowhere
+    uint32_t there = 0;                // lanes whose runs are to be brought
+
+    __device__ __forceinline__ int key_of_run(int tile, bool pers) const {
+        return (pers ? tile : at.lo / KT + tile - p.pers_tiles) * KT;
+    }
+    // Looks the pages of the runs from the next tile on up, if that has no plan yet.
+    __device__ __forceinline__ void look() {
+        const int tile = at.tile();
+        if (tile >= planned && tile < planned + p.run) return;  // (32 runs are those of p.run tiles)
+        planned = tile;
+        const int lane = threadIdx.x & 31, r = lane * p.run, mine = tile + r / KT;
+        const bool pers = mine < p.pers_tiles;
+        const int j = key_of_run(mine, pers) + r % KT;
+        page = -1;
+        row = -1;
+        if (mine < at.n - COST && j <= (pers ? p.np - 1 : at.pos) && j + p.run > (pers ? 0 : at.lo)) {
+            row = j;
+            if (!pers) {
+                const uint32_t column = p.map.page.div((uint32_t)j);
+                row = j - (int)(column * p.map.page.d);
+                page = __ldg(p.map.table + at.b * p.map.table_stride + column);
+            }
+        }
+        there = 0;
+    }
+    // A whole plan's rows, once their pages have come.
+    __device__ __forceinline__ void find() {
+        const int lane = threadIdx.x & 31, mine = planned + lane * p.run / KT;
+        if (row >= 0) {
+            if (mine < p.pers_tiles) row += at.head * p.np;
+            else row = (uint32_t)page < (uint32_t)p.map.pages ? (page * p.map.kv_heads + at.head) * (int)p.map.page.d + row : -2;
+        }
+        there = __ballot_sync(0xffffffffu, row >= 0);
+    }
+    __device__ __forceinline__ void issue(int stage) {
+        const int tile = at.tile();
+        const bool pers = tile < p.pers_tiles;
+        if (tile == planned) find();
+        const int runs = KT / p.run, first_run = (tile - planned) * runs;
+        const int j0 = key_of_run(tile, pers), first = pers ? 0 : max(at.lo - j0, 0), last = min((pers ? p.np - 1 : at.pos) - j0, KT - 1);
+        const uint32_t bar = ring.arrived + stage * 8;
+        constexpr int kBoxes = Layout::kBoxes, kHalf = KT * Layout::kBoxBytes;
+        const int box = p.run * Layout::kBoxBytes, here = __popc(there >> first_run & ((1u << runs) - 1));
+        const uint32_t seen = (2u << last) - (1u << first);
+        uint32_t lost = 0;
+        int run[KT / 8];
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+            run[i] = -1;
+            if (i >= 2 && runs == 2) continue;
+            run[i] = __shfl_sync(0xffffffffu, row, first_run + i);
+            if (run[i] == -2) lost |= ((1u << p.run) - 1) << i * p.run;
+        }
+        if (kScaled<P> && pers) {  // scales that need not begin on sixteen bytes
+            const int r = threadIdx.x & 31;
+            const bool mine = r <= last;
+            const int of = at.head * p.np + j0 + r;
+            ring.scales[stage * 2 * KT + r] = mine ? __ldg(p.k_pers_scales + of) : 0.f;
+            ring.scales[stage * 2 * KT + KT + r] = mine ? __ldg(p.v_pers_scales + of) : 0.f;
+            ptx::fence_proxy_async_smem();  // (before the copies of a later tile write there)
+            __syncwarp();
+        }
+        if (ptx::elect_one()) {  // (all of it in one such branch: what one lane alone runs needs no loop over the lanes' operands)
+            ring.marks[stage] = make_uint2(seen, lost & seen);
+            if (TREE) ring.places[stage] = pers ? -1 : j0;
+            const uint32_t keys = (uint32_t)__cvta_generic_to_shared(ring.tiles) + stage * 2 * KT * Layout::pitch();
+            const uint32_t scales = (uint32_t)__cvta_generic_to_shared(ring.scales) + stage * 2 * KT * 4;
+            const CUtensorMap *k = pers ? &p.k_pers_map : &p.k_map, *v = pers ? &p.v_pers_map : &p.v_map;
+            const int scale_bytes = kScaled<P> && !pers ? p.run * 4 : 0;
+            ptx::mbar_expect_tx(bar, here * 2 * (kBoxes * box + scale_bytes));
+#pragma unroll
+            for (int i = 0; i < KT / 8; ++i) {
+                if (run[i] < 0) continue;
+#pragma unroll
+                for (int c = 0; c < kBoxes; ++c) {
+                    ptx::tma_load_2d(keys + c * kHalf + i * box, k, bar, c * Layout::kBoxBytes / 2, run[i]);
+                    ptx::tma_load_2d(keys + KT * Layout::pitch() + c * kHalf + i * box, v, bar, c * Layout::kBoxBytes / 2, run[i]);
+                }
+                if (kScaled<P> && !pers) {
+                    ptx::bulk_load(scales + i * scale_bytes, p.k_scales + run[i], scale_bytes, bar);
+                    ptx::bulk_load(scales + KT * 4 + i * scale_bytes, p.v_scales + run[i], scale_bytes, bar);
+                }
+            }
+        }
+    }
+};
+
+// queries and outputs of either 16-bit type, which p.bf16 tells apart
+struct Any16 {
+    uint16_t bits;
+};
+template <typename T>
+__device__ __forceinline__ void put(const PagedAttention& p, T* to, float x) {
+    if constexpr (std::is_same<T, Any16>::value) {
+        to->bits = p.bf16 ? __bfloat16_as_ushort(from_f32<__nv_bfloat16>(x)) : __half_as_ushort(from_f32<__half>(x));
+    } else {
+        *to = from_f32<T>(x);
+    }
+}
+template <typename T>
+__device__ __forceinline__ float get(const PagedAttention& p, const T* from) {
+    if constexpr (std::is_same<T, Any16>::value) {
+        return p.bf16 ? __uint_as_float((uint32_t)from->bits << 16) : __half2float(__ushort_as_half(from->bits));
+    } else {
+        return to_f32<T>(*from);
+    }
+}
+
 // ---- the core on CUDA cores: every type, head_dim a multiple of 8 --------------------------------------------------------
 // Lane l has key l % 16 of a tile and one half of the head's dimensions of its scores; then the four dimensions from 4 l on (and
 // from 128 + 4 l, with QUADS 2) of the outputs.  kRows query heads, their numbers as fp32 in shared memory.
@@ -404,6 +536,9 @@ template <typename T, typename P, int ROWS, int QUADS, bool TREE = false>
 struct SimtCore {
     static constexpr int kRows = ROWS, KT = 16;
     using Layout = SimtLayout<P>;
+    static constexpr int kItemCost = 1;
+    using Load = Loader<P, KT, TREE, kItemCost, Layout>;
+    using Args = PagedAttention;
     const PagedAttention& p;
     float* q;        // [kRows][head_dim], of the CTA's warp
     float* weights;  // [KT][kRows]
@@ -426,7 +561,7 @@ struct SimtCore {
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const T* from = static_cast<const T*>(p.q) + row_at<TREE>(p, p.qs, of, r);
-            for (int i = lane; i < dim; i += 32) q[r * dim + i] = r < of.n ? to_f32<T>(from[i]) : 0.f;
+            for (int i = lane; i < dim; i += 32) q[r * dim + i] = r < of.n ? get(p, from + i) : 0.f;
             if constexpr (TREE) {
                 const int node = (of.first + r) / p.group;
                 low[r] = r < of.n ? first_seen(p, of.b, start, node) : 0;
@@ -536,10 +671,34 @@ struct SimtCore {
             const float scale = inverse_of<TREE>(p, rows, r, sum);
             T* at = static_cast<T*>(p.o) + row_at<TREE>(p, p.os, rows, r) + d;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) at[e] = from_f32<T>(x[e] * scale);
+            for (int e = 0; e < 4; ++e) put(p, at + e, x[e] * scale);
         });
     }
 };
+
+// Four codes as fp16 numbers, two to a register: the first and third, the second and fourth.  (int8 as subnormal numbers, a byte with its
+// sign bit turned over as it stands: two instructions less, but then 128 too much, and sums that begin at what takes it off wait for the
+// weights' own sum: 8 x 40000 tokens of 32 heads on 4 of 128 86 us instead of 80.)
+template <typename P>
+__device__ __forceinline__ void to_pairs(uint32_t w, uint32_t& even, uint32_t& odd);
+template <>
+__device__ __forceinline__ void to_pairs<int8_t>(uint32_t w, uint32_t& even, uint32_t& odd) {
+    w ^= 0x80808080u;  // 0 .. 255 under the exponent of 1024, less 1024 + 128
+    const uint32_t bias = 0x64806480u;
+    const auto less = [&](uint32_t x) {
+        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    };
+    even = less(__byte_perm(w, 0x64646464u, 0x4240));
+    odd = less(__byte_perm(w, 0x64646464u, 0x4341));
+}
+template <>
+__device__ __forceinline__ void to_pairs<E4m3>(uint32_t w, uint32_t& even, uint32_t& odd) {
+    w = __byte_perm(w, w, 0x3120);
+    const __half2 a = from_e4m3(w), b = from_e4m3(w >> 16);
+    even = *reinterpret_cast<const uint32_t*>(&a);
+    odd = *reinterpret_cast<const uint32_t*>(&b);
+}
 
 // ---- the core on tensor cores: 16-bit types, head_dim 16, 32, 64, 80, 96, 128, 192 or 256 -------------------------------------------------
 // mma.sync with the keys, then the dimensions of the values, as the sixteen rows of a tile and eight query heads as its columns
@@ -653,6 +812,9 @@ struct MmaCore {
     static constexpr int kRows = kMaxRows, KT = DH > 128 ? 16 : 32;
     static constexpr float kRaise = std::is_same<T, __half>::value ? 12.f : 0.f;
     using Layout = MmaLayout<DH>;
+    static constexpr int kItemCost = 1;
+    using Load = Loader<T, KT, false, kItemCost, Layout>;
+    using Args = PagedAttention;
     const PagedAttention& p;
     uint32_t q[EIGHTS][DH / 16][2];
     float m[EIGHTS][2], l[EIGHTS][2];  // l: of this lane's keys
@@ -852,9 +1014,14 @@ struct Part {
 };
 
 template <typename T, typename P, bool TREE, typename Core, int W, int S>  // up to W warps
-__global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_constant__ PagedAttention p) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int KT = Core::KT;
+__global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_constant__ typename Core::Args p) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    constexpr int KT = Core::KT, COST = Core::kItemCost;
+    constexpr bool kBulk = Core::Load::kBulk;
+    __shared__ alignas(8) uint64_t arrived[W][kBulk ? S : 1];
+    __shared__ int given_up;
+    // (what TMA writes turns its chunks by the address: tiles on 1024 bytes)
+    unsigned char* smem = kBulk ? dynamic + (1024 - (uint32_t)__cvta_generic_to_shared(dynamic)) % 1024 : dynamic;
     __shared__ uint2 marks[W][S];
     __shared__ int places[W][TREE ? S : 1];
     __shared__ Part parts[2 * W];
@@ -863,39 +1030,53 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
     const typename Core::Layout lay{p.row_bytes};
     const int tile_bytes = S * 2 * KT * lay.pitch(), ring_bytes = tile_bytes + (kScaled<P> ? S * 2 * KT * (int)sizeof(float) : 0);
     const int extra = Core::extra(dim);
-    unsigned char* mine = smem + warp * (ring_bytes + extra);
-    const Ring ring{mine, marks[warp], places[warp], reinterpret_cast<float*>(mine + tile_bytes)};
+    // a warp's tiles and scales; or the tiles of all of them, then all scales
+    const int step = kBulk ? tile_bytes : ring_bytes + extra;
+    unsigned char* mine = smem + warp * step;
+    unsigned char* scales = kBulk ? smem + warps * tile_bytes + warp * (ring_bytes - tile_bytes) : mine + tile_bytes;
+    const Ring ring{mine, marks[warp], places[warp], reinterpret_cast<float*>(scales), (uint32_t)__cvta_generic_to_shared(arrived[warp])};
     float2* part_sums = reinterpret_cast<float2*>(smem + warps * (ring_bytes + extra));  // [2 * warps][rows]
     // a warp's first part [rows][head_dim] goes through memory; its second one, made when all its tiles are done, where they were
     auto part_out = [&](int w, int which) {
         return which == 0 ? p.firsts + (blockIdx.x * warps + w) * (long long)p.rows * dim
-                          : reinterpret_cast<float*>(smem + w * (ring_bytes + extra));
+                          : reinterpret_cast<float*>(smem + w * step);
     };
 
     if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (lane < 2) parts[2 * warp + lane].there = 0;
+    if constexpr (kBulk) {
+        if (tid == 0) given_up = 0;
+        if (lane < S) ptx::mbar_init(ring.arrived + lane * 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        ptx::fence_proxy_async_smem();
+        __syncthreads();
+    }
     __syncwarp();
 
-    Cursor<KT, TREE> at;
-    const Share share = find_share<KT, TREE>(p, at);
+    Cursor<KT, TREE, COST> at;
+    const Share share = find_share<KT, TREE, COST>(p, at, warp, warps);
     if (share.first < share.end) {
-        Loader<P, KT, TREE, typename Core::Layout> ahead{p, ring, lay, at};  // of the tile to load next, unit `load` of the line
+        typename Core::Load ahead{p, ring, lay, at};  // of the tile to load next, unit `load` of the line
         long long load = share.first;
         int stage_in = 0, stage_out = 0;
+        uint32_t phase = 0;  // a bit for each stage
         auto look = [&]() {
-            if (load < share.end && ahead.at.t < kItemCost) {
-                load += kItemCost - ahead.at.t;
-                ahead.at.t = kItemCost;
+            if (load < share.end && ahead.at.t < COST) {
+                load += COST - ahead.at.t;
+                ahead.at.t = COST;
             }
             if (load < share.end) ahead.look();
         };
         auto fetch = [&]() {
             if (load < share.end) {
                 ahead.issue(stage_in);
-                if (++load < share.end && ++ahead.at.t == ahead.at.n) ahead.at.next_item(p);
+                if (++load < share.end && ++ahead.at.t == ahead.at.n) {
+                    ahead.at.next_item(p);
+                    if constexpr (kBulk) ahead.planned = 1 << 30;
+                }
                 look();
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if constexpr (!kBulk) asm volatile("cp.async.commit_group;" ::: "memory");
             stage_in = stage_in + 1 == S ? 0 : stage_in + 1;
         };
         look();
@@ -903,7 +1084,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
         for (int s = 0; s < S - 1; ++s) fetch();
 
         Core core(p, mine + ring_bytes);
-        auto queries = [&](const Cursor<KT, TREE>& c) {
+        auto queries = [&](const Cursor<KT, TREE, COST>& c) {
             const Rows rows = rows_of<TREE>(p, c.b, c.head, c.item - c.head * c.parts(p), c.count);
             core.load_queries(rows, c.count);
             return rows;
@@ -913,10 +1094,14 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
         Rows rows = queries(at);
         while (begin < share.end) {
             const long long item_end = begin + (at.n - at.t), end = item_end < share.end ? item_end : share.end;
-            const int tiles = (int)(end - begin) - max(kItemCost - at.t, 0);
+            const int tiles = (int)(end - begin) - max(COST - at.t, 0);
             core.reset();
             for (int i = 0; i < tiles; ++i) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+                if constexpr (!kBulk) asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+                if constexpr (kBulk) {
+                    ptx::mbar_wait(ring.arrived + stage_out * 8, phase >> stage_out & 1, &given_up, p.status);
+                    phase ^= 1u << stage_out;
+                }
                 __syncwarp();
                 fetch();
                 const uint2 mark = ring.marks[stage_out];
@@ -924,7 +1109,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
                 core.tile(ring, stage_out, mark, lay);
                 stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
             }
-            const Cursor<KT, TREE> done = at;
+            const Cursor<KT, TREE, COST> done = at;
             const Rows done_rows = rows;
             if (item_end < share.end) {  // the next item's queries load while this one's results are stored
                 at.next_item(p);
@@ -932,7 +1117,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
             }
             begin = end;
             if (tiles <= 0) continue;
-            const bool starts = done.t <= kItemCost, ends = end == item_end;
+            const bool starts = done.t <= COST, ends = end == item_end;
             if (starts && ends) {
                 core.store(done_rows);
             } else {
@@ -984,10 +1169,10 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
             if (starts && ends) {
                 T* to = static_cast<T*>(p.o) + row_at<TREE>(p, p.os, rows, r) + (x * 4 - r * dim);
                 const float scale = inverse_of<TREE>(p, rows, r, l);
-                to[0] = from_f32<T>(o.x * scale);
-                to[1] = from_f32<T>(o.y * scale);
-                to[2] = from_f32<T>(o.z * scale);
-                to[3] = from_f32<T>(o.w * scale);
+                put(p, to + 0, o.x * scale);
+                put(p, to + 1, o.y * scale);
+                put(p, to + 2, o.z * scale);
+                put(p, to + 3, o.w * scale);
             } else {
                 reinterpret_cast<float4*>(p.partial + slot * dim)[x] = o;
                 if (x * 4 == r * dim) p.sums[slot + r] = make_float2(m, l);
@@ -1011,7 +1196,7 @@ __global__ void __launch_bounds__(W * 32) paged_attention_kernel(const __grid_co
             const int d = i % dim, row = i / dim, node = TREE ? row / heads : 0, h = row - node * heads;
             T* to = static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + d;
             if (TREE) to += node * p.os[2];
-            *to = from_f32<T>(bad ? CUDART_NAN_F : 0.f);
+            put(p, to, bad ? CUDART_NAN_F : 0.f);
         }
     }
 }
@@ -1078,10 +1263,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     }
     const float scale = inverse_of<TREE>(p, rows, r, sum);
     T* to = static_cast<T*>(p.o) + row_at<TREE>(p, p.os, rows, r) + d;
-    to[0] = from_f32<T>(out.x * scale);
-    to[1] = from_f32<T>(out.y * scale);
-    to[2] = from_f32<T>(out.z * scale);
-    to[3] = from_f32<T>(out.w * scale);
+    put(p, to + 0, out.x * scale);
+    put(p, to + 1, out.y * scale);
+    put(p, to + 2, out.z * scale);
+    put(p, to + 3, out.w * scale);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -1090,6 +1275,42 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
 // way, and they come from L2 twice (32 heads on 4, 553,000 tokens, rings of three tiles in 226 KB: 231 us when this took 189).  Head
 // size 64 has eleven warps here; with twelve its 256 windows of 512 take the same 68.5 us.
 constexpr int kMostShared = 193 * 1024 + 512;
+// What TMA brings does not go through L1.
+constexpr int kMostSharedBulk = 216 * 1024;
+
+// Keys and values as TMA's swizzles leave their rows: boxes of 128, 64 or 32 bytes, one behind the other for all 32 rows, the sixteen-byte
+// chunks of a row turned so that eight rows' same chunk stands on different banks.
+template <int ROWB>
+struct BoxLayout {
+    int bytes;
+    static constexpr int kBoxBytes = ROWB % 128 == 0 ? 128 : ROWB % 64 == 0 ? 64 : 32, kBoxes = ROWB / kBoxBytes, kInBox = kBoxBytes / 16;
+    __host__ __device__ static constexpr int pitch() { return ROWB; }
+    __host__ __device__ static constexpr int chunks() { return ROWB / 16; }
+    __device__ __forceinline__ static int turn(int r) { return kInBox == 8 ? r & 7 : kInBox == 4 ? r >> 1 & 3 : r >> 2 & 1; }
+    __device__ __forceinline__ static int offset(int r, int c) {
+        return c / kInBox * 32 * kBoxBytes + r * kBoxBytes + ((c % kInBox ^ turn(r)) << 4);
+    }
+};
+
+// the maps of what TMA reads, rows of pairs of bytes; none of what does not exist
+template <typename Layout>
+bool make_maps(const tmw_paged_attention_desc& d, PagedAttentionBulk& p) {
+    const CUtensorMapSwizzle turns = Layout::kBoxBytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : Layout::kBoxBytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                               : CU_TENSOR_MAP_SWIZZLE_32B;
+    const auto make = [&](CUtensorMap* map, const void* base, int rows) {
+        return rows == 0 || make_map_2d(map, base, TMW_F16, rows, Layout::pitch() / 2, Layout::pitch() / 2, p.run, Layout::kBoxBytes / 2, turns);
+    };
+    const int rows = d.at.pages * d.at.kv_heads * d.at.page_size, pers = d.at.kv_heads * d.n_persistent;
+    return make(&p.k_map, d.at.k_pages, rows) && make(&p.v_map, d.at.v_pages, rows) && make(&p.k_pers_map, d.k_pers, pers) &&
+           make(&p.v_pers_map, d.v_pers, pers);
+}
+// whether pages can come by TMA: runs of eight neighbours at least, rows numbered in 32 bits, scales that begin on sixteen bytes
+inline bool can_bulk(const tmw_paged_attention_desc& d, const tmw_page_scales& s) {
+    return d.at.page_size % 8 == 0 && (reinterpret_cast<uintptr_t>(s.k_scales) | reinterpret_cast<uintptr_t>(s.v_scales)) % 16 == 0 &&
+           (long long)d.at.pages * d.at.kv_heads * d.at.page_size <= 0x7fffffffLL - 32 &&
+           (long long)d.at.kv_heads * d.n_persistent <= 0x7fffffffLL - 32;
+}
 
 struct Plan {
     int rows, parts, warps, grid, smem;
@@ -1098,6 +1319,7 @@ struct Plan {
 
 template <typename T, typename P, bool TREE, typename Core, int W, int S>
 struct Kernel {
+    using CoreOf = Core;
     static constexpr int KT = Core::KT;
     // nodes: drafted ones of a sequence, 1 without
     static Plan plan(const tmw_paged_attention_desc& d, int row_bytes, int nodes) {
@@ -1107,8 +1329,9 @@ struct Kernel {
         n.rows = (group + n.parts - 1) / n.parts;
         const int tile = S * 2 * KT * (typename Core::Layout{row_bytes}.pitch() + (kScaled<P> ? (int)sizeof(float) : 0));
         const int warp = tile + Core::extra(d.at.head_dim) + 2 * n.rows * (int)sizeof(float2);
-        n.warps = kMostShared / warp < W ? kMostShared / warp : W;
-        n.smem = n.warps * warp;
+        constexpr int most = Core::Load::kBulk ? kMostSharedBulk - 1024 : kMostShared;
+        n.warps = most / warp < W ? most / warp : W;
+        n.smem = n.warps * warp + (Core::Load::kBulk ? 1024 : 0);
         // no more CTAs than the longest sequences could have work for
         const long long capacity = (long long)d.at.columns * d.at.page_size;
         const long long keys = d.window >= 0 && d.window + (long long)nodes < capacity ? d.window + (long long)nodes : capacity;
@@ -1121,7 +1344,7 @@ struct Kernel {
         n.bytes = n.firsts_at + (size_t)n.grid * n.warps * out;
         return n;
     }
-    static int launch(PagedAttention& p, const Plan& n, unsigned char* scratch, cudaStream_t stream) {
+    static int launch(typename Core::Args& p, const Plan& n, unsigned char* scratch, cudaStream_t stream) {
         p.rows = n.rows;
         p.parts = n.parts;
         p.items = p.map.kv_heads * n.parts;
@@ -1137,7 +1360,7 @@ struct Kernel {
         TMW_CUDA_TRY(cudaGetLastError());
         if (n.grid > 1)
             TMW_CUDA_TRY(launch_ex(paged_join_kernel<T, TREE>, dim3((unsigned)n.grid - 1, (unsigned)(n.rows * ((p.map.head_dim + 127) / 128))),
-                                   dim3(kJoinWarps * 32), 0, stream, true, 1, p));
+                                   dim3(kJoinWarps * 32), 0, stream, true, 1, static_cast<const PagedAttention&>(p)));
         return TMW_OK;
     }
 };
@@ -1199,7 +1422,9 @@ inline int arguments(const tmw_paged_attention_desc& d, const tmw_page_scales& s
     }
     p.pos = d.pos;
     p.batch = d.at.batch; p.np = d.n_persistent; p.window = d.window;
+    p.bf16 = d.at.dtype == TMW_BF16;
     p.whole_runs = d.at.page_size % 16 == 0;
+    p.run = d.at.page_size % 16 == 0 ? 16 : d.at.page_size % 8 == 0 ? 8 : 0;
     p.group = d.heads / d.at.kv_heads;
     p.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.at.head_dim)) * 1.4426950408889634f;
     p.row_bytes = d.at.head_dim * (scales.format == 0 ? (int)size : 1);

@@ -1,4 +1,6 @@
-// Attention of one new token per sequence over pages in 8 bits (tmw_paged_attention_scaled): which kernel takes a call.
+// Attention of one new token per sequence over pages in 8 bits: the core on tensor cores, and which kernel takes a call.
+#pragma once
+
 #include "paged_attention.cuh"
 
 namespace tmw {
@@ -21,43 +23,20 @@ namespace {
 // HEADS: of an item at most, 1, 2, 4, 8 or 16.  With fewer than eight the columns hold them several times over, and each of the 8 / HEADS
 // copies deals with its own share of the tile's keys: its weights are zero in the rows of the others', its running maximum
 // is its own, and the copies are added up when the item ends.  So a lane has KT HEADS / 32 exponentials to a tile instead of KT / 4.
-template <int DH>
-struct Mma8Layout {
-    int bytes;
-    static constexpr int kChunks = DH / 16;
-    static constexpr bool kTurned = (kChunks & (kChunks - 1)) == 0;
-    __host__ __device__ static constexpr int pitch() { return DH + (kTurned ? 0 : 16); }
-    __host__ __device__ static constexpr int chunks() { return kChunks; }
-    // eight rows' same chunk stands on different banks: by its place in the row, or by rows of an odd number of chunks
-    __device__ __forceinline__ static int offset(int r, int c) {
-        const int turn = !kTurned ? 0 : kChunks >= 8 ? r & 7 : kChunks == 4 ? r >> 1 & 3 : r >> 2 & 1;
-        return r * pitch() + ((c ^ turn) << 4);
-    }
-};
-
-// Four codes as fp16 numbers, two to a register: the first and third, the second and fourth.
-template <typename P>
-__device__ __forceinline__ void to_pairs(uint32_t w, uint32_t& even, uint32_t& odd);
-template <>
-__device__ __forceinline__ void to_pairs<int8_t>(uint32_t w, uint32_t& even, uint32_t& odd) {
-    w ^= 0x80808080u;  // 0 .. 255 under the exponent of 1024, less 1024 + 128
-    const uint32_t bias = 0x64806480u;
-    const auto less = [&](uint32_t x) {
-        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
-        return *reinterpret_cast<const uint32_t*>(&d);
-    };
-    even = less(__byte_perm(w, 0x64646464u, 0x4240));
-    odd = less(__byte_perm(w, 0x64646464u, 0x4341));
+// d = a b + c for one 16 x 8 x 16 tile, and d += a b (not volatile: in whichever order the results are needed)
+__device__ __forceinline__ void mma_more(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <>
-__device__ __forceinline__ void to_pairs<E4m3>(uint32_t w, uint32_t& even, uint32_t& odd) {
-    w = __byte_perm(w, w, 0x3120);
-    const __half2 a = from_e4m3(w), b = from_e4m3(w >> 16);
-    even = *reinterpret_cast<const uint32_t*>(&a);
-    odd = *reinterpret_cast<const uint32_t*>(&b);
+__device__ __forceinline__ void mma_onto(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                         float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-template <typename T, typename P, int DH, int HEADS>
+template <typename P, int DH, int HEADS, bool BULK>
 struct Mma8Core {
     static constexpr int kRows = HEADS, KT = 32, kChunks = DH / 16;
     static constexpr int EIGHTS = HEADS > 8 ? 2 : 1, kCopies = HEADS < 8 ? 8 / HEADS : 1;
@@ -65,7 +44,10 @@ struct Mma8Core {
     static constexpr int kOfLane = HEADS == 1 ? 1 : 2;                     // heads of each eight
     static constexpr int kTerms8 = HEADS == 1 ? 1 : 2;  // products of a weight with the values
     static constexpr float kRaise = 12.f;  // as far as fp16 allows: a weight is at most 2^13
-    using Layout = Mma8Layout<DH>;
+    using Layout = BoxLayout<DH>;
+    static constexpr int kItemCost = 2;
+    using Load = std::conditional_t<BULK, BulkLoader<P, KT, false, kItemCost, Layout>, Loader<P, KT, false, kItemCost, Layout>>;
+    using Args = std::conditional_t<BULK, PagedAttentionBulk, PagedAttention>;
     const PagedAttention& p;
     uint32_t q[EIGHTS][kChunks][2];
     float q_scale[EIGHTS][2];
@@ -80,7 +62,7 @@ struct Mma8Core {
 #pragma unroll
         for (int h = 0; h < EIGHTS; ++h) {
             const int r = h * 8 + lane / 4 % HEADS;
-            const T* from = static_cast<const T*>(p.q) + row_at<false>(p, p.qs, of, r) + lane % 4 * 4;
+            const uint16_t* from = static_cast<const uint16_t*>(p.q) + row_at<false>(p, p.qs, of, r) + lane % 4 * 4;
             uint32_t raw[kChunks][2];
             float top = 0.f;
 #pragma unroll
@@ -89,16 +71,15 @@ struct Mma8Core {
                 for (int i = 0; i < 2; ++i) {
                     uint32_t w = 0;
                     if (r < of.n) {
-                        const T* at = from + k * 16 + i * 2;
-                        if (p.q_pairs) w = *reinterpret_cast<const uint32_t*>(at);
-                        else w = *reinterpret_cast<const uint16_t*>(at) | (uint32_t)*reinterpret_cast<const uint16_t*>(at + 1) << 16;
+                        const uint16_t* at = from + k * 16 + i * 2;
+                        w = p.q_pairs ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16;
                     }
                     raw[k][i] = w;
-                    const float2 x = unpack2<T>(w);
+                    const float2 x = unpack2<__nv_bfloat16>(w);
                     top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
                 }
             float scale = p.scale;
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            if (p.bf16) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // the largest number becomes one from 2^14 on; an infinite one stays infinite
@@ -109,7 +90,7 @@ struct Mma8Core {
                 for (int k = 0; k < kChunks; ++k)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float2 x = unpack2<T>(raw[k][i]);
+                        const float2 x = unpack2<__nv_bfloat16>(raw[k][i]);
                         raw[k][i] = pack2<__half>(x.x * up, x.y * up);
                     }
             }
@@ -137,26 +118,30 @@ struct Mma8Core {
         const int lane = threadIdx.x & 31;
         const uint32_t keys = (uint32_t)__cvta_generic_to_shared(ring.tiles + stage * 2 * KT * Layout::pitch()), values = keys + KT * Layout::pitch();
         const float* scales = ring.scales + stage * 2 * KT + lane / 4;
+        // of the lane's row and the first chunk of two, turned: two chunks further on is another number in the same bits, or the next box
+        const uint32_t lane_at = Layout::offset(lane & 15, lane >> 4);
+        const auto chunk_at = [&](int g, int k) {
+            constexpr int in = Layout::kInBox;
+            return (lane_at ^ (k % in << 4)) + k / in * KT * Layout::kBoxBytes + g * 16 * Layout::kBoxBytes;
+        };
         float s[EIGHTS][KT / 16][4];  // of each sixteen: keys lane / 4 and 8 + lane / 4, both heads each
-#pragma unroll
-        for (int h = 0; h < EIGHTS; ++h)
-#pragma unroll
-            for (int g = 0; g < KT / 16; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[h][g][i] = 0.f;
 #pragma unroll
         for (int k = 0; k < kChunks; k += 2)
 #pragma unroll
             for (int g = 0; g < KT / 16; ++g) {
                 uint32_t a[4];
-                ldmatrix4(a, keys + lay.offset(g * 16 + (lane & 15), k + (lane >> 4)));
+                ldmatrix4(a, keys + chunk_at(g, k));
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t even[2], odd[2];
                     to_pairs<P>(a[2 * c], even[0], odd[0]);
                     to_pairs<P>(a[2 * c + 1], even[1], odd[1]);
 #pragma unroll
-                    for (int h = 0; h < EIGHTS; ++h) mma_16816<__half>(s[h][g], even[0], even[1], odd[0], odd[1], q[h][k + c][0], q[h][k + c][1]);
+                    for (int h = 0; h < EIGHTS; ++h) {
+                        const uint32_t(&b)[2] = q[h][k + c];
+                        if (k + c == 0) mma_onto(s[h][g], even[0], even[1], odd[0], odd[1], b[0], b[1], 0.f, 0.f, 0.f, 0.f);
+                        else mma_more(s[h][g], even[0], even[1], odd[0], odd[1], b[0], b[1]);
+                    }
                 }
             }
         // this lane's keys, with the values' scales in their two parts
@@ -170,7 +155,7 @@ struct Mma8Core {
             const int bits = __float_as_int(fmaxf(vs, 0x1p-100f));
             e[j] = __int_as_float(0x4b000000 | (bits >> 23)) - (8388608.f + 127.f) + (vs - vs);  // (NaN stays that)
             f[j] = __int_as_float((bits & 0x007fffff) | 0x3f800000);
-            back[j] = __int_as_float(0x7f000000 - (bits & 0x7f800000));
+            back[j] = __int_as_float(0x7f000000 - min(bits & 0x7f800000, 0x7e800000));  // (finite under keys that are not seen)
         }
         // all heads side by side: their chains of shuffles and exponentials overlap
         uint32_t weights[EIGHTS][KT / 16][2][kTerms8];
@@ -186,15 +171,26 @@ struct Mma8Core {
                     if constexpr (kCopies == 1) x = s[h][j / 2][j % 2 * 2 + a];
                     else if constexpr (kCopies == 2) x = t < 2 ? s[h][0][j * 2 + a] : s[h][1][j * 2 + a];
                     else x = t < 2 ? (t == 0 ? s[h][0][a] : s[h][0][2 + a]) : (t == 2 ? s[h][1][a] : s[h][1][2 + a]);
-                    x = fmaf(x * ks[j], q_scale[h][a], e[j]);
-                    if (marks.x != 0xffffffffu || marks.y != 0) {
-                        const int key = key_of(j) + lane / 4;
-                        x = marks.y >> key & 1 ? CUDART_NAN_F : marks.x >> key & 1 ? x : -CUDART_INF_F;
-                    }
-                    w[h][j][a] = x;
-                    top[h][a] = fmaxf(top[h][a], x);
+                    w[h][j][a] = fmaf(x * ks[j], q_scale[h][a], e[j]);
                 }
             }
+        if (marks.x != 0xffffffffu || marks.y != 0) {
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j) {
+                const int key = key_of(j) + lane / 4;
+                const bool seen = marks.x >> key & 1, bad = marks.y >> key & 1;
+#pragma unroll
+                for (int h = 0; h < EIGHTS; ++h)
+#pragma unroll
+                    for (int a = 0; a < kOfLane; ++a) w[h][j][a] = bad ? CUDART_NAN_F : seen ? w[h][j][a] : -CUDART_INF_F;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < EIGHTS; ++h)
+#pragma unroll
+            for (int a = 0; a < kOfLane; ++a)
+#pragma unroll
+                for (int j = 0; j < kKeys; ++j) top[h][a] = fmaxf(top[h][a], w[h][j][a]);
 #pragma unroll
         for (int d = 4; d < 32; d *= 2)
 #pragma unroll
@@ -249,35 +245,48 @@ struct Mma8Core {
                         weights[h][g][i][n] = turned(x);
                     }
         }
+        if constexpr (BULK && std::is_same<P, E4m3>::value) {
+            // rows that are not seen may hold codes that are no number, and nothing times these is no number either
+            const uint32_t want = marks.x & ~marks.y;
+            if (want != 0xffffffffu) {
+                if ((want >> lane & 1) == 0) {
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + lay.offset(lane, c)), "r"(0) : "memory");
+                }
+                ptx::fence_proxy_async_smem();  // (before TMA writes there again)
+                __syncwarp();
+            }
+        }
 #pragma unroll
         for (int k = 0; k < kChunks; k += 2) {
             uint32_t a[KT / 16][4];
 #pragma unroll
-            for (int g = 0; g < KT / 16; ++g) ldmatrix4_trans(a[g], values + lay.offset(g * 16 + (lane & 15), k + (lane >> 4)));
+            for (int g = 0; g < KT / 16; ++g) ldmatrix4_trans(a[g], values + chunk_at(g, k));
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float sum[KT / 16][EIGHTS][4];  // of this tile
+                float sum[EIGHTS][KT / 16][4];  // of this tile, one chain of products for each sixteen keys
 #pragma unroll
                 for (int g = 0; g < KT / 16; ++g) {
                     uint32_t even[2], odd[2];
                     to_pairs<P>(a[g][2 * c], even[0], odd[0]);
                     to_pairs<P>(a[g][2 * c + 1], even[1], odd[1]);
 #pragma unroll
-                    for (int h = 0; h < EIGHTS; ++h) {
+                    for (int h = 0; h < EIGHTS; ++h)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[g][h][i] = 0.f;
-#pragma unroll
-                        for (int n = 0; n < kTerms8; ++n)
-                            mma_16816<__half>(sum[g][h], even[0], odd[0], even[1], odd[1], weights[h][g][0][n], weights[h][g][1][n]);
-                    }
+                        for (int n = 0; n < kTerms8; ++n) {
+                            const uint32_t b0 = weights[h][g][0][n], b1 = weights[h][g][1][n];
+                            if (n == 0) mma_onto(sum[h][g], even[0], odd[0], even[1], odd[1], b0, b1, 0.f, 0.f, 0.f, 0.f);
+                            else mma_more(sum[h][g], even[0], odd[0], even[1], odd[1], b0, b1);
+                        }
                 }
 #pragma unroll
                 for (int h = 0; h < EIGHTS; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float x = sum[0][h][i];
+                        float x = sum[h][0][i];
 #pragma unroll
-                        for (int g = 1; g < KT / 16; ++g) x += sum[g][h][i];
+                        for (int g = 1; g < KT / 16; ++g) x += sum[h][g][i];
                         o[h][k + c][i] = fmaf(o[h][k + c][i], keep[h][i & 1], x);
                     }
             }
@@ -323,89 +332,86 @@ struct Mma8Core {
     __device__ __forceinline__ void store(const Rows& rows) {
         results(rows, [&](int r, float, float sum, int d, const float (&x)[2]) {
             const float scale = inverse(sum);
-            T* at = static_cast<T*>(p.o) + row_at<false>(p, p.os, rows, r) + d;
+            Any16* at = static_cast<Any16*>(p.o) + row_at<false>(p, p.os, rows, r) + d;
             if (p.o_pairs) {
-                *reinterpret_cast<uint32_t*>(at) = pack2<T>(x[0] * scale, x[1] * scale);
+                const uint32_t b = pack2<__nv_bfloat16>(x[0] * scale, x[1] * scale), h = pack2<__half>(x[0] * scale, x[1] * scale);
+                *reinterpret_cast<uint32_t*>(at) = p.bf16 ? b : h;
             } else {
-                at[0] = from_f32<T>(x[0] * scale);
-                at[1] = from_f32<T>(x[1] * scale);
+                put(p, at, x[0] * scale);
+                put(p, at + 1, x[1] * scale);
             }
         });
     }
 };
 
-// as many heads as a group has, the next power of two of them
-template <typename T, typename P, int DH, typename F>
-int with_mma(const tmw_paged_attention_desc& d, F&& use) {
+// Pages made of eights or sixteens come by TMA, with as many heads as a group has, the next power of two of them; others by copies of sixteen bytes, with
+// eight or sixteen heads.
+template <typename P, int DH, typename F>
+int with_mma(const tmw_paged_attention_desc& d, bool bulk, F&& use) {
     constexpr int W = DH > 128 ? 6 : DH > 64 ? 12 : 16;
     const int group = d.heads / d.at.kv_heads;
-    if (group == 1) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 1>, W, 2>());
-    if (group == 2) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 2>, W, 2>());
-    if (group <= 4) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 4>, W, 2>());
-    if (group <= 8) return use(Kernel<T, P, false, Mma8Core<T, P, DH, 8>, W, 2>());
-    return use(Kernel<T, P, false, Mma8Core<T, P, DH, 16>, (DH > 64 ? W : 12), 2>());
-}
-template <typename T, typename P, typename F>
-int with_16_bits(const tmw_paged_attention_desc& d, F&& use) {
-    if constexpr (sizeof(T) == 2) {
-        switch (d.at.head_dim) {
-            case 32: return with_mma<T, P, 32>(d, use);
-            case 64: return with_mma<T, P, 64>(d, use);
-            case 96: return with_mma<T, P, 96>(d, use);
-            case 128: return with_mma<T, P, 128>(d, use);
-            case 256: return with_mma<T, P, 256>(d, use);
-        }
+    if (!bulk) {
+        if (group <= 8) return use(Kernel<Any16, P, false, Mma8Core<P, DH, 8, false>, W, 2>());
+        return use(Kernel<Any16, P, false, Mma8Core<P, DH, 16, false>, (DH > 64 ? W : 12), 2>());
     }
-    return with_simt<T, P, false>(d, 1, use);
-}
-template <typename T, typename F>
-int with_pages(const tmw_paged_attention_desc& d, const tmw_page_scales& s, F&& use) {
-    return s.format == TMW_PAGES_INT8 ? with_16_bits<T, int8_t>(d, use) : with_16_bits<T, E4m3>(d, use);
+    if (group == 1) return use(Kernel<Any16, P, false, Mma8Core<P, DH, 1, true>, W, 2>());
+    if (group == 2) return use(Kernel<Any16, P, false, Mma8Core<P, DH, 2, true>, W, 2>());
+    if (group <= 4) return use(Kernel<Any16, P, false, Mma8Core<P, DH, 4, true>, W, 2>());
+    if (group <= 8) return use(Kernel<Any16, P, false, Mma8Core<P, DH, 8, true>, W, 2>());
+    return use(Kernel<Any16, P, false, Mma8Core<P, DH, 16, true>, (DH > 64 ? W : 12), 2>());
 }
 // `use` with the Kernel that takes the call
-template <typename F>
+template <typename P, typename F>
 int with_kernel(const tmw_paged_attention_desc& d, const tmw_page_scales& s, F&& use) {
-    if (d.at.dtype == TMW_F32) return with_pages<float>(d, s, use);
-    return d.at.dtype == TMW_BF16 ? with_pages<__nv_bfloat16>(d, s, use) : with_pages<__half>(d, s, use);
+    const bool bulk = can_bulk(d, s);
+    if (d.at.dtype != TMW_F32) {
+        switch (d.at.head_dim) {
+            case 32: return with_mma<P, 32>(d, bulk, use);
+            case 64: return with_mma<P, 64>(d, bulk, use);
+            case 96: return with_mma<P, 96>(d, bulk, use);
+            case 128: return with_mma<P, 128>(d, bulk, use);
+            case 256: return with_mma<P, 256>(d, bulk, use);
+        }
+        return with_simt<Any16, P, false>(d, 1, use);
+    }
+    return with_simt<float, P, false>(d, 1, use);
 }
 
-int validate(const tmw_paged_attention_desc* d, const tmw_page_scales* s, bool& used) {
-    const int rc = validate(d, used);
-    if (rc != TMW_OK) return rc;
-    if (s == nullptr || s->format == TMW_PAGES_SAME) return TMW_ERR_INVALID_ARGUMENT;
-    return validate_scales(d->at, *s, false, false);
-}
-
-}  // namespace
-}  // namespace tmw
-
-extern "C" size_t tmw_paged_attention_scaled_scratch_bytes(const tmw_paged_attention_desc* d, const tmw_page_scales* s) {
-    using namespace tmw;
-    bool used = false;
-    if (validate(d, s, used) != TMW_OK || !used) return 0;
+template <typename P>
+size_t scratch_bytes_of(const tmw_paged_attention_desc& d, const tmw_page_scales& s) {
     size_t bytes = 0;
-    with_kernel(*d, *s, [&](auto kernel) {
-        bytes = kernel.plan(*d, d->at.head_dim, 1).bytes;
+    with_kernel<P>(d, s, [&](auto kernel) {
+        bytes = kernel.plan(d, d.at.head_dim, 1).bytes;
         return TMW_OK;
     });
     return bytes;
 }
 
-extern "C" int tmw_paged_attention_scaled(const tmw_paged_attention_desc* d, const tmw_page_scales* s, void* scratch, size_t scratch_bytes,
-                                          void* stream) {
-    using namespace tmw;
-    bool used = false;
-    const int rc = validate(d, s, used);
-    if (rc != TMW_OK || !used) return rc;
-    PagedAttention p;
-    const int bad = arguments(*d, *s, scratch, p);
+template <typename P>
+int launch_of(const tmw_paged_attention_desc& d, const tmw_page_scales& s, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+    PagedAttentionBulk p;
+    const int bad = arguments(d, s, scratch, p);
     if (bad != TMW_OK) return bad;
-    return with_kernel(*d, *s, [&](auto kernel) {
-        const Plan n = kernel.plan(*d, p.row_bytes, 1);
+    return with_kernel<P>(d, s, [&](auto kernel) {
+        using K = decltype(kernel);
+        const Plan n = kernel.plan(d, p.row_bytes, 1);
         if (scratch_bytes < n.bytes) {
             set_error_text("tmw_paged_attention_scaled: scratch smaller than tmw_paged_attention_scaled_scratch_bytes()");
             return (int)TMW_ERR_INVALID_ARGUMENT;
         }
-        return kernel.launch(p, n, static_cast<unsigned char*>(scratch), static_cast<cudaStream_t>(stream));
+        if constexpr (K::CoreOf::Load::kBulk) {
+            if (!make_maps<typename K::CoreOf::Layout>(d, p)) return (int)TMW_ERR_CUDA;
+        }
+        return kernel.launch(p, n, static_cast<unsigned char*>(scratch), stream);
     });
 }
+
+}  // namespace
+
+// one for each form of the pages, in files of their own
+size_t paged_attention_int8_scratch(const tmw_paged_attention_desc& d, const tmw_page_scales& s);
+size_t paged_attention_e4m3_scratch(const tmw_paged_attention_desc& d, const tmw_page_scales& s);
+int paged_attention_int8(const tmw_paged_attention_desc& d, const tmw_page_scales& s, void* scratch, size_t scratch_bytes, cudaStream_t stream);
+int paged_attention_e4m3(const tmw_paged_attention_desc& d, const tmw_page_scales& s, void* scratch, size_t scratch_bytes, cudaStream_t stream);
+
+}  // namespace tmw

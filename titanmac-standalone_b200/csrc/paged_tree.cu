@@ -1,5 +1,5 @@
 // Attention of the drafted tokens of a tree over paged keys (tmw_paged_tree_attention).
-#include "paged_attention.cuh"
+#include "paged_tree.cuh"
 
 namespace tmw {
 namespace {
@@ -22,17 +22,21 @@ tmw_paged_attention_desc shared_part(const tmw_paged_tree_desc& d) {
     return one;
 }
 
+// what the kernel on tensor cores does not take: fp32, head sizes that it is not built for
 template <typename T, typename F>
 int with_pages(const tmw_paged_attention_desc& d, const tmw_page_scales& s, int nodes, F&& use) {
     if (s.format == TMW_PAGES_INT8) return with_simt<T, int8_t, true>(d, nodes, use);
     if (s.format == TMW_PAGES_E4M3) return with_simt<T, E4m3, true>(d, nodes, use);
-    return with_simt<T, T, true>(d, nodes, use);
+    if constexpr (std::is_same<T, Any16>::value) {
+        return d.at.dtype == TMW_BF16 ? with_simt<T, __nv_bfloat16, true>(d, nodes, use) : with_simt<T, __half, true>(d, nodes, use);
+    } else {
+        return with_simt<T, T, true>(d, nodes, use);
+    }
 }
 // `use` with the Kernel that takes the call
 template <typename F>
 int with_kernel(const tmw_paged_attention_desc& d, const tmw_page_scales& s, int nodes, F&& use) {
-    if (d.at.dtype == TMW_F32) return with_pages<float>(d, s, nodes, use);
-    return d.at.dtype == TMW_BF16 ? with_pages<__nv_bfloat16>(d, s, nodes, use) : with_pages<__half>(d, s, nodes, use);
+    return d.at.dtype == TMW_F32 ? with_pages<float>(d, s, nodes, use) : with_pages<Any16>(d, s, nodes, use);
 }
 
 int validate(const tmw_paged_tree_desc* d, const tmw_page_scales& s, bool& used) {
@@ -62,6 +66,13 @@ extern "C" size_t tmw_paged_tree_attention_scratch_bytes(const tmw_paged_tree_de
     if (validate(d, s, used) != TMW_OK || !used) return 0;
     const tmw_paged_attention_desc one = shared_part(*d);
     size_t bytes = 0;
+    if (d->at.dtype != TMW_F32) {
+        const auto of = s.format == TMW_PAGES_INT8   ? tree_scratch_int8
+                        : s.format == TMW_PAGES_E4M3 ? tree_scratch_e4m3
+                        : d->at.dtype == TMW_BF16    ? tree_scratch_bf16
+                                                     : tree_scratch_f16;
+        if (of(one, s, d->nodes, bytes)) return bytes;
+    }
     with_kernel(one, s, d->nodes, [&](auto kernel) {
         bytes = kernel.plan(one, row_bytes(*d, s), d->nodes).bytes;
         return TMW_OK;
@@ -84,22 +95,24 @@ extern "C" int tmw_paged_tree_attention(const tmw_paged_tree_desc* d, const tmw_
         return TMW_ERR_INVALID_ARGUMENT;
     }
     const tmw_paged_attention_desc one = shared_part(*d);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (d->at.dtype != TMW_F32) {
+        const auto run = s.format == TMW_PAGES_INT8   ? tree_launch_int8
+                         : s.format == TMW_PAGES_E4M3 ? tree_launch_e4m3
+                         : d->at.dtype == TMW_BF16    ? tree_launch_bf16
+                                                      : tree_launch_f16;
+        int status = TMW_OK;
+        if (run(one, s, *d, scratch, scratch_bytes, st, status)) return status;
+    }
     PagedAttention p;
-    const int bad = arguments(one, s, scratch, p);
+    const int bad = tree_arguments(one, s, *d, scratch, p);
     if (bad != TMW_OK) return bad;
-    p.qs[2] = d->q_stride[2];
-    p.os[2] = d->o_stride[2];
-    p.q_pairs = p.q_pairs && d->q_stride[2] % 2 == 0;
-    p.o_pairs = p.o_pairs && d->o_stride[2] % 2 == 0;
-    p.counts = d->counts; p.positions = d->positions;
-    p.seen = d->seen;
-    p.nodes = d->nodes;
     return with_kernel(one, s, d->nodes, [&](auto kernel) {
         const Plan n = kernel.plan(one, p.row_bytes, d->nodes);
         if (scratch_bytes < n.bytes) {
             set_error_text("tmw_paged_tree_attention: scratch smaller than tmw_paged_tree_attention_scratch_bytes()");
             return (int)TMW_ERR_INVALID_ARGUMENT;
         }
-        return kernel.launch(p, n, static_cast<unsigned char*>(scratch), static_cast<cudaStream_t>(stream));
+        return kernel.launch(p, n, static_cast<unsigned char*>(scratch), st);
     });
 }
