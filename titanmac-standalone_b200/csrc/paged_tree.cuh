@@ -18,7 +18,7 @@ namespace tmw {
 namespace {
 
 constexpr int kTreeKeys = 32, kTreeCost = 2;  // keys of a tile; what an item costs besides its tiles
-constexpr int kMostSlots = 16;
+constexpr int kMostSlots = 16, kMostTree = 212 * 1024;  // slots of a ring; bytes of rings and rows
 
 // d = a b (+ d) in the type of P's products
 template <typename M>
@@ -67,15 +67,6 @@ __device__ __forceinline__ void split_in_two(float a, float b, uint32_t& first, 
         second = *reinterpret_cast<const uint32_t*>(&rest);
     }
 }
-// the same pair with what is infinite or no number made zero; whether there was any
-template <typename M>
-__device__ __forceinline__ uint32_t finite_part(uint32_t w, bool& wild) {
-    constexpr uint32_t e = std::is_same<M, __half>::value ? 0x7c00u : 0x7f80u;
-    const bool low = (w & e) == e, high = (w >> 16 & e) == e;
-    wild |= low || high;
-    return w & ((low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u));
-}
-
 // One warp's sixteen rows of an item.  P: of keys and values; M: of the products, P itself or fp16 for codes of 8 bits.
 template <typename P, int DH>
 struct TreeCore {
@@ -84,15 +75,19 @@ struct TreeCore {
     static constexpr int KT = kTreeKeys, kRowBytes = DH * (int)sizeof(P), kSteps = DH / 16;
     static constexpr float kRaise = std::is_same<M, __half>::value ? 12.f : 0.f;
     using Layout = BoxLayout<kRowBytes>;
+    // What a warp has of its rows in shared memory (in registers the queries alone would be 32 of head_dim 128, next to 64 of
+    // outputs): the queries, a row's sixteen bytes off the last one's banks, the first token that a row sees, the nodes that it sees.
+    static constexpr int kQueryPitch = DH * 2 + 16, kQueries = 16 * kQueryPitch, kRowsBytes = kQueries + 16 * 16;
     const PagedAttention& p;
-    uint32_t q[kSteps][4];
-    float q_scale[2];           // of rows lane / 4 and 8 + lane / 4
-    float m[2], l[2];           // l: of this lane's keys
-    float o[DH / 8][4];         // 16-bit pages: dimensions 8 n + 2 t and the next, of both rows; codes: see dim_of
-    int start, low[2], lowest;  // tokens in front of the nodes, the first of these that a row sees, the largest of these
-    uint64_t nodes[2];          // those that a row sees
+    unsigned char* mine;
+    float q_scale[2];   // of rows lane / 4 and 8 + lane / 4
+    float m[2], l[2];   // l: of this lane's keys
+    float o[DH / 8][4]; // 16-bit pages: dimensions 8 n + 2 t and the next, of both rows; codes: see dim_of
+    int start, lowest;  // tokens in front of the nodes, the last begin of a row's window
 
-    __device__ __forceinline__ TreeCore(const PagedAttention& p) : p(p) {}
+    __device__ __forceinline__ TreeCore(const PagedAttention& p, unsigned char* mine) : p(p), mine(mine) {}
+    __device__ __forceinline__ uint64_t* nodes_of(int r) const { return reinterpret_cast<uint64_t*>(mine + kQueries + r * 16); }
+    __device__ __forceinline__ int* low_of(int r) const { return reinterpret_cast<int*>(mine + kQueries + r * 16 + 8); }
     // 16-bit pages: the first of a lane's two neighbouring dimensions of tile n.  Codes: tiles 2 c and 2 c + 1 have the even and the odd
     // dimensions of the sixteen from 16 c on, a lane's four are neighbours.
     __device__ __forceinline__ static int dim_of(int n) { return (threadIdx.x & 3) * (k8 ? 4 : 2) + (k8 ? n / 2 * 16 : n * 8); }
@@ -101,60 +96,63 @@ struct TreeCore {
         const int lane = threadIdx.x & 31, t = lane & 3;
         start = __ldg(p.pos + of.b);
         lowest = 0;
-        float top[2] = {0.f, 0.f};
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int r = warp_rows + i * 8 + lane / 4;
+            const int own = i * 8 + lane / 4, r = warp_rows + own;
             const bool there = r < of.n;
             const int node = (of.first + r) / p.group;
-            low[i] = there ? first_seen(p, of.b, start, node) : 0;
-            nodes[i] = there ? nodes_seen(p, of.b, count, node) : 0;
-            lowest = max(lowest, low[i]);
+            const int low = there ? first_seen(p, of.b, start, node) : 0;
+            lowest = max(lowest, low);
+            if (t == 0) {
+                *low_of(own) = low;
+                *nodes_of(own) = there ? nodes_seen(p, of.b, count, node) : 0;
+            }
             const uint16_t* from = static_cast<const uint16_t*>(p.q) + (there ? row_at<true>(p, p.qs, of, r) : 0);
+            uint32_t w[kSteps][2];
+            float top = 0.f;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                uint32_t w[2];
+            for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint16_t* at = from + k * 16 + (k8 ? t * 4 + h * 2 : t * 2 + h * 8);
-                    w[h] = 0;
-                    if (there) w[h] = p.q_pairs ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16;
+                    w[k][h] = 0;
+                    if (there) w[k][h] = p.q_pairs ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16;
                     if constexpr (k8) {
-                        const float2 x = unpack2<__nv_bfloat16>(w[h]);
-                        top[i] = fmaxf(top[i], fmaxf(fabsf(x.x), fabsf(x.y)));
+                        const float2 x = unpack2<__nv_bfloat16>(w[k][h]);
+                        top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
                     }
                 }
-                q[k][i] = w[0];
-                q[k][2 + i] = w[1];
-            }
-        }
-        for (int d = 4; d < 32; d *= 2) lowest = max(lowest, __shfl_xor_sync(0xffffffffu, lowest, d));
-        q_scale[0] = q_scale[1] = p.scale;
-        if constexpr (k8) {  // bf16 as fp16 times a power of two of the row's own; then in the order of the codes
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            q_scale[i] = p.scale;
+            if constexpr (k8) {  // bf16 as fp16 times a power of two of the row's own; then in the order of the codes
                 if (p.bf16) {
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                    const int e = max((__float_as_int(top[i]) >> 23) - 127, -100);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const int e = max((__float_as_int(top) >> 23) - 127, -100);
                     const float up = __int_as_float((127 + 14 - e) << 23);
                     q_scale[i] *= __int_as_float((127 - 14 + e) << 23);
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float2 x = unpack2<__nv_bfloat16>(q[k][2 * h + i]);
-                            q[k][2 * h + i] = pack2<__half>(x.x * up, x.y * up);
+                            const float2 x = unpack2<__nv_bfloat16>(w[k][h]);
+                            w[k][h] = pack2<__half>(x.x * up, x.y * up);
                         }
                 }
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    const uint32_t a = q[k][i], b = q[k][2 + i];
-                    q[k][i] = __byte_perm(a, b, 0x5410);
-                    q[k][2 + i] = __byte_perm(a, b, 0x7632);
+                    const uint32_t a = w[k][0], b = w[k][1];
+                    w[k][0] = __byte_perm(a, b, 0x5410);
+                    w[k][1] = __byte_perm(a, b, 0x7632);
                 }
             }
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) *reinterpret_cast<uint32_t*>(mine + own * kQueryPitch + k * 32 + h * 16 + t * 4) = w[k][h];
         }
+        for (int d = 4; d < 32; d *= 2) lowest = max(lowest, __shfl_xor_sync(0xffffffffu, lowest, d));
+        __syncwarp();
     }
     __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -169,6 +167,7 @@ struct TreeCore {
     __device__ __forceinline__ void tile(const Ring& ring, int slot, uint2 marks, int place) {
         const int lane = threadIdx.x & 31, t = lane & 3;
         const uint32_t keys = (uint32_t)__cvta_generic_to_shared(ring.tiles) + slot * 2 * KT * kRowBytes, values = keys + KT * kRowBytes;
+        const uint32_t query_at = (uint32_t)__cvta_generic_to_shared(mine) + (lane & 15) * kQueryPitch + (lane >> 4) * 16;
         float s[KT / 8][4];
         // of 16-bit rows: eight keys' first and second chunk of a step, then the next eight's; of codes two steps of eight keys, of the next eight
         const uint32_t key_at = Layout::offset((lane >> 4) * 8 + (lane & 7), lane >> 3 & 1);
@@ -177,7 +176,10 @@ struct TreeCore {
             return (at ^ (c % in << 4)) + c / in * KT * Layout::kBoxBytes + g * 16 * Layout::kBoxBytes;
         };
 #pragma unroll
-        for (int c = 0; c < kRowBytes / 16; c += 2)
+        for (int c = 0; c < kRowBytes / 16; c += 2) {
+            uint32_t q[k8 ? 2 : 1][4];
+#pragma unroll
+            for (int h = 0; h < (k8 ? 2 : 1); ++h) ldmatrix4(q[h], query_at + (k8 ? c + h : c / 2) * 32);
 #pragma unroll
             for (int g = 0; g < KT / 16; ++g) {
                 uint32_t b[4];
@@ -189,15 +191,16 @@ struct TreeCore {
                         for (int h = 0; h < 2; ++h) {
                             uint32_t even, odd;
                             to_pairs<P>(b[2 * n + h], even, odd);
-                            if (c + h == 0) mma_from_zero<M>(s[2 * g + n], q[0], even, odd);
-                            else mma_onto_it<M>(s[2 * g + n], q[c + h], even, odd);
+                            if (c + h == 0) mma_from_zero<M>(s[2 * g + n], q[h], even, odd);
+                            else mma_onto_it<M>(s[2 * g + n], q[h], even, odd);
                         }
                     } else {
                         if (c == 0) mma_from_zero<M>(s[2 * g + n], q[0], b[2 * n], b[2 * n + 1]);
-                        else mma_onto_it<M>(s[2 * g + n], q[c / 2], b[2 * n], b[2 * n + 1]);
+                        else mma_onto_it<M>(s[2 * g + n], q[0], b[2 * n], b[2 * n + 1]);
                     }
                 }
             }
+        }
         // scores in powers of two; of codes with the values' scales in two parts (as in the attention of one token)
         float f[KT / 8][2], back[KT / 8][2];
 #pragma unroll
@@ -225,13 +228,15 @@ struct TreeCore {
             for (int i = 0; i < 2; ++i) {
                 // the row's tile as a word of bits: nodes' from theirs, tokens' from its window's begin on
                 uint32_t seen = marks.x;
+                const uint64_t nodes = *nodes_of(i * 8 + lane / 4);
+                const int low = *low_of(i * 8 + lane / 4);
                 if (place >= 0) {
                     const int nodes_at = start - place;  // of node 0 in the tile
                     uint32_t of_nodes = 0;
-                    if (nodes_at >= 0) of_nodes = nodes_at < 32 ? (uint32_t)(nodes[i] << nodes_at) : 0u;
-                    else of_nodes = -nodes_at < 64 ? (uint32_t)(nodes[i] >> -nodes_at) : 0u;
+                    if (nodes_at >= 0) of_nodes = nodes_at < 32 ? (uint32_t)(nodes << nodes_at) : 0u;
+                    else of_nodes = -nodes_at < 64 ? (uint32_t)(nodes >> -nodes_at) : 0u;
                     const uint32_t tokens = nodes_at <= 0 ? 0u : nodes_at >= 32 ? 0xffffffffu : (1u << nodes_at) - 1;
-                    const int first = low[i] - place;
+                    const int first = low - place;
                     const uint32_t from = first <= 0 ? 0xffffffffu : first >= 32 ? 0u : 0xffffffffu << first;
                     seen &= (tokens & from) | (of_nodes & ~tokens);
                 }
@@ -284,7 +289,6 @@ struct TreeCore {
                 }
                 split_in_two<M>(s[n][2 * i], s[n][2 * i + 1], w[0][n / 2][n % 2 * 2 + i], w[1][n / 2][n % 2 * 2 + i]);
             }
-        bool wild = false;
         if constexpr (MASKED) {
             // rows that nobody sees may hold anything, and nothing times that need not be nothing (each warp makes them zero for itself: the
             // same zeros)
@@ -297,6 +301,12 @@ struct TreeCore {
                 }
                 ptx::fence_proxy_async_smem();  // (before TMA writes there again)
                 __syncwarp();
+            }
+            if constexpr (!k8) {
+                if (has_wild(values)) {
+                    add_by_numbers(values, s, keep);
+                    return;
+                }
             }
         }
         // of 16-bit rows: keys 0 - 7 and 8 - 15 of a step's eight dimensions, then of the next eight; of codes of sixteen dimensions
@@ -335,11 +345,7 @@ struct TreeCore {
                     float sum[4];
 #pragma unroll
                     for (int g = 0; g < KT / 16; ++g) {
-                        uint32_t b0 = b[g][2 * h], b1 = b[g][2 * h + 1];
-                        if constexpr (MASKED) {  // (what a row does not see must not reach it)
-                            b0 = finite_part<M>(b0, wild);
-                            b1 = finite_part<M>(b1, wild);
-                        }
+                        const uint32_t b0 = b[g][2 * h], b1 = b[g][2 * h + 1];
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
                             if (g + n == 0) mma_from_zero<M>(sum, w[0][0], b0, b1);
@@ -353,13 +359,32 @@ struct TreeCore {
                 }
             }
         }
-        if constexpr (MASKED && !k8) {
-            if (__any_sync(0xffffffffu, wild)) add_wild(values, s);
-        }
     }
-    // What is infinite or no number among a tile's values, to the rows that see it: s holds the weights.
-    __device__ __forceinline__ void add_wild(uint32_t values, const float (&s)[KT / 8][4]) {
+    // Whether the values of a tile hold an infinity or a NaN: a row to a lane.
+    __device__ __forceinline__ bool has_wild(uint32_t values) const {
+        const int lane = threadIdx.x & 31;
+        constexpr uint32_t up = std::is_same<M, __half>::value ? 0x04000400u : 0x00800080u;  // carries the largest exponent into the sign
+        uint32_t found = 0;
+#pragma unroll 4
+        for (int c = 0; c < kRowBytes / 16; ++c) {
+            uint32_t v[4];
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                         : "r"(values + Layout::offset(lane, c))
+                         : "memory");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) found |= (v[i] & 0x7fff7fffu) + up;
+        }
+        return __any_sync(0xffffffffu, (found & 0x80008000u) != 0);
+    }
+    // O += P V of a tile with such values: number by number, so that what a row does not see stays out of it.  s: the weights.
+    __device__ __forceinline__ void add_by_numbers(uint32_t values, const float (&s)[KT / 8][4], const float (&keep)[2]) {
         const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < DH / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= keep[i / 2];
+#pragma unroll 1
         for (int key = 0; key < KT; ++key) {
             float w[2];
 #pragma unroll
@@ -374,15 +399,12 @@ struct TreeCore {
             for (int n = 0; n < DH / 8; ++n) {
                 uint32_t v;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(values + Layout::offset(key, n) + t * 4) : "memory");
-                bool wild = false;
-                const uint32_t finite = finite_part<M>(v, wild);
-                if (!wild) continue;
-                const float2 x = unpack2<M>(v), y = unpack2<M>(finite);
+                const float2 x = unpack2<M>(v);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (w[i] == 0.f) continue;
-                    o[n][2 * i] += w[i] * x.x - w[i] * y.x;
-                    o[n][2 * i + 1] += w[i] * x.y - w[i] * y.y;
+                    o[n][2 * i] = fmaf(w[i], x.x, o[n][2 * i]);
+                    o[n][2 * i + 1] = fmaf(w[i], x.y, o[n][2 * i + 1]);
                 }
             }
         }
@@ -500,9 +522,10 @@ __global__ void __launch_bounds__(W * 32, 1) paged_tree_kernel(const __grid_cons
         };
         if (leads) {
             look();
-            for (int s = 0; s < slots - 1; ++s) fetch();
+            // (some slots behind: the leading warp need not wait for the slowest one's last tile)
+            for (int s = 0; s < slots - (slots > 4 ? slots / 4 + 1 : 1); ++s) fetch();
         }
-        Core core(p);
+        Core core(p, smem + workers * slots * (kUnit + 2 * KT * 4) + warp * Core::kRowsBytes);
         auto queries = [&](const Cursor<KT, true, COST>& c) {
             const Rows rows = rows_of<true>(p, c.b, c.head, c.item - c.head * c.parts(p), c.count);
             core.load_queries(rows, c.count, warp_rows);
@@ -701,11 +724,13 @@ struct TreeKernel {
         const int parts = (teams + W - 1) / W;
         n.rows = (all + parts - 1) / parts;
         n.team = (n.rows + 15) / 16;
-        constexpr int unit = 2 * kTreeKeys * (DH * (int)sizeof(P) + (kScaled<P> ? 4 : 0));
-        constexpr int units = (200 * 1024) / unit;
-        n.workers = W / n.team < units / 2 ? W / n.team : units / 2;
-        n.slots = units / n.workers < kMostSlots ? units / n.workers : kMostSlots;
-        n.smem = 1024 + n.workers * n.slots * unit;
+        constexpr int unit = 2 * kTreeKeys * (DH * (int)sizeof(P) + 4);
+        const int rows = n.team * TreeCore<P, DH>::kRowsBytes;  // of a worker
+        n.workers = W / n.team;
+        while (n.workers > 1 && n.workers * (rows + 2 * unit) > kMostTree) --n.workers;
+        n.slots = (kMostTree / n.workers - rows) / unit;
+        if (n.slots > kMostSlots) n.slots = kMostSlots;
+        n.smem = 1024 + n.workers * (n.slots * unit + rows);
         const long long capacity = (long long)d.at.columns * d.at.page_size;
         const long long keys = d.window >= 0 && d.window + (long long)nodes < capacity ? d.window + (long long)nodes : capacity;
         const long long tiles = ((d.n_persistent + 31) / 32 + keys / 32 + 2) * (long long)d.at.kv_heads * parts * d.at.batch;
