@@ -47,6 +47,7 @@ struct PagedAttention {
     int run;                // as many from a multiple of that on do, 16, 8 or none
     bool bf16;              // of two types with 16 bits
     bool q_pairs, o_pairs;  // queries can be read, outputs stored two at a time
+    bool q_wide, o_wide;    // sixteen bytes at a time
     int group;              // query heads of a key head
     int rows, parts;        // query heads of an item at most; items of a key head
     int items;              // of a sequence
@@ -1430,6 +1431,8 @@ inline int arguments(const tmw_paged_attention_desc& d, const tmw_page_scales& s
     p.row_bytes = d.at.head_dim * (scales.format == 0 ? (int)size : 1);
     p.q_pairs = bits(d.q) % 4 == 0 && (d.q_stride[0] | d.q_stride[1]) % 2 == 0;
     p.o_pairs = bits(d.o) % 4 == 0 && (d.o_stride[0] | d.o_stride[1]) % 2 == 0;
+    p.q_wide = bits(d.q) % 16 == 0 && (d.q_stride[0] | d.q_stride[1]) * (long long)size % 16 == 0;
+    p.o_wide = bits(d.o) % 16 == 0 && (d.o_stride[0] | d.o_stride[1]) * (long long)size % 16 == 0;
     p.status = device_status_word();
     return p.status == nullptr ? TMW_ERR_CUDA : TMW_OK;
 }

@@ -67,6 +67,7 @@ extern "C" size_t tmw_paged_tree_attention_scratch_bytes(const tmw_paged_tree_de
     const tmw_paged_attention_desc one = shared_part(*d);
     size_t bytes = 0;
     if (d->at.dtype != TMW_F32) {
+        if (tree_scratch_tc(one, s, d->nodes, bytes)) return bytes;
         const auto of = s.format == TMW_PAGES_INT8   ? tree_scratch_int8
                         : s.format == TMW_PAGES_E4M3 ? tree_scratch_e4m3
                         : d->at.dtype == TMW_BF16    ? tree_scratch_bf16
@@ -102,6 +103,7 @@ extern "C" int tmw_paged_tree_attention(const tmw_paged_tree_desc* d, const tmw_
                          : d->at.dtype == TMW_BF16    ? tree_launch_bf16
                                                       : tree_launch_f16;
         int status = TMW_OK;
+        if (tree_launch_tc(one, s, *d, scratch, scratch_bytes, st, status)) return status;
         if (run(one, s, *d, scratch, scratch_bytes, st, status)) return status;
     }
     PagedAttention p;

@@ -702,6 +702,8 @@ inline int tree_arguments(const tmw_paged_attention_desc& one, const tmw_page_sc
     p.os[2] = d.o_stride[2];
     p.q_pairs = p.q_pairs && d.q_stride[2] % 2 == 0;
     p.o_pairs = p.o_pairs && d.o_stride[2] % 2 == 0;
+    p.q_wide = p.q_wide && d.q_stride[2] % 8 == 0;  // (used with 16-bit numbers)
+    p.o_wide = p.o_wide && d.o_stride[2] % 8 == 0;
     p.counts = d.counts; p.positions = d.positions;
     p.seen = d.seen;
     p.nodes = d.nodes;
@@ -809,6 +811,14 @@ TMW_TREE_OF(bf16)
 TMW_TREE_OF(f16)
 TMW_TREE_OF(int8)
 TMW_TREE_OF(e4m3)
+TMW_TREE_OF(tc)
 #undef TMW_TREE_OF
+
+// Which calls tcgen05 takes: 16-bit pages that come by TMA, head_dim 64 or 128, and more rows to a key head than mma.sync's two or three warps
+// have, TREE_ROWS.
+inline bool tree_takes_tc(const tmw_paged_attention_desc& d, const tmw_page_scales& s, int nodes) {
+    return s.format == TMW_PAGES_SAME && d.at.dtype != TMW_F32 && (d.at.head_dim == 64 || d.at.head_dim == 128) && can_bulk(d, s) &&
+           d.heads / d.at.kv_heads * nodes > 32;
+}
 
 }  // namespace tmw

@@ -1,0 +1,549 @@
+// Attention of a tree's drafted tokens over pages of 16-bit numbers, many rows to a key head (tcgen05; head_dim 64 or 128).
+//
+// Up to 128 (node, head) rows of a key head are one tile of tcgen05.mma, so that 64 keys cost the tensor core the same for 33 rows as for
+// 128, a fifth of what mma.sync takes for them (9 cycles of a scheduler for each 16 x 8 x 16).  A CTA, two to an SM, is one worker of the
+// line of tiles (paged_attention.cuh), here of 64 keys, and its warps have fixed roles:
+//   warp  0    pages looked up, K and V brought by TMA, a run of up to 64 neighbouring tokens at a time
+//   warp  1    issues the products (one elected thread)
+//   warps 4-7  softmax, a thread to a row; queries into shared memory, outputs out of tensor memory
+// S = Q K^T (two buffers in tensor memory, the next scores are multiplied while these are exponentiated); P goes over its S as two 16-bit
+// numbers a weight, 64 columns for 64 fp32 ones; O += P V.  The running maximum follows only a score that is 2^4 above it: O is brought
+// up in tensor memory then.  Tiles that some row does not see in full, at a window's begin and among the nodes, have the rows' bits
+// applied to the scores, and their values made harmless: rows that nobody sees are zeros, and what is infinite or no number is added
+// row by row to those that see it.
+//
+// All waits are bounded (paged_attention.cuh); the tensor memory is given back on every way.
+#include "paged_tree.cuh"
+
+namespace tmw {
+namespace {
+
+using namespace ptx;
+
+constexpr int kTcKeys = 64, kTcRows = 128, kTcThreads = 256, kTcCost = 2;
+constexpr int kRegsService = 56, kRegsSoftmax = 200;
+static_assert(kTcThreads / 2 * (kRegsService + kRegsSoftmax) <= 65536 / 2, "setmaxnreg: what the softmax warps ask for the others release");
+
+template <int DH>
+struct TcLayout {
+    static constexpr int kSubs = DH / 64, kStages = DH == 64 ? 4 : 2;  // sub-tiles of 64 columns; tiles in a ring
+    static constexpr int kQSub = kTcRows * 128, kSub = kTcKeys * 128, kTile = kSub * kSubs;
+    static constexpr int kK = kQSub * kSubs, kV = kK + kStages * kTile, kBytes = kV + kStages * kTile;
+};
+// of a tile: its first key's token (-1: persistent ones), its keys that exist, runs without a page
+struct TileInfo {
+    int place, first, last, lost, run;
+};
+
+// A CTA's parts of items, one after the other, as every role walks over them.
+struct Walk {
+    Cursor<kTcKeys, true, kTcCost> at, now;  // the next part's first unit; the present part's
+    long long begin, end, item_end;
+    int first_tile, tiles;
+    bool starts, ends;
+    __device__ __forceinline__ bool next(const PagedAttention& p, long long limit) {
+        while (begin < limit) {
+            now = at;
+            item_end = begin + (at.n - at.t);
+            end = item_end < limit ? item_end : limit;
+            first_tile = max(at.t - kTcCost, 0);
+            tiles = (int)(end - begin) - max(kTcCost - at.t, 0);
+            starts = at.t <= kTcCost;
+            ends = end == item_end;
+            begin = end;
+            if (item_end < limit) at.next_item(p);
+            if (tiles > 0) return true;
+        }
+        return false;
+    }
+};
+
+template <int DH, bool BF16>
+__global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
+    using L = TcLayout<DH>;
+    using M = std::conditional_t<BF16, __nv_bfloat16, __half>;
+    constexpr int KT = kTcKeys, ST = L::kStages;
+    constexpr float kRaise = BF16 ? 0.f : 11.f;  // a weight is at most 2^4 under it
+    constexpr uint32_t kO = 2 * KT, kColumns = 256;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ alignas(8) uint64_t bars[8 + 4 * ST];
+    __shared__ TileInfo infos[ST];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int given_up, wild, first_adds, lows[4];
+    unsigned char* smem = dynamic + (1024 - smem_u32(dynamic)) % 1024;
+    const uint32_t base = smem_u32(smem);
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t q_ready = bar0, s_full = bar0 + 8, p_ready = bar0 + 24, o_done = bar0 + 40, pv_done = bar0 + 48;
+    const uint32_t k_full = bar0 + 64, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        mbar_init(q_ready, 4);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
+        mbar_init(o_done, 1);
+        mbar_init(pv_done, 1);
+        for (int i = 0; i < 4 * ST; ++i) mbar_init(k_full + 8 * i, 1);
+        given_up = wild = first_adds = 0;
+        p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), kColumns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_trigger();
+
+    Walk walk;
+    const Share share = find_share<KT, true, kTcCost>(p, walk.at, 0, 1);
+    walk.begin = share.first;
+    const long long limit = share.first < share.end ? share.end : share.first;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService) : "memory");
+        if (warp == 0) {
+            // ---- K and V ----
+            const int runs = KT / p.run;
+            int stage = 0;
+            uint32_t phase = 1;
+            while (walk.next(p, limit)) {
+                const auto& at = walk.now;
+                int row = -1, page = -1;
+                bool pers = false;
+                int j0 = 0, first = 0, last = 0;
+                auto look = [&](int tile) {  // this lane's run of a tile
+                    pers = tile < p.pers_tiles;
+                    j0 = (pers ? tile : at.lo / KT + tile - p.pers_tiles) * KT;
+                    first = pers ? 0 : max(at.lo - j0, 0);
+                    last = min((pers ? p.np - 1 : at.pos) - j0, KT - 1);
+                    row = -1;
+                    const int j = lane * p.run;
+                    if (lane < runs && j <= last && j + p.run > first) {
+                        row = j0 + j;
+                        if (!pers) {
+                            const uint32_t column = p.map.page.div((uint32_t)row);
+                            row -= (int)(column * p.map.page.d);
+                            page = __ldg(p.map.table + at.b * p.map.table_stride + column);
+                        }
+                    }
+                };
+                look(walk.first_tile);
+                for (int i = 0; i < walk.tiles; ++i) {
+                    if (row >= 0) {
+                        if (pers) row += at.head * p.np;
+                        else row = (uint32_t)page < (uint32_t)p.map.pages ? (page * p.map.kv_heads + at.head) * (int)p.map.page.d + row : -2;
+                    }
+                    const uint32_t there = __ballot_sync(0xffffffffu, row >= 0), lost = __ballot_sync(0xffffffffu, row == -2);
+                    const uint32_t bytes = __popc(there) * p.run * DH * 2;
+                    const CUtensorMap *km = pers ? &p.k_pers_map : &p.k_map, *vm = pers ? &p.v_pers_map : &p.v_map;
+                    mbar_wait(k_free + 8 * stage, phase, &given_up, p.status);
+                    if (elect_one()) mbar_expect_tx(k_full + 8 * stage, bytes);
+                    for (uint32_t todo = there; todo != 0; todo &= todo - 1) {
+                        const int r = __ffs(todo) - 1, from = __shfl_sync(0xffffffffu, row, r);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int s = 0; s < L::kSubs; ++s)
+                                tma_load_2d(base + L::kK + stage * L::kTile + s * L::kSub + r * p.run * 128, km, k_full + 8 * stage, s * 64, from);
+                        }
+                    }
+                    mbar_wait(v_free + 8 * stage, phase, &given_up, p.status);
+                    if (elect_one()) {
+                        infos[stage] = {pers ? -1 : j0, first, last, (int)lost, p.run};
+                        mbar_expect_tx(v_full + 8 * stage, bytes);
+                    }
+                    for (uint32_t todo = there; todo != 0; todo &= todo - 1) {
+                        const int r = __ffs(todo) - 1, from = __shfl_sync(0xffffffffu, row, r);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int s = 0; s < L::kSubs; ++s)
+                                tma_load_2d(base + L::kV + stage * L::kTile + s * L::kSub + r * p.run * 128, vm, v_full + 8 * stage, s * 64, from);
+                        }
+                    }
+                    if (lost != 0 && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+                    if (++stage == ST) stage = 0, phase ^= 1;
+                    if (i + 1 < walk.tiles) look(walk.first_tile + i + 1);
+                }
+            }
+        } else if (warp == 1 && elect_one()) {
+            // ---- the products ----
+            constexpr uint32_t fmt = BF16 ? 1u : 0u;
+            const uint32_t idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((KT >> 3) << 17) | ((kTcRows >> 4) << 24);
+            const uint32_t idesc_pv = idesc_b_mnmajor(fmt, DH);
+            int k_stage = 0, v_stage = 0, n = 0;  // n: tiles whose scores have been issued, of all parts
+            uint32_t k_phase = 0, v_phase = 0, q_phase = 0;
+            auto scores = [&]() {
+                mbar_wait(k_full + 8 * k_stage, k_phase, &given_up, p.status);
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < DH / 16; ++k)
+                    mma_ss(tmem + (n & 1) * KT, kmajor_desc(base + k / 4 * L::kQSub) + k % 4 * 2,
+                           kmajor_desc(base + L::kK + k_stage * L::kTile + k / 4 * L::kSub) + k % 4 * 2, idesc_qk, k > 0 ? 1u : 0u);
+                tc_commit(s_full + 8 * (n & 1));
+                tc_commit(k_free + 8 * k_stage);
+                if (++k_stage == ST) k_stage = 0, k_phase ^= 1;
+                ++n;
+            };
+            int m = 0;  // tiles whose values have been issued
+            while (walk.next(p, limit)) {
+                mbar_wait(q_ready, q_phase, &given_up, p.status);
+                q_phase ^= 1;
+                tc_fence_after();
+                for (int i = 0; i < 2 && i < walk.tiles; ++i) scores();
+                for (int i = 0; i < walk.tiles; ++i) {
+                    mbar_wait(v_full + 8 * v_stage, v_phase, &given_up, p.status);
+                    mbar_wait(p_ready + 8 * (m & 1), (m >> 1) & 1, &given_up, p.status);
+                    tc_fence_after();
+                    const uint32_t pt = tmem + (m & 1) * KT;
+                    const uint64_t v = mnmajor_desc(base + L::kV + v_stage * L::kTile, L::kSub);
+                    const uint32_t onto = i > 0 || *(volatile int*)&first_adds ? 1u : 0u;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int k = 0; k < KT / 16; ++k) mma_ts(tmem + kO, pt + half * 32 + k * 8, v + k * 128, idesc_pv, half + k > 0 ? 1u : onto);
+                    ++m;
+                    if (i + 2 < walk.tiles) scores();
+                    else if (i + 2 == walk.tiles) tc_commit(pv_done);  // the last tile but one
+                    else tc_commit(o_done);
+                    tc_commit(v_free + 8 * v_stage);
+                    if (++v_stage == ST) v_stage = 0, v_phase ^= 1;
+                }
+            }
+        }
+    } else {
+        // ---- softmax: a thread to a row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax) : "memory");
+        const int row = tid - 128;
+        const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lane_at + kO;
+        int n = 0, v_stage = 0;
+        uint32_t v_phase = 0, o_phase = 0, pv_phase = 0;
+        while (walk.next(p, limit)) {
+            const auto& at = walk.now;
+            const Rows rows = rows_of<true>(p, at.b, at.head, at.item - at.head * at.parts(p), at.count);
+            const int start = __ldg(p.pos + at.b);
+            const bool there = row < rows.n, warp_there = (warp & 3) * 32 < rows.n;
+            int low = 0;
+            uint64_t nodes = 0;
+            {   // the row's queries, as TMA would leave them
+                const uint16_t* from = static_cast<const uint16_t*>(p.q);
+                if (there) {
+                    const int node = (rows.first + row) / p.group;
+                    low = first_seen(p, at.b, start, node);
+                    nodes = nodes_seen(p, at.b, at.count, node);
+                    from += row_at<true>(p, p.qs, rows, row);
+                }
+                const bool wide = p.q_wide;
+#pragma unroll 4
+                for (int c = 0; c < DH / 8; ++c) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (there) {
+                        if (wide) {
+                            w = *reinterpret_cast<const uint4*>(from + c * 8);
+                        } else {
+                            uint32_t x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = from[c * 8 + 2 * e] | (uint32_t)from[c * 8 + 2 * e + 1] << 16;
+                            w = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(smem + c / 8 * L::kQSub + row * 128 + ((c % 8 ^ (row & 7)) << 4)) = w;
+                }
+                int warp_low = low;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) warp_low = max(warp_low, __shfl_xor_sync(0xffffffffu, warp_low, d));
+                if (lane == 0) lows[warp & 3] = warp_low;
+                if (row == 0) first_adds = 0;
+                fence_proxy_async_smem();
+                named_barrier_sync(1, 128);
+                if (lane == 0) mbar_arrive(q_ready);
+            }
+            const int lowest = max(max(lows[0], lows[1]), max(lows[2], lows[3]));
+            float m_used = -CUDART_INF_F, l = 0.f;
+            for (int i = 0; i < walk.tiles; ++i, ++n) {
+                const int buf = n & 1;
+                const uint32_t s_at = tmem + lane_at + buf * KT;
+                mbar_wait(s_full + 8 * buf, (n >> 1) & 1, &given_up, p.status);
+                mbar_wait(v_full + 8 * v_stage, v_phase, &given_up, p.status);
+                tc_fence_after();
+                const TileInfo info = infos[v_stage];
+                const bool whole = info.first == 0 && info.last == KT - 1 && info.lost == 0 &&
+                                   (info.place < 0 || (info.place + KT <= start && info.place >= lowest));
+                uint32_t s[KT];
+                if (warp_there) {
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t(&part)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + c * 32);
+                        tmem_ld32(s_at + c * 32, part);
+                    }
+                    tc_wait_ld();
+                }
+                uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first, bad = 0;
+                if (!whole) {
+                    for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1) bad |= (info.run == 64 ? ~0ull : (1ull << info.run) - 1) << (__ffs(todo) - 1) * info.run;
+                    uint64_t seen = exists;
+                    if (info.place >= 0) {
+                        const int nodes_at = start - info.place, from = low - info.place;  // of node 0, of the window's begin
+                        const uint64_t of_nodes = nodes_at >= 0 ? (nodes_at < 64 ? nodes << nodes_at : 0) : (nodes_at > -64 ? nodes >> -nodes_at : 0);
+                        const uint64_t tokens = nodes_at <= 0 ? 0 : nodes_at >= 64 ? ~0ull : (1ull << nodes_at) - 1;
+                        const uint64_t behind = from <= 0 ? ~0ull : from >= 64 ? 0 : ~0ull << from;
+                        seen &= (tokens & behind) | (of_nodes & ~tokens);
+                    }
+                    const uint64_t nan = bad & seen;
+#pragma unroll
+                    for (int j = 0; j < KT; ++j)
+                        if ((seen >> j & 1) == 0) s[j] = 0xff800000u;
+                    if (nan != 0) {
+#pragma unroll
+                        for (int j = 0; j < KT; ++j)
+                            if (nan >> j & 1) s[j] = 0x7fffffffu;
+                    }
+                }
+                // what the last product but one left in O is final; may O be changed?
+                auto wait_products = [&]() {
+                    if (i + 1 < walk.tiles) mbar_wait(s_full + 8 * (buf ^ 1), ((n + 1) >> 1) & 1, &given_up, p.status);
+                    else if (walk.tiles > 1) mbar_wait(pv_done, pv_phase, &given_up, p.status);
+                    tc_fence_after();
+                };
+                if (warp_there) {
+                    float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                    for (int j = 0; j < KT; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(s[j]));
+                    const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
+                    if (i == 0) {
+                        m_used = tile_top;
+                    } else if (__any_sync(0xffffffffu, tile_top > m_used + 4.f)) {
+                        const float now = tile_top > m_used + 4.f ? tile_top : m_used;
+                        const float keep = m_used == -CUDART_INF_F ? 1.f : ex2_ftz(m_used - now);  // (nothing to keep: zeros, or NaN)
+                        m_used = now;
+                        l *= keep;
+                        wait_products();
+#pragma unroll 1
+                        for (int c = 0; c < DH; c += 16) {
+                            uint32_t x[16];
+                            tmem_ld16(o_at + c, x);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
+                            tmem_st16(o_at + c, x);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                const float less = (m_used == -CUDART_INF_F ? 0.f : m_used) - kRaise;
+                if (warp_there) {
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t first[16], second[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float a = ex2_ftz(fmaf(__uint_as_float(s[c * 32 + 2 * e]), p.scale, -less));
+                            const float b = ex2_ftz(fmaf(__uint_as_float(s[c * 32 + 2 * e + 1]), p.scale, -less));
+                            l += a + b;
+                            split_in_two<M>(a, b, first[e], second[e]);
+                        }
+                        tmem_st16(s_at + c * 16, first);
+                        tmem_st16(s_at + 32 + c * 16, second);
+                    }
+                    tc_wait_st();
+                }
+                if (!whole) {
+                    // values that must not count: a thread has half a row of them
+                    const int key = row >> 1;
+                    unsigned char* half = smem + L::kV + v_stage * L::kTile + key * 128;
+                    constexpr int kChunks = DH / 16;  // sixteen-byte pieces of a half
+                    auto piece = [&](int c) {
+                        c += (row & 1) * kChunks;
+                        return reinterpret_cast<uint4*>(half + c / 8 * L::kSub + ((c % 8 ^ (key & 7)) << 4));
+                    };
+                    constexpr uint32_t up = BF16 ? 0x00800080u : 0x04000400u, inf = BF16 ? 0x7f80u : 0x7c00u;
+                    bool found = false;
+                    if (((exists & ~bad) >> key & 1) == 0) {
+                        for (int c = 0; c < kChunks; ++c) *piece(c) = make_uint4(0, 0, 0, 0);
+                    } else {
+                        uint32_t any = 0;
+                        for (int c = 0; c < kChunks; ++c) {
+                            const uint4 v = *piece(c);
+                            any |= ((v.x & 0x7fff7fffu) + up) | ((v.y & 0x7fff7fffu) + up) | ((v.z & 0x7fff7fffu) + up) | ((v.w & 0x7fff7fffu) + up);
+                        }
+                        found = (any & 0x80008000u) != 0;
+                        if (found) wild = 1;
+                    }
+                    named_barrier_sync(1, 128);
+                    const bool any_wild = *(volatile int*)&wild != 0;
+                    named_barrier_sync(1, 128);  // (all have read it: the next such tile may set it)
+                    if (any_wild) {
+                        // Infinities and NaN to the rows that see them, number by number, into O: in front of a part's first product O
+                        // is made zero, and that product told to add.
+                        if (i == 0) {
+                            for (int c = 0; c < DH; c += 16) {
+                                const uint32_t zero[16] = {};
+                                tmem_st16(o_at + c, zero);
+                            }
+                            tc_wait_st();
+                            if (row == 0) first_adds = 1;
+                        } else {
+                            wait_products();
+                        }
+                        uint64_t mine = 0;  // keys that have a weight
+#pragma unroll
+                        for (int j = 0; j < KT; ++j)
+                            if (warp_there && !(ex2_ftz(fmaf(__uint_as_float(s[j]), p.scale, -less)) == 0.f)) mine |= 1ull << j;
+                        for (int j = 0; j < KT; ++j) {
+                            const unsigned char* v = smem + L::kV + v_stage * L::kTile + j * 128;
+                            for (int d = 0; d < DH; ++d) {
+                                const uint32_t x = *reinterpret_cast<const uint16_t*>(v + d / 64 * L::kSub + ((d % 64 / 8 ^ (j & 7)) << 4) + d % 8 * 2);
+                                if ((x & 0x7fffu) < inf) continue;  // (the same for all rows)
+                                uint32_t o;
+                                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_at + d) : "memory");
+                                tc_wait_ld();
+                                const float add = (x & 0x7fffu) > inf ? CUDART_NAN_F : x & 0x8000u ? -CUDART_INF_F : CUDART_INF_F;
+                                if (mine >> j & 1) o = __float_as_uint(__uint_as_float(o) + add);
+                                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(o_at + d), "r"(o) : "memory");
+                                tc_wait_st();
+                            }
+                        }
+                        named_barrier_sync(1, 128);
+                        if (found) {
+                            for (int c = 0; c < kChunks; ++c) {
+                                uint16_t* x = reinterpret_cast<uint16_t*>(piece(c));
+                                for (int e = 0; e < 8; ++e)
+                                    if ((x[e] & 0x7fffu) >= inf) x[e] = 0;
+                            }
+                        }
+                        if (row == 0) wild = 0;
+                        named_barrier_sync(1, 128);
+                    }
+                    fence_proxy_async_smem();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + 8 * buf);
+                if (++v_stage == ST) v_stage = 0, v_phase ^= 1;
+            }
+            mbar_wait(o_done, o_phase, &given_up, p.status);
+            o_phase ^= 1;
+            if (walk.tiles > 1) pv_phase ^= 1;
+            tc_fence_after();
+            if (warp_there) {
+                const bool out = walk.starts && walk.ends;
+                const long long slot = (blockIdx.x * 2 + (walk.starts ? 1 : 0)) * (long long)p.rows + row;
+                const float scale = there && out ? inverse_of<true>(p, rows, row, l) : 0.f;
+                uint16_t* to = static_cast<uint16_t*>(p.o) + (there ? row_at<true>(p, p.os, rows, row) : 0);
+#pragma unroll 2
+                for (int c = 0; c < DH; c += 16) {
+                    uint32_t x[16];
+                    tmem_ld16(o_at + c, x);
+                    tc_wait_ld();
+                    if (there && out) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e] = pack2<M>(__uint_as_float(x[2 * e]) * scale, __uint_as_float(x[2 * e + 1]) * scale);
+                        if (p.o_wide) {
+                            reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                            reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) to[c + 2 * e] = (uint16_t)w[e], to[c + 2 * e + 1] = (uint16_t)(w[e] >> 16);
+                        }
+                    } else if (there) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<uint4*>(p.partial + slot * DH + c + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                    }
+                    __syncwarp();  // (the next load is the whole warp's)
+                }
+                if (there && !out) p.sums[slot] = make_float2(m_used, l);
+            }
+            if (walk.starts && !walk.ends && row == 0) p.joins[blockIdx.x] = make_int4(at.b, at.item, (int)((walk.item_end - 1) / share.per), 0);
+            tc_fence_before();
+            named_barrier_sync(1, 128);  // (O and the queries may be written again)
+        }
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kColumns);
+
+    // sequences without a place
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        int lo, pos, count;
+        bool bad;
+        if (tiles_of<KT, true>(p, b, lo, pos, count, bad) > 0 || !bad) continue;
+        if (tid == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+        const int heads = p.group * p.map.kv_heads, all = count < 0 || count > p.nodes ? p.nodes : count;
+        for (int i = tid; i < all * heads * DH; i += blockDim.x) {
+            const int d = i % DH, r = i / DH, node = r / heads, h = r - node * heads;
+            put(p, static_cast<Any16*>(p.o) + b * p.os[0] + h * p.os[1] + node * p.os[2] + d, CUDART_NAN_F);
+        }
+    }
+}
+
+struct TcPlan {
+    int rows, grid;
+    size_t sums_at, partial_at, bytes;
+};
+TcPlan tc_plan(const tmw_paged_attention_desc& d, int nodes) {
+    TcPlan n;
+    const int all = d.heads / d.at.kv_heads * nodes, parts = (all + kTcRows - 1) / kTcRows;
+    n.rows = (all + parts - 1) / parts;
+    const long long capacity = (long long)d.at.columns * d.at.page_size;
+    const long long keys = d.window >= 0 && d.window + (long long)nodes < capacity ? d.window + (long long)nodes : capacity;
+    const long long tiles = ((d.n_persistent + kTcKeys - 1) / kTcKeys + keys / kTcKeys + 2) * (long long)d.at.kv_heads * parts * d.at.batch;
+    n.grid = (int)(tiles < 2 * sm_count() ? tiles : 2 * sm_count());
+    n.sums_at = (size_t)n.grid * sizeof(int4);
+    n.partial_at = (n.sums_at + (size_t)n.grid * 2 * n.rows * sizeof(float2) + 15) & ~(size_t)15;
+    n.bytes = n.partial_at + (size_t)n.grid * 2 * n.rows * d.at.head_dim * sizeof(float);
+    return n;
+}
+
+template <int DH, bool BF16>
+int launch_tc(const tmw_paged_attention_desc& d, PagedAttentionBulk& p, const TcPlan& n, cudaStream_t stream) {
+    using L = TcLayout<DH>;
+    const auto make = [&](CUtensorMap* map, const void* base, int rows) {
+        return rows == 0 || make_map_2d(map, base, TMW_F16, rows, DH, DH, p.run, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    const int rows = d.at.pages * d.at.kv_heads * d.at.page_size, pers = d.at.kv_heads * d.n_persistent;
+    if (!make(&p.k_map, d.at.k_pages, rows) || !make(&p.v_map, d.at.v_pages, rows) || !make(&p.k_pers_map, d.k_pers, pers) ||
+        !make(&p.v_pers_map, d.v_pers, pers))
+        return TMW_ERR_CUDA;
+    auto kern = paged_tree_tc_kernel<DH, BF16>;
+    const int smem = L::kBytes + 1024, rc = allow_shared_memory(reinterpret_cast<const void*>(kern), smem);
+    if (rc != TMW_OK) return rc;
+    kern<<<n.grid, kTcThreads, smem, stream>>>(p);
+    TMW_CUDA_TRY(cudaGetLastError());
+    if (n.grid > 1)
+        TMW_CUDA_TRY(launch_ex(tree_join_kernel<DH>, dim3((unsigned)n.grid - 1, (unsigned)((n.rows + kTreeJoinWarps - 1) / kTreeJoinWarps)),
+                               dim3(kTreeJoinWarps * 32), 0, stream, true, 1, static_cast<const PagedAttention&>(p)));
+    return TMW_OK;
+}
+
+}  // namespace
+
+bool tree_scratch_tc(const tmw_paged_attention_desc& d, const tmw_page_scales& s, int nodes, size_t& bytes) {
+    if (!tree_takes_tc(d, s, nodes)) return false;
+    bytes = tc_plan(d, nodes).bytes;
+    return true;
+}
+
+bool tree_launch_tc(const tmw_paged_attention_desc& d, const tmw_page_scales& s, const tmw_paged_tree_desc& tree, void* scratch,
+                    size_t scratch_bytes, cudaStream_t stream, int& status) {
+    if (!tree_takes_tc(d, s, tree.nodes)) return false;
+    PagedAttentionBulk p;
+    status = tree_arguments(d, s, tree, scratch, p);
+    if (status != TMW_OK) return true;
+    const TcPlan n = tc_plan(d, tree.nodes);
+    if (scratch_bytes < n.bytes) {
+        set_error_text("tmw_paged_tree_attention: scratch smaller than tmw_paged_tree_attention_scratch_bytes()");
+        status = TMW_ERR_INVALID_ARGUMENT;
+        return true;
+    }
+    unsigned char* at = static_cast<unsigned char*>(scratch);
+    p.rows = n.rows;
+    p.pers_tiles = (p.np + kTcKeys - 1) / kTcKeys;
+    p.joins = reinterpret_cast<int4*>(at);
+    p.sums = reinterpret_cast<float2*>(at + n.sums_at);
+    p.partial = reinterpret_cast<float*>(at + n.partial_at);
+    p.run = d.at.page_size % 64 == 0 ? 64 : d.at.page_size % 32 == 0 ? 32 : d.at.page_size % 16 == 0 ? 16 : 8;
+    const bool bf16 = d.at.dtype == TMW_BF16;
+    if (d.at.head_dim == 64) status = bf16 ? launch_tc<64, true>(d, p, n, stream) : launch_tc<64, false>(d, p, n, stream);
+    else status = bf16 ? launch_tc<128, true>(d, p, n, stream) : launch_tc<128, false>(d, p, n, stream);
+    return true;
+}
+
+}  // namespace tmw
