@@ -310,3 +310,87 @@ def test_keep_leaves_alone_what_does_not_hold(rows, count, start, break_page):
     want_k = k.clone()
     want_k[int(table[1, 0]), :, 5] = k[int(table[1, 0]), :, 6]
     assert torch.equal(d[0].cpu(), want_k)
+
+
+# ---- many rows to a key head ------------------------------------------------------------------------------------------------
+
+MANY = [
+    ([300, 3, 50], [33, 33, 17], 33, 8, 2, 128, 32, None, 3),             # 132 rows: one block of 128 and a small one
+    ([513, 77, 20, 0], [64, 1, 40, 64], 64, 4, 4, 64, 64, 100, 5),        # 64 rows, a window, a tree without tokens in front
+    ([1000], [64], 64, 8, 1, 64, 16, None, 0),                            # 512 rows: four blocks
+    ([129, 64, 63, 1], [40, 40, 40, 40], 40, 4, 2, 128, 8, 37, 0),        # runs of eight, windows that begin in tiles
+    ([700], [20], 20, 10, 5, 64, 128, None, 100),                         # more persistent keys than a tile
+    ([90, 200], [50, 12], 50, 3, 1, 128, 24, None, 64),
+]
+
+
+@pytest.mark.parametrize("dtype,form", [(BF, None), (HF, None), (BF, I8), (HF, E4)])
+@pytest.mark.parametrize("start,counts,nodes,heads,kv_heads,dh,page,window,n_p", MANY)
+def test_many_rows_against_64_bits(start, counts, nodes, heads, kv_heads, dh, page, window, n_p, dtype, form):
+    case = Case(start, counts, nodes, heads, kv_heads, dh, page, dtype, form, window, n_p, seed=dh + nodes)
+    got = case.run()
+    _native.poll_status(DEV)
+    check(got, *case.want())
+
+
+@pytest.mark.parametrize("dtype,dh,start", [(BF, 64, 70), (HF, 128, 70), (BF, 128, 200), (HF, 64, 3), (BF, 128, 0)])
+def test_what_many_rows_do_not_see_does_not_matter(dtype, dh, start):
+    """As above with 40 nodes of a chain and a half: infinities and NaN in nodes that some see, in one tile and across two."""
+    nodes, page = 40, 16
+    case = Case([start], [nodes], nodes, 4, 2, dh, page, dtype, seed=1)
+    parents = [-1] + [0 if i == 20 else i - 1 for i in range(1, nodes)]  # 1 .. 19 and 20 .. 39 are two branches
+    case.seen = dr.ancestors(parents)[0][None]
+    want, bound = case.want()
+    for node, what in ((10, math.inf), (30, math.nan)):
+        at = int(case.table[0, (start + node) // page]), slice(None), (start + node) % page
+        case.v[at] = what
+    case.v[int(case.table[0, (start + 35) // page]), :, (start + 35) % page, ::2] = -math.inf
+    got = case.run().cpu()
+    _native.poll_status(DEV)
+    assert torch.isinf(got[:, :, 10:20]).all() and (got[:, :, 10:20] > 0).all() and torch.isnan(got[:, :, 30:]).all()
+    free = list(range(10)) + list(range(20, 30))
+    check(got[:, :, free], want[:, :, free], bound[:, :, free])
+
+
+@pytest.mark.parametrize("dtype,form", [(BF, None), (HF, None), (BF, I8)])
+def test_many_rows_with_any_mask(dtype, form):
+    case = Case([0, 130, 64], [64, 40, 64], 64, 4, 2, 64, 16, dtype, form, 70, 0, seed=3, shape="any")
+    got = case.run()
+    _native.poll_status(DEV)
+    check(got, *case.want())
+    assert (got[0, :, 0] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,dh", [(BF, 64), (HF, 128)])
+def test_many_rows_and_what_has_no_place(dtype, dh):
+    case = Case([150, 40, 40], [40] * 3, 40, 4, 2, dh, 16, dtype, seed=3, branch=1)
+    want, bound = case.want()
+    case.table[0, 3] = -1           # context that every node sees
+    case.table[1, 4] = 1 << 30      # nodes 24 .. 39
+    got = case.run()
+    reported()
+    assert torch.isnan(got[0]).all() and torch.isnan(got[1, :, 24:]).all()
+    check(got[1, :, :24], want[1, :, :24], bound[1, :, :24])
+    check(got[2:], want[2:], bound[2:])
+
+
+@pytest.mark.parametrize("dtype,dh,heads,nodes", [(BF, 64, 4, 48), (HF, 128, 8, 33)])
+def test_many_rows_of_a_long_sequence_and_of_many(dtype, dh, heads, nodes):
+    case = Case([9000], [nodes], nodes, heads, 1, dh, 64, dtype, seed=6)
+    got = case.run()
+    assert all(torch.equal(got, case.run()) for _ in range(3))
+    check(got, *case.want())
+    case = Case([(37 * b) % 200 for b in range(90)], [(5 * b) % (nodes + 1) for b in range(90)], nodes, heads, 1, dh, 16, dtype, n_p=3, seed=7)
+    got = case.run()
+    _native.poll_status(DEV)
+    check(got, *case.want())
+
+
+def test_many_rows_with_strides():
+    case = Case([140], [40], 40, 2, 2, 64, 16, BF, seed=2)
+    q, out = torch.zeros(1, 40, 2, 67, dtype=BF), torch.zeros(1, 40, 2, 71, dtype=BF, device=DEV)
+    q[..., 1:65] = case.q.permute(0, 2, 1, 3)
+    got = paged_tree_attention(q.to(DEV).permute(0, 2, 1, 3)[..., 1:65], *dev(case.k, case.v, case.table), numbers([140]), case.seen.to(DEV),
+                               out=out.permute(0, 2, 1, 3)[..., 3:67])
+    check(got, *case.want())
+    assert (out[..., :3] == 0).all() and (out[..., 67:] == 0).all()

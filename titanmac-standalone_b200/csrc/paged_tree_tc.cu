@@ -1,16 +1,18 @@
 // Attention of a tree's drafted tokens over pages of 16-bit numbers, many rows to a key head (tcgen05; head_dim 64 or 128).
 //
 // Up to 128 (node, head) rows of a key head are one tile of tcgen05.mma, so that 64 keys cost the tensor core the same for 33 rows as for
-// 128, a fifth of what mma.sync takes for them (9 cycles of a scheduler for each 16 x 8 x 16).  A CTA, two to an SM, is one worker of the
+// 128, a fifth of what mma.sync takes for them (9 cycles of a scheduler for each 16 x 8 x 16).  A CTA, one to an SM, is one worker of the
 // line of tiles (paged_attention.cuh), here of 64 keys, and its warps have fixed roles:
-//   warp  0    pages looked up, K and V brought by TMA, a run of up to 64 neighbouring tokens at a time
-//   warp  1    issues the products (one elected thread)
-//   warps 4-7  softmax, a thread to a row; queries into shared memory, outputs out of tensor memory
-// S = Q K^T (two buffers in tensor memory, the next scores are multiplied while these are exponentiated); P goes over its S as two 16-bit
-// numbers a weight, 64 columns for 64 fp32 ones; O += P V.  The running maximum follows only a score that is 2^4 above it: O is brought
-// up in tensor memory then.  Tiles that some row does not see in full, at a window's begin and among the nodes, have the rows' bits
-// applied to the scores, and their values made harmless: rows that nobody sees are zeros, and what is infinite or no number is added
-// row by row to those that see it.
+//   warp  0     pages looked up, K and V brought by TMA, a run of up to 64 neighbouring tokens at a time
+//   warp  1     issues the products (one elected thread)
+//   warps 4-11  softmax, a thread to a row; queries into shared memory, outputs out of tensor memory
+// A tile's chain - products, hand-over, exponentials, hand-over, products - is several times as long as its parts, so two streams of
+// softmax warps take the tiles by turns, each with a running maximum, a sum and an output of its own, and two buffers of scores: S = Q K^T
+// of four tiles is under way while P goes over its S as two 16-bit numbers a weight (64 columns for 64 fp32 ones) and O += P V.  The streams are joined
+// when the part ends.  (As two CTAs to an SM, with two tiles of each of K and V: 16 ragged sequences of 32 heads on 8, 32 nodes, 160 us.)
+// The running maximum follows only a score that is 2^4 above it: O is brought up in tensor memory then.  Tiles that some row does not
+// see in full, at a window's begin and among the nodes, have the rows' bits applied to the scores, and their values made harmless: rows
+// that nobody sees are zeros, and what is infinite or no number is added row by row to those that see it.
 //
 // All waits are bounded (paged_attention.cuh); the tensor memory is given back on every way.
 #include "paged_tree.cuh"
@@ -20,19 +22,18 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTcKeys = 64, kTcRows = 128, kTcThreads = 256, kTcCost = 2;
-constexpr int kRegsService = 56, kRegsSoftmax = 200;
-static_assert(kTcThreads / 2 * (kRegsService + kRegsSoftmax) <= 65536 / 2, "setmaxnreg: what the softmax warps ask for the others release");
+constexpr int kTcKeys = 64, kTcRows = 128, kTcThreads = 384, kTcCost = 2;
+constexpr int kTcAhead = 4;  // tiles whose scores are under way
 
 template <int DH>
 struct TcLayout {
-    static constexpr int kSubs = DH / 64, kStages = DH == 64 ? 4 : 2;  // sub-tiles of 64 columns; tiles in a ring
+    static constexpr int kSubs = DH / 64, kKStages = DH == 64 ? 10 : 5, kVStages = DH == 64 ? 10 : 6;  // sub-tiles of 64 columns; tiles in the rings
     static constexpr int kQSub = kTcRows * 128, kSub = kTcKeys * 128, kTile = kSub * kSubs;
-    static constexpr int kK = kQSub * kSubs, kV = kK + kStages * kTile, kBytes = kV + kStages * kTile;
+    static constexpr int kK = kQSub * kSubs, kV = kK + kKStages * kTile, kBytes = kV + kVStages * kTile;
 };
-// of a tile: its first key's token (-1: persistent ones), its keys that exist, runs without a page
+// of a tile: its first key's token (-1: persistent ones), its keys that exist, runs that are there and that have no page, where they are
 struct TileInfo {
-    int place, first, last, lost, run;
+    int place, first, last, there, lost, rows[kTcKeys / 8];
 };
 
 // A CTA's parts of items, one after the other, as every role walks over them.
@@ -59,30 +60,31 @@ struct Walk {
 };
 
 template <int DH, bool BF16>
-__global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
+__global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
     using L = TcLayout<DH>;
     using M = std::conditional_t<BF16, __nv_bfloat16, __half>;
-    constexpr int KT = kTcKeys, ST = L::kStages;
+    constexpr int KT = kTcKeys, KS = L::kKStages, VS = L::kVStages;
     constexpr float kRaise = BF16 ? 0.f : 11.f;  // a weight is at most 2^4 under it
-    constexpr uint32_t kO = 2 * KT, kColumns = 256;
+    constexpr uint32_t kO = 4 * KT, kColumns = 512;  // two buffers of scores for each stream, then their outputs
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ alignas(8) uint64_t bars[8 + 4 * ST];
-    __shared__ TileInfo infos[ST];
+    __shared__ alignas(8) uint64_t bars[14 + 2 * (KS + VS)];
+    __shared__ TileInfo infos[16];  // of the last tiles
+    __shared__ float2 stream_sums[2][kTcRows];
     __shared__ uint32_t tmem_slot;
-    __shared__ int given_up, wild, first_adds, lows[4];
+    __shared__ int given_up, wild[2], first_adds[2], lows[8];
     unsigned char* smem = dynamic + (1024 - smem_u32(dynamic)) % 1024;
     const uint32_t base = smem_u32(smem);
     const uint32_t bar0 = smem_u32(bars);
-    const uint32_t q_ready = bar0, s_full = bar0 + 8, p_ready = bar0 + 24, o_done = bar0 + 40, pv_done = bar0 + 48;
-    const uint32_t k_full = bar0 + 64, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST;
+    // [stream][buffer], or [stream]
+    const uint32_t q_ready = bar0, s_full = bar0 + 8, p_ready = bar0 + 40, o_done = bar0 + 72, pv_done = bar0 + 88;
+    const uint32_t k_full = bar0 + 112, k_free = k_full + 8 * KS, v_full = k_free + 8 * KS, v_free = v_full + 8 * VS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        mbar_init(q_ready, 4);
-        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
-        mbar_init(o_done, 1);
-        mbar_init(pv_done, 1);
-        for (int i = 0; i < 4 * ST; ++i) mbar_init(k_full + 8 * i, 1);
-        given_up = wild = first_adds = 0;
+        mbar_init(q_ready, 8);
+        for (int i = 0; i < 4; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
+        for (int i = 0; i < 2; ++i) mbar_init(o_done + 8 * i, 1), mbar_init(pv_done + 8 * i, 1), wild[i] = first_adds[i] = 0;
+        for (int i = 0; i < 2 * (KS + VS); ++i) mbar_init(k_full + 8 * i, 1);
+        given_up = 0;
         p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -98,12 +100,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
     walk.begin = share.first;
     const long long limit = share.first < share.end ? share.end : share.first;
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService) : "memory");
         if (warp == 0) {
-            // ---- K and V ----
+            // ---- K and V, in the order in which they are used: four tiles' keys, then the values of one and the keys of the fourth behind it ----
             const int runs = KT / p.run;
-            int stage = 0;
-            uint32_t phase = 1;
+            int k_stage = 0, v_stage = 0, n = 0;  // n: tiles whose keys have been asked for, of all parts
+            uint32_t k_phase = 1, v_phase = 1;
             while (walk.next(p, limit)) {
                 const auto& at = walk.now;
                 int row = -1, page = -1;
@@ -125,41 +126,44 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                         }
                     }
                 };
-                look(walk.first_tile);
-                for (int i = 0; i < walk.tiles; ++i) {
-                    if (row >= 0) {
-                        if (pers) row += at.head * p.np;
-                        else row = (uint32_t)page < (uint32_t)p.map.pages ? (page * p.map.kv_heads + at.head) * (int)p.map.page.d + row : -2;
-                    }
-                    const uint32_t there = __ballot_sync(0xffffffffu, row >= 0), lost = __ballot_sync(0xffffffffu, row == -2);
-                    const uint32_t bytes = __popc(there) * p.run * DH * 2;
-                    const CUtensorMap *km = pers ? &p.k_pers_map : &p.k_map, *vm = pers ? &p.v_pers_map : &p.v_map;
-                    mbar_wait(k_free + 8 * stage, phase, &given_up, p.status);
-                    if (elect_one()) mbar_expect_tx(k_full + 8 * stage, bytes);
-                    for (uint32_t todo = there; todo != 0; todo &= todo - 1) {
-                        const int r = __ffs(todo) - 1, from = __shfl_sync(0xffffffffu, row, r);
-                        if (elect_one()) {
-#pragma unroll
-                            for (int s = 0; s < L::kSubs; ++s)
-                                tma_load_2d(base + L::kK + stage * L::kTile + s * L::kSub + r * p.run * 128, km, k_full + 8 * stage, s * 64, from);
-                        }
-                    }
-                    mbar_wait(v_free + 8 * stage, phase, &given_up, p.status);
+                auto bring = [&](const CUtensorMap* map, uint32_t to, uint32_t bar, const TileInfo& info) {
                     if (elect_one()) {
-                        infos[stage] = {pers ? -1 : j0, first, last, (int)lost, p.run};
-                        mbar_expect_tx(v_full + 8 * stage, bytes);
-                    }
-                    for (uint32_t todo = there; todo != 0; todo &= todo - 1) {
-                        const int r = __ffs(todo) - 1, from = __shfl_sync(0xffffffffu, row, r);
-                        if (elect_one()) {
+                        mbar_expect_tx(bar, __popc(info.there) * p.run * DH * 2);
+                        for (uint32_t todo = info.there; todo != 0; todo &= todo - 1) {
+                            const int r = __ffs(todo) - 1;
 #pragma unroll
-                            for (int s = 0; s < L::kSubs; ++s)
-                                tma_load_2d(base + L::kV + stage * L::kTile + s * L::kSub + r * p.run * 128, vm, v_full + 8 * stage, s * 64, from);
+                            for (int s = 0; s < L::kSubs; ++s) tma_load_2d(to + s * L::kSub + r * p.run * 128, map, bar, s * 64, info.rows[r]);
                         }
                     }
-                    if (lost != 0 && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
-                    if (++stage == ST) stage = 0, phase ^= 1;
-                    if (i + 1 < walk.tiles) look(walk.first_tile + i + 1);
+                    __syncwarp();
+                };
+                look(walk.first_tile);
+                for (int i = 0; i < walk.tiles + kTcAhead; ++i) {
+                    if (i >= kTcAhead) {
+                        mbar_wait(v_free + 8 * v_stage, v_phase, &given_up, p.status);
+                        // (of tile i - kTcAhead, the place of whose description is not written again before its values are used)
+                        const int behind = n - (i < walk.tiles ? kTcAhead : walk.tiles + kTcAhead - i);
+                        const TileInfo& info = infos[behind & 15];
+                        bring(info.place < 0 ? &p.v_pers_map : &p.v_map, base + L::kV + v_stage * L::kTile, v_full + 8 * v_stage, info);
+                        if (++v_stage == VS) v_stage = 0, v_phase ^= 1;
+                    }
+                    if (i < walk.tiles) {
+                        if (row >= 0) {
+                            if (pers) row += at.head * p.np;
+                            else row = (uint32_t)page < (uint32_t)p.map.pages ? (page * p.map.kv_heads + at.head) * (int)p.map.page.d + row : -2;
+                        }
+                        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0), lost = __ballot_sync(0xffffffffu, row == -2);
+                        if (lost != 0 && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+                        mbar_wait(k_free + 8 * k_stage, k_phase, &given_up, p.status);
+                        TileInfo& info = infos[n & 15];
+                        if (lane < runs) info.rows[lane] = row;
+                        if (lane == 0) info.place = pers ? -1 : j0, info.first = first, info.last = last, info.there = (int)there, info.lost = (int)lost;
+                        __syncwarp();
+                        bring(pers ? &p.k_pers_map : &p.k_map, base + L::kK + k_stage * L::kTile, k_full + 8 * k_stage, info);
+                        if (++k_stage == KS) k_stage = 0, k_phase ^= 1;
+                        ++n;
+                        if (i + 1 < walk.tiles) look(walk.first_tile + i + 1);
+                    }
                 }
             }
         } else if (warp == 1 && elect_one()) {
@@ -167,53 +171,58 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
             constexpr uint32_t fmt = BF16 ? 1u : 0u;
             const uint32_t idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((KT >> 3) << 17) | ((kTcRows >> 4) << 24);
             const uint32_t idesc_pv = idesc_b_mnmajor(fmt, DH);
-            int k_stage = 0, v_stage = 0, n = 0;  // n: tiles whose scores have been issued, of all parts
+            int k_stage = 0, v_stage = 0;
+            int in[2] = {0, 0}, out[2] = {0, 0};  // tiles of a stream whose scores, whose values have been issued, of all parts
             uint32_t k_phase = 0, v_phase = 0, q_phase = 0;
-            auto scores = [&]() {
+            auto scores = [&](int g) {
                 mbar_wait(k_full + 8 * k_stage, k_phase, &given_up, p.status);
                 tc_fence_after();
+                const int buf = 2 * g + (in[g] & 1);
 #pragma unroll
                 for (int k = 0; k < DH / 16; ++k)
-                    mma_ss(tmem + (n & 1) * KT, kmajor_desc(base + k / 4 * L::kQSub) + k % 4 * 2,
+                    mma_ss(tmem + buf * KT, kmajor_desc(base + k / 4 * L::kQSub) + k % 4 * 2,
                            kmajor_desc(base + L::kK + k_stage * L::kTile + k / 4 * L::kSub) + k % 4 * 2, idesc_qk, k > 0 ? 1u : 0u);
-                tc_commit(s_full + 8 * (n & 1));
+                tc_commit(s_full + 8 * buf);
                 tc_commit(k_free + 8 * k_stage);
-                if (++k_stage == ST) k_stage = 0, k_phase ^= 1;
-                ++n;
+                if (++k_stage == KS) k_stage = 0, k_phase ^= 1;
+                ++in[g];
             };
-            int m = 0;  // tiles whose values have been issued
             while (walk.next(p, limit)) {
                 mbar_wait(q_ready, q_phase, &given_up, p.status);
                 q_phase ^= 1;
                 tc_fence_after();
-                for (int i = 0; i < 2 && i < walk.tiles; ++i) scores();
+                for (int i = 0; i < kTcAhead && i < walk.tiles; ++i) scores(i & 1);
                 for (int i = 0; i < walk.tiles; ++i) {
+                    const int g = i & 1, buf = 2 * g + (out[g] & 1);
                     mbar_wait(v_full + 8 * v_stage, v_phase, &given_up, p.status);
-                    mbar_wait(p_ready + 8 * (m & 1), (m >> 1) & 1, &given_up, p.status);
+                    mbar_wait(p_ready + 8 * buf, (out[g] >> 1) & 1, &given_up, p.status);
                     tc_fence_after();
-                    const uint32_t pt = tmem + (m & 1) * KT;
+                    const uint32_t pt = tmem + buf * KT, to = tmem + kO + g * DH;
                     const uint64_t v = mnmajor_desc(base + L::kV + v_stage * L::kTile, L::kSub);
-                    const uint32_t onto = i > 0 || *(volatile int*)&first_adds ? 1u : 0u;
+                    const uint32_t onto = i > 1 || *(volatile int*)&first_adds[g] ? 1u : 0u;
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
 #pragma unroll
-                        for (int k = 0; k < KT / 16; ++k) mma_ts(tmem + kO, pt + half * 32 + k * 8, v + k * 128, idesc_pv, half + k > 0 ? 1u : onto);
-                    ++m;
-                    if (i + 2 < walk.tiles) scores();
-                    else if (i + 2 == walk.tiles) tc_commit(pv_done);  // the last tile but one
-                    else tc_commit(o_done);
+                        for (int k = 0; k < KT / 16; ++k) mma_ts(to, pt + half * 32 + k * 8, v + k * 128, idesc_pv, half + k > 0 ? 1u : onto);
+                    ++out[g];
+                    if (i + kTcAhead < walk.tiles) scores(g);
+                    else if (i + 2 >= walk.tiles) tc_commit(o_done + 8 * g);  // the stream's last tile
+                    else tc_commit(pv_done + 8 * g);                          // its last but one
                     tc_commit(v_free + 8 * v_stage);
-                    if (++v_stage == ST) v_stage = 0, v_phase ^= 1;
+                    if (++v_stage == VS) v_stage = 0, v_phase ^= 1;
                 }
             }
         }
     } else {
         // ---- softmax: a thread to a row ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax) : "memory");
-        const int row = tid - 128;
-        const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lane_at + kO;
-        int n = 0, v_stage = 0;
+        const int g = (warp - 4) >> 2, row = tid & 127;
+        const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lane_at + kO + g * DH;
+        int n = 0, v_stage = 0, tile = 0;  // n: the stream's tiles, tile: everybody's, of all parts
         uint32_t v_phase = 0, o_phase = 0, pv_phase = 0;
+        const auto next_stage = [&]() {
+            if (++v_stage == VS) v_stage = 0, v_phase ^= 1;
+            ++tile;
+        };
         while (walk.next(p, limit)) {
             const auto& at = walk.now;
             const Rows rows = rows_of<true>(p, at.b, at.head, at.item - at.head * at.parts(p), at.count);
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                 }
                 const bool wide = p.q_wide;
 #pragma unroll 4
-                for (int c = 0; c < DH / 8; ++c) {
+                for (int c = g; c < DH / 8; c += 2) {
                     uint4 w = make_uint4(0, 0, 0, 0);
                     if (there) {
                         if (wide) {
@@ -248,21 +257,23 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                 int warp_low = low;
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) warp_low = max(warp_low, __shfl_xor_sync(0xffffffffu, warp_low, d));
-                if (lane == 0) lows[warp & 3] = warp_low;
-                if (row == 0) first_adds = 0;
+                if (lane == 0) lows[warp - 4] = warp_low;
+                if (row == 0) first_adds[g] = 0;
                 fence_proxy_async_smem();
-                named_barrier_sync(1, 128);
+                named_barrier_sync(3, 256);
                 if (lane == 0) mbar_arrive(q_ready);
             }
             const int lowest = max(max(lows[0], lows[1]), max(lows[2], lows[3]));
             float m_used = -CUDART_INF_F, l = 0.f;
-            for (int i = 0; i < walk.tiles; ++i, ++n) {
-                const int buf = n & 1;
+            const int mine_of = (walk.tiles + 1 - g) / 2;  // tiles of this stream
+            if (g == 1) next_stage();  // (the first tile is the other stream's)
+            for (int i = 0; i < mine_of; ++i, ++n) {
+                const int buf = 2 * g + (n & 1);
                 const uint32_t s_at = tmem + lane_at + buf * KT;
-                mbar_wait(s_full + 8 * buf, (n >> 1) & 1, &given_up, p.status);
                 mbar_wait(v_full + 8 * v_stage, v_phase, &given_up, p.status);
+                mbar_wait(s_full + 8 * buf, (n >> 1) & 1, &given_up, p.status);
                 tc_fence_after();
-                const TileInfo info = infos[v_stage];
+                const TileInfo& info = infos[tile & 15];
                 const bool whole = info.first == 0 && info.last == KT - 1 && info.lost == 0 &&
                                    (info.place < 0 || (info.place + KT <= start && info.place >= lowest));
                 uint32_t s[KT];
@@ -276,7 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                 }
                 uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first, bad = 0;
                 if (!whole) {
-                    for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1) bad |= (info.run == 64 ? ~0ull : (1ull << info.run) - 1) << (__ffs(todo) - 1) * info.run;
+                    for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1) bad |= (p.run == 64 ? ~0ull : (1ull << p.run) - 1) << (__ffs(todo) - 1) * p.run;
                     uint64_t seen = exists;
                     if (info.place >= 0) {
                         const int nodes_at = start - info.place, from = low - info.place;  // of node 0, of the window's begin
@@ -297,8 +308,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                 }
                 // what the last product but one left in O is final; may O be changed?
                 auto wait_products = [&]() {
-                    if (i + 1 < walk.tiles) mbar_wait(s_full + 8 * (buf ^ 1), ((n + 1) >> 1) & 1, &given_up, p.status);
-                    else if (walk.tiles > 1) mbar_wait(pv_done, pv_phase, &given_up, p.status);
+                    if (i + 1 < mine_of) mbar_wait(s_full + 8 * (buf ^ 1), ((n + 1) >> 1) & 1, &given_up, p.status);
+                    else if (mine_of > 1) mbar_wait(pv_done + 8 * g, pv_phase, &given_up, p.status);
                     tc_fence_after();
                 };
                 if (warp_there) {
@@ -329,17 +340,17 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                 const float less = (m_used == -CUDART_INF_F ? 0.f : m_used) - kRaise;
                 if (warp_there) {
 #pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) {
-                        uint32_t first[16], second[16];
+                    for (int c = 0; c < KT / 16; ++c) {
+                        uint32_t first[8], second[8];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float a = ex2_ftz(fmaf(__uint_as_float(s[c * 32 + 2 * e]), p.scale, -less));
-                            const float b = ex2_ftz(fmaf(__uint_as_float(s[c * 32 + 2 * e + 1]), p.scale, -less));
+                        for (int e = 0; e < 8; ++e) {
+                            const float a = ex2_ftz(fmaf(__uint_as_float(s[c * 16 + 2 * e]), p.scale, -less));
+                            const float b = ex2_ftz(fmaf(__uint_as_float(s[c * 16 + 2 * e + 1]), p.scale, -less));
                             l += a + b;
                             split_in_two<M>(a, b, first[e], second[e]);
                         }
-                        tmem_st16(s_at + c * 16, first);
-                        tmem_st16(s_at + 32 + c * 16, second);
+                        tmem_st8(s_at + c * 8, first);
+                        tmem_st8(s_at + 32 + c * 8, second);
                     }
                     tc_wait_st();
                 }
@@ -363,11 +374,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                             any |= ((v.x & 0x7fff7fffu) + up) | ((v.y & 0x7fff7fffu) + up) | ((v.z & 0x7fff7fffu) + up) | ((v.w & 0x7fff7fffu) + up);
                         }
                         found = (any & 0x80008000u) != 0;
-                        if (found) wild = 1;
+                        if (found) wild[g] = 1;
                     }
-                    named_barrier_sync(1, 128);
-                    const bool any_wild = *(volatile int*)&wild != 0;
-                    named_barrier_sync(1, 128);  // (all have read it: the next such tile may set it)
+                    named_barrier_sync(1 + g, 128);
+                    const bool any_wild = *(volatile int*)&wild[g] != 0;
+                    named_barrier_sync(1 + g, 128);  // (all have read it: the next such tile may set it)
                     if (any_wild) {
                         // Infinities and NaN to the rows that see them, number by number, into O: in front of a part's first product O
                         // is made zero, and that product told to add.
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                                 tmem_st16(o_at + c, zero);
                             }
                             tc_wait_st();
-                            if (row == 0) first_adds = 1;
+                            if (row == 0) first_adds[g] = 1;
                         } else {
                             wait_products();
                         }
@@ -399,7 +410,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                                 tc_wait_st();
                             }
                         }
-                        named_barrier_sync(1, 128);
+                        named_barrier_sync(1 + g, 128);
                         if (found) {
                             for (int c = 0; c < kChunks; ++c) {
                                 uint16_t* x = reinterpret_cast<uint16_t*>(piece(c));
@@ -407,34 +418,55 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                                     if ((x[e] & 0x7fffu) >= inf) x[e] = 0;
                             }
                         }
-                        if (row == 0) wild = 0;
-                        named_barrier_sync(1, 128);
+                        if (row == 0) wild[g] = 0;
+                        named_barrier_sync(1 + g, 128);
                     }
                     fence_proxy_async_smem();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready + 8 * buf);
-                if (++v_stage == ST) v_stage = 0, v_phase ^= 1;
+                next_stage();
+                if (2 * i + g + 1 < walk.tiles) next_stage();  // (the other stream's)
             }
-            mbar_wait(o_done, o_phase, &given_up, p.status);
-            o_phase ^= 1;
-            if (walk.tiles > 1) pv_phase ^= 1;
+            if (mine_of > 0) {
+                mbar_wait(o_done + 8 * g, o_phase, &given_up, p.status);
+                o_phase ^= 1;
+            }
+            if (mine_of > 1) pv_phase ^= 1;
+            tc_fence_after();
+            stream_sums[g][row] = make_float2(m_used, l);
+            tc_fence_before();
+            named_barrier_sync(3, 256);
             tc_fence_after();
             if (warp_there) {
+                // both streams' outputs, a half of the dimensions each
+                const float2 other = stream_sums[g ^ 1][row];
+                const float m = fmaxf(m_used, other.x), of = m == -CUDART_INF_F ? 0.f : m;
+                float own_part = part_weight(m_used, of), other_part = part_weight(other.x, of);
+                if (walk.tiles == 1) (g == 0 ? other_part : own_part) = 0.f;  // (the second stream had none)
+                const float sum = (walk.tiles == 1 && g == 1 ? 0.f : l * own_part) + (walk.tiles == 1 && g == 0 ? 0.f : other.y * other_part);
+                const bool single = walk.tiles == 1;
+                const float w0 = g == 0 ? own_part : other_part, w1 = g == 0 ? other_part : own_part;
                 const bool out = walk.starts && walk.ends;
                 const long long slot = (blockIdx.x * 2 + (walk.starts ? 1 : 0)) * (long long)p.rows + row;
-                const float scale = there && out ? inverse_of<true>(p, rows, row, l) : 0.f;
+                const float scale = there && out ? inverse_of<true>(p, rows, row, sum) : 1.f;
                 uint16_t* to = static_cast<uint16_t*>(p.o) + (there ? row_at<true>(p, p.os, rows, row) : 0);
 #pragma unroll 2
-                for (int c = 0; c < DH; c += 16) {
-                    uint32_t x[16];
-                    tmem_ld16(o_at + c, x);
+                for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 16) {
+                    uint32_t x[16], y[16];
+                    tmem_ld16(tmem + lane_at + kO + c, x);
+                    tmem_ld16(tmem + lane_at + kO + DH + c, y);
                     tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float a = __uint_as_float(x[e]) * w0;
+                        x[e] = __float_as_uint((single ? a : fmaf(__uint_as_float(y[e]), w1, a)) * scale);
+                    }
                     if (there && out) {
                         uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = pack2<M>(__uint_as_float(x[2 * e]) * scale, __uint_as_float(x[2 * e + 1]) * scale);
+                        for (int e = 0; e < 8; ++e) w[e] = pack2<M>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
                         if (p.o_wide) {
                             reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
                             reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
@@ -449,11 +481,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_tree_tc_kernel(const __gr
                     }
                     __syncwarp();  // (the next load is the whole warp's)
                 }
-                if (there && !out) p.sums[slot] = make_float2(m_used, l);
+                if (there && !out && g == 0) p.sums[slot] = make_float2(m, sum);
             }
-            if (walk.starts && !walk.ends && row == 0) p.joins[blockIdx.x] = make_int4(at.b, at.item, (int)((walk.item_end - 1) / share.per), 0);
+            if (walk.starts && !walk.ends && tid == 128) p.joins[blockIdx.x] = make_int4(at.b, at.item, (int)((walk.item_end - 1) / share.per), 0);
             tc_fence_before();
-            named_barrier_sync(1, 128);  // (O and the queries may be written again)
+            named_barrier_sync(3, 256);  // (O, the queries and the sums may be written again)
         }
     }
     __syncthreads();
@@ -481,11 +513,11 @@ struct TcPlan {
 TcPlan tc_plan(const tmw_paged_attention_desc& d, int nodes) {
     TcPlan n;
     const int all = d.heads / d.at.kv_heads * nodes, parts = (all + kTcRows - 1) / kTcRows;
-    n.rows = (all + parts - 1) / parts;
+    n.rows = all < kTcRows ? all : kTcRows;  // (a tile costs the same however many rows it has)
     const long long capacity = (long long)d.at.columns * d.at.page_size;
     const long long keys = d.window >= 0 && d.window + (long long)nodes < capacity ? d.window + (long long)nodes : capacity;
     const long long tiles = ((d.n_persistent + kTcKeys - 1) / kTcKeys + keys / kTcKeys + 2) * (long long)d.at.kv_heads * parts * d.at.batch;
-    n.grid = (int)(tiles < 2 * sm_count() ? tiles : 2 * sm_count());
+    n.grid = (int)(tiles < sm_count() ? tiles : sm_count());
     n.sums_at = (size_t)n.grid * sizeof(int4);
     n.partial_at = (n.sums_at + (size_t)n.grid * 2 * n.rows * sizeof(float2) + 15) & ~(size_t)15;
     n.bytes = n.partial_at + (size_t)n.grid * 2 * n.rows * d.at.head_dim * sizeof(float);
