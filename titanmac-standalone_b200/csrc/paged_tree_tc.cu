@@ -3,8 +3,10 @@
 // Up to 128 (node, head) rows of a key head are one tile of tcgen05.mma, so that 64 keys cost the tensor core the same for 33 rows as for
 // 128, a fifth of what mma.sync takes for them (9 cycles of a scheduler for each 16 x 8 x 16).  A CTA, one to an SM, is one worker of the
 // line of tiles (paged_attention.cuh), here of 64 keys, and its warps have fixed roles:
-//   warp  0     pages looked up, K and V brought by TMA, a run of up to 64 neighbouring tokens at a time
-//   warp  1     issues the products (one elected thread)
+//   warp  0, 3  bring K, bring V by TMA, a run of up to 64 neighbouring tokens at a time; every lane looks the page of one run up, for
+//               4 to 32 tiles in one go (one warp for both, tile by tile, needed 2050 cycles for each: 183 us instead of PRODUCED)
+//   warp  1, 2  issue the products for the scores, and those with the values (one elected thread each: a product costs its thread some
+//               thirty cycles, and a commit hundreds)
 //   warps 4-11  softmax, a thread to a row; queries into shared memory, outputs out of tensor memory
 // A tile's chain - products, hand-over, exponentials, hand-over, products - is several times as long as its parts, so two streams of
 // softmax warps take the tiles by turns, each with a running maximum, a sum and an output of its own, and two buffers of scores: S = Q K^T
@@ -23,17 +25,17 @@ namespace {
 using namespace ptx;
 
 constexpr int kTcKeys = 64, kTcRows = 128, kTcThreads = 384, kTcCost = 2;
-constexpr int kTcAhead = 4;  // tiles whose scores are under way
+constexpr int kTcAhead = 4;  // tiles whose scores are under way: buffers of scores, and tiles in the ring of keys
 
 template <int DH>
 struct TcLayout {
-    static constexpr int kSubs = DH / 64, kKStages = DH == 64 ? 10 : 5, kVStages = DH == 64 ? 10 : 6;  // sub-tiles of 64 columns; tiles in the rings
+    static constexpr int kSubs = DH / 64, kKStages = kTcAhead, kVStages = DH == 64 ? 12 : 7;  // sub-tiles of 64 columns; tiles in the rings
     static constexpr int kQSub = kTcRows * 128, kSub = kTcKeys * 128, kTile = kSub * kSubs;
     static constexpr int kK = kQSub * kSubs, kV = kK + kKStages * kTile, kBytes = kV + kVStages * kTile;
 };
-// of a tile: its first key's token (-1: persistent ones), its keys that exist, runs that are there and that have no page, where they are
+// of a tile: its first key's token (-1: persistent ones), its keys that exist, its runs that have no page
 struct TileInfo {
-    int place, first, last, there, lost, rows[kTcKeys / 8];
+    int place, first, last, lost;
 };
 
 // A CTA's parts of items, one after the other, as every role walks over them.
@@ -63,11 +65,11 @@ template <int DH, bool BF16>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
     using L = TcLayout<DH>;
     using M = std::conditional_t<BF16, __nv_bfloat16, __half>;
-    constexpr int KT = kTcKeys, KS = L::kKStages, VS = L::kVStages;
+    constexpr int KT = kTcKeys, VS = L::kVStages;
     constexpr float kRaise = BF16 ? 0.f : 11.f;  // a weight is at most 2^4 under it
     constexpr uint32_t kO = 4 * KT, kColumns = 512;  // two buffers of scores for each stream, then their outputs
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ alignas(8) uint64_t bars[14 + 2 * (KS + VS)];
+    __shared__ alignas(8) uint64_t bars[1 + 3 * kTcAhead + 2 * VS];
     __shared__ TileInfo infos[16];  // of the last tiles
     __shared__ float2 stream_sums[2][kTcRows];
     __shared__ uint32_t tmem_slot;
@@ -75,15 +77,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
     unsigned char* smem = dynamic + (1024 - smem_u32(dynamic)) % 1024;
     const uint32_t base = smem_u32(smem);
     const uint32_t bar0 = smem_u32(bars);
-    // [stream][buffer], or [stream]
-    const uint32_t q_ready = bar0, s_full = bar0 + 8, p_ready = bar0 + 40, o_done = bar0 + 72, pv_done = bar0 + 88;
-    const uint32_t k_full = bar0 + 112, k_free = k_full + 8 * KS, v_full = k_free + 8 * KS, v_free = v_full + 8 * VS;
+    // Of tile t, counted over all parts: stream t & 1, buffer of scores and place of its keys t & 3, place of its values t % VS; a barrier's
+    // phase is the turn's.  Keys are let go with their scores, scores and weights with the products with the values (v_free).
+    const uint32_t q_ready = bar0, k_full = bar0 + 8, s_full = k_full + 32, p_ready = s_full + 32, v_full = p_ready + 32, v_free = v_full + 8 * VS;
+    const auto turn = [](int t) { return (uint32_t)(t >> 2) & 1; };
+    const auto v_turn = [](int t) { return (uint32_t)(t / VS) & 1; };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         mbar_init(q_ready, 8);
-        for (int i = 0; i < 4; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
-        for (int i = 0; i < 2; ++i) mbar_init(o_done + 8 * i, 1), mbar_init(pv_done + 8 * i, 1), wild[i] = first_adds[i] = 0;
-        for (int i = 0; i < 2 * (KS + VS); ++i) mbar_init(k_full + 8 * i, 1);
+        for (int i = 0; i < kTcAhead; ++i) mbar_init(k_full + 8 * i, 1), mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
+        for (int i = 0; i < 2 * VS; ++i) mbar_init(v_full + 8 * i, 1);
+        wild[0] = wild[1] = first_adds[0] = first_adds[1] = 0;
         given_up = 0;
         p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -100,116 +104,109 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
     walk.begin = share.first;
     const long long limit = share.first < share.end ? share.end : share.first;
     if (warp < 4) {
-        if (warp == 0) {
-            // ---- K and V, in the order in which they are used: four tiles' keys, then the values of one and the keys of the fourth behind it ----
+        if (warp == 0 || warp == 3) {
+            // ---- the keys; the values ----
+            const bool values = warp == 3;
             const int runs = KT / p.run;
-            int k_stage = 0, v_stage = 0, n = 0;  // n: tiles whose keys have been asked for, of all parts
-            uint32_t k_phase = 1, v_phase = 1;
+            int t = 0;
             while (walk.next(p, limit)) {
                 const auto& at = walk.now;
-                int row = -1, page = -1;
-                bool pers = false;
-                int j0 = 0, first = 0, last = 0;
-                auto look = [&](int tile) {  // this lane's run of a tile
-                    pers = tile < p.pers_tiles;
-                    j0 = (pers ? tile : at.lo / KT + tile - p.pers_tiles) * KT;
-                    first = pers ? 0 : max(at.lo - j0, 0);
-                    last = min((pers ? p.np - 1 : at.pos) - j0, KT - 1);
+                int planned = 0, row = -1, page = -1;  // the first tile of the plan; this lane's run: -1 not wanted, -2 nowhere
+                uint32_t there = 0, lost = 0;          // lanes
+                auto look = [&](int tile) {
+                    planned = tile;
+                    tile += lane / runs;
+                    const bool pers = tile < p.pers_tiles;
+                    const int j = (pers ? tile : at.lo / KT + tile - p.pers_tiles) * KT + lane % runs * p.run;
                     row = -1;
-                    const int j = lane * p.run;
-                    if (lane < runs && j <= last && j + p.run > first) {
-                        row = j0 + j;
+                    if (tile < at.n - kTcCost && j <= (pers ? p.np - 1 : at.pos) && j + p.run > (pers ? 0 : at.lo)) {
+                        row = j;
                         if (!pers) {
-                            const uint32_t column = p.map.page.div((uint32_t)row);
+                            const uint32_t column = p.map.page.div((uint32_t)j);
                             row -= (int)(column * p.map.page.d);
                             page = __ldg(p.map.table + at.b * p.map.table_stride + column);
                         }
                     }
                 };
-                auto bring = [&](const CUtensorMap* map, uint32_t to, uint32_t bar, const TileInfo& info) {
-                    if (elect_one()) {
-                        mbar_expect_tx(bar, __popc(info.there) * p.run * DH * 2);
-                        for (uint32_t todo = info.there; todo != 0; todo &= todo - 1) {
-                            const int r = __ffs(todo) - 1;
-#pragma unroll
-                            for (int s = 0; s < L::kSubs; ++s) tma_load_2d(to + s * L::kSub + r * p.run * 128, map, bar, s * 64, info.rows[r]);
-                        }
-                    }
-                    __syncwarp();
-                };
                 look(walk.first_tile);
-                for (int i = 0; i < walk.tiles + kTcAhead; ++i) {
-                    if (i >= kTcAhead) {
-                        mbar_wait(v_free + 8 * v_stage, v_phase, &given_up, p.status);
-                        // (of tile i - kTcAhead, the place of whose description is not written again before its values are used)
-                        const int behind = n - (i < walk.tiles ? kTcAhead : walk.tiles + kTcAhead - i);
-                        const TileInfo& info = infos[behind & 15];
-                        bring(info.place < 0 ? &p.v_pers_map : &p.v_map, base + L::kV + v_stage * L::kTile, v_full + 8 * v_stage, info);
-                        if (++v_stage == VS) v_stage = 0, v_phase ^= 1;
-                    }
-                    if (i < walk.tiles) {
+                for (int i = 0; i < walk.tiles; ++i, ++t) {
+                    const int tile = walk.first_tile + i;
+                    if (tile == planned) {  // the pages have come
                         if (row >= 0) {
-                            if (pers) row += at.head * p.np;
+                            if (tile + lane / runs < p.pers_tiles) row += at.head * p.np;
                             else row = (uint32_t)page < (uint32_t)p.map.pages ? (page * p.map.kv_heads + at.head) * (int)p.map.page.d + row : -2;
                         }
-                        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0), lost = __ballot_sync(0xffffffffu, row == -2);
-                        if (lost != 0 && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
-                        mbar_wait(k_free + 8 * k_stage, k_phase, &given_up, p.status);
-                        TileInfo& info = infos[n & 15];
-                        if (lane < runs) info.rows[lane] = row;
-                        if (lane == 0) info.place = pers ? -1 : j0, info.first = first, info.last = last, info.there = (int)there, info.lost = (int)lost;
-                        __syncwarp();
-                        bring(pers ? &p.k_pers_map : &p.k_map, base + L::kK + k_stage * L::kTile, k_full + 8 * k_stage, info);
-                        if (++k_stage == KS) k_stage = 0, k_phase ^= 1;
-                        ++n;
-                        if (i + 1 < walk.tiles) look(walk.first_tile + i + 1);
+                        there = __ballot_sync(0xffffffffu, row >= 0);
+                        lost = __ballot_sync(0xffffffffu, row == -2);
                     }
+                    const bool pers = tile < p.pers_tiles;
+                    const int from = (tile - planned) * runs, mask = (1 << runs) - 1;
+                    const int slot = values ? t % VS : t & 3;
+                    const uint32_t full = values ? v_full + 8 * slot : k_full + 8 * slot;
+                    const uint32_t to = base + (values ? L::kV : L::kK) + slot * L::kTile;
+                    const CUtensorMap* map = values ? (pers ? &p.v_pers_map : &p.v_map) : (pers ? &p.k_pers_map : &p.k_map);
+                    if (values) {
+                        if (t >= VS) mbar_wait(v_free + 8 * slot, v_turn(t - VS), &given_up, p.status);
+                    } else if (t >= kTcAhead) {
+                        mbar_wait(s_full + 8 * slot, turn(t - kTcAhead), &given_up, p.status);
+                    }
+                    if (elect_one()) {
+                        if (values) {
+                            const int j0 = (pers ? tile : at.lo / KT + tile - p.pers_tiles) * KT;
+                            infos[t & 15] = {pers ? -1 : j0, pers ? 0 : max(at.lo - j0, 0), min((pers ? p.np - 1 : at.pos) - j0, KT - 1), (int)(lost >> from) & mask};
+                        }
+                        mbar_expect_tx(full, __popc(there >> from & mask) * p.run * DH * 2);
+                    }
+                    __syncwarp();
+                    for (uint32_t todo = there >> from & mask; todo != 0; todo &= todo - 1) {
+                        const int r = __ffs(todo) - 1, first = __shfl_sync(0xffffffffu, row, from + r);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int s = 0; s < L::kSubs; ++s) tma_load_2d(to + s * L::kSub + r * p.run * 128, map, full, s * 64, first);
+                        }
+                    }
+                    if (values && (lost >> from & mask) != 0 && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
+                    if (from + runs == 32 && i + 1 < walk.tiles) look(tile + 1);
                 }
             }
         } else if (warp == 1 && elect_one()) {
-            // ---- the products ----
-            constexpr uint32_t fmt = BF16 ? 1u : 0u;
-            const uint32_t idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((KT >> 3) << 17) | ((kTcRows >> 4) << 24);
-            const uint32_t idesc_pv = idesc_b_mnmajor(fmt, DH);
-            int k_stage = 0, v_stage = 0;
-            int in[2] = {0, 0}, out[2] = {0, 0};  // tiles of a stream whose scores, whose values have been issued, of all parts
-            uint32_t k_phase = 0, v_phase = 0, q_phase = 0;
-            auto scores = [&](int g) {
-                mbar_wait(k_full + 8 * k_stage, k_phase, &given_up, p.status);
-                tc_fence_after();
-                const int buf = 2 * g + (in[g] & 1);
-#pragma unroll
-                for (int k = 0; k < DH / 16; ++k)
-                    mma_ss(tmem + buf * KT, kmajor_desc(base + k / 4 * L::kQSub) + k % 4 * 2,
-                           kmajor_desc(base + L::kK + k_stage * L::kTile + k / 4 * L::kSub) + k % 4 * 2, idesc_qk, k > 0 ? 1u : 0u);
-                tc_commit(s_full + 8 * buf);
-                tc_commit(k_free + 8 * k_stage);
-                if (++k_stage == KS) k_stage = 0, k_phase ^= 1;
-                ++in[g];
-            };
+            // ---- the scores ----
+            constexpr uint32_t fmt = BF16 ? 1u : 0u, idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((KT >> 3) << 17) | ((kTcRows >> 4) << 24);
+            int t = 0;
+            uint32_t q_phase = 0;
             while (walk.next(p, limit)) {
                 mbar_wait(q_ready, q_phase, &given_up, p.status);
                 q_phase ^= 1;
-                tc_fence_after();
-                for (int i = 0; i < kTcAhead && i < walk.tiles; ++i) scores(i & 1);
-                for (int i = 0; i < walk.tiles; ++i) {
-                    const int g = i & 1, buf = 2 * g + (out[g] & 1);
-                    mbar_wait(v_full + 8 * v_stage, v_phase, &given_up, p.status);
-                    mbar_wait(p_ready + 8 * buf, (out[g] >> 1) & 1, &given_up, p.status);
+                for (int i = 0; i < walk.tiles; ++i, ++t) {
+                    mbar_wait(k_full + 8 * (t & 3), turn(t), &given_up, p.status);
+                    if (t >= kTcAhead) mbar_wait(v_free + 8 * ((t - kTcAhead) % VS), v_turn(t - kTcAhead), &given_up, p.status);
                     tc_fence_after();
-                    const uint32_t pt = tmem + buf * KT, to = tmem + kO + g * DH;
-                    const uint64_t v = mnmajor_desc(base + L::kV + v_stage * L::kTile, L::kSub);
-                    const uint32_t onto = i > 1 || *(volatile int*)&first_adds[g] ? 1u : 0u;
+                    const uint64_t q = kmajor_desc(base), keys = kmajor_desc(base + L::kK + (t & 3) * L::kTile);
+#pragma unroll
+                    for (int k = 0; k < DH / 16; ++k)
+                        mma_ss(tmem + (t & 3) * KT, q + k / 4 * (L::kQSub >> 4) + k % 4 * 2, keys + k / 4 * (L::kSub >> 4) + k % 4 * 2, idesc, k > 0 ? 1u : 0u);
+                    tc_commit(s_full + 8 * (t & 3));
+                }
+            }
+        } else if (warp == 2 && elect_one()) {
+            // ---- the products with the values ----
+            const uint32_t idesc = idesc_b_mnmajor(BF16 ? 1u : 0u, DH);
+            int t = 0;
+            while (walk.next(p, limit)) {
+                for (int i = 0; i < walk.tiles; ++i, ++t) {
+                    const int v = t % VS;
+                    mbar_wait(v_full + 8 * v, v_turn(t), &given_up, p.status);
+                    mbar_wait(p_ready + 8 * (t & 3), turn(t), &given_up, p.status);
+                    tc_fence_after();
+                    const uint32_t weights = tmem + (t & 3) * KT, to = tmem + kO + (t & 1) * DH;
+                    const uint64_t values = mnmajor_desc(base + L::kV + v * L::kTile, L::kSub);
+                    const uint32_t onto = i > 1 || *(volatile int*)&first_adds[t & 1] ? 1u : 0u;  // (a stream's first tile of a part begins its O)
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
 #pragma unroll
-                        for (int k = 0; k < KT / 16; ++k) mma_ts(to, pt + half * 32 + k * 8, v + k * 128, idesc_pv, half + k > 0 ? 1u : onto);
-                    ++out[g];
-                    if (i + kTcAhead < walk.tiles) scores(g);
-                    else if (i + 2 >= walk.tiles) tc_commit(o_done + 8 * g);  // the stream's last tile
-                    else tc_commit(pv_done + 8 * g);                          // its last but one
-                    tc_commit(v_free + 8 * v_stage);
-                    if (++v_stage == VS) v_stage = 0, v_phase ^= 1;
+                        for (int k = 0; k < KT / 16; ++k)
+                            mma_ts(to, weights + half * 32 + k * 8, values + k * 128, idesc, half + k > 0 ? 1u : onto);
+                    tc_commit(v_free + 8 * v);
                 }
             }
         }
@@ -217,12 +214,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
         // ---- softmax: a thread to a row ----
         const int g = (warp - 4) >> 2, row = tid & 127;
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lane_at + kO + g * DH;
-        int n = 0, v_stage = 0, tile = 0;  // n: the stream's tiles, tile: everybody's, of all parts
-        uint32_t v_phase = 0, o_phase = 0, pv_phase = 0;
-        const auto next_stage = [&]() {
-            if (++v_stage == VS) v_stage = 0, v_phase ^= 1;
-            ++tile;
-        };
+        int t0 = 0;  // the part's first tile
         while (walk.next(p, limit)) {
             const auto& at = walk.now;
             const Rows rows = rows_of<true>(p, at.b, at.head, at.item - at.head * at.parts(p), at.count);
@@ -265,15 +257,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
             }
             const int lowest = max(max(lows[0], lows[1]), max(lows[2], lows[3]));
             float m_used = -CUDART_INF_F, l = 0.f;
-            const int mine_of = (walk.tiles + 1 - g) / 2;  // tiles of this stream
-            if (g == 1) next_stage();  // (the first tile is the other stream's)
-            for (int i = 0; i < mine_of; ++i, ++n) {
-                const int buf = 2 * g + (n & 1);
+            const int t1 = t0 + walk.tiles;
+            int t = t0 + ((t0 & 1) != g ? 1 : 0);
+            const bool none = t >= t1;  // (a part of one tile is the other stream's)
+            for (bool begins = true; t < t1; t += 2, begins = false) {
+                const int buf = t & 3, v_stage = t % VS;
                 const uint32_t s_at = tmem + lane_at + buf * KT;
-                mbar_wait(v_full + 8 * v_stage, v_phase, &given_up, p.status);
-                mbar_wait(s_full + 8 * buf, (n >> 1) & 1, &given_up, p.status);
+                mbar_wait(v_full + 8 * v_stage, v_turn(t), &given_up, p.status);
+                mbar_wait(s_full + 8 * buf, turn(t), &given_up, p.status);
                 tc_fence_after();
-                const TileInfo& info = infos[tile & 15];
+                const TileInfo& info = infos[t & 15];
                 const bool whole = info.first == 0 && info.last == KT - 1 && info.lost == 0 &&
                                    (info.place < 0 || (info.place + KT <= start && info.place >= lowest));
                 uint32_t s[KT];
@@ -306,10 +299,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                             if (nan >> j & 1) s[j] = 0x7fffffffu;
                     }
                 }
-                // what the last product but one left in O is final; may O be changed?
+                // O may be changed: the products of the stream's last tile are done
                 auto wait_products = [&]() {
-                    if (i + 1 < mine_of) mbar_wait(s_full + 8 * (buf ^ 1), ((n + 1) >> 1) & 1, &given_up, p.status);
-                    else if (mine_of > 1) mbar_wait(pv_done + 8 * g, pv_phase, &given_up, p.status);
+                    mbar_wait(v_free + 8 * ((t - 2) % VS), v_turn(t - 2), &given_up, p.status);
                     tc_fence_after();
                 };
                 if (warp_there) {
@@ -317,7 +309,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
 #pragma unroll
                     for (int j = 0; j < KT; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(s[j]));
                     const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
-                    if (i == 0) {
+                    if (begins) {
                         m_used = tile_top;
                     } else if (__any_sync(0xffffffffu, tile_top > m_used + 4.f)) {
                         const float now = tile_top > m_used + 4.f ? tile_top : m_used;
@@ -382,7 +374,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                     if (any_wild) {
                         // Infinities and NaN to the rows that see them, number by number, into O: in front of a part's first product O
                         // is made zero, and that product told to add.
-                        if (i == 0) {
+                        if (begins) {
                             for (int c = 0; c < DH; c += 16) {
                                 const uint32_t zero[16] = {};
                                 tmem_st16(o_at + c, zero);
@@ -426,15 +418,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready + 8 * buf);
-                next_stage();
-                if (2 * i + g + 1 < walk.tiles) next_stage();  // (the other stream's)
             }
-            if (mine_of > 0) {
-                mbar_wait(o_done + 8 * g, o_phase, &given_up, p.status);
-                o_phase ^= 1;
-            }
-            if (mine_of > 1) pv_phase ^= 1;
-            tc_fence_after();
+            if (!none) mbar_wait(v_free + 8 * ((t - 2) % VS), v_turn(t - 2), &given_up, p.status);
+            t0 = t1;
             stream_sums[g][row] = make_float2(m_used, l);
             tc_fence_before();
             named_barrier_sync(3, 256);
@@ -443,11 +429,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                 // both streams' outputs, a half of the dimensions each
                 const float2 other = stream_sums[g ^ 1][row];
                 const float m = fmaxf(m_used, other.x), of = m == -CUDART_INF_F ? 0.f : m;
-                float own_part = part_weight(m_used, of), other_part = part_weight(other.x, of);
-                if (walk.tiles == 1) (g == 0 ? other_part : own_part) = 0.f;  // (the second stream had none)
-                const float sum = (walk.tiles == 1 && g == 1 ? 0.f : l * own_part) + (walk.tiles == 1 && g == 0 ? 0.f : other.y * other_part);
+                // (a part of one tile: the stream that had none has an O of anything, which must not count)
                 const bool single = walk.tiles == 1;
-                const float w0 = g == 0 ? own_part : other_part, w1 = g == 0 ? other_part : own_part;
+                const float own_part = none ? 0.f : part_weight(m_used, of), other_part = single && !none ? 0.f : part_weight(other.x, of);
+                const float sum = l * own_part + other.y * other_part;
                 const bool out = walk.starts && walk.ends;
                 const long long slot = (blockIdx.x * 2 + (walk.starts ? 1 : 0)) * (long long)p.rows + row;
                 const float scale = there && out ? inverse_of<true>(p, rows, row, sum) : 1.f;
@@ -455,13 +440,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
 #pragma unroll 2
                 for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 16) {
                     uint32_t x[16], y[16];
-                    tmem_ld16(tmem + lane_at + kO + c, x);
-                    tmem_ld16(tmem + lane_at + kO + DH + c, y);
+                    tmem_ld16(o_at + c, x);
+                    tmem_ld16(tmem + lane_at + kO + (g ^ 1) * DH + c, y);
                     tc_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float a = __uint_as_float(x[e]) * w0;
-                        x[e] = __float_as_uint((single ? a : fmaf(__uint_as_float(y[e]), w1, a)) * scale);
+                        const float a = none ? 0.f : __uint_as_float(x[e]) * own_part;
+                        const float b = single && !none ? 0.f : __uint_as_float(y[e]) * other_part;
+                        x[e] = __float_as_uint((a + b) * scale);
                     }
                     if (there && out) {
                         uint32_t w[8];
