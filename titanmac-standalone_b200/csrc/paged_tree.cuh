@@ -817,7 +817,7 @@ TMW_TREE_OF(tc)
 // Which calls tcgen05 takes: 16-bit pages that come by TMA, head_dim 64 or 128, and more rows to a key head than mma.sync's two or three warps
 // have, TREE_ROWS.
 inline bool tree_takes_tc(const tmw_paged_attention_desc& d, const tmw_page_scales& s, int nodes) {
-    return s.format == TMW_PAGES_SAME && d.at.dtype != TMW_F32 && (d.at.head_dim == 64 || d.at.head_dim == 128) && can_bulk(d, s) &&
+    return d.at.dtype != TMW_F32 && (d.at.head_dim == 64 || d.at.head_dim == 128) && can_bulk(d, s) &&
            d.heads / d.at.kv_heads * nodes > 32;
 }
 

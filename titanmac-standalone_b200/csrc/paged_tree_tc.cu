@@ -1,4 +1,4 @@
-// Attention of a tree's drafted tokens over pages of 16-bit numbers, many rows to a key head (tcgen05; head_dim 64 or 128).
+// Attention of a tree's drafted tokens, many rows to a key head, over pages of 16-bit numbers or of codes (tcgen05; head_dim 64 or 128).
 //
 // Up to 128 (node, head) rows of a key head are one tile of tcgen05.mma, so that 64 keys cost the tensor core the same for 33 rows as for
 // 128, a fifth of what mma.sync takes for them (9 cycles of a scheduler for each 16 x 8 x 16).  A CTA, one to an SM, is one worker of the
@@ -16,6 +16,10 @@
 // see in full, at a window's begin and among the nodes, have the rows' bits applied to the scores, and their values made harmless: rows
 // that nobody sees are zeros, and what is infinite or no number is added row by row to those that see it.
 //
+// Pages of 8 bits: TMA brings codes, and four more warps (12-15) turn them into fp16 tiles of the same form, once for all rows, and every key's
+// scales into the numbers that the softmax warps use (see the attention of one token): scores times the key's scale, weights times the
+// value's in two parts.
+//
 // All waits are bounded (paged_attention.cuh); the tensor memory is given back on every way.
 #include "paged_tree.cuh"
 
@@ -24,15 +28,26 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTcKeys = 64, kTcRows = 128, kTcThreads = 384, kTcCost = 2;
+constexpr int kTcKeys = 64, kTcRows = 128, kTcCost = 9;  // (what an item costs besides its tiles: 2 | 4 | 6 | 9 made the ragged sequences 149 | 135 | 127 | 124 us)
 constexpr int kTcAhead = 4;  // tiles whose scores are under way: buffers of scores, and tiles in the ring of keys
 
-template <int DH>
+template <typename P, int DH>
 struct TcLayout {
-    static constexpr int kSubs = DH / 64, kKStages = kTcAhead, kVStages = DH == 64 ? 12 : 7;  // sub-tiles of 64 columns; tiles in the rings
+    static constexpr bool k8 = kScaled<P>;
+    static constexpr int kSubs = DH / 64, kKStages = k8 ? 2 : kTcAhead, kVStages = k8 ? 4 : DH == 64 ? 12 : 7;  // sub-tiles of 64 columns; tiles in the rings
+    // (who waits for the values of four tiles ago must not find the barrier a turn further)
+    static_assert(kVStages >= kTcAhead, "a phase is asked for before the next but one");
     static constexpr int kQSub = kTcRows * 128, kSub = kTcKeys * 128, kTile = kSub * kSubs;
-    static constexpr int kK = kQSub * kSubs, kV = kK + kKStages * kTile, kBytes = kV + kVStages * kTile;
+    static constexpr int kK = kQSub * kSubs, kV = kK + kKStages * kTile;
+    // codes: rings of four tiles, with scales of keys and values; then what becomes of the scales, of eight tiles, {key's scale, exponent} and {rest, back}
+    static constexpr int kRawTile = kTcKeys * DH, kRawK = kV + kVStages * kTile, kRawV = kRawK + (k8 ? 4 * kRawTile : 0);
+    static constexpr int kScales = kRawV + (k8 ? 4 * kRawTile : 0), kParts = kScales + (k8 ? 4 * 2 * kTcKeys * 4 : 0);
+    static constexpr int kBytes = kParts + (k8 ? 8 * 2 * kTcKeys * 8 : 0);
+    static constexpr int kThreads = k8 ? 512 : 384;
 };
+// registers of the codes' form: sixteen warps have 128 each at launch
+constexpr int kRegsService = 80, kRegsSoftmax = 176;
+static_assert(8 * 32 * (kRegsService + kRegsSoftmax) <= 512 * 128, "setmaxnreg: what the softmax warps ask for the others release");
 // of a tile: its first key's token (-1: persistent ones), its keys that exist, its runs that have no page
 struct TileInfo {
     int place, first, last, lost;
@@ -61,15 +76,41 @@ struct Walk {
     }
 };
 
-template <int DH, bool BF16>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
-    using L = TcLayout<DH>;
+// sixteen codes as fp16 numbers, in their order
+template <typename P>
+__device__ __forceinline__ void to_halves(const uint4& codes, uint4 (&out)[2]) {
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<P, E4m3>::value) {
+            const __half2 a = from_e4m3(w[i]), b = from_e4m3(w[i] >> 16);
+            x[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+            x[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {  // 0 .. 255 under the exponent of 1024, less 1024 + 128
+            const uint32_t u = w[i] ^ 0x80808080u, bias = 0x64806480u;
+            const auto less = [&](uint32_t v) {
+                const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&bias));
+                return *reinterpret_cast<const uint32_t*>(&d);
+            };
+            x[2 * i] = less(__byte_perm(u, 0x64646464u, 0x4140));
+            x[2 * i + 1] = less(__byte_perm(u, 0x64646464u, 0x4342));
+        }
+    }
+    out[0] = make_uint4(x[0], x[1], x[2], x[3]);
+    out[1] = make_uint4(x[4], x[5], x[6], x[7]);
+}
+
+template <typename P, int DH>
+__global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
+    using L = TcLayout<P, DH>;
+    constexpr bool k8 = L::k8, BF16 = std::is_same<P, __nv_bfloat16>::value;
     using M = std::conditional_t<BF16, __nv_bfloat16, __half>;
-    constexpr int KT = kTcKeys, VS = L::kVStages;
-    constexpr float kRaise = BF16 ? 0.f : 11.f;  // a weight is at most 2^4 under it
+    constexpr int KT = kTcKeys, KS = L::kKStages, VS = L::kVStages;
+    constexpr float kRaise = BF16 ? 0.f : k8 ? 10.f : 11.f;  // (a weight is at most 2^4, of codes 2^5, times that)
     constexpr uint32_t kO = 4 * KT, kColumns = 512;  // two buffers of scores for each stream, then their outputs
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ alignas(8) uint64_t bars[1 + 3 * kTcAhead + 2 * VS];
+    __shared__ alignas(8) uint64_t bars[1 + 3 * kTcAhead + 2 * VS + (k8 ? 16 : 0)];
     __shared__ TileInfo infos[16];  // of the last tiles
     __shared__ float2 stream_sums[2][kTcRows];
     __shared__ uint32_t tmem_slot;
@@ -77,16 +118,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
     unsigned char* smem = dynamic + (1024 - smem_u32(dynamic)) % 1024;
     const uint32_t base = smem_u32(smem);
     const uint32_t bar0 = smem_u32(bars);
-    // Of tile t, counted over all parts: stream t & 1, buffer of scores and place of its keys t & 3, place of its values t % VS; a barrier's
-    // phase is the turn's.  Keys are let go with their scores, scores and weights with the products with the values (v_free).
+    // Of tile t, counted over all parts: stream t & 1, buffer of scores t & 3, places of its keys t % KS and of its values t % VS (of its codes
+    // t & 3); a barrier's phase is the turn's.  Keys are let go with their scores, scores and weights with the products with the values (v_free).
     const uint32_t q_ready = bar0, k_full = bar0 + 8, s_full = k_full + 32, p_ready = s_full + 32, v_full = p_ready + 32, v_free = v_full + 8 * VS;
+    const uint32_t raw_k_full = v_free + 8 * VS, raw_k_free = raw_k_full + 32, raw_v_full = raw_k_free + 32, raw_v_free = raw_v_full + 32;  // codes
     const auto turn = [](int t) { return (uint32_t)(t >> 2) & 1; };
     const auto v_turn = [](int t) { return (uint32_t)(t / VS) & 1; };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         mbar_init(q_ready, 8);
-        for (int i = 0; i < kTcAhead; ++i) mbar_init(k_full + 8 * i, 1), mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
-        for (int i = 0; i < 2 * VS; ++i) mbar_init(v_full + 8 * i, 1);
+        for (int i = 0; i < kTcAhead; ++i) mbar_init(k_full + 8 * i, k8 ? 4 : 1), mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
+        for (int i = 0; i < VS; ++i) mbar_init(v_full + 8 * i, k8 ? 4 : 1), mbar_init(v_free + 8 * i, 1);
+        if (k8)
+            for (int i = 0; i < 4; ++i)
+                mbar_init(raw_k_full + 8 * i, 1), mbar_init(raw_k_free + 8 * i, 4), mbar_init(raw_v_full + 8 * i, 1), mbar_init(raw_v_free + 8 * i, 4);
         wild[0] = wild[1] = first_adds[0] = first_adds[1] = 0;
         given_up = 0;
         p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -104,6 +149,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
     walk.begin = share.first;
     const long long limit = share.first < share.end ? share.end : share.first;
     if (warp < 4) {
+        if constexpr (k8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService) : "memory");
         if (warp == 0 || warp == 3) {
             // ---- the keys; the values ----
             const bool values = warp == 3;
@@ -141,28 +187,57 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                     }
                     const bool pers = tile < p.pers_tiles;
                     const int from = (tile - planned) * runs, mask = (1 << runs) - 1;
-                    const int slot = values ? t % VS : t & 3;
-                    const uint32_t full = values ? v_full + 8 * slot : k_full + 8 * slot;
-                    const uint32_t to = base + (values ? L::kV : L::kK) + slot * L::kTile;
-                    const CUtensorMap* map = values ? (pers ? &p.v_pers_map : &p.v_map) : (pers ? &p.k_pers_map : &p.k_map);
-                    if (values) {
-                        if (t >= VS) mbar_wait(v_free + 8 * slot, v_turn(t - VS), &given_up, p.status);
-                    } else if (t >= kTcAhead) {
-                        mbar_wait(s_full + 8 * slot, turn(t - kTcAhead), &given_up, p.status);
+                    const int slot = values && !k8 ? t % VS : t & 3;
+                    uint32_t full, to;
+                    if constexpr (k8) {
+                        full = (values ? raw_v_full : raw_k_full) + 8 * slot;
+                        to = base + (values ? L::kRawV : L::kRawK) + slot * L::kRawTile;
+                        if (t >= 4) mbar_wait((values ? raw_v_free : raw_k_free) + 8 * slot, turn(t - 4), &given_up, p.status);
+                    } else {
+                        full = values ? v_full + 8 * slot : k_full + 8 * slot;
+                        to = base + (values ? L::kV : L::kK) + slot * L::kTile;  // (KS is four here)
+                        if (values) {
+                            if (t >= VS) mbar_wait(v_free + 8 * slot, v_turn(t - VS), &given_up, p.status);
+                        } else if (t >= kTcAhead) {
+                            mbar_wait(s_full + 8 * slot, turn(t - kTcAhead), &given_up, p.status);
+                        }
                     }
+                    const CUtensorMap* map = values ? (pers ? &p.v_pers_map : &p.v_map) : (pers ? &p.k_pers_map : &p.k_map);
+                    const bool with_scales = k8 && !values;
+                    float* scales = reinterpret_cast<float*>(smem + L::kScales) + slot * 2 * KT;
+                    if (with_scales && pers) {  // (they need not begin on sixteen bytes)
+                        const int j0 = tile * KT;
+#pragma unroll
+                        for (int h = 0; h < KT; h += 32) {
+                            const bool mine = j0 + h + lane < p.np;
+                            scales[h + lane] = mine ? __ldg(p.k_pers_scales + at.head * p.np + j0 + h + lane) : 0.f;
+                            scales[KT + h + lane] = mine ? __ldg(p.v_pers_scales + at.head * p.np + j0 + h + lane) : 0.f;
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    const int scale_bytes = with_scales && !pers ? p.run * 4 : 0;
                     if (elect_one()) {
                         if (values) {
                             const int j0 = (pers ? tile : at.lo / KT + tile - p.pers_tiles) * KT;
                             infos[t & 15] = {pers ? -1 : j0, pers ? 0 : max(at.lo - j0, 0), min((pers ? p.np - 1 : at.pos) - j0, KT - 1), (int)(lost >> from) & mask};
                         }
-                        mbar_expect_tx(full, __popc(there >> from & mask) * p.run * DH * 2);
+                        mbar_expect_tx(full, __popc(there >> from & mask) * (p.run * DH * (int)sizeof(P) + 2 * scale_bytes));
                     }
                     __syncwarp();
                     for (uint32_t todo = there >> from & mask; todo != 0; todo &= todo - 1) {
                         const int r = __ffs(todo) - 1, first = __shfl_sync(0xffffffffu, row, from + r);
                         if (elect_one()) {
+                            if constexpr (k8) {
+                                tma_load_2d(to + r * p.run * DH, map, full, 0, first);
+                                if (scale_bytes != 0) {
+                                    bulk_load(smem_u32(scales) + r * scale_bytes, p.k_scales + first, scale_bytes, full);
+                                    bulk_load(smem_u32(scales + KT) + r * scale_bytes, p.v_scales + first, scale_bytes, full);
+                                }
+                            } else {
 #pragma unroll
-                            for (int s = 0; s < L::kSubs; ++s) tma_load_2d(to + s * L::kSub + r * p.run * 128, map, full, s * 64, first);
+                                for (int s = 0; s < L::kSubs; ++s) tma_load_2d(to + s * L::kSub + r * p.run * 128, map, full, s * 64, first);
+                            }
                         }
                     }
                     if (values && (lost >> from & mask) != 0 && lane == 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
@@ -181,7 +256,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                     mbar_wait(k_full + 8 * (t & 3), turn(t), &given_up, p.status);
                     if (t >= kTcAhead) mbar_wait(v_free + 8 * ((t - kTcAhead) % VS), v_turn(t - kTcAhead), &given_up, p.status);
                     tc_fence_after();
-                    const uint64_t q = kmajor_desc(base), keys = kmajor_desc(base + L::kK + (t & 3) * L::kTile);
+                    const uint64_t q = kmajor_desc(base), keys = kmajor_desc(base + L::kK + t % KS * L::kTile);
 #pragma unroll
                     for (int k = 0; k < DH / 16; ++k)
                         mma_ss(tmem + (t & 3) * KT, q + k / 4 * (L::kQSub >> 4) + k % 4 * 2, keys + k / 4 * (L::kSub >> 4) + k % 4 * 2, idesc, k > 0 ? 1u : 0u);
@@ -210,8 +285,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                 }
             }
         }
+    } else if (k8 && warp >= 12) {
+        if constexpr (k8) {
+            // ---- codes into fp16 tiles: the keys of a tile, with the scales of both, then the values of the tile two in front of it ----
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService) : "memory");
+            const int mine = tid - 384;
+            auto convert = [&](const unsigned char* from, uint32_t to, uint64_t exists) {
+                constexpr int kPieces = KT * DH / 16 / 128, kOfRow = DH / 16;
+                uint4 codes[kPieces];
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) codes[i] = reinterpret_cast<const uint4*>(from)[i * 128 + mine];
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int row = (i * 128 + mine) / kOfRow, c = (i * 128 + mine) % kOfRow * 2;
+                    uint4 x[2];
+                    to_halves<P>(codes[i], x);
+                    if ((exists >> row & 1) == 0) x[0] = x[1] = make_uint4(0, 0, 0, 0);  // (may be no number)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        *reinterpret_cast<uint4*>(smem + to + c / 8 * L::kSub + row * 128 + (((c + h) % 8 ^ (row & 7)) << 4)) = x[h];
+                }
+            };
+            int t = 0;  // the part's first tile
+            while (walk.next(p, limit)) {
+                for (int i = 0; i < walk.tiles + 2; ++i) {
+                    if (i < walk.tiles) {
+                        const int k = t + i;
+                        mbar_wait(raw_k_full + 8 * (k & 3), turn(k), &given_up, p.status);
+                        if (k >= KS) mbar_wait(s_full + 8 * ((k - KS) & 3), turn(k - KS), &given_up, p.status);
+                        convert(smem + L::kRawK + (k & 3) * L::kRawTile, L::kK + k % KS * L::kTile, ~0ull);
+                        if (mine < KT) {
+                            const float* scales = reinterpret_cast<const float*>(smem + L::kScales) + (k & 3) * 2 * KT;
+                            const float vs = scales[KT + mine];
+                            const int bits = __float_as_int(fmaxf(vs, 0x1p-100f));
+                            float2* parts = reinterpret_cast<float2*>(smem + L::kParts) + (k & 7) * 2 * KT;
+                            parts[mine] = make_float2(scales[mine], __int_as_float(0x4b000000 | (bits >> 23)) - (8388608.f + 127.f) + (vs - vs));
+                            parts[KT + mine] = make_float2(__int_as_float((bits & 0x007fffff) | 0x3f800000),
+                                                           __int_as_float(0x7f000000 - min(bits & 0x7f800000, 0x7e800000)));
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(k_full + 8 * (k & 3)), mbar_arrive(raw_k_free + 8 * (k & 3));
+                    }
+                    if (i >= 2) {
+                        const int v = t + i - 2, slot = v % VS;
+                        mbar_wait(raw_v_full + 8 * (v & 3), turn(v), &given_up, p.status);
+                        if (v >= VS) mbar_wait(v_free + 8 * slot, v_turn(v - VS), &given_up, p.status);
+                        const TileInfo& info = infos[v & 15];
+                        uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first;
+                        for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1)
+                            exists &= ~((p.run == 64 ? ~0ull : (1ull << p.run) - 1) << (__ffs(todo) - 1) * p.run);
+                        convert(smem + L::kRawV + (v & 3) * L::kRawTile, L::kV + slot * L::kTile, exists);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_full + 8 * slot), mbar_arrive(raw_v_free + 8 * (v & 3));
+                    }
+                }
+                t += walk.tiles;
+            }
+        }
     } else {
         // ---- softmax: a thread to a row ----
+        if constexpr (k8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax) : "memory");
         const int g = (warp - 4) >> 2, row = tid & 127;
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lane_at + kO + g * DH;
         int t0 = 0;  // the part's first tile
@@ -222,6 +357,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
             const bool there = row < rows.n, warp_there = (warp & 3) * 32 < rows.n;
             int low = 0;
             uint64_t nodes = 0;
+            float q_scale = p.scale;
             {   // the row's queries, as TMA would leave them
                 const uint16_t* from = static_cast<const uint16_t*>(p.q);
                 if (there) {
@@ -230,19 +366,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                     nodes = nodes_seen(p, at.b, at.count, node);
                     from += row_at<true>(p, p.qs, rows, row);
                 }
-                const bool wide = p.q_wide;
+                const auto eight = [&](int c) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (there && p.q_wide) {
+                        w = *reinterpret_cast<const uint4*>(from + c * 8);
+                    } else if (there) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = from[c * 8 + 2 * e] | (uint32_t)from[c * 8 + 2 * e + 1] << 16;
+                        w = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                    return w;
+                };
+                float up = 1.f;
+                if (k8 && p.bf16) {  // as fp16 numbers times a power of two of the row's own
+                    float top = 0.f;
+#pragma unroll 4
+                    for (int c = 0; c < DH / 8; ++c) {
+                        const uint4 w = eight(c);
+                        for (uint32_t x : {w.x, w.y, w.z, w.w}) {
+                            const float2 two = tmw::unpack2<__nv_bfloat16>(x);
+                            top = fmaxf(top, fmaxf(fabsf(two.x), fabsf(two.y)));
+                        }
+                    }
+                    const int e = max((__float_as_int(top) >> 23) - 127, -100);
+                    up = __int_as_float((127 + 14 - e) << 23);
+                    q_scale *= __int_as_float((127 - 14 + e) << 23);
+                }
 #pragma unroll 4
                 for (int c = g; c < DH / 8; c += 2) {
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (there) {
-                        if (wide) {
-                            w = *reinterpret_cast<const uint4*>(from + c * 8);
-                        } else {
-                            uint32_t x[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] = from[c * 8 + 2 * e] | (uint32_t)from[c * 8 + 2 * e + 1] << 16;
-                            w = make_uint4(x[0], x[1], x[2], x[3]);
-                        }
+                    uint4 w = eight(c);
+                    if (k8 && p.bf16) {
+                        const auto half = [&](uint32_t x) {
+                            const float2 two = tmw::unpack2<__nv_bfloat16>(x);
+                            return tmw::pack2<__half>(two.x * up, two.y * up);
+                        };
+                        w = make_uint4(half(w.x), half(w.y), half(w.z), half(w.w));
                     }
                     *reinterpret_cast<uint4*>(smem + c / 8 * L::kQSub + row * 128 + ((c % 8 ^ (row & 7)) << 4)) = w;
                 }
@@ -278,6 +437,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                     }
                     tc_wait_ld();
                 }
+                const float2* parts = reinterpret_cast<const float2*>(smem + L::kParts) + (t & 7) * 2 * KT;
+                if constexpr (k8) {
+#pragma unroll
+                    for (int j = 0; j < KT; ++j) {
+                        const float2 part = parts[j];
+                        s[j] = __float_as_uint(fmaf(__uint_as_float(s[j]) * part.x, q_scale, part.y));
+                    }
+                }
+                const float scale = k8 ? 1.f : p.scale;  // (of codes the scores are what they are)
                 uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first, bad = 0;
                 if (!whole) {
                     for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1) bad |= (p.run == 64 ? ~0ull : (1ull << p.run) - 1) << (__ffs(todo) - 1) * p.run;
@@ -307,8 +475,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                 if (warp_there) {
                     float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-                    for (int j = 0; j < KT; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(s[j]));
-                    const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
+                    for (int j = 0; j < KT; j += 2)
+                        asm("max.f32 %0, %0, %1, %2;" : "+f"(top[j / 2 & 3]) : "f"(__uint_as_float(s[j])), "f"(__uint_as_float(s[j + 1])));
+                    const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
                     if (begins) {
                         m_used = tile_top;
                     } else if (__any_sync(0xffffffffu, tile_top > m_used + 4.f)) {
@@ -331,22 +500,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                 }
                 const float less = (m_used == -CUDART_INF_F ? 0.f : m_used) - kRaise;
                 if (warp_there) {
+                    const uint64_t scale2 = ptx::pack2(scale, scale), less2 = ptx::pack2(-less, -less);
+                    uint64_t sums[2] = {0, 0};  // two at a time
 #pragma unroll
                     for (int c = 0; c < KT / 16; ++c) {
                         uint32_t first[8], second[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const float a = ex2_ftz(fmaf(__uint_as_float(s[c * 16 + 2 * e]), p.scale, -less));
-                            const float b = ex2_ftz(fmaf(__uint_as_float(s[c * 16 + 2 * e + 1]), p.scale, -less));
-                            l += a + b;
+                            float a, b;
+                            ptx::unpack2(fma2(ptx::pack2(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1])), scale2, less2), a, b);
+                            a = ex2_ftz(a), b = ex2_ftz(b);
+                            if constexpr (k8) {
+                                const float4 two = *reinterpret_cast<const float4*>(parts + KT + c * 16 + 2 * e);
+                                sums[e & 1] = fma2(ptx::pack2(a, b), ptx::pack2(two.y, two.w), sums[e & 1]);
+                                a *= two.x, b *= two.z;
+                            } else {
+                                sums[e & 1] = add2(sums[e & 1], ptx::pack2(a, b));
+                            }
                             split_in_two<M>(a, b, first[e], second[e]);
                         }
                         tmem_st8(s_at + c * 8, first);
                         tmem_st8(s_at + 32 + c * 8, second);
                     }
+                    float a, b, c, d;
+                    ptx::unpack2(sums[0], a, b);
+                    ptx::unpack2(sums[1], c, d);
+                    l += (a + b) + (c + d);
                     tc_wait_st();
                 }
-                if (!whole) {
+                if (!k8 && !whole) {
                     // values that must not count: a thread has half a row of them
                     const int key = row >> 1;
                     unsigned char* half = smem + L::kV + v_stage * L::kTile + key * 128;
@@ -452,7 +634,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tree_tc_kernel(const __gr
                     if (there && out) {
                         uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = pack2<M>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                        for (int e = 0; e < 8; ++e) {
+                            const float a = __uint_as_float(x[2 * e]), b = __uint_as_float(x[2 * e + 1]);
+                            w[e] = (k8 ? p.bf16 : BF16) ? tmw::pack2<__nv_bfloat16>(a, b) : tmw::pack2<__half>(a, b);
+                        }
                         if (p.o_wide) {
                             reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
                             reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
@@ -510,25 +695,32 @@ TcPlan tc_plan(const tmw_paged_attention_desc& d, int nodes) {
     return n;
 }
 
-template <int DH, bool BF16>
+template <typename P, int DH>
 int launch_tc(const tmw_paged_attention_desc& d, PagedAttentionBulk& p, const TcPlan& n, cudaStream_t stream) {
-    using L = TcLayout<DH>;
-    const auto make = [&](CUtensorMap* map, const void* base, int rows) {
-        return rows == 0 || make_map_2d(map, base, TMW_F16, rows, DH, DH, p.run, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    using L = TcLayout<P, DH>;
+    const auto make = [&](CUtensorMap* map, const void* base, int rows) {  // (codes as pairs, rows as they lie)
+        return rows == 0 || make_map_2d(map, base, TMW_F16, rows, DH * (int)sizeof(P) / 2, DH * (int)sizeof(P) / 2, p.run, L::k8 ? DH / 2 : 64,
+                                        L::k8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
     };
     const int rows = d.at.pages * d.at.kv_heads * d.at.page_size, pers = d.at.kv_heads * d.n_persistent;
     if (!make(&p.k_map, d.at.k_pages, rows) || !make(&p.v_map, d.at.v_pages, rows) || !make(&p.k_pers_map, d.k_pers, pers) ||
         !make(&p.v_pers_map, d.v_pers, pers))
         return TMW_ERR_CUDA;
-    auto kern = paged_tree_tc_kernel<DH, BF16>;
+    auto kern = paged_tree_tc_kernel<P, DH>;
     const int smem = L::kBytes + 1024, rc = allow_shared_memory(reinterpret_cast<const void*>(kern), smem);
     if (rc != TMW_OK) return rc;
-    kern<<<n.grid, kTcThreads, smem, stream>>>(p);
+    kern<<<n.grid, L::kThreads, smem, stream>>>(p);
     TMW_CUDA_TRY(cudaGetLastError());
     if (n.grid > 1)
         TMW_CUDA_TRY(launch_ex(tree_join_kernel<DH>, dim3((unsigned)n.grid - 1, (unsigned)((n.rows + kTreeJoinWarps - 1) / kTreeJoinWarps)),
                                dim3(kTreeJoinWarps * 32), 0, stream, true, 1, static_cast<const PagedAttention&>(p)));
     return TMW_OK;
+}
+template <int DH>
+int launch_tc(const tmw_paged_attention_desc& d, int format, PagedAttentionBulk& p, const TcPlan& n, cudaStream_t stream) {
+    if (format == TMW_PAGES_INT8) return launch_tc<int8_t, DH>(d, p, n, stream);
+    if (format == TMW_PAGES_E4M3) return launch_tc<E4m3, DH>(d, p, n, stream);
+    return d.at.dtype == TMW_BF16 ? launch_tc<__nv_bfloat16, DH>(d, p, n, stream) : launch_tc<__half, DH>(d, p, n, stream);
 }
 
 }  // namespace
@@ -558,9 +750,7 @@ bool tree_launch_tc(const tmw_paged_attention_desc& d, const tmw_page_scales& s,
     p.sums = reinterpret_cast<float2*>(at + n.sums_at);
     p.partial = reinterpret_cast<float*>(at + n.partial_at);
     p.run = d.at.page_size % 64 == 0 ? 64 : d.at.page_size % 32 == 0 ? 32 : d.at.page_size % 16 == 0 ? 16 : 8;
-    const bool bf16 = d.at.dtype == TMW_BF16;
-    if (d.at.head_dim == 64) status = bf16 ? launch_tc<64, true>(d, p, n, stream) : launch_tc<64, false>(d, p, n, stream);
-    else status = bf16 ? launch_tc<128, true>(d, p, n, stream) : launch_tc<128, false>(d, p, n, stream);
+    status = d.at.head_dim == 64 ? launch_tc<64>(d, s.format, p, n, stream) : launch_tc<128>(d, s.format, p, n, stream);
     return true;
 }
 
