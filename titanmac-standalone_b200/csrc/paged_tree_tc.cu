@@ -16,8 +16,8 @@
 // see in full, at a window's begin and among the nodes, have the rows' bits applied to the scores, and their values made harmless: rows
 // that nobody sees are zeros, and what is infinite or no number is added row by row to those that see it.
 //
-// Pages of 8 bits: TMA brings codes, and four more warps (12-15) turn them into fp16 tiles of the same form, once for all rows, and every key's
-// scales into the numbers that the softmax warps use (see the attention of one token): scores times the key's scale, weights times the
+// Pages of 8 bits: TMA brings codes, and eight more warps (12-19, four for the keys, four for the values) turn them into fp16 tiles of the same form, once for all
+// rows, and every key's scales into the numbers that the softmax warps use (see the attention of one token): scores times the key's scale, weights times the
 // value's in two parts.
 //
 // All waits are bounded (paged_attention.cuh); the tensor memory is given back on every way.
@@ -39,15 +39,15 @@ struct TcLayout {
     static_assert(kVStages >= kTcAhead, "a phase is asked for before the next but one");
     static constexpr int kQSub = kTcRows * 128, kSub = kTcKeys * 128, kTile = kSub * kSubs;
     static constexpr int kK = kQSub * kSubs, kV = kK + kKStages * kTile;
-    // codes: rings of four tiles, with scales of keys and values; then what becomes of the scales, of eight tiles, {key's scale, exponent} and {rest, back}
+    // codes: rings of four tiles, with scales of keys and values; then what becomes of the scales, of eight tiles
     static constexpr int kRawTile = kTcKeys * DH, kRawK = kV + kVStages * kTile, kRawV = kRawK + (k8 ? 4 * kRawTile : 0);
     static constexpr int kScales = kRawV + (k8 ? 4 * kRawTile : 0), kParts = kScales + (k8 ? 4 * 2 * kTcKeys * 4 : 0);
     static constexpr int kBytes = kParts + (k8 ? 8 * 2 * kTcKeys * 8 : 0);
-    static constexpr int kThreads = k8 ? 512 : 384;
+    static constexpr int kThreads = k8 ? 640 : 384;
 };
-// registers of the codes' form: sixteen warps have 128 each at launch
-constexpr int kRegsService = 80, kRegsSoftmax = 176;
-static_assert(8 * 32 * (kRegsService + kRegsSoftmax) <= 512 * 128, "setmaxnreg: what the softmax warps ask for the others release");
+// registers of the codes' form: twenty warps have 96 each at launch
+constexpr int kRegsService = 56, kRegsSoftmax = 152;
+static_assert(32 * (12 * kRegsService + 8 * kRegsSoftmax) <= 640 * 96, "setmaxnreg: what the softmax warps ask for the others release");
 // of a tile: its first key's token (-1: persistent ones), its keys that exist, its runs that have no page
 struct TileInfo {
     int place, first, last, lost;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
     constexpr float kRaise = BF16 ? 0.f : k8 ? 10.f : 11.f;  // (a weight is at most 2^4, of codes 2^5, times that)
     constexpr uint32_t kO = 4 * KT, kColumns = 512;  // two buffers of scores for each stream, then their outputs
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ alignas(8) uint64_t bars[1 + 3 * kTcAhead + 2 * VS + (k8 ? 16 : 0)];
+    __shared__ alignas(8) uint64_t bars[1 + 3 * kTcAhead + 2 * VS + (k8 ? 24 : 0)];
     __shared__ TileInfo infos[16];  // of the last tiles
     __shared__ float2 stream_sums[2][kTcRows];
     __shared__ uint32_t tmem_slot;
@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
     // t & 3); a barrier's phase is the turn's.  Keys are let go with their scores, scores and weights with the products with the values (v_free).
     const uint32_t q_ready = bar0, k_full = bar0 + 8, s_full = k_full + 32, p_ready = s_full + 32, v_full = p_ready + 32, v_free = v_full + 8 * VS;
     const uint32_t raw_k_full = v_free + 8 * VS, raw_k_free = raw_k_full + 32, raw_v_full = raw_k_free + 32, raw_v_free = raw_v_full + 32;  // codes
+    const uint32_t parts_full = raw_v_free + 32;  // of tile t, t & 7
     const auto turn = [](int t) { return (uint32_t)(t >> 2) & 1; };
     const auto v_turn = [](int t) { return (uint32_t)(t / VS) & 1; };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -131,7 +132,8 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
         for (int i = 0; i < VS; ++i) mbar_init(v_full + 8 * i, k8 ? 4 : 1), mbar_init(v_free + 8 * i, 1);
         if (k8)
             for (int i = 0; i < 4; ++i)
-                mbar_init(raw_k_full + 8 * i, 1), mbar_init(raw_k_free + 8 * i, 4), mbar_init(raw_v_full + 8 * i, 1), mbar_init(raw_v_free + 8 * i, 4);
+                mbar_init(raw_k_full + 8 * i, 1), mbar_init(raw_k_free + 8 * i, 4), mbar_init(raw_v_full + 8 * i, 1), mbar_init(raw_v_free + 8 * i, 4),
+                    mbar_init(parts_full + 16 * i, 4), mbar_init(parts_full + 16 * i + 8, 4);
         wild[0] = wild[1] = first_adds[0] = first_adds[1] = 0;
         given_up = 0;
         p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -287,9 +289,9 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
         }
     } else if (k8 && warp >= 12) {
         if constexpr (k8) {
-            // ---- codes into fp16 tiles: the keys of a tile, with the scales of both, then the values of the tile two in front of it ----
+            // ---- codes into fp16 tiles: four warps the keys, with the scales of both, four warps the values ----
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsService) : "memory");
-            const int mine = tid - 384;
+            const int mine = tid & 127;
             auto convert = [&](const unsigned char* from, uint32_t to, uint64_t exists) {
                 constexpr int kPieces = KT * DH / 16 / 128, kOfRow = DH / 16;
                 uint4 codes[kPieces];
@@ -305,43 +307,43 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
                     for (int h = 0; h < 2; ++h)
                         *reinterpret_cast<uint4*>(smem + to + c / 8 * L::kSub + row * 128 + (((c + h) % 8 ^ (row & 7)) << 4)) = x[h];
                 }
+                fence_proxy_async_smem();
+                __syncwarp();
             };
-            int t = 0;  // the part's first tile
+            int t = 0;
             while (walk.next(p, limit)) {
-                for (int i = 0; i < walk.tiles + 2; ++i) {
-                    if (i < walk.tiles) {
-                        const int k = t + i;
-                        mbar_wait(raw_k_full + 8 * (k & 3), turn(k), &given_up, p.status);
-                        if (k >= KS) mbar_wait(s_full + 8 * ((k - KS) & 3), turn(k - KS), &given_up, p.status);
-                        convert(smem + L::kRawK + (k & 3) * L::kRawTile, L::kK + k % KS * L::kTile, ~0ull);
+                for (int i = 0; i < walk.tiles; ++i, ++t) {
+                    if (warp < 16) {
+                        mbar_wait(raw_k_full + 8 * (t & 3), turn(t), &given_up, p.status);
+                        if (t >= KS) mbar_wait(s_full + 8 * ((t - KS) & 3), turn(t - KS), &given_up, p.status);
+                        convert(smem + L::kRawK + (t & 3) * L::kRawTile, L::kK + t % KS * L::kTile, ~0ull);
+                        if (lane == 0) mbar_arrive(k_full + 8 * (t & 3));
+                        const float* scales = reinterpret_cast<const float*>(smem + L::kScales) + (t & 3) * 2 * KT;
+                        const float vs = scales[KT + (mine & 63)];
+                        const int bits = __float_as_int(fmaxf(vs, 0x1p-100f));
+                        // of two keys: their own scales and the exponents of their values', then what the exponents leave and their inverses
+                        float* parts = reinterpret_cast<float*>(smem + L::kParts) + (t & 7) * 4 * KT + (mine & 63) / 2 * 4 + (mine & 1);
                         if (mine < KT) {
-                            const float* scales = reinterpret_cast<const float*>(smem + L::kScales) + (k & 3) * 2 * KT;
-                            const float vs = scales[KT + mine];
-                            const int bits = __float_as_int(fmaxf(vs, 0x1p-100f));
-                            float2* parts = reinterpret_cast<float2*>(smem + L::kParts) + (k & 7) * 2 * KT;
-                            parts[mine] = make_float2(scales[mine], __int_as_float(0x4b000000 | (bits >> 23)) - (8388608.f + 127.f) + (vs - vs));
-                            parts[KT + mine] = make_float2(__int_as_float((bits & 0x007fffff) | 0x3f800000),
-                                                           __int_as_float(0x7f000000 - min(bits & 0x7f800000, 0x7e800000)));
+                            parts[0] = scales[mine];
+                            parts[2] = __int_as_float(0x4b000000 | (bits >> 23)) - (8388608.f + 127.f) + (vs - vs);
+                        } else {
+                            parts[2 * KT] = __int_as_float((bits & 0x007fffff) | 0x3f800000);
+                            parts[2 * KT + 2] = __int_as_float(0x7f000000 - min(bits & 0x7f800000, 0x7e800000));
                         }
-                        fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(k_full + 8 * (k & 3)), mbar_arrive(raw_k_free + 8 * (k & 3));
-                    }
-                    if (i >= 2) {
-                        const int v = t + i - 2, slot = v % VS;
-                        mbar_wait(raw_v_full + 8 * (v & 3), turn(v), &given_up, p.status);
-                        if (v >= VS) mbar_wait(v_free + 8 * slot, v_turn(v - VS), &given_up, p.status);
-                        const TileInfo& info = infos[v & 15];
+                        if (lane == 0) mbar_arrive(parts_full + 8 * (t & 7)), mbar_arrive(raw_k_free + 8 * (t & 3));
+                    } else {
+                        const int slot = t % VS;
+                        mbar_wait(raw_v_full + 8 * (t & 3), turn(t), &given_up, p.status);
+                        if (t >= VS) mbar_wait(v_free + 8 * slot, v_turn(t - VS), &given_up, p.status);
+                        const TileInfo& info = infos[t & 15];
                         uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first;
                         for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1)
                             exists &= ~((p.run == 64 ? ~0ull : (1ull << p.run) - 1) << (__ffs(todo) - 1) * p.run);
-                        convert(smem + L::kRawV + (v & 3) * L::kRawTile, L::kV + slot * L::kTile, exists);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(v_full + 8 * slot), mbar_arrive(raw_v_free + 8 * (v & 3));
+                        convert(smem + L::kRawV + (t & 3) * L::kRawTile, L::kV + slot * L::kTile, exists);
+                        if (lane == 0) mbar_arrive(v_full + 8 * slot), mbar_arrive(raw_v_free + 8 * (t & 3));
                     }
                 }
-                t += walk.tiles;
             }
         }
     } else {
@@ -424,6 +426,7 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
                 const uint32_t s_at = tmem + lane_at + buf * KT;
                 mbar_wait(v_full + 8 * v_stage, v_turn(t), &given_up, p.status);
                 mbar_wait(s_full + 8 * buf, turn(t), &given_up, p.status);
+                if constexpr (k8) mbar_wait(parts_full + 8 * (t & 7), (uint32_t)(t >> 3) & 1, &given_up, p.status);
                 tc_fence_after();
                 const TileInfo& info = infos[t & 15];
                 const bool whole = info.first == 0 && info.last == KT - 1 && info.lost == 0 &&
@@ -437,12 +440,16 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
                     }
                     tc_wait_ld();
                 }
-                const float2* parts = reinterpret_cast<const float2*>(smem + L::kParts) + (t & 7) * 2 * KT;
+                const float4* parts = reinterpret_cast<const float4*>(smem + L::kParts) + (t & 7) * KT;
                 if constexpr (k8) {
+                    const uint64_t q_scale2 = ptx::pack2(q_scale, q_scale);
 #pragma unroll
-                    for (int j = 0; j < KT; ++j) {
-                        const float2 part = parts[j];
-                        s[j] = __float_as_uint(fmaf(__uint_as_float(s[j]) * part.x, q_scale, part.y));
+                    for (int j = 0; j < KT; j += 2) {
+                        const float4 part = parts[j / 2];
+                        const uint64_t x = mul2(ptx::pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), ptx::pack2(part.x, part.y));
+                        float a, b;
+                        ptx::unpack2(fma2(x, q_scale2, ptx::pack2(part.z, part.w)), a, b);
+                        s[j] = __float_as_uint(a), s[j + 1] = __float_as_uint(b);
                     }
                 }
                 const float scale = k8 ? 1.f : p.scale;  // (of codes the scores are what they are)
@@ -508,12 +515,14 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             float a, b;
-                            ptx::unpack2(fma2(ptx::pack2(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1])), scale2, less2), a, b);
+                            const uint64_t two_scores = ptx::pack2(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1]));
+                            ptx::unpack2(k8 ? add2(two_scores, less2) : fma2(two_scores, scale2, less2), a, b);
                             a = ex2_ftz(a), b = ex2_ftz(b);
                             if constexpr (k8) {
-                                const float4 two = *reinterpret_cast<const float4*>(parts + KT + c * 16 + 2 * e);
-                                sums[e & 1] = fma2(ptx::pack2(a, b), ptx::pack2(two.y, two.w), sums[e & 1]);
-                                a *= two.x, b *= two.z;
+                                const float4 two = parts[KT / 2 + c * 8 + e];
+                                const uint64_t w = ptx::pack2(a, b);
+                                sums[e & 1] = fma2(w, ptx::pack2(two.z, two.w), sums[e & 1]);
+                                ptx::unpack2(mul2(w, ptx::pack2(two.x, two.y)), a, b);
                             } else {
                                 sums[e & 1] = add2(sums[e & 1], ptx::pack2(a, b));
                             }
