@@ -32,7 +32,7 @@ import torch.nn.functional as F
 
 from .. import _native, _stack, _train
 from ..blocks.titan_block import RMSNorm, TitanBlock
-from ..paged_cache import PagedCache
+from ..paged_cache import PagedCache, draft_tree
 from ..logprobs import TokenLogprobs, token_logprobs
 
 
@@ -167,11 +167,13 @@ class TitanMAC(nn.Module):
         storage = torch.zeros((len(self.layers), _native.RingCache.elements(*geometry)), dtype=dtype, device=device)
         return [_native.RingCache(*geometry, dtype, device, storage=storage[i]) for i in range(len(self.layers))]
 
-    def new_paged_caches(self, page_table: torch.Tensor, pages: int, page_size: int, dtype) -> List[PagedCache]:
+    def new_paged_caches(self, page_table: torch.Tensor, pages: int, page_size: int, dtype,
+                         page_dtype: Optional[torch.dtype] = None) -> List[PagedCache]:
         """Caches for ``prefill`` and ``decode_step`` whose sequences live in pages: ``page_table [B, columns]`` (int32, on the
         device, shared by the layers), a pool of ``pages`` pages of ``page_size`` tokens per layer.  ``prefill`` fills every
         sequence's pages with the whole prompt it is given, all prompts of one length; ``decode_step`` takes positions of -1 for
-        rows without a sequence (their logits mean nothing).
+        rows without a sequence (their logits mean nothing).  ``page_dtype`` int8 or float8_e4m3fn: keys and values, the persistent
+        ones too, in 8 bits with a scale for every token and head.
 
         An id outside the vocabulary, a position of ``decode_step`` outside the model's or the pages' table: that row's logits are
         NaN, what it adds to its pages is too (steps that see it are NaN again), the other rows are as they would be, and
@@ -179,7 +181,7 @@ class TitanMAC(nn.Module):
         it has no place in the pages is left out and reported."""
         self._need_windowed()
         c = self.config
-        return [PagedCache(page_table, pages, page_size, c.n_heads, c.d_head, c.window_size, c.n_persistent, dtype)
+        return [PagedCache(page_table, pages, page_size, c.n_heads, c.d_head, c.window_size, c.n_persistent, dtype, page_dtype=page_dtype)
                 for _ in self.layers]
 
     @torch.no_grad()
@@ -270,6 +272,52 @@ class TitanMAC(nn.Module):
             pending = layer.mlp(h)
         h = self.norm(x) if pending is None else self.norm.add_forward(x, pending, inplace=True)[1]
         return self.lm_head(h)
+
+    @torch.no_grad()
+    def decode_tree(self, token_ids: torch.Tensor, parents: torch.Tensor, start: torch.Tensor, caches: List[PagedCache],
+                    counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One step of drafted tokens, a tree of them per sequence: ``token_ids``, ``parents [B, nodes]`` (at most 64; a node's parent is an
+        earlier node, -1 where it follows the cached tokens), ``start [B] int32`` = how many tokens are cached (-1: no sequence in this row),
+        ``counts [B] int32`` nodes of each (None: all).  Returns logits ``[B, nodes, V]``: at node ``i`` what ``decode_step`` would return
+        for its token behind the cached ones and its ancestors.  The nodes' keys and values are tokens ``start ..`` of the pages, where
+        ``keep_drafts`` leaves those of an accepted path; the next step, or tree, writes over the others.  Ids and positions outside
+        their tables: as for ``new_paged_caches``, node by node; rows from ``counts`` on mean nothing."""
+        self._need_windowed()
+        if not all(isinstance(cache, PagedCache) for cache in caches):
+            raise TypeError("decode_tree works with paged caches (new_paged_caches)")
+        B, N = token_ids.shape
+        tree = draft_tree(parents, start, self.config.window_size)
+        ids, unknown = _in_table(self.embed_tokens, token_ids)
+        at, outside = _in_table(self.embed_positions, tree.positions.long())
+        there = (start >= 0)[:, None].expand(B, N)
+        if counts is not None:
+            there = there & (torch.arange(N, device=start.device) < counts[:, None])
+        bad = (unknown | outside) & there
+        x = (self.embed_tokens(ids) + self.embed_positions(at)).masked_fill(bad[..., None], float("nan"))
+        pending, reported = None, False
+        for layer, cache in zip(self.layers, caches):
+            attn = layer.attention
+            if pending is None:
+                h = layer.norm_attn(x)
+            else:
+                x, h = layer.norm_attn.add_forward(x, pending, inplace=True)
+            q, k, v = attn.split_qkv(_native.project(attn.qkv_proj, h))
+            o = cache.decode_tree(q, k, v, start, tree, counts)
+            if not reported and N > 0:  # (a start of -2 stores nothing: it reports)
+                cache.append(k[:, :, :1], v[:, :, :1], -1 - bad.any(dim=1).to(torch.int32))
+                reported = True
+            o = o.permute(0, 2, 1, 3).reshape(B, N, -1)
+            x, h = layer.norm_mlp.add_forward(x, _native.project(attn.out_proj, o), inplace=True)
+            pending = layer.mlp(h)
+        h = self.norm(x) if pending is None else self.norm.add_forward(x, pending, inplace=True)[1]
+        return _native.project(self.lm_head, h)
+
+    @torch.no_grad()
+    def keep_drafts(self, caches: List[PagedCache], start: torch.Tensor, kept: torch.Tensor, counts: torch.Tensor) -> None:
+        """The accepted path of ``decode_tree``'s nodes: nodes ``kept[b, : counts[b]]`` (int32, rising) become tokens ``start[b] ..`` of every
+        layer's pages; the sequence then has ``start + counts`` tokens."""
+        for cache in caches:
+            cache.keep(start, kept, counts)
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, use_cuda_graph: bool = True) -> torch.Tensor:
