@@ -19,30 +19,13 @@ struct PagedRead {
     int* status;
 };
 
-template <typename T, typename P>
-__device__ __forceinline__ void read8(const P* from, float scale, T (&x)[8]) {
-    if constexpr (sizeof(P) == 1) {
-        const uint2 w = *reinterpret_cast<const uint2*>(from);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t two = (i < 2 ? w.x : w.y) >> i % 2 * 16;
-            float2 c;
-            if constexpr (std::is_same<P, E4m3>::value) c = __half22float2(from_e4m3(two));
-            else c = make_float2((float)(int8_t)two, (float)(int8_t)(two >> 8));
-            x[2 * i] = from_f32<T>(c.x * scale);
-            x[2 * i + 1] = from_f32<T>(c.y * scale);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(x) / 16; ++i) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(from)[i];
-    }
-}
-
-// A CTA has kReadTokens tokens of a sequence, all heads of theirs; a thread eight numbers at a time.
-constexpr int kReadTokens = 8;
+// A CTA has kReadTokens tokens of a sequence, all heads of theirs; a thread sixteen bytes of a row of a page at a time, at the same
+// place of every row it has, two rows under way.
+constexpr int kReadTokens = 16, kReadAhead = 2;
 template <typename T, typename P, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) paged_read_kernel(const __grid_constant__ PagedRead p) {
+__global__ void __launch_bounds__(kThreads, 6) paged_read_kernel(const __grid_constant__ PagedRead p) {
     __shared__ long long place[kReadTokens];
+    constexpr int kOne = 16 / sizeof(P);
     const int b = blockIdx.y, r0 = blockIdx.x * kReadTokens, tid = threadIdx.x;
     const int start = p.start[b];
     int count = p.counts != nullptr ? p.counts[b] : p.rows;
@@ -57,30 +40,64 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const __grid_const
         if (at < 0) atomicCAS(p.status, 0, (int)TMW_ERR_INVALID_ARGUMENT);
         place[tid] = at;
     }
+    const int units = p.map.head_dim / kOne, slots = 2 * p.map.kv_heads, step = kThreads / units;
+    const int step_r = step / slots, step_slot = step - step_r * slots;
+    const int row = tid / units, d = (tid - row * units) * kOne;
+    int r = row < step ? row / slots : tokens, slot = row % slots;  // (threads behind the last whole row have none)
     __syncthreads();
-    const int units = p.map.head_dim / 8, slots = 2 * p.map.kv_heads;
-    for (int i = tid; i < tokens * slots * units; i += kThreads) {
-        const int row = i / units, d = (i - row * units) * 8, r = row / slots, slot = row - r * slots;
-        const bool value = slot >= p.map.kv_heads;
-        const int head = value ? slot - p.map.kv_heads : slot;
-        alignas(16) T x[8];
-        if (place[r] >= 0) {
-            const long long at = place[r] + (long long)head * p.map.page.d;
-            float scale = 1.f;
-            if constexpr (sizeof(P) == 1) scale = __ldg((value ? p.v_scales : p.k_scales) + at);
-            read8<T, P>(static_cast<const P*>(value ? p.v_pages : p.k_pages) + at * p.map.head_dim + d, scale, x);
-        } else {
+    while (r < tokens) {
+        uint4 w[kReadAhead];
+        float scale[kReadAhead];
+        T* to[kReadAhead];  // NULL: no row
+        bool there[kReadAhead];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = from_f32<T>(__int_as_float(0x7fffffff));
+        for (int i = 0; i < kReadAhead; ++i) {
+            to[i] = nullptr;
+            there[i] = false;
+            if (r < tokens) {
+                const bool value = slot >= p.map.kv_heads;
+                const int head = value ? slot - p.map.kv_heads : slot;
+                to[i] = value ? static_cast<T*>(p.v) + b * p.vs[0] + head * p.vs[1] + (r0 + r) * p.vs[2] + d
+                              : static_cast<T*>(p.k) + b * p.ks[0] + head * p.ks[1] + (r0 + r) * p.ks[2] + d;
+                there[i] = place[r] >= 0;
+                if (there[i]) {
+                    const long long at = place[r] + (long long)head * p.map.page.d;
+                    w[i] = *reinterpret_cast<const uint4*>(static_cast<const P*>(value ? p.v_pages : p.k_pages) + at * p.map.head_dim + d);
+                    if constexpr (sizeof(P) == 1) scale[i] = (value ? p.v_scales : p.k_scales)[at];
+                }
+                r += step_r;
+                slot += step_slot;
+                if (slot >= slots) slot -= slots, ++r;
+            }
         }
-        const long long(&s)[3] = value ? p.vs : p.ks;
-        T* to = static_cast<T*>(value ? p.v : p.k) + b * s[0] + head * s[1] + (r0 + r) * s[2] + d;
-        if constexpr (WHOLE) {
 #pragma unroll
-            for (int e = 0; e < (int)sizeof(x) / 16; ++e) reinterpret_cast<uint4*>(to)[e] = reinterpret_cast<const uint4*>(x)[e];
-        } else {
+        for (int i = 0; i < kReadAhead; ++i) {
+            if (to[i] == nullptr) continue;
+            alignas(16) T x[kOne];
+            if (!there[i]) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) to[e] = x[e];
+                for (int e = 0; e < kOne; ++e) x[e] = from_f32<T>(__int_as_float(0x7fffffff));
+            } else if constexpr (sizeof(P) == 1) {
+                const uint32_t codes[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t two = codes[e / 2] >> e % 2 * 16;
+                    float2 c;
+                    if constexpr (std::is_same<P, E4m3>::value) c = __half22float2(from_e4m3(two));
+                    else c = make_float2((float)(int8_t)two, (float)(int8_t)(two >> 8));
+                    x[2 * e] = from_f32<T>(c.x * scale[i]);
+                    x[2 * e + 1] = from_f32<T>(c.y * scale[i]);
+                }
+            } else {
+                *reinterpret_cast<uint4*>(x) = w[i];
+            }
+            if constexpr (WHOLE) {
+#pragma unroll
+                for (int e = 0; e < (int)sizeof(x) / 16; ++e) reinterpret_cast<uint4*>(to[i])[e] = reinterpret_cast<const uint4*>(x)[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < kOne; ++e) to[i][e] = x[e];
+            }
         }
     }
 }
