@@ -285,8 +285,12 @@ class TitanMAC(nn.Module):
         self._need_windowed()
         if not all(isinstance(cache, PagedCache) for cache in caches):
             raise TypeError("decode_tree works with paged caches (new_paged_caches)")
+        if parents.shape != token_ids.shape:
+            raise ValueError(f"token_ids and parents must be [batch, nodes] alike, got {list(token_ids.shape)} and {list(parents.shape)}")
         B, N = token_ids.shape
         tree = draft_tree(parents, start, self.config.window_size)
+        if token_ids.numel() == 0:
+            return self.lm_head.weight.new_empty(B, N, self.config.vocab_size)
         ids, unknown = _in_table(self.embed_tokens, token_ids)
         at, outside = _in_table(self.embed_positions, tree.positions.long())
         there = (start >= 0)[:, None].expand(B, N)
@@ -303,7 +307,7 @@ class TitanMAC(nn.Module):
                 x, h = layer.norm_attn.add_forward(x, pending, inplace=True)
             q, k, v = attn.split_qkv(_native.project(attn.qkv_proj, h))
             o = cache.decode_tree(q, k, v, start, tree, counts)
-            if not reported and N > 0:  # (a start of -2 stores nothing: it reports)
+            if not reported:  # (a start of -2 stores nothing: it reports)
                 cache.append(k[:, :, :1], v[:, :, :1], -1 - bad.any(dim=1).to(torch.int32))
                 reported = True
             o = o.permute(0, 2, 1, 3).reshape(B, N, -1)

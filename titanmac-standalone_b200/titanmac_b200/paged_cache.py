@@ -219,6 +219,7 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
         _refuse_devices("paged_read", k_pages, v_pages, page_table, start)
     if not (k_pages.dtype is v_pages.dtype and torch.int32 is page_table.dtype is start.dtype):
         raise TypeError("paged_read: the pages must share one dtype; page_table and start must be int32")
+    _native.refuse_tangents("paged_read", k_pages, v_pages, k_out, v_out)
     if start.dim() != 1:
         raise ValueError("start must be a contiguous vector of one number per sequence")
     B = start.shape[0]
@@ -498,6 +499,7 @@ def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
         _refuse_devices("paged_keep", k_pages, v_pages, page_table, start, kept, counts)
     if not (k_pages.dtype is v_pages.dtype and torch.int32 is page_table.dtype is start.dtype is kept.dtype is counts.dtype):
         raise TypeError("paged_keep: the pages must share one dtype; page_table, start, kept and counts must be int32")
+    _native.refuse_tangents("paged_keep", k_pages, v_pages)
     if kept.dim() != 2 or not kept.is_contiguous():
         raise ValueError("kept must be contiguous [batch, most]")
     B, most = kept.shape
