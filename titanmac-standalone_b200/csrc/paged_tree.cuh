@@ -814,11 +814,17 @@ TMW_TREE_OF(e4m3)
 TMW_TREE_OF(tc)
 #undef TMW_TREE_OF
 
-// Which calls tcgen05 takes: 16-bit pages that come by TMA, head_dim 64 or 128, and more rows to a key head than mma.sync's two or three warps
-// have, TREE_ROWS.
+// Which calls tcgen05 takes: pages that come by TMA, head_dim 64 or 128, and so many rows to a key head that mma.sync's work outweighs the longer
+// hand-overs here.  us, tcgen05 | mma.sync:
+//   16-bit pages, heads of 128: 16 sequences of up to 16384, 32 heads on 8: 8 rows 115 | 134, 16 rows 116 | 161, 32 rows 118 | 175;
+//     64 windows of 512 of 10 heads: 8 rows 87 | 70, 16 rows 90 | 85, 33 rows 94 | 100
+//   16-bit pages, heads of 64: the same sequences: 32 rows 108 | 99, 48 rows 108 | 121; 32 sequences of 10 heads, 20 rows 346 | 298,
+//     33 rows 349 | 365; the windows: 33 rows 76 | 64, 64 rows 82 | 88
+//   codes, 6 of up to 65536, 32 heads on 4: of 128: 32 rows 202 | 164, 40 rows 207 | 215; of 64: 48 rows 166 | 148, 56 rows 168 | 216
 inline bool tree_takes_tc(const tmw_paged_attention_desc& d, const tmw_page_scales& s, int nodes) {
-    return d.at.dtype != TMW_F32 && (d.at.head_dim == 64 || d.at.head_dim == 128) && can_bulk(d, s) &&
-           d.heads / d.at.kv_heads * nodes > 32;
+    const bool codes = s.format != TMW_PAGES_SAME, wide = d.at.head_dim == 128;
+    const int few = codes ? (wide ? 32 : 48) : (wide ? 8 : 32);
+    return d.at.dtype != TMW_F32 && (d.at.head_dim == 64 || wide) && can_bulk(d, s) && d.heads / d.at.kv_heads * nodes > few;
 }
 
 }  // namespace tmw

@@ -4,7 +4,7 @@
 // 128, a fifth of what mma.sync takes for them (9 cycles of a scheduler for each 16 x 8 x 16).  A CTA, one to an SM, is one worker of the
 // line of tiles (paged_attention.cuh), here of 64 keys, and its warps have fixed roles:
 //   warp  0, 3  bring K, bring V by TMA, a run of up to 64 neighbouring tokens at a time; every lane looks the page of one run up, for
-//               4 to 32 tiles in one go (one warp for both, tile by tile, needed 2050 cycles for each: 183 us instead of PRODUCED)
+//               4 to 32 tiles in one go (one warp for both, tile by tile, needed 2050 cycles for each: 183 us instead of 149)
 //   warp  1, 2  issue the products for the scores, and those with the values (one elected thread each: a product costs its thread some
 //               thirty cycles, and a commit hundreds)
 //   warps 4-11  softmax, a thread to a row; queries into shared memory, outputs out of tensor memory
