@@ -4,6 +4,9 @@
 // scale = max |x| / largest, code = the nearest one to x / scale.  A row's numbers are spread over up to sixteen lanes, sixteen each - eight
 // pairs that turn together -, and its largest is found by shuffles, so a row is read once and written once.  The sines are
 // computed once for a CTA's tokens, as in the append to wider pages.
+//
+// A byte read or written here costs more instructions than in the append to wider pages: 77 million for 21600 tokens of 16 heads of 128
+// each of queries, keys and values, bf16 into e4m3, which take 93 us (80 % of what can be issued; their 415 MB alone 63 us).
 #include "paged_append.cuh"
 
 namespace tmw {

@@ -1,6 +1,7 @@
 // Tokens out of their pages and from place to place in them: tmw_paged_read, tmw_paged_keep.
 //
-// Both move bytes: bound by HBM, or for a few tokens by launch and latency.
+// Both move bytes: bound by HBM, or for a few tokens by launch and latency (reading 21600 tokens of 16 heads of 128 from e4m3 in bf16,
+// 250 MB, takes 48 us cold, 5.2 TB/s; one row after the other in a thread, eight numbers of it, 62).
 #include "paged.cuh"
 
 namespace tmw {
@@ -129,7 +130,7 @@ struct PagedKeep {
 
 // A CTA has keys and values of some heads of a sequence, as many as its threads can have under way at once, or of one: every CTA looks the tokens'
 // places up first, four loads one after the other, so that fewer CTAs are faster (256 sequences, 6 of 32 tokens, 10 heads of 64: keys and
-// values of every head apart 18.3 us, 5.8 us).  Tokens come from further back than they go to, in the order of both,
+// values of every head apart 18.3 us, so 5.8).  Tokens come from further back than they go to, in the order of both,
 // so a batch of them is read, and when every thread has its part, written: no later token of its head has been written over by then.
 constexpr int kKeepAhead = 4;
 __global__ void __launch_bounds__(kThreads) paged_keep_kernel(const __grid_constant__ PagedKeep p) {

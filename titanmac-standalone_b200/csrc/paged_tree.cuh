@@ -7,8 +7,8 @@
 // attention of one token.  No barrier but the ring's own.
 //
 // S = Q K^T and O += P V by mma.sync with the rows as the sixteen of a tile: the scores' registers are the operand of the second
-// product as they are.  (tcgen05's 128 rows would be half empty for most trees; here M is what bounds it: 2.25 cycles of the SM for each
-// 16 x 8 x 16.)  A weight is two 16-bit numbers, as far as a tile's mask goes; only tiles that some row does not see in full, at the
+// product as they are.  (Here M is what bounds it: 2.25 cycles of the SM for each 16 x 8 x 16; which rows tcgen05's 128 take instead is
+// said below, at tree_takes_tc.)  64 windows of 512, 16 nodes, 10 heads of 64, bf16, 86 MB: 39 us, latency: two or three tiles to a worker.  A weight is two 16-bit numbers, as far as a tile's mask goes; only tiles that some row does not see in full, at the
 // window's begin and among the nodes, run the body with the mask.
 #pragma once
 

@@ -20,6 +20,9 @@
 // rows, and every key's scales into the numbers that the softmax warps use (see the attention of one token): scores times the key's scale, weights times the
 // value's in two parts.
 //
+// 16 sequences of up to 16384, 33 nodes, 32 heads on 8 of 128, fp16, 576 MB: 154 us from HBM alone, 2200 cycles for the 64 keys of a tile in either
+// stream; 6 of up to 65536, 12 nodes, 32 heads on 4 of 128, int8, 307 MB: 220 us, 5500 cycles, the softmax warps'.
+//
 // All waits are bounded (paged_attention.cuh); the tensor memory is given back on every way.
 #include "paged_tree.cuh"
 
