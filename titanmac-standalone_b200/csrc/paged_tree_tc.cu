@@ -10,15 +10,15 @@
 //   warps 4-11  softmax, a thread to a row; queries into shared memory, outputs out of tensor memory
 // A tile's chain - products, hand-over, exponentials, hand-over, products - is several times as long as its parts, so two streams of
 // softmax warps take the tiles by turns, each with a running maximum, a sum and an output of its own, and two buffers of scores: S = Q K^T
-// of four tiles is under way while P goes over its S as two 16-bit numbers a weight (64 columns for 64 fp32 ones) and O += P V.  The streams are joined
-// when the part ends.  (As two CTAs to an SM, with two tiles of each of K and V: 16 ragged sequences of 32 heads on 8, 32 nodes, 160 us.)
+// of four tiles is under way while P goes over its S as two 16-bit numbers a weight (64 columns for 64 fp32 ones) and O += P V.
+// The streams are joined when the part ends.  (As two CTAs to an SM, with two tiles of each of K and V: 16 ragged sequences of 32 heads on 8, 32 nodes, 160 us.)
 // The running maximum follows only a score that is 2^4 above it: O is brought up in tensor memory then.  Tiles that some row does not
 // see in full, at a window's begin and among the nodes, have the rows' bits applied to the scores, and their values made harmless: rows
 // that nobody sees are zeros, and what is infinite or no number is added row by row to those that see it.
 //
-// Pages of 8 bits: TMA brings codes, and eight more warps (12-19, four for the keys, four for the values) turn them into fp16 tiles of the same form, once for all
-// rows, and every key's scales into the numbers that the softmax warps use (see the attention of one token): scores times the key's scale, weights times the
-// value's in two parts.
+// Pages of 8 bits: TMA brings codes, and eight more warps (12-19, four for the keys, four for the values) turn them into fp16 tiles of
+// the same form, once for all rows, and every key's scales into the numbers that the softmax warps use (see the attention of one token):
+// scores times the key's scale, weights times the value's in two parts.
 //
 // 16 sequences of up to 16384, 33 nodes, 32 heads on 8 of 128, fp16, 576 MB: 154 us from HBM alone, 2200 cycles for the 64 keys of a tile in either
 // stream; 6 of up to 65536, 12 nodes, 32 heads on 4 of 128, int8, 307 MB: 220 us, 5500 cycles, the softmax warps'.
@@ -31,13 +31,15 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTcKeys = 64, kTcRows = 128, kTcCost = 9;  // (what an item costs besides its tiles: 2 | 4 | 6 | 9 made the ragged sequences 149 | 135 | 127 | 124 us)
+// kTcCost: what an item costs besides its tiles (2 | 4 | 6 | 9: the ragged sequences 149 | 135 | 127 | 124 us)
+constexpr int kTcKeys = 64, kTcRows = 128, kTcCost = 9;
 constexpr int kTcAhead = 4;  // tiles whose scores are under way: buffers of scores, and tiles in the ring of keys
 
 template <typename P, int DH>
 struct TcLayout {
     static constexpr bool k8 = kScaled<P>;
-    static constexpr int kSubs = DH / 64, kKStages = k8 ? 2 : kTcAhead, kVStages = k8 ? 4 : DH == 64 ? 12 : 7;  // sub-tiles of 64 columns; tiles in the rings
+    // sub-tiles of 64 columns; tiles in the rings
+    static constexpr int kSubs = DH / 64, kKStages = k8 ? 2 : kTcAhead, kVStages = k8 ? 4 : DH == 64 ? 12 : 7;
     // (who waits for the values of four tiles ago must not find the barrier a turn further)
     static_assert(kVStages >= kTcAhead, "a phase is asked for before the next but one");
     static constexpr int kQSub = kTcRows * 128, kSub = kTcKeys * 128, kTile = kSub * kSubs;

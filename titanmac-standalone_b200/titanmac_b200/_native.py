@@ -370,6 +370,14 @@ def launch(index: int, fn, *args) -> None:
         check(status)
 
 
+def ask(index: int, fn, *args):
+    """``fn(*args)`` with device ``index`` current: what needs no stream and has no status."""
+    if _raw_stream is not None and index == _raw_device():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def refuse_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
     """Raises where a tensor carries a forward-mode derivative: the call would drop it without a word.  (Outside every dual level,
     as almost always, one comparison.)"""

@@ -308,7 +308,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         window = -1  # (no sequence is longer)
     n_persistent = 0
     if k_pers is not None or v_pers is not None:
-        n_persistent = _check_persistent("paged_attention", k_pages, k_pers, v_pers)
+        n_persistent = _check_persistent("paged_attention", k_pages, index, kv_heads, head_dim, k_pers, v_pers)
     scaled = None
     if eight or scales is not None or pers_scales is not None:
         scaled = _scale_numbers("paged_attention", k_pages, v_pages, scales, pers_scales, (kv_heads, n_persistent) if n_persistent else None)
@@ -332,8 +332,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                            q.data_ptr(), k_pers.data_ptr() if n_persistent else 0, v_pers.data_ptr() if n_persistent else 0,
                            out.data_ptr(), qs[0], qs[1], os_[0], os_[1], pos.data_ptr())
     lib, device = _native.lib(), k_pages.device
-    with _native._on(device):  # (how much depends on the device's SMs)
-        nbytes = lib.tmw_paged_attention_scratch_bytes(desc) if scaled is None else lib.tmw_paged_attention_scaled_scratch_bytes(desc, scaled)
+    # (how much depends on the device's SMs)
+    nbytes = (_native.ask(index, lib.tmw_paged_attention_scratch_bytes, desc) if scaled is None
+              else _native.ask(index, lib.tmw_paged_attention_scaled_scratch_bytes, desc, scaled))
     # of this call alone: calls on two streams, or of two captured graphs, have nothing in common
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
     if scaled is None:
@@ -343,16 +344,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
-def _check_persistent(name: str, k_pages: torch.Tensor, k_pers: Optional[torch.Tensor], v_pers: Optional[torch.Tensor]) -> int:
+def _check_persistent(name: str, k_pages: torch.Tensor, index: int, kv_heads: int, head_dim: int, k_pers: Optional[torch.Tensor],
+                      v_pers: Optional[torch.Tensor]) -> int:
     """How many persistent keys there are."""
     if k_pers is None or v_pers is None:
         raise ValueError("k_pers and v_pers go together")
-    if not k_pages.get_device() == k_pers.get_device() == v_pers.get_device():
+    if not index == k_pers.get_device() == v_pers.get_device():
         _refuse_devices(name, k_pages, k_pers, v_pers)
     if not k_pages.dtype is k_pers.dtype is v_pers.dtype:
         raise TypeError("k_pers and v_pers must have the dtype of the pages")
     pers = k_pers.shape
-    if len(pers) != 3 or pers[0] != k_pages.shape[1] or pers[2] != k_pages.shape[3] or v_pers.shape != pers or not k_pers.is_contiguous() \
+    if len(pers) != 3 or pers[0] != kv_heads or pers[2] != head_dim or v_pers.shape != pers or not k_pers.is_contiguous() \
             or not v_pers.is_contiguous():
         raise ValueError("k_pers and v_pers must be contiguous [kv_heads, n_persistent, head_dim]")
     return pers[1]
@@ -455,7 +457,7 @@ def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
             raise ValueError("positions must be contiguous [batch, nodes]")
     n_persistent = 0
     if k_pers is not None or v_pers is not None:
-        n_persistent = _check_persistent("paged_tree_attention", k_pages, k_pers, v_pers)
+        n_persistent = _check_persistent("paged_tree_attention", k_pages, index, kv_heads, head_dim, k_pers, v_pers)
     scaled = None
     if eight or scales is not None or pers_scales is not None:
         scaled = _scale_numbers("paged_tree_attention", k_pages, v_pages, scales, pers_scales,
@@ -481,8 +483,7 @@ def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
                       qs[2], os_[0], os_[1], os_[2], start.data_ptr(), counts.data_ptr() if counts is not None else 0,
                       positions.data_ptr() if positions is not None else 0, seen.data_ptr())
     lib, device = _native.lib(), k_pages.device
-    with _native._on(device):
-        nbytes = lib.tmw_paged_tree_attention_scratch_bytes(desc, scaled)
+    nbytes = _native.ask(index, lib.tmw_paged_tree_attention_scratch_bytes, desc, scaled)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)  # (of this call alone)
     _native.launch(index, lib.tmw_paged_tree_attention, desc, scaled, scratch.data_ptr() or None, nbytes)
     return out
