@@ -394,3 +394,14 @@ def test_many_rows_with_strides():
                                out=out.permute(0, 2, 1, 3)[..., 3:67])
     check(got, *case.want())
     assert (out[..., :3] == 0).all() and (out[..., 67:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,form", [(BF, None), (HF, None), (BF, I8), (HF, E4)])
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("dh,nodes,group", [(128, 8, 1), (128, 9, 1), (128, 4, 4), (128, 31, 1), (128, 8, 4), (128, 33, 1), (64, 16, 2), (64, 33, 1),
+                                            (64, 12, 4), (64, 49, 1), (64, 7, 7)])
+def test_rows_on_both_sides_of_what_tcgen05_takes(dh, nodes, group, page, dtype, form):
+    case = Case([210, 0, 65], [nodes, nodes, 1], nodes, 2 * group, 2, dh, page, dtype, form, 90, 3, seed=nodes)
+    got = case.run()
+    _native.poll_status(DEV)
+    check(got, *case.want())
