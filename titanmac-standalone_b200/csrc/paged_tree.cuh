@@ -72,7 +72,7 @@ __device__ __forceinline__ void split_in_two(float a, float b, uint32_t& first, 
 // One warp's sixteen rows of an item.  P: of keys and values; M: of the products, P itself or fp16 for codes of 8 bits.
 template <typename P, int DH>
 struct TreeCore {
-    static constexpr bool k8 = kScaled<P>;
+    static constexpr bool k8 = kScaled<P>, kMayBeWild = !std::is_same<P, int8_t>::value;  // infinities and NaN among the values
     using M = std::conditional_t<k8, __half, P>;
     static constexpr int KT = kTreeKeys, kRowBytes = DH * (int)sizeof(P), kSteps = DH / 16;
     static constexpr float kRaise = std::is_same<M, __half>::value ? 12.f : 0.f;
@@ -304,7 +304,7 @@ struct TreeCore {
                 ptx::fence_proxy_async_smem();  // (before TMA writes there again)
                 __syncwarp();
             }
-            if constexpr (!k8) {
+            if constexpr (kMayBeWild) {
                 if (has_wild(values)) {
                     add_by_numbers(values, s, keep);
                     return;
@@ -362,10 +362,12 @@ struct TreeCore {
             }
         }
     }
-    // Whether the values of a tile hold an infinity or a NaN: a row to a lane.
+    // Whether the values of a tile hold an infinity or a NaN (e4m3: codes that are no number, all seven bits): a row to a lane.
     __device__ __forceinline__ bool has_wild(uint32_t values) const {
         const int lane = threadIdx.x & 31;
-        constexpr uint32_t up = std::is_same<M, __half>::value ? 0x04000400u : 0x00800080u;  // carries the largest exponent into the sign
+        // carries the largest exponent, or all seven bits, into the sign
+        constexpr uint32_t up = k8 ? 0x01010101u : std::is_same<M, __half>::value ? 0x04000400u : 0x00800080u;
+        constexpr uint32_t signs = k8 ? 0x80808080u : 0x80008000u;
         uint32_t found = 0;
 #pragma unroll 4
         for (int c = 0; c < kRowBytes / 16; ++c) {
@@ -375,9 +377,9 @@ struct TreeCore {
                          : "r"(values + Layout::offset(lane, c))
                          : "memory");
 #pragma unroll
-            for (int i = 0; i < 4; ++i) found |= (v[i] & 0x7fff7fffu) + up;
+            for (int i = 0; i < 4; ++i) found |= (v[i] & ~signs) + up;
         }
-        return __any_sync(0xffffffffu, (found & 0x80008000u) != 0);
+        return __any_sync(0xffffffffu, (found & signs) != 0);
     }
     // O += P V of a tile with such values: number by number, so that what a row does not see stays out of it.  s: the weights.
     __device__ __forceinline__ void add_by_numbers(uint32_t values, const float (&s)[KT / 8][4], const float (&keep)[2]) {
@@ -398,15 +400,24 @@ struct TreeCore {
                 w[i] = __shfl_sync(0xffffffffu, x, (lane & ~3) + key % 8 / 2);
             }
 #pragma unroll
-            for (int n = 0; n < DH / 8; ++n) {
+            for (int c = 0; c < kRowBytes / 16; ++c) {
                 uint32_t v;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(values + Layout::offset(key, n) + t * 4) : "memory");
-                const float2 x = unpack2<M>(v);
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(values + Layout::offset(key, c) + t * 4) : "memory");
+                float2 x, y = make_float2(0.f, 0.f);  // two neighbouring dimensions; codes: and the next two
+                if constexpr (std::is_same<P, E4m3>::value) x = __half22float2(from_e4m3(v)), y = __half22float2(from_e4m3(v >> 16));
+                else x = unpack2<M>(v);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (w[i] == 0.f) continue;
-                    o[n][2 * i] = fmaf(w[i], x.x, o[n][2 * i]);
-                    o[n][2 * i + 1] = fmaf(w[i], x.y, o[n][2 * i + 1]);
+                    if constexpr (k8) {
+                        o[2 * c][2 * i] = fmaf(w[i], x.x, o[2 * c][2 * i]);
+                        o[2 * c + 1][2 * i] = fmaf(w[i], x.y, o[2 * c + 1][2 * i]);
+                        o[2 * c][2 * i + 1] = fmaf(w[i], y.x, o[2 * c][2 * i + 1]);
+                        o[2 * c + 1][2 * i + 1] = fmaf(w[i], y.y, o[2 * c + 1][2 * i + 1]);
+                    } else {
+                        o[c][2 * i] = fmaf(w[i], x.x, o[c][2 * i]);
+                        o[c][2 * i + 1] = fmaf(w[i], x.y, o[c][2 * i + 1]);
+                    }
                 }
             }
         }

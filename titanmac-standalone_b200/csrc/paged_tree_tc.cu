@@ -110,6 +110,7 @@ template <typename P, int DH>
 __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_kernel(const __grid_constant__ PagedAttentionBulk p) {
     using L = TcLayout<P, DH>;
     constexpr bool k8 = L::k8, BF16 = std::is_same<P, __nv_bfloat16>::value;
+    constexpr bool kMayBeWild = !std::is_same<P, int8_t>::value;  // infinities and NaN among the values
     using M = std::conditional_t<BF16, __nv_bfloat16, __half>;
     constexpr int KT = kTcKeys, KS = L::kKStages, VS = L::kVStages;
     constexpr float kRaise = BF16 ? 0.f : k8 ? 10.f : 11.f;  // (a weight is at most 2^4, of codes 2^5, times that)
@@ -542,8 +543,8 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
                     l += (a + b) + (c + d);
                     tc_wait_st();
                 }
-                if (!k8 && !whole) {
-                    // values that must not count: a thread has half a row of them
+                if (kMayBeWild && !whole) {
+                    // values that must not count: a thread has half a row of them (of codes they are fp16 numbers already)
                     const int key = row >> 1;
                     unsigned char* half = smem + L::kV + v_stage * L::kTile + key * 128;
                     constexpr int kChunks = DH / 16;  // sixteen-byte pieces of a half
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
                         uint64_t mine = 0;  // keys that have a weight
 #pragma unroll
                         for (int j = 0; j < KT; ++j)
-                            if (warp_there && !(ex2_ftz(fmaf(__uint_as_float(s[j]), p.scale, -less)) == 0.f)) mine |= 1ull << j;
+                            if (warp_there && !(ex2_ftz(fmaf(__uint_as_float(s[j]), scale, -less)) == 0.f)) mine |= 1ull << j;
                         for (int j = 0; j < KT; ++j) {
                             const unsigned char* v = smem + L::kV + v_stage * L::kTile + j * 128;
                             for (int d = 0; d < DH; ++d) {
