@@ -1,11 +1,14 @@
-"""Drafted trees where their sums are delicate: what single numbers of a value do to the rows that see them and to those that do not."""
+"""Drafted trees where their sums are delicate: what single numbers of a value do to the rows that see them and to those that do not,
+sums over very many keys."""
+
+import math
 
 import pytest
 import torch
 
 import paged_drafts_reference as dr
-from test_paged_drafts_gpu import BF, DEV, E4, FF, HF, Case, check
-from titanmac_b200 import _native
+from test_paged_drafts_gpu import BF, DEV, E4, FF, HF, I8, Case, check, dev, numbers
+from titanmac_b200 import _native, paged_tree_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +55,77 @@ def test_codes_that_are_no_number_reach_those_that_see_them(dtype, dh, nodes, he
     _native.poll_status(DEV)
     assert torch.equal(torch.isnan(got), nan)
     check(got.masked_fill(nan, 0), want.masked_fill(nan, 0), bound)
+
+
+# ---- very many keys ----------------------------------------------------------------------------------------------------------
+
+
+def pages_of(form, dh, values, g):
+    """One page of 64 tokens, keys of normal numbers; ``(k, v, scales)`` and what they stand for."""
+    k = torch.randn(1, 1, 64, dh, generator=g)
+    if form is None:
+        k, v = k.to(HF), values.to(HF)
+        return (k, v, None), (k.double(), v.double())
+    (k, ks), (v, vs) = dr.coded(k, form), dr.coded(values, form)
+    if (values == 1).all():
+        v, vs = torch.full(v.shape, 64.0).to(form), torch.full_like(vs, 2.0 ** -6)
+    return (k, v, (ks, vs)), (dr.meant(k, ks), dr.meant(v, vs))
+
+
+def long_chains(B, tokens, nodes, dh, held, g):
+    """Chains of ``nodes`` behind ``tokens`` that all lie in one page, which the tables name over and over."""
+    k, v, scales = held
+    table = torch.zeros(B, (tokens + nodes + 63) // 64, dtype=torch.int32, device=DEV)
+    q = torch.randn(B, 1, nodes, dh, generator=g).to(HF).to(DEV)
+    seen = torch.tensor([[-1 if i == 63 else (2 << i) - 1 for i in range(nodes)]] * B, device=DEV)
+    out = paged_tree_attention(q, k.to(DEV), v.to(DEV), table, numbers([tokens] * B), seen, scales=dev(scales)[0])
+    _native.poll_status(DEV)
+    return q, out
+
+
+# With as many sequences as SMs one CTA has all the keys of each; with one sequence every CTA has an equal part of it.  (64 tokens to a tile:
+# 8202 and 40 are a tile more than 128, 16484 two more than 256.)
+MUCH = [("all", 5000), ("all", 8202), ("all", 16484), ("all", 400_000), (1, 2_500_000)]
+
+
+def batch(B):
+    return torch.cuda.get_device_properties(DEV).multi_processor_count if B == "all" else B
+
+
+@pytest.mark.parametrize("form", [None, I8, E4])
+@pytest.mark.parametrize("dh,nodes", [(128, 6), (128, 40), (64, 60)])
+@pytest.mark.parametrize("B,tokens", MUCH)
+def test_sums_over_very_many_keys_lose_nothing(B, tokens, dh, nodes, form):
+    """Values that are all one: an output is one, whatever the weights.  512 products in a row may each cut off 2^-23 of the sum; a row's
+    sum of weights is rounded by 2^-24 some 100 times on the way through as many keys, parts are added up at most 200 times; a weight is held
+    in 22 bits: 6.1e-5 + 1.8e-5 + 2.4e-7 at the most, less than the half step 2^-12 of fp16 below one."""
+    g = torch.Generator().manual_seed(2)
+    held, _ = pages_of(form, dh, torch.ones(1, 1, 64, dh), g)
+    _, out = long_chains(batch(B), tokens, nodes, dh, held, g)
+    assert (out == 1).all(), (out.float() - 1).abs().max().item()
+
+
+@pytest.mark.parametrize("form", [None, I8, E4])
+@pytest.mark.parametrize("dh,nodes", [(128, 40), (64, 60)])
+@pytest.mark.parametrize("B,tokens", MUCH[1:3] + MUCH[4:])
+def test_outputs_over_very_many_keys(B, tokens, dh, nodes, form):
+    """The same with values of normal numbers, against the formula in 64 bits, a page's token counted as often as it is seen.  A sum is off by what
+    its weights are, by what the scores are, and by what the test above allows, all of the largest value; then one rounding."""
+    g = torch.Generator().manual_seed(3)
+    held, (k, v) = pages_of(form, dh, torch.randn(1, 1, 64, dh, generator=g), g)
+    B = batch(B)
+    q, out = long_chains(B, tokens, nodes, dh, held, g)
+    k, v = k[0, 0].to(DEV), v[0, 0].to(DEV)
+    s = q[:, 0].double() @ k.T / math.sqrt(dh)  # [B, nodes, 64]
+    slot = torch.arange(64, device=DEV)
+    times = (tokens // 64 + (slot < tokens % 64)).double()
+    node = torch.arange(nodes, device=DEV)
+    times = times + ((node[None, :, None] <= node[:, None, None]) & ((tokens + node)[None, :, None] % 64 == slot)).sum(1)  # [nodes, 64]
+    w = torch.exp(s - s.amax(-1, keepdim=True)) * times
+    want = w @ v / w.sum(-1, keepdim=True)
+    u = 2.0 ** -23
+    off = (dh + 16) * u * (q[:, 0].double().abs() @ k.abs().T).amax() / math.sqrt(dh) + 2 * u * s.abs().amax()
+    bound = 2 * v.abs().amax() * (1.01 * off + 2.0 ** -22 + 6.1e-5 + 1.8e-5)
+    step = torch.finfo(HF).eps / 2
+    error = (out[:, 0].double() - want).abs() - step * (want.abs() + bound)
+    assert (error <= bound).all(), (error / bound).max().item()

@@ -33,6 +33,10 @@ using namespace ptx;
 
 // kTcCost: what an item costs besides its tiles (2 | 4 | 6 | 9: the ragged sequences 149 | 135 | 127 | 124 us)
 constexpr int kTcKeys = 64, kTcRows = 128, kTcCost = 9;
+// Tensor memory's sums are cut off, not rounded: a product of sixteen keys loses 2^-24 of the sum on the average, 400,000 keys of one part 1.5e-3
+// of it.  After so many tiles, 512 products in either stream (3e-5), a part's outputs leave tensor memory and are added up with rounding
+// (148 sequences of 100,000 tokens that lie in L2, 40 nodes, fp16: 1125 us without, 1183 so; shorter parts the same).
+constexpr int kTcMost = 128;
 constexpr int kTcAhead = 4;  // tiles whose scores are under way: buffers of scores, and tiles in the ring of keys
 
 template <typename P, int DH>
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
                     tc_fence_after();
                     const uint32_t weights = tmem + (t & 3) * KT, to = tmem + kO + (t & 1) * DH;
                     const uint64_t values = mnmajor_desc(base + L::kV + v * L::kTile, L::kSub);
-                    const uint32_t onto = i > 1 || *(volatile int*)&first_adds[t & 1] ? 1u : 0u;  // (a stream's first tile of a part begins its O)
+                    const uint32_t onto = i % kTcMost > 1 || *(volatile int*)&first_adds[t & 1] ? 1u : 0u;  // (else it begins its stream's O)
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -417,261 +421,296 @@ __global__ void __launch_bounds__(TcLayout<P, DH>::kThreads, 1) paged_tree_tc_ke
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) warp_low = max(warp_low, __shfl_xor_sync(0xffffffffu, warp_low, d));
                 if (lane == 0) lows[warp - 4] = warp_low;
-                if (row == 0) first_adds[g] = 0;
                 fence_proxy_async_smem();
                 named_barrier_sync(3, 256);
                 if (lane == 0) mbar_arrive(q_ready);
             }
             const int lowest = max(max(lows[0], lows[1]), max(lows[2], lows[3]));
-            float m_used = -CUDART_INF_F, l = 0.f;
-            const int t1 = t0 + walk.tiles;
-            int t = t0 + ((t0 & 1) != g ? 1 : 0);
-            const bool none = t >= t1;  // (a part of one tile is the other stream's)
-            for (bool begins = true; t < t1; t += 2, begins = false) {
-                const int buf = t & 3, v_stage = t % VS;
-                const uint32_t s_at = tmem + lane_at + buf * KT;
-                mbar_wait(v_full + 8 * v_stage, v_turn(t), &given_up, p.status);
-                mbar_wait(s_full + 8 * buf, turn(t), &given_up, p.status);
-                if constexpr (k8) mbar_wait(parts_full + 8 * (t & 7), (uint32_t)(t >> 3) & 1, &given_up, p.status);
-                tc_fence_after();
-                const TileInfo& info = infos[t & 15];
-                const bool whole = info.first == 0 && info.last == KT - 1 && info.lost == 0 &&
-                                   (info.place < 0 || (info.place + KT <= start && info.place >= lowest));
-                uint32_t s[KT];
-                if (warp_there) {
+            const int t_end = t0 + walk.tiles;
+            while (t0 < t_end) {
+                const int t1 = min(t0 + kTcMost, t_end);
+                float m_used = -CUDART_INF_F, l = 0.f;
+                int t = t0 + ((t0 & 1) != g ? 1 : 0);
+                const bool none = t >= t1;  // (a single tile is the other stream's)
+                for (bool begins = true; t < t1; t += 2, begins = false) {
+                    const int buf = t & 3, v_stage = t % VS;
+                    const uint32_t s_at = tmem + lane_at + buf * KT;
+                    mbar_wait(v_full + 8 * v_stage, v_turn(t), &given_up, p.status);
+                    mbar_wait(s_full + 8 * buf, turn(t), &given_up, p.status);
+                    if constexpr (k8) mbar_wait(parts_full + 8 * (t & 7), (uint32_t)(t >> 3) & 1, &given_up, p.status);
+                    tc_fence_after();
+                    const TileInfo& info = infos[t & 15];
+                    const bool whole = info.first == 0 && info.last == KT - 1 && info.lost == 0 &&
+                                       (info.place < 0 || (info.place + KT <= start && info.place >= lowest));
+                    uint32_t s[KT];
+                    if (warp_there) {
 #pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) {
-                        uint32_t(&part)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + c * 32);
-                        tmem_ld32(s_at + c * 32, part);
+                        for (int c = 0; c < KT / 32; ++c) {
+                            uint32_t(&part)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + c * 32);
+                            tmem_ld32(s_at + c * 32, part);
+                        }
+                        tc_wait_ld();
                     }
-                    tc_wait_ld();
-                }
-                const float4* parts = reinterpret_cast<const float4*>(smem + L::kParts) + (t & 7) * KT;
-                if constexpr (k8) {
-                    const uint64_t q_scale2 = ptx::pack2(q_scale, q_scale);
+                    const float4* parts = reinterpret_cast<const float4*>(smem + L::kParts) + (t & 7) * KT;
+                    if constexpr (k8) {
+                        const uint64_t q_scale2 = ptx::pack2(q_scale, q_scale);
 #pragma unroll
-                    for (int j = 0; j < KT; j += 2) {
-                        const float4 part = parts[j / 2];
-                        const uint64_t x = mul2(ptx::pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), ptx::pack2(part.x, part.y));
-                        float a, b;
-                        ptx::unpack2(fma2(x, q_scale2, ptx::pack2(part.z, part.w)), a, b);
-                        s[j] = __float_as_uint(a), s[j + 1] = __float_as_uint(b);
+                        for (int j = 0; j < KT; j += 2) {
+                            const float4 part = parts[j / 2];
+                            const uint64_t x = mul2(ptx::pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), ptx::pack2(part.x, part.y));
+                            float a, b;
+                            ptx::unpack2(fma2(x, q_scale2, ptx::pack2(part.z, part.w)), a, b);
+                            s[j] = __float_as_uint(a), s[j + 1] = __float_as_uint(b);
+                        }
                     }
-                }
-                const float scale = k8 ? 1.f : p.scale;  // (of codes the scores are what they are)
-                uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first, bad = 0;
-                if (!whole) {
-                    for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1) bad |= (p.run == 64 ? ~0ull : (1ull << p.run) - 1) << (__ffs(todo) - 1) * p.run;
-                    uint64_t seen = exists;
-                    if (info.place >= 0) {
-                        const int nodes_at = start - info.place, from = low - info.place;  // of node 0, of the window's begin
-                        const uint64_t of_nodes = nodes_at >= 0 ? (nodes_at < 64 ? nodes << nodes_at : 0) : (nodes_at > -64 ? nodes >> -nodes_at : 0);
-                        const uint64_t tokens = nodes_at <= 0 ? 0 : nodes_at >= 64 ? ~0ull : (1ull << nodes_at) - 1;
-                        const uint64_t behind = from <= 0 ? ~0ull : from >= 64 ? 0 : ~0ull << from;
-                        seen &= (tokens & behind) | (of_nodes & ~tokens);
-                    }
-                    const uint64_t nan = bad & seen;
-#pragma unroll
-                    for (int j = 0; j < KT; ++j)
-                        if ((seen >> j & 1) == 0) s[j] = 0xff800000u;
-                    if (nan != 0) {
+                    const float scale = k8 ? 1.f : p.scale;  // (of codes the scores are what they are)
+                    uint64_t exists = ~0ull >> (63 - info.last) & ~0ull << info.first, bad = 0;
+                    if (!whole) {
+                        for (uint32_t todo = info.lost; todo != 0; todo &= todo - 1) bad |= (p.run == 64 ? ~0ull : (1ull << p.run) - 1) << (__ffs(todo) - 1) * p.run;
+                        uint64_t seen = exists;
+                        if (info.place >= 0) {
+                            const int nodes_at = start - info.place, from = low - info.place;  // of node 0, of the window's begin
+                            const uint64_t of_nodes = nodes_at >= 0 ? (nodes_at < 64 ? nodes << nodes_at : 0) : (nodes_at > -64 ? nodes >> -nodes_at : 0);
+                            const uint64_t tokens = nodes_at <= 0 ? 0 : nodes_at >= 64 ? ~0ull : (1ull << nodes_at) - 1;
+                            const uint64_t behind = from <= 0 ? ~0ull : from >= 64 ? 0 : ~0ull << from;
+                            seen &= (tokens & behind) | (of_nodes & ~tokens);
+                        }
+                        const uint64_t nan = bad & seen;
 #pragma unroll
                         for (int j = 0; j < KT; ++j)
-                            if (nan >> j & 1) s[j] = 0x7fffffffu;
-                    }
-                }
-                // O may be changed: the products of the stream's last tile are done
-                auto wait_products = [&]() {
-                    mbar_wait(v_free + 8 * ((t - 2) % VS), v_turn(t - 2), &given_up, p.status);
-                    tc_fence_after();
-                };
-                if (warp_there) {
-                    float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+                            if ((seen >> j & 1) == 0) s[j] = 0xff800000u;
+                        if (nan != 0) {
 #pragma unroll
-                    for (int j = 0; j < KT; j += 2)
-                        asm("max.f32 %0, %0, %1, %2;" : "+f"(top[j / 2 & 3]) : "f"(__uint_as_float(s[j])), "f"(__uint_as_float(s[j + 1])));
-                    const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-                    if (begins) {
-                        m_used = tile_top;
-                    } else if (__any_sync(0xffffffffu, tile_top > m_used + 4.f)) {
-                        const float now = tile_top > m_used + 4.f ? tile_top : m_used;
-                        const float keep = m_used == -CUDART_INF_F ? 1.f : ex2_ftz(m_used - now);  // (nothing to keep: zeros, or NaN)
-                        m_used = now;
-                        l *= keep;
-                        wait_products();
+                            for (int j = 0; j < KT; ++j)
+                                if (nan >> j & 1) s[j] = 0x7fffffffu;
+                        }
+                    }
+                    // O may be changed: the products of the stream's last tile are done
+                    auto wait_products = [&]() {
+                        mbar_wait(v_free + 8 * ((t - 2) % VS), v_turn(t - 2), &given_up, p.status);
+                        tc_fence_after();
+                    };
+                    if (warp_there) {
+                        float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                        for (int j = 0; j < KT; j += 2)
+                            asm("max.f32 %0, %0, %1, %2;" : "+f"(top[j / 2 & 3]) : "f"(__uint_as_float(s[j])), "f"(__uint_as_float(s[j + 1])));
+                        const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+                        if (begins) {
+                            m_used = tile_top;
+                        } else if (__any_sync(0xffffffffu, tile_top > m_used + 4.f)) {
+                            const float now = tile_top > m_used + 4.f ? tile_top : m_used;
+                            const float keep = m_used == -CUDART_INF_F ? 1.f : ex2_ftz(m_used - now);  // (nothing to keep: zeros, or NaN)
+                            m_used = now;
+                            l *= keep;
+                            wait_products();
 #pragma unroll 1
-                        for (int c = 0; c < DH; c += 16) {
-                            uint32_t x[16];
-                            tmem_ld16(o_at + c, x);
+                            for (int c = 0; c < DH; c += 16) {
+                                uint32_t x[16];
+                                tmem_ld16(o_at + c, x);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
+                                tmem_st16(o_at + c, x);
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    const float less = (m_used == -CUDART_INF_F ? 0.f : m_used) - kRaise;
+                    if (warp_there) {
+                        const uint64_t scale2 = ptx::pack2(scale, scale), less2 = ptx::pack2(-less, -less);
+                        uint64_t sums[2] = {0, 0};  // two at a time
+#pragma unroll
+                        for (int c = 0; c < KT / 16; ++c) {
+                            uint32_t first[8], second[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                float a, b;
+                                const uint64_t two_scores = ptx::pack2(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1]));
+                                ptx::unpack2(k8 ? add2(two_scores, less2) : fma2(two_scores, scale2, less2), a, b);
+                                a = ex2_ftz(a), b = ex2_ftz(b);
+                                if constexpr (k8) {
+                                    const float4 two = parts[KT / 2 + c * 8 + e];
+                                    const uint64_t w = ptx::pack2(a, b);
+                                    sums[e & 1] = fma2(w, ptx::pack2(two.z, two.w), sums[e & 1]);
+                                    ptx::unpack2(mul2(w, ptx::pack2(two.x, two.y)), a, b);
+                                } else {
+                                    sums[e & 1] = add2(sums[e & 1], ptx::pack2(a, b));
+                                }
+                                split_in_two<M>(a, b, first[e], second[e]);
+                            }
+                            tmem_st8(s_at + c * 8, first);
+                            tmem_st8(s_at + 32 + c * 8, second);
+                        }
+                        float a, b, c, d;
+                        ptx::unpack2(sums[0], a, b);
+                        ptx::unpack2(sums[1], c, d);
+                        l += (a + b) + (c + d);
+                        tc_wait_st();
+                    }
+                    if (kMayBeWild && !whole) {
+                        // values that must not count: a thread has half a row of them (of codes they are fp16 numbers already)
+                        const int key = row >> 1;
+                        unsigned char* half = smem + L::kV + v_stage * L::kTile + key * 128;
+                        constexpr int kChunks = DH / 16;  // sixteen-byte pieces of a half
+                        auto piece = [&](int c) {
+                            c += (row & 1) * kChunks;
+                            return reinterpret_cast<uint4*>(half + c / 8 * L::kSub + ((c % 8 ^ (key & 7)) << 4));
+                        };
+                        constexpr uint32_t up = BF16 ? 0x00800080u : 0x04000400u, inf = BF16 ? 0x7f80u : 0x7c00u;
+                        bool found = false;
+                        if (((exists & ~bad) >> key & 1) == 0) {
+                            for (int c = 0; c < kChunks; ++c) *piece(c) = make_uint4(0, 0, 0, 0);
+                        } else {
+                            uint32_t any = 0;
+                            for (int c = 0; c < kChunks; ++c) {
+                                const uint4 v = *piece(c);
+                                any |= ((v.x & 0x7fff7fffu) + up) | ((v.y & 0x7fff7fffu) + up) | ((v.z & 0x7fff7fffu) + up) | ((v.w & 0x7fff7fffu) + up);
+                            }
+                            found = (any & 0x80008000u) != 0;
+                            if (found) wild[g] = 1;
+                        }
+                        named_barrier_sync(1 + g, 128);
+                        const bool any_wild = *(volatile int*)&wild[g] != 0;
+                        named_barrier_sync(1 + g, 128);  // (all have read it: the next such tile may set it)
+                        if (any_wild) {
+                            // Infinities and NaN to the rows that see them, number by number, into O: in front of a part's first product O
+                            // is made zero, and that product told to add.
+                            if (begins) {
+                                for (int c = 0; c < DH; c += 16) {
+                                    const uint32_t zero[16] = {};
+                                    tmem_st16(o_at + c, zero);
+                                }
+                                tc_wait_st();
+                                if (row == 0) first_adds[g] = 1;
+                            } else {
+                                wait_products();
+                            }
+                            uint64_t mine = 0;  // keys that have a weight
+#pragma unroll
+                            for (int j = 0; j < KT; ++j)
+                                if (warp_there && !(ex2_ftz(fmaf(__uint_as_float(s[j]), scale, -less)) == 0.f)) mine |= 1ull << j;
+                            for (int j = 0; j < KT; ++j) {
+                                const unsigned char* v = smem + L::kV + v_stage * L::kTile + j * 128;
+                                for (int d = 0; d < DH; ++d) {
+                                    const uint32_t x = *reinterpret_cast<const uint16_t*>(v + d / 64 * L::kSub + ((d % 64 / 8 ^ (j & 7)) << 4) + d % 8 * 2);
+                                    if ((x & 0x7fffu) < inf) continue;  // (the same for all rows)
+                                    uint32_t o;
+                                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_at + d) : "memory");
+                                    tc_wait_ld();
+                                    const float add = (x & 0x7fffu) > inf ? CUDART_NAN_F : x & 0x8000u ? -CUDART_INF_F : CUDART_INF_F;
+                                    if (mine >> j & 1) o = __float_as_uint(__uint_as_float(o) + add);
+                                    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(o_at + d), "r"(o) : "memory");
+                                    tc_wait_st();
+                                }
+                            }
+                            named_barrier_sync(1 + g, 128);
+                            if (found) {
+                                for (int c = 0; c < kChunks; ++c) {
+                                    uint16_t* x = reinterpret_cast<uint16_t*>(piece(c));
+                                    for (int e = 0; e < 8; ++e)
+                                        if ((x[e] & 0x7fffu) >= inf) x[e] = 0;
+                                }
+                            }
+                            if (row == 0) wild[g] = 0;
+                            named_barrier_sync(1 + g, 128);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready + 8 * buf);
+                }
+                if (none) {  // (an O of anything, which must not count)
+#pragma unroll 1
+                    for (int c = 0; c < DH; c += 16) {
+                        const uint32_t zero[16] = {};
+                        tmem_st16(o_at + c, zero);
+                    }
+                    tc_wait_st();
+                } else {
+                    mbar_wait(v_free + 8 * ((t - 2) % VS), v_turn(t - 2), &given_up, p.status);
+                }
+                const bool goes_on = t0 + walk.tiles > t_end, last = t1 == t_end;
+                const long long slot = (blockIdx.x * 2 + (walk.starts ? 1 : 0)) * (long long)p.rows + row;
+                t0 = t1;
+                float2 before = make_float2(-CUDART_INF_F, 0.f);  // what the part has so far
+                if (goes_on && there) before = p.sums[slot];
+                if (row == 0) first_adds[g] = 0;
+                stream_sums[g][row] = make_float2(m_used, l);
+                tc_fence_before();
+                named_barrier_sync(3, 256);
+                tc_fence_after();
+                // both streams' outputs, a half of the dimensions each
+                const float2 other = stream_sums[g ^ 1][row];
+                const float m = fmaxf(fmaxf(m_used, other.x), before.x), of = m == -CUDART_INF_F ? 0.f : m;
+                float own_part = part_weight(m_used, of);
+                float* so_far = p.partial + (slot - row) * DH + row;
+                if (goes_on) {  // what the part had goes onto this stream's half (sixteen numbers at a time: every tile of codes 2.5 % slower)
+                    const float weight = part_weight(before.x, of);
+                    if (warp_there) {
+#pragma unroll 1
+                        for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 8) {
+                            uint32_t x[8];
+                            tmem_ld8(o_at + c, x);
+                            float had[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) had[e] = there ? so_far[(c + e) * p.rows] : 0.f;
                             tc_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
-                            tmem_st16(o_at + c, x);
+                            for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(fmaf(had[e], weight, __uint_as_float(x[e]) * own_part));
+                            tmem_st8(o_at + c, x);
                         }
                         tc_wait_st();
                     }
+                    own_part = 1.f;
+                    named_barrier_sync(3, 256);  // (rows of the last outputs lie across what others had)
                 }
-                const float less = (m_used == -CUDART_INF_F ? 0.f : m_used) - kRaise;
                 if (warp_there) {
-                    const uint64_t scale2 = ptx::pack2(scale, scale), less2 = ptx::pack2(-less, -less);
-                    uint64_t sums[2] = {0, 0};  // two at a time
+                    const float other_part = part_weight(other.x, of);
+                    const float sum = l * part_weight(m_used, of) + other.y * other_part + before.y * part_weight(before.x, of);
+                    const bool out = walk.starts && walk.ends && last;
+                    const float scale = there && out ? inverse_of<true>(p, rows, row, sum) : 1.f;
+                    uint16_t* to = static_cast<uint16_t*>(p.o) + (there ? row_at<true>(p, p.os, rows, row) : 0);
+#pragma unroll 2
+                    for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 16) {
+                        uint32_t x[16], y[16];
+                        tmem_ld16(o_at + c, x);
+                        tmem_ld16(tmem + lane_at + kO + (g ^ 1) * DH + c, y);
+                        tc_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < KT / 16; ++c) {
-                        uint32_t first[8], second[8];
+                        for (int e = 0; e < 16; ++e)
+                            x[e] = __float_as_uint((__uint_as_float(x[e]) * own_part + __uint_as_float(y[e]) * other_part) * scale);
+                        if (there && out) {
+                            uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            float a, b;
-                            const uint64_t two_scores = ptx::pack2(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1]));
-                            ptx::unpack2(k8 ? add2(two_scores, less2) : fma2(two_scores, scale2, less2), a, b);
-                            a = ex2_ftz(a), b = ex2_ftz(b);
-                            if constexpr (k8) {
-                                const float4 two = parts[KT / 2 + c * 8 + e];
-                                const uint64_t w = ptx::pack2(a, b);
-                                sums[e & 1] = fma2(w, ptx::pack2(two.z, two.w), sums[e & 1]);
-                                ptx::unpack2(mul2(w, ptx::pack2(two.x, two.y)), a, b);
+                            for (int e = 0; e < 8; ++e) {
+                                const float a = __uint_as_float(x[2 * e]), b = __uint_as_float(x[2 * e + 1]);
+                                w[e] = (k8 ? p.bf16 : BF16) ? tmw::pack2<__nv_bfloat16>(a, b) : tmw::pack2<__half>(a, b);
+                            }
+                            if (p.o_wide) {
+                                reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                                reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
                             } else {
-                                sums[e & 1] = add2(sums[e & 1], ptx::pack2(a, b));
-                            }
-                            split_in_two<M>(a, b, first[e], second[e]);
-                        }
-                        tmem_st8(s_at + c * 8, first);
-                        tmem_st8(s_at + 32 + c * 8, second);
-                    }
-                    float a, b, c, d;
-                    ptx::unpack2(sums[0], a, b);
-                    ptx::unpack2(sums[1], c, d);
-                    l += (a + b) + (c + d);
-                    tc_wait_st();
-                }
-                if (kMayBeWild && !whole) {
-                    // values that must not count: a thread has half a row of them (of codes they are fp16 numbers already)
-                    const int key = row >> 1;
-                    unsigned char* half = smem + L::kV + v_stage * L::kTile + key * 128;
-                    constexpr int kChunks = DH / 16;  // sixteen-byte pieces of a half
-                    auto piece = [&](int c) {
-                        c += (row & 1) * kChunks;
-                        return reinterpret_cast<uint4*>(half + c / 8 * L::kSub + ((c % 8 ^ (key & 7)) << 4));
-                    };
-                    constexpr uint32_t up = BF16 ? 0x00800080u : 0x04000400u, inf = BF16 ? 0x7f80u : 0x7c00u;
-                    bool found = false;
-                    if (((exists & ~bad) >> key & 1) == 0) {
-                        for (int c = 0; c < kChunks; ++c) *piece(c) = make_uint4(0, 0, 0, 0);
-                    } else {
-                        uint32_t any = 0;
-                        for (int c = 0; c < kChunks; ++c) {
-                            const uint4 v = *piece(c);
-                            any |= ((v.x & 0x7fff7fffu) + up) | ((v.y & 0x7fff7fffu) + up) | ((v.z & 0x7fff7fffu) + up) | ((v.w & 0x7fff7fffu) + up);
-                        }
-                        found = (any & 0x80008000u) != 0;
-                        if (found) wild[g] = 1;
-                    }
-                    named_barrier_sync(1 + g, 128);
-                    const bool any_wild = *(volatile int*)&wild[g] != 0;
-                    named_barrier_sync(1 + g, 128);  // (all have read it: the next such tile may set it)
-                    if (any_wild) {
-                        // Infinities and NaN to the rows that see them, number by number, into O: in front of a part's first product O
-                        // is made zero, and that product told to add.
-                        if (begins) {
-                            for (int c = 0; c < DH; c += 16) {
-                                const uint32_t zero[16] = {};
-                                tmem_st16(o_at + c, zero);
-                            }
-                            tc_wait_st();
-                            if (row == 0) first_adds[g] = 1;
-                        } else {
-                            wait_products();
-                        }
-                        uint64_t mine = 0;  // keys that have a weight
 #pragma unroll
-                        for (int j = 0; j < KT; ++j)
-                            if (warp_there && !(ex2_ftz(fmaf(__uint_as_float(s[j]), scale, -less)) == 0.f)) mine |= 1ull << j;
-                        for (int j = 0; j < KT; ++j) {
-                            const unsigned char* v = smem + L::kV + v_stage * L::kTile + j * 128;
-                            for (int d = 0; d < DH; ++d) {
-                                const uint32_t x = *reinterpret_cast<const uint16_t*>(v + d / 64 * L::kSub + ((d % 64 / 8 ^ (j & 7)) << 4) + d % 8 * 2);
-                                if ((x & 0x7fffu) < inf) continue;  // (the same for all rows)
-                                uint32_t o;
-                                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_at + d) : "memory");
-                                tc_wait_ld();
-                                const float add = (x & 0x7fffu) > inf ? CUDART_NAN_F : x & 0x8000u ? -CUDART_INF_F : CUDART_INF_F;
-                                if (mine >> j & 1) o = __float_as_uint(__uint_as_float(o) + add);
-                                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(o_at + d), "r"(o) : "memory");
-                                tc_wait_st();
+                                for (int e = 0; e < 8; ++e) to[c + 2 * e] = (uint16_t)w[e], to[c + 2 * e + 1] = (uint16_t)(w[e] >> 16);
                             }
+                        } else if (there && !last) {  // (dimension by dimension: the rows of a warp side by side)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) so_far[(c + e) * p.rows] = __uint_as_float(x[e]);
+                        } else if (there) {
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4)
+                                *reinterpret_cast<uint4*>(p.partial + slot * DH + c + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
                         }
-                        named_barrier_sync(1 + g, 128);
-                        if (found) {
-                            for (int c = 0; c < kChunks; ++c) {
-                                uint16_t* x = reinterpret_cast<uint16_t*>(piece(c));
-                                for (int e = 0; e < 8; ++e)
-                                    if ((x[e] & 0x7fffu) >= inf) x[e] = 0;
-                            }
-                        }
-                        if (row == 0) wild[g] = 0;
-                        named_barrier_sync(1 + g, 128);
+                        __syncwarp();  // (the next load is the whole warp's)
                     }
-                    fence_proxy_async_smem();
+                    if (there && !out && g == 0) p.sums[slot] = make_float2(m, sum);
                 }
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + 8 * buf);
-            }
-            if (!none) mbar_wait(v_free + 8 * ((t - 2) % VS), v_turn(t - 2), &given_up, p.status);
-            t0 = t1;
-            stream_sums[g][row] = make_float2(m_used, l);
-            tc_fence_before();
-            named_barrier_sync(3, 256);
-            tc_fence_after();
-            if (warp_there) {
-                // both streams' outputs, a half of the dimensions each
-                const float2 other = stream_sums[g ^ 1][row];
-                const float m = fmaxf(m_used, other.x), of = m == -CUDART_INF_F ? 0.f : m;
-                // (a part of one tile: the stream that had none has an O of anything, which must not count)
-                const bool single = walk.tiles == 1;
-                const float own_part = none ? 0.f : part_weight(m_used, of), other_part = single && !none ? 0.f : part_weight(other.x, of);
-                const float sum = l * own_part + other.y * other_part;
-                const bool out = walk.starts && walk.ends;
-                const long long slot = (blockIdx.x * 2 + (walk.starts ? 1 : 0)) * (long long)p.rows + row;
-                const float scale = there && out ? inverse_of<true>(p, rows, row, sum) : 1.f;
-                uint16_t* to = static_cast<uint16_t*>(p.o) + (there ? row_at<true>(p, p.os, rows, row) : 0);
-#pragma unroll 2
-                for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 16) {
-                    uint32_t x[16], y[16];
-                    tmem_ld16(o_at + c, x);
-                    tmem_ld16(tmem + lane_at + kO + (g ^ 1) * DH + c, y);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float a = none ? 0.f : __uint_as_float(x[e]) * own_part;
-                        const float b = single && !none ? 0.f : __uint_as_float(y[e]) * other_part;
-                        x[e] = __float_as_uint((a + b) * scale);
-                    }
-                    if (there && out) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float a = __uint_as_float(x[2 * e]), b = __uint_as_float(x[2 * e + 1]);
-                            w[e] = (k8 ? p.bf16 : BF16) ? tmw::pack2<__nv_bfloat16>(a, b) : tmw::pack2<__half>(a, b);
-                        }
-                        if (p.o_wide) {
-                            reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                            reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) to[c + 2 * e] = (uint16_t)w[e], to[c + 2 * e + 1] = (uint16_t)(w[e] >> 16);
-                        }
-                    } else if (there) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4)
-                            *reinterpret_cast<uint4*>(p.partial + slot * DH + c + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                    }
-                    __syncwarp();  // (the next load is the whole warp's)
-                }
-                if (there && !out && g == 0) p.sums[slot] = make_float2(m, sum);
+                named_barrier_sync(3, 256);  // (O, the queries and the sums may be written again)
             }
             if (walk.starts && !walk.ends && tid == 128) p.joins[blockIdx.x] = make_int4(at.b, at.item, (int)((walk.item_end - 1) / share.per), 0);
-            tc_fence_before();
-            named_barrier_sync(3, 256);  // (O, the queries and the sums may be written again)
         }
     }
     __syncthreads();
