@@ -574,7 +574,8 @@ TMW_API int tmw_paged_attention_scaled(const tmw_paged_attention_desc* desc, con
  * that sees nothing has an output of zero.  What it does not see does not matter, infinities and NaN included.  Rows of o from counts[b] on are left as they
  * are, and with start[b] = -1 all of them.  A count outside 0 .. nodes, a start below -1 or nodes behind the table's end make the
  * sequence's outputs NaN (with such a count all nodes'), a page outside the pool those of the nodes that see it; tmw_poll_status reports
- * it.  Pages of either form (scales NULL: in dtype).  The rest is as with tmw_paged_attention.
+ * it.  Pages of either form (scales NULL: in dtype).  The rest is as with tmw_paged_attention, but that a weight meets its value with 16 bits
+ * in bf16 (off by at most 2^-16 of itself; 24 bits there), with 22 in fp16 and over pages of 8 bits as there.
  */
 typedef struct tmw_paged_tree_desc {
     tmw_pages at;

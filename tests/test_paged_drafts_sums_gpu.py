@@ -1,5 +1,5 @@
 """Drafted trees where their sums are delicate: what single numbers of a value do to the rows that see them and to those that do not,
-sums over very many keys."""
+sums over very many keys, values that cancel."""
 
 import math
 
@@ -8,7 +8,7 @@ import torch
 
 import paged_drafts_reference as dr
 from test_paged_drafts_gpu import BF, DEV, E4, FF, HF, I8, Case, check, dev, numbers
-from titanmac_b200 import _native, paged_tree_attention
+from titanmac_b200 import _native, paged_attention, paged_tree_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,53 @@ def test_outputs_over_very_many_keys(B, tokens, dh, nodes, form):
     step = torch.finfo(HF).eps / 2
     error = (out[:, 0].double() - want).abs() - step * (want.abs() + bound)
     assert (error <= bound).all(), (error / bound).max().item()
+
+
+# ---- values that cancel ------------------------------------------------------------------------------------------------------
+
+
+# How much of itself a weight may be off by, besides what the values' product makes of it: its score, a number of a key here, exact but
+# for three roundings of at most 2^3 / 2 (the exponent of two), ex2.approx to 2^-22, sums of at most 16 products that may each cut off
+# 2^-23 and of 12 roundings; the weight itself as it meets the values, 24 bits in the attention of one token, 16 in a tree over bf16
+# pages, 22 over fp16 pages and codes.
+SUMS = 3 * 2.0 ** -22 + 2.0 ** -22 + 16 * 2.0 ** -23 + 12 * 2.0 ** -24
+TREE = {BF: 2.0 ** -16, HF: 2.0 ** -22, FF: 2.0 ** -23}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF])
+@pytest.mark.parametrize("nodes", [6, 40])
+def test_values_that_cancel(nodes, dtype):
+    """Four tokens' values leave next to nothing of one another, so an output is what its weights have lost; a chain's last node and the
+    attention of one token at its place."""
+    g = torch.Generator().manual_seed(nodes)
+    start, page, dh, heads = 70, 16, 64, 2
+    tokens = start + nodes
+    columns = (tokens + page - 1) // page
+    k, v = torch.zeros(columns, heads, page, dh), torch.zeros(columns, heads, page, dh)
+    k[..., 0] = (torch.randn(columns, heads, page, generator=g) * 0.8).clamp(-2, 2).to(dtype).float()
+    table = torch.randperm(columns, generator=g)[None].to(torch.int32)
+    q = torch.zeros(1, heads, nodes, dh)
+    q[..., 0] = 8.0  # times 1 / sqrt(64)
+    size = torch.zeros(heads, dh, dtype=torch.float64)
+    want = torch.zeros(heads, dh, dtype=torch.float64)
+    for h in range(heads):
+        at = [(int(table[0, t // page]), t % page) for t in range(tokens)]
+        w = torch.softmax(torch.stack([k[a, h, b, 0].double() for a, b in at]), 0)
+        left = torch.zeros(dh, dtype=torch.float64)
+        for n, t in enumerate(torch.tensor([5, 20, 41, 66]) + torch.tensor(nodes // 3)):
+            x = 50 + 50 * torch.rand(dh, generator=g) if n == 0 else (-left / w[t]).float()
+            x = x.to(dtype).float()
+            v[at[t][0], h, at[t][1]] = x
+            left += w[t] * x.double()
+            size[h] += w[t] * x.double().abs()
+        want[h] = left
+    case = [t.to(dtype) for t in (k, v)] + [table]
+    seen = torch.tensor([[(2 << i) - 1 for i in range(nodes)]], device=DEV)
+    tree = paged_tree_attention(*dev(q.to(dtype), *case), numbers([start]), seen)[0, :, -1]
+    one = paged_attention(*dev(q[:, :, -1].to(dtype), *case), numbers([tokens - 1]))[0]
+    _native.poll_status(DEV)
+    for got, more in ((tree, TREE[dtype]), (one, 2.0 ** -23)):
+        off = (got.double().cpu() - want).abs()
+        bound = size * (SUMS + more)
+        step = torch.finfo(dtype).eps / 2 * (want.abs() + bound) + torch.finfo(dtype).tiny
+        assert (off <= bound + step).all(), (off / (bound + step)).max().item()
