@@ -1,0 +1,51 @@
+"""Calls over pages of 8 bits and drafted trees that took, or dropped, something without a word."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from test_model_drafts_gpu import BF, DEV, E4, FF, I8, build, numbers
+from titanmac_b200 import (PagedCache, _native, paged_append, paged_attention, paged_keep, paged_read, paged_tree_attention)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _fresh_status():
+    _native.poll_status(DEV)
+    yield
+
+
+@pytest.mark.parametrize("which", ["k_scales", "v_scales", "k_pers_scales", "v_pers_scales"])
+def test_scales_with_a_forward_mode_derivative_are_refused(which):
+    codes, pers = torch.zeros(2, 1, 8, 16, dtype=I8, device=DEV), torch.zeros(1, 3, 16, dtype=I8, device=DEV)
+    table, x = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, 1, 1, 16, device=DEV)
+    seen = torch.ones(1, 1, dtype=torch.int64, device=DEV)
+    s = {n: torch.ones(2, 1, 8, device=DEV) if "pers" not in n else torch.ones(1, 3, device=DEV)
+         for n in ("k_scales", "v_scales", "k_pers_scales", "v_pers_scales")}
+
+    def calls():
+        scales, more = (s["k_scales"], s["v_scales"]), dict(k_pers=pers, v_pers=pers, pers_scales=(s["k_pers_scales"], s["v_pers_scales"]))
+        yield lambda: paged_attention(x[:, :, 0], codes, codes, table, numbers([0]), scales=scales, **more)
+        yield lambda: paged_tree_attention(x, codes, codes, table, numbers([0]), seen, scales=scales, **more)
+        if "pers" not in which:
+            yield lambda: paged_append(x, x, codes, codes.clone(), table, numbers([0]), scales=scales)
+            yield lambda: paged_read(codes, codes, table, numbers([0]), 1, dtype=FF, scales=scales)
+            yield lambda: paged_keep(codes, codes.clone(), table, numbers([0]), numbers([[0]]), numbers([1]), scales=scales)
+
+    for call in calls():  # nothing is refused outside
+        call()
+    with forward_ad.dual_level():
+        s[which] = forward_ad.make_dual(s[which], torch.ones_like(s[which]))
+        for call in calls():
+            with pytest.raises(NotImplementedError):
+                call()
+    _native.poll_status(DEV)
+
+
+def test_angles_with_a_forward_mode_derivative_are_refused():
+    pages, table = torch.zeros(2, 1, 8, 16, device=DEV), torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    x, inv_freq = torch.zeros(1, 1, 1, 16, device=DEV), torch.ones(8, device=DEV)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            paged_append(x, x, pages, pages.clone(), table, numbers([0]), inv_freq=forward_ad.make_dual(inv_freq, torch.ones_like(inv_freq)))

@@ -72,6 +72,7 @@ def _number_of(name: str, dtype: torch.dtype) -> int:
 def _check_scales(name: str, scales: Optional[Scales], index: int, shape, what: str) -> Scales:
     if scales is None or len(scales) != 2:
         raise ValueError(f"{name}: pages of 8 bits go with {what}, a pair of tensors")
+    _native.refuse_tangents(name, *scales)
     for t in scales:
         if t.get_device() != index:
             _native._require_cuda(t)
@@ -136,7 +137,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if not (dtype is v.dtype and (eight or dtype is k_pages.dtype) and k_pages.dtype is v_pages.dtype
             and torch.int32 is page_table.dtype is start.dtype):
         raise TypeError("paged_append: k, v and the pages must share one dtype; page_table and start must be int32")
-    _native.refuse_tangents("paged_append", k, v, k_pages, v_pages, q)
+    _native.refuse_tangents("paged_append", k, v, k_pages, v_pages, q, inv_freq)
     shape = k.shape
     if len(shape) != 4:
         raise ValueError("paged_append: k and v must be [batch, kv_heads, rows, head_dim]")
