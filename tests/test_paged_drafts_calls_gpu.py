@@ -49,3 +49,20 @@ def test_angles_with_a_forward_mode_derivative_are_refused():
     with forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             paged_append(x, x, pages, pages.clone(), table, numbers([0]), inv_freq=forward_ad.make_dual(inv_freq, torch.ones_like(inv_freq)))
+
+
+@pytest.mark.parametrize("page_dtype", [None, I8, E4])
+def test_persistent_rows_of_any_strides(page_dtype):
+    """Keys and values whose numbers are not neighbours in memory, as a cache in the model's type takes them."""
+    g = torch.Generator().manual_seed(0)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(32, 2, 5, generator=g).to(BF).to(DEV).permute(1, 2, 0) for _ in range(2))
+    caches = [PagedCache(table, 1, 8, 2, 32, None, 5, BF, page_dtype=page_dtype) for _ in range(2)]
+    caches[0].set_persistent(k, v)
+    caches[1].set_persistent(k.contiguous(), v.contiguous())
+    for name in ("k_pers", "v_pers"):
+        a, b = (getattr(c, name).float() for c in caches)
+        assert torch.equal(a, b) and a.abs().max() > 0
+    if page_dtype is not None:
+        assert all(torch.equal(a, b) for a, b in zip(caches[0].pers_scales, caches[1].pers_scales))
+    _native.poll_status(DEV)

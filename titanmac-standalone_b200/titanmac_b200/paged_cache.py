@@ -559,8 +559,9 @@ class PagedCache:
             self.k_pers.copy_(k_pers)
             self.v_pers.copy_(v_pers)
         elif self.n_persistent:  # as one page, of tokens from 0 on
-            paged_append(k_pers[None].to(self.dtype), v_pers[None].to(self.dtype), self.k_pers[None], self.v_pers[None], self._one_page,
-                         self._one_page[0], scales=tuple(t[None] for t in self.pers_scales))
+            k, v = (t[None].to(device=self.device, dtype=self.dtype).contiguous() for t in (k_pers, v_pers))
+            paged_append(k, v, self.k_pers[None], self.v_pers[None], self._one_page, self._one_page[0],
+                         scales=tuple(t[None] for t in self.pers_scales))
 
     def append(self, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: Optional[torch.Tensor] = None,
                q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
