@@ -66,3 +66,19 @@ def test_persistent_rows_of_any_strides(page_dtype):
     if page_dtype is not None:
         assert all(torch.equal(a, b) for a, b in zip(caches[0].pers_scales, caches[1].pers_scales))
     _native.poll_status(DEV)
+
+
+def test_a_tree_goes_through_every_layer():
+    """Fewer or more caches than layers: not a model's answer that leaves layers out."""
+    model = build(FF)
+    table = torch.arange(2 * 8).view(2, 8).to(torch.int32).to(DEV)
+    _, caches = model.prefill(torch.randint(0, 64, (2, 9), device=DEV), model.new_paged_caches(table, 16, 8, FF))
+    drafts, parents = torch.zeros(2, 3, dtype=torch.int64, device=DEV), torch.tensor([[-1, 0, 0]] * 2, device=DEV)
+    before = [c.k_pages.clone() for c in caches]
+    for some in (caches[:1], caches + caches[:1], []):
+        with pytest.raises(ValueError):
+            model.decode_tree(drafts, parents, numbers([9, 9]), some)
+        with pytest.raises(ValueError):
+            model.keep_drafts(some, numbers([9, 9]), numbers([[0]] * 2), numbers([1, 1]))
+    assert all(torch.equal(c.k_pages, b) for c, b in zip(caches, before))
+    _native.poll_status(DEV)

@@ -158,6 +158,10 @@ class TitanMAC(nn.Module):
                 "the ring-cache generation path (prefill / decode_step / generate) is built for WindowedAttention; "
                 "build the config with use_block_sparse=False (forward() works with either attention class)")
 
+    def _need_caches(self, caches) -> None:
+        if len(caches) != len(self.layers):
+            raise ValueError(f"one cache for each of the {len(self.layers)} layers expected, got {len(caches)}")
+
     def new_caches(self, batch: int, device, dtype) -> List[_native.RingCache]:
         self._need_windowed()
         c = self.config
@@ -285,6 +289,7 @@ class TitanMAC(nn.Module):
         self._need_windowed()
         if not all(isinstance(cache, PagedCache) for cache in caches):
             raise TypeError("decode_tree works with paged caches (new_paged_caches)")
+        self._need_caches(caches)
         if parents.shape != token_ids.shape:
             raise ValueError(f"token_ids and parents must be [batch, nodes] alike, got {list(token_ids.shape)} and {list(parents.shape)}")
         B, N = token_ids.shape
@@ -320,6 +325,7 @@ class TitanMAC(nn.Module):
     def keep_drafts(self, caches: List[PagedCache], start: torch.Tensor, kept: torch.Tensor, counts: torch.Tensor) -> None:
         """The accepted path of ``decode_tree``'s nodes: nodes ``kept[b, : counts[b]]`` (int32, rising) become tokens ``start[b] ..`` of every
         layer's pages; the sequence then has ``start + counts`` tokens."""
+        self._need_caches(caches)
         for cache in caches:
             cache.keep(start, kept, counts)
 
