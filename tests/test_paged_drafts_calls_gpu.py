@@ -82,3 +82,20 @@ def test_a_tree_goes_through_every_layer():
             model.keep_drafts(some, numbers([9, 9]), numbers([[0]] * 2), numbers([1, 1]))
     assert all(torch.equal(c.k_pages, b) for c, b in zip(caches, before))
     _native.poll_status(DEV)
+
+
+@pytest.mark.parametrize("dtype,nodes", [(FF, 4), (BF, 4), (BF, 40)])
+def test_a_tree_that_does_not_end_within_its_pages(dtype, nodes):
+    """Its nodes are NaN, all of them, and that is reported; the other sequence's are as they are alone, and so are the pages."""
+    model = build(dtype, positions=200)
+    table = torch.arange(2 * 8).view(2, 8).to(torch.int32).to(DEV)  # room for 64 tokens
+    _, caches = model.prefill(torch.randint(0, 64, (2, 62), device=DEV), model.new_paged_caches(table, 16, 8, dtype))
+    drafts, parents = torch.randint(0, 64, (2, nodes), device=DEV), torch.arange(-1, nodes - 1, device=DEV).expand(2, nodes).contiguous()
+    alone = model.decode_tree(drafts, parents, numbers([20, -1]), caches)
+    _native.poll_status(DEV)
+    before = [c.k_pages[8:14].clone() for c in caches]
+    got = model.decode_tree(drafts, parents, numbers([20, 62]), caches)
+    with pytest.raises(_native.TmwError):
+        _native.poll_status(DEV)
+    assert torch.isnan(got[1]).all() and torch.equal(got[0], alone[0])
+    assert all(torch.equal(c.k_pages[8:14], b) for c, b in zip(caches, before))

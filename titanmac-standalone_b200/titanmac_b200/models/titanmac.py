@@ -285,7 +285,8 @@ class TitanMAC(nn.Module):
         ``counts [B] int32`` nodes of each (None: all).  Returns logits ``[B, nodes, V]``: at node ``i`` what ``decode_step`` would return
         for its token behind the cached ones and its ancestors.  The nodes' keys and values are tokens ``start ..`` of the pages, where
         ``keep_drafts`` leaves those of an accepted path; the next step, or tree, writes over the others.  Ids and positions outside
-        their tables: as for ``new_paged_caches``, node by node; rows from ``counts`` on mean nothing."""
+        their tables: as for ``new_paged_caches``, node by node, but a tree that does not end within its pages has NaN at every node; rows
+        from ``counts`` on mean nothing."""
         self._need_windowed()
         if not all(isinstance(cache, PagedCache) for cache in caches):
             raise TypeError("decode_tree works with paged caches (new_paged_caches)")
