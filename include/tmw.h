@@ -526,7 +526,9 @@ TMW_API int tmw_paged_attention(const tmw_paged_attention_desc* desc, void* scra
  *
  * A row x of head_dim numbers (a key rotated already) is written as scale = max(max |x| / largest, 2^-100), largest being 127 or 448,
  * and the codes nearest to x / scale, halves to the even one.  A row with a NaN or an infinity has a scale of NaN and codes of 0: it
- * reads as NaN.  Scales that the caller writes are positive and below 2^126; what is below 2^-100 counts as that under a value.
+ * reads as NaN.  Scales that the caller writes are positive and below 2^126; what is below 2^-100 counts as that under a value.  Where
+ * the scales of the values that a query sees are more than 2^112 apart, tokens with the smaller ones may be missing from its sum of weights:
+ * beside a row of zeros, whose scale is 2^-100, rows that the append writes may have numbers up to 2^18.
  */
 enum { TMW_PAGES_SAME = 0, TMW_PAGES_INT8 = 1, TMW_PAGES_E4M3 = 2 };
 typedef struct tmw_page_scales {

@@ -179,3 +179,23 @@ def test_values_that_cancel(nodes, dtype):
         bound = size * (SUMS + more)
         step = torch.finfo(dtype).eps / 2 * (want.abs() + bound) + torch.finfo(dtype).tiny
         assert (off <= bound + step).all(), (off / (bound + step)).max().item()
+
+
+# ---- values whose scales lie far apart ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("form", [I8, E4])
+@pytest.mark.parametrize("dh,nodes,heads,page", [(64, 6, 2, 16), (64, 6, 2, 12), (128, 40, 2, 16), (64, 60, 1, 16), (144, 6, 2, 16)])
+def test_scales_as_far_apart_as_is_allowed(dh, nodes, heads, page, form):
+    """Values of zeros, whose scale is the least one, between some of 2^12: the zeros count in a row's sum of weights."""
+    case = Case([70], [nodes], nodes, heads, 1, dh, page, BF, form, seed=nodes, branch=1)
+    for t in range(70 + nodes):
+        at = int(case.table[0, t // page]), slice(None), t % page
+        if t % 3 == 1:
+            case.v.view(torch.uint8)[at] = 0
+        case.scales[1][at] = dr.LEAST if t % 3 == 1 else 2.0 ** 12
+    got, (want, bound) = case.run(), case.want()
+    check(got, want, bound)
+    one = paged_attention(*dev(case.q[:, :, -1].contiguous(), case.k, case.v, case.table), numbers([70 + nodes - 1]), scales=dev(case.scales)[0])
+    check(one, want[:, :, -1], bound[:, :, -1])
+    _native.poll_status(DEV)

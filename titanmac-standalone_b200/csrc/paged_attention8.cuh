@@ -16,9 +16,11 @@ namespace {
 // lanes.  Queries in bf16 go in as fp16 times a power of two of each head's own: what their largest number leaves no bits for is 2^-38 of it.
 //
 // A key's scale multiplies its score.  A value's, 2^e f with 1 <= f < 2, must not meet the 16-bit weights as it is, since scales may differ by
-// any factor: x_j = s_j + e_j takes the score's place under the running maximum, u_j = 2^(x_j - m) f_j are the weights of the
+// far more than these hold: x_j = s_j + e_j takes the score's place under the running maximum, u_j = 2^(x_j - m) f_j are the weights of the
 // codes, and u_j / scale_j = 2^(x_j - m) 2^-e_j those that are summed up for the denominator; both with one exponential and no
-// logarithm, and a token whose values are small counts as much in the sum as any other.
+// logarithm, and a token whose values are small counts as much in the sum as any other.  That ends where 2^(x_j - m) is no fp32 number any
+// more, 2^-126: with scales 2^114 apart for a token whose weight is 2^-24 of the largest (2^112 in the tcgen05 form, whose weights are
+// raised by two less).
 //
 // HEADS: of an item at most, 1, 2, 4, 8 or 16.  With fewer than eight the columns hold them several times over, and each of the 8 / HEADS
 // copies deals with its own share of the tile's keys: its weights are zero in the rows of the others', its running maximum

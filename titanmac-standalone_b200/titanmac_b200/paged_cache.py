@@ -10,7 +10,8 @@ positions on the way into the cache.
 Pages hold the model's type, or 8 bits: ``int8`` or ``float8_e4m3fn`` codes with an fp32 scale for every token and key head, half the
 memory and half the traffic.  ``scales``, a pair ``(k_scales, v_scales)`` of ``[pages, kv_heads, page_size]``, goes with such pages
 wherever these go; a code stands for itself times its row's scale.  A row is written with ``scale = max(max |x| / largest, 2^-100)``,
-``largest`` 127 or 448, and the codes nearest to ``x / scale``; one with a NaN or an infinity reads as NaN.
+``largest`` 127 or 448, and the codes nearest to ``x / scale``; one with a NaN or an infinity reads as NaN.  Beside values that are all
+zeros others may be up to 2^18 (scales 2^112 apart): beyond that the attention may leave the zeros out of its sum of weights.
 
 Drafted tokens: ``paged_append`` takes several rows of a sequence, with ``positions`` if they form a tree, ``paged_tree_attention``
 attends with all of them at once, and ``paged_keep`` moves the accepted ones together.
