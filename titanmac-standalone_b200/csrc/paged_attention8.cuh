@@ -27,9 +27,9 @@ namespace {
 // is its own, and the copies are added up when the item ends.  So a lane has KT HEADS / 32 exponentials to a tile instead of KT / 4
 // (256 windows of 512, 10 heads of 64: 127 us with one copy, 86 with eight; by TMA then 56).
 //
-// A warp's chain of copies, products and exponentials bounds it, at 50 to 60 % of the issue slots: 256 windows of 512 of 10 heads of 64,
-// int8, 180 MB, 56 us; 48 sequences of up to 16384, 32 heads on 8 of 128, e4m3 under fp16, 350 MB, 78 us; 12 of up to 65536, 32
-// heads on 4 of 128, int8, 583 MB, 131 us.
+// A warp's chain of copies, products and exponentials bounds it, at 51 to 66 % of the issue slots: 256 windows of 512 of 10 heads of 64,
+// int8, 180 MB, 56 us; 48 sequences of up to 16384, 32 heads on 8 of 128, e4m3 under fp16, 350 MB, 77 us; 12 of up to 65536, 32
+// heads on 4 of 128, int8, 583 MB, 129 us.
 //
 // d = a b + c for one 16 x 8 x 16 tile, and d += a b (not volatile: in whichever order the results are needed)
 __device__ __forceinline__ void mma_more(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -8,7 +8,8 @@
 //
 // S = Q K^T and O += P V by mma.sync with the rows as the sixteen of a tile: the scores' registers are the operand of the second
 // product as they are.  (Here M is what bounds it: 2.25 cycles of the SM for each 16 x 8 x 16; which rows tcgen05's 128 take instead is
-// said below, at tree_takes_tc.)  64 windows of 512, 16 nodes, 10 heads of 64, bf16, 86 MB: 39 us, latency: two or three tiles to a worker.  A weight is two 16-bit numbers, as far as a tile's mask goes; only tiles that some row does not see in full, at the
+// said below, at tree_takes_tc.)  64 windows of 512, 16 nodes, 10 heads of 64, bf16, 86 MB: 39 us, a third of the issue slots: seven or eight tiles to a worker and eighteen to an
+// item, so that every item is cut, and its parts go through memory twice.  A weight is two 16-bit numbers, as far as a tile's mask goes; only tiles that some row does not see in full, at the
 // window's begin and among the nodes, run the body with the mask.
 #pragma once
 
@@ -831,7 +832,8 @@ TMW_TREE_OF(tc)
 #undef TMW_TREE_OF
 
 // Which calls tcgen05 takes: pages that come by TMA, head_dim 64 or 128, and so many rows to a key head that mma.sync's work outweighs the longer
-// hand-overs here.  us, tcgen05 | mma.sync:
+// hand-overs here.  One border for all lengths, that of long sequences: windows of a few hundred keys, with fewer tiles to a worker, would want a
+// later one (up to a fifth: 16-bit heads of 64 up to some 48 rows, of 128 up to 24).  us, tcgen05 | mma.sync:
 //   16-bit pages, heads of 128: 16 sequences of up to 16384, 32 heads on 8: 8 rows 115 | 134, 16 rows 116 | 161, 32 rows 118 | 175;
 //     64 windows of 512 of 10 heads: 8 rows 87 | 70, 16 rows 90 | 85, 33 rows 94 | 100
 //   16-bit pages, heads of 64: the same sequences: 32 rows 108 | 99, 48 rows 108 | 121; 32 sequences of 10 heads, 20 rows 346 | 298,

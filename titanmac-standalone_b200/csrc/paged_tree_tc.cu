@@ -11,7 +11,7 @@
 // A tile's chain - products, hand-over, exponentials, hand-over, products - is several times as long as its parts, so two streams of
 // softmax warps take the tiles by turns, each with a running maximum, a sum and an output of its own, and two buffers of scores: S = Q K^T
 // of four tiles is under way while P goes over its S as two 16-bit numbers a weight (64 columns for 64 fp32 ones) and O += P V.
-// The streams are joined when the part ends.  (As two CTAs to an SM, with two tiles of each of K and V: 16 ragged sequences of 32 heads on 8, 32 nodes, 160 us.)
+// The streams are joined when the part ends, or has had kTcMost tiles.  (As two CTAs to an SM, with two tiles of each of K and V: 16 ragged sequences of 32 heads on 8, 32 nodes, 160 us.)
 // The running maximum follows only a score that is 2^4 above it: O is brought up in tensor memory then.  Tiles that some row does not
 // see in full, at a window's begin and among the nodes, have the rows' bits applied to the scores, and their values made harmless: rows
 // that nobody sees are zeros, and what is infinite or no number is added row by row to those that see it.
@@ -20,10 +20,11 @@
 // the same form, once for all rows, and every key's scales into the numbers that the softmax warps use (see the attention of one token):
 // scores times the key's scale, weights times the value's in two parts.
 //
-// 16 sequences of up to 16384, 33 nodes, 32 heads on 8 of 128, fp16, 576 MB: 154 us from HBM alone, 2200 cycles for the 64 keys of a tile in either
-// stream; 6 of up to 65536, 12 nodes, 32 heads on 4 of 128, int8, 307 MB: 220 us, 5500 cycles, the softmax warps'.
+// 16 sequences of up to 16384, 33 nodes, 32 heads on 8 of 128, fp16, 576 MB: 153 us with the join; 118 tiles of 64 keys to a CTA, 2100 cycles
+// each, 1410 for their bytes.  6 of up to 65536, 12 nodes, 32 heads on 4 of 128, int8, 307 MB: 218 us; 122 tiles, 3500 cycles each.  Issue slots are
+// 38 % busy either way: two softmax warps to a scheduler, each a row's 64 keys in one dependent chain.
 //
-// All waits are bounded (paged_attention.cuh); the tensor memory is given back on every way.
+// All waits are bounded (tc_ptx.cuh); the tensor memory is given back on every way.
 #include "paged_tree.cuh"
 
 namespace tmw {
