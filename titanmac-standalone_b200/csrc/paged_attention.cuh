@@ -58,7 +58,11 @@ struct PagedAttention {
     float* firsts;   // [CTA][warp][rows][head_dim]: what a warp has of the item that its piece begins in
     int4* joins;     // [CTA]: the item that begins in it and ends in another one - sequence (-1: none), item, last CTA
     int* status;
+    long long room[3];
 };
+// What a launch takes of the host goes by its arguments' size, in steps that repeat every 64 bytes (driver 580.159; this kernel's launch and
+// its join's, us: 232 bytes 4.3, 240 - 272 4.7, 280 - 288 4.0, 296 4.4, 304 - 336 4.7, 344 - 352 4.0).
+static_assert(sizeof(PagedAttention) % 64 == 24 || sizeof(PagedAttention) % 64 == 32, "a size that launches quickly");
 
 // Tiles, of KT keys, of sequence b's items; lo, pos: its first and last token seen (lo > pos: none); count: its drafted nodes, the last
 // tokens.  0 with bad: no such position.  TREE: with drafted nodes instead of one new token.
